@@ -194,6 +194,131 @@ typedef struct RoostQkvQkNormRopeCacheWriteParams {
 ROOST_API RoostStatus roost_qkv_qk_norm_rope_cache_write_run(RoostContext* ctx, const void* params,
                                                              const RoostWorkspace* ws, void* stream);
 
+/* The fused ops between a layer's residual stream and its projections: ROOST_OP_ADD_RMS_NORM (64),
+ * ROOST_OP_ADD_RMS_NORM_QUANT (65), ROOST_OP_SILU_MUL_QUANT (66) and ROOST_OP_GEMM_LORA_EPILOGUE (68), of which the
+ * reference's C header names the ids only. They are reached by name, outside the registration table, whose variants a
+ * Roost loader checks against its manifest. Every call may be captured into a HIP graph, is deterministic, allocates
+ * nothing and does not synchronise; the context's device must be current. Row strides are elements between rows, 0 for
+ * contiguous rows; rows need only their element type's alignment unless stated. */
+
+/* AddRmsNorm. Per row, in f32: s = input + residual; residual_out = s; output = s / sqrt(mean(s^2) + eps) * weight.
+ * The norm takes the f32 sum, not the rounded residual_out; each output is rounded once. Without a residual (NULL
+ * address) s = input; without a residual_out the sum is not stored. output and residual_out may each be exactly the
+ * input or the residual (same address, stride and type); any other overlap is refused. A row's result does not depend on
+ * the other rows of the call. dim <= 32768. */
+typedef struct RoostAmdAddRmsNormParams {
+  uint32_t struct_size;
+  uint32_t abi_minor;
+  RoostDeviceSpan input;        /* [rows, dim] bf16 or f32 */
+  RoostDeviceSpan residual;     /* [rows, dim] bf16 or f32, or NULL */
+  RoostDeviceSpan weight;       /* [dim] bf16 or f32 */
+  RoostDeviceSpan residual_out; /* [rows, dim] the residual's type (the input's without one), or NULL */
+  RoostDeviceSpan output;       /* [rows, dim] the input's type */
+  uint32_t rows;
+  uint32_t dim;
+  uint32_t input_stride;
+  uint32_t residual_stride;
+  uint32_t residual_out_stride;
+  uint32_t output_stride;
+  float eps;
+  uint32_t reserved0;
+} RoostAmdAddRmsNormParams;
+
+ROOST_API RoostStatus roost_amd_add_rms_norm_run(RoostContext* ctx, const void* params, void* stream);
+
+/* AddRmsNormQuant. AddRmsNorm with its output y in 8 bits (OCP e4m3) and a scale for each cell: a whole row
+ * (group_size 0) or group_size consecutive columns of it (a power of two from 16 to 512; the last cell of a row may be
+ * shorter). scale = max(max|y| / 448, 2^-126) over the cell's f32 values, code = y / scale rounded to nearest, ties to
+ * even, so code * scale stands for y and a cell of zeros has zero codes. A cell that holds a NaN has a NaN scale and NaN
+ * codes; one that holds an infinity has an infinite scale, zero codes for its finite values and NaN codes for the others. */
+typedef struct RoostAmdAddRmsNormQuantParams {
+  uint32_t struct_size;
+  uint32_t abi_minor;
+  RoostDeviceSpan input;        /* [rows, dim] bf16 or f32 */
+  RoostDeviceSpan residual;     /* [rows, dim] bf16 or f32, or NULL */
+  RoostDeviceSpan weight;       /* [dim] bf16 or f32 */
+  RoostDeviceSpan residual_out; /* [rows, dim] the residual's type (the input's without one), or NULL */
+  RoostDeviceSpan output;       /* [rows, dim] f8e4m3 */
+  RoostDeviceSpan scales;       /* [rows, cells of a row] f32, contiguous */
+  uint32_t rows;
+  uint32_t dim;
+  uint32_t input_stride;
+  uint32_t residual_stride;
+  uint32_t residual_out_stride;
+  uint32_t output_stride;
+  float eps;
+  uint32_t group_size;
+} RoostAmdAddRmsNormQuantParams;
+
+ROOST_API RoostStatus roost_amd_add_rms_norm_quant_run(RoostContext* ctx, const void* params, void* stream);
+
+/* SiluMulQuant. y = gate * sigmoid(gate) * up in f32, then 8 bits and scales as AddRmsNormQuant's. gate and up may be the
+ * halves of one fused projection (row strides); the outputs overlap nothing. dim <= 32768. */
+typedef struct RoostAmdSiluMulQuantParams {
+  uint32_t struct_size;
+  uint32_t abi_minor;
+  RoostDeviceSpan gate;   /* [rows, dim] bf16 or f32 */
+  RoostDeviceSpan up;     /* [rows, dim] the gate's type */
+  RoostDeviceSpan output; /* [rows, dim] f8e4m3 */
+  RoostDeviceSpan scales; /* [rows, cells of a row] f32, contiguous */
+  uint32_t rows;
+  uint32_t dim;
+  uint32_t gate_stride;
+  uint32_t up_stride;
+  uint32_t output_stride;
+  uint32_t group_size;
+} RoostAmdSiluMulQuantParams;
+
+ROOST_API RoostStatus roost_amd_silu_mul_quant_run(RoostContext* ctx, const void* params, void* stream);
+
+/* GemmLora: a projection shared by every sequence, with each sequence's own low-rank adapter on top. For row t of sequence
+ * b (cu_seqlens[b] <= t < cu_seqlens[b + 1]) with adapter a = lora_slots[b] (a C2 step plan's lora_slot):
+ *   output_t = weight x_t + lora_scale[a] * B_a[:, :rank] (A_a[:rank] x_t) + addend_t,  rank = ranks[a] (max_rank if NULL).
+ * A slot below 0 or at or past `adapters` means no adapter; ranks are clamped to [0, max_rank], and what a pool holds past
+ * an adapter's rank is not read into a result. Rows of no sequence (behind cu_seqlens[batch], in a padded batch) are left
+ * as they were. One adapter's values never reach another sequence's rows, NaN and infinity included.
+ *   - x bf16: weight bf16, adapters bf16, output bf16 or f32. x f32: all f32. x f8e4m3 (as AddRmsNormQuant leaves rows with
+ *     group_size 0): weight f8e4m3, a scale for each row of x and of weight, adapters bf16, output bf16 or f32.
+ *   - weight NULL: the adapters alone, on top of the addend (a product that ran elsewhere) or alone.
+ *   - lora_a NULL: no adapters (adapters = max_rank = 0; lora_slots, lora_b, lora_scale and ranks unused).
+ *   - addend: bf16 or f32, may be exactly the output (same address, stride and type); any other overlap of the output is refused.
+ * Sums are f32. In bf16 the low-rank rows A_a x are rounded to bf16 once where many rows are multiplied together.
+ * x, weight, lora_a and lora_b are 16-byte aligned; in_dim and x_stride are multiples of 16 bytes; max_rank is a multiple of
+ * 8 up to 128. cu_seqlens[0] = 0 and cu_seqlens does not go backwards (device data, not checked; a table that breaks this
+ * leaves rows unwritten or gives them a neighbour's adapter, and reads and writes nothing outside the spans). The results
+ * of a row may differ in rounding with the number of tokens of the call. */
+typedef struct RoostAmdGemmLoraParams {
+  uint32_t struct_size;
+  uint32_t abi_minor;
+  RoostDeviceSpan x;          /* [tokens, in_dim] */
+  RoostDeviceSpan x_scale;    /* [tokens] f32 with f8e4m3 rows, else NULL */
+  RoostDeviceSpan weight;     /* [out_dim, in_dim] or NULL */
+  RoostDeviceSpan w_scale;    /* [out_dim] f32 with f8e4m3 weights, else NULL */
+  RoostDeviceSpan lora_a;     /* [adapters, max_rank, in_dim] or NULL */
+  RoostDeviceSpan lora_b;     /* [adapters, out_dim, max_rank] */
+  RoostDeviceSpan lora_scale; /* [adapters] f32, or NULL for 1 */
+  RoostDeviceSpan ranks;      /* [adapters] i32, or NULL */
+  RoostDeviceSpan lora_slots; /* [batch] i32 */
+  RoostDeviceSpan cu_seqlens; /* [batch + 1] i32 */
+  RoostDeviceSpan addend;     /* [tokens, out_dim] or NULL */
+  RoostDeviceSpan output;     /* [tokens, out_dim] */
+  uint32_t tokens;
+  uint32_t batch;
+  uint32_t in_dim;
+  uint32_t out_dim;
+  uint32_t adapters;
+  uint32_t max_rank;
+  uint32_t x_stride;
+  uint32_t addend_stride;
+  uint32_t output_stride;
+  uint32_t reserved0;
+} RoostAmdGemmLoraParams;
+
+/* Device scratch of a call (sizes->device_bytes; the low-rank rows). Its contents are undefined before and after. */
+ROOST_API RoostStatus roost_amd_gemm_lora_workspace(RoostContext* ctx, const void* params, RoostWorkspaceSizes* sizes);
+ROOST_API RoostStatus roost_amd_gemm_lora_run(RoostContext* ctx, const void* params, const RoostWorkspace* ws,
+                                              void* stream);
+
 /* The plan region: the batch tables and slot mapping of one worker step, from its sequences. Replaces the worker's
  * PlanRegionWriter.Fill (reference src/Starlings.Roost.Worker/Eager/PlanRegionWriter.cs:19-64), which the reference runs
  * in C# on a host mirror of the region before one host-to-device copy. For sequence b (in order):

@@ -115,6 +115,12 @@ class KernelLibrary:
         self.dll.roost_amd_gdn_layer_run.argtypes = [C.c_void_p] * 7
         self.dll.roost_amd_gdn_layer_run.restype = C.c_int32
         self.dll.roost_amd_gdn_chunk_layer_plan.restype = C.c_int32
+        for name in ("roost_amd_add_rms_norm_run", "roost_amd_add_rms_norm_quant_run", "roost_amd_silu_mul_quant_run",
+                     "roost_amd_gemm_lora_workspace"):
+            getattr(self.dll, name).argtypes = [C.c_void_p] * 3
+            getattr(self.dll, name).restype = C.c_int32
+        self.dll.roost_amd_gemm_lora_run.argtypes = [C.c_void_p] * 4
+        self.dll.roost_amd_gemm_lora_run.restype = C.c_int32
         self.dll.roost_amd_plan_region_from_step.argtypes = [C.c_void_p, C.c_uint64, C.POINTER(abi.StepTables)]
         self.dll.roost_amd_plan_region_from_step.restype = C.c_int32
         version = self.dll.roost_abi_version()
@@ -186,7 +192,7 @@ def dtype_of(t) -> int:
     torch = _torch()
     return {torch.float32: abi.DTYPE_F32, torch.float16: abi.DTYPE_F16, torch.bfloat16: abi.DTYPE_BF16,
             torch.float64: abi.DTYPE_F64, torch.int32: abi.DTYPE_I32, torch.int64: abi.DTYPE_I64,
-            torch.uint8: abi.DTYPE_U8}[t.dtype]
+            torch.uint8: abi.DTYPE_U8, torch.float8_e4m3fn: abi.DTYPE_F8E4M3}[t.dtype]
 
 
 def span(t, *, length: Optional[int] = None, dtype: Optional[int] = None, offset_elems: int = 0) -> abi.DeviceSpan:
@@ -236,9 +242,12 @@ class OpSession:
         return sizes
 
     def _workspace(self, entry: Entry, params, key) -> abi.Workspace:
+        return self.workspace_of((entry.variant_id, key), self.workspace_sizes(entry, params))
+
+    def workspace_of(self, key, sizes: abi.WorkspaceSizes) -> list:
+        """The buffers kept under `key`, allocated anew when they do not hold `sizes`."""
         torch = _torch()
-        sizes = self.workspace_sizes(entry, params)
-        slot = self._ws.get((entry.variant_id, key))
+        slot = self._ws.get(key)
         fits = slot is not None and slot[3].device_bytes >= sizes.device_bytes and \
             slot[3].pinned_host_bytes >= sizes.pinned_host_bytes and slot[3].plan_bytes >= sizes.plan_bytes
         if not fits:
@@ -255,7 +264,7 @@ class OpSession:
             ws.plan = C.addressof(plan)
             ws.plan_bytes = sizes.plan_bytes
             slot = [dev, pinned, plan, ws, None]
-            self._ws[(entry.variant_id, key)] = slot
+            self._ws[key] = slot
         return slot
 
     def prepare(self, entry: Entry, params, key=0, plan: bool = True) -> Optional[abi.Workspace]:
@@ -542,6 +551,163 @@ def gdn_chunk_layer(session: OpSession, conv_params, gates_params, gdn_params, n
         C.addressof(gdn_params), C.addressof(norm_params), C.addressof(ws), C.c_void_p(session.stream_handle))
     if status != abi.OK:
         raise KernelError("gdn_chunk_layer", status, session.lib.last_error())
+
+
+# ---- the fused ops between the residual stream and the projections (AddRmsNorm, AddRmsNormQuant, SiluMulQuant, GemmLora) ----
+
+def _rows(t, name, rows, dim, dtypes=None):
+    """(span, row stride) of a [rows, dim] tensor whose columns are contiguous; an empty span for None."""
+    if t is None:
+        return abi.DeviceSpan(), 0
+    if t.dim() != 2 or tuple(t.shape) != (rows, dim):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, not {(rows, dim)}")
+    if dtypes is not None and t.dtype not in dtypes:
+        raise ValueError(f"{name}: {t.dtype} is not one of {dtypes}")
+    if dim > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: columns are {t.stride(1)} elements apart, not 1")
+    stride = t.stride(0) if rows > 1 else dim
+    if stride < dim:
+        raise ValueError(f"{name}: rows are {stride} elements apart, below their {dim} columns")
+    return span(t, length=0 if rows == 0 else (rows - 1) * stride + dim), stride
+
+
+def _flat(t, name, shape, dtype=None):
+    """The span of a contiguous tensor of `shape`; an empty span for None."""
+    if t is None:
+        return abi.DeviceSpan()
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name}: shape {tuple(t.shape)} (contiguous: {t.is_contiguous()}), not a contiguous {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name}: {t.dtype}, not {dtype}")
+    return span(t)
+
+
+def _one_device(**tensors):
+    """Every tensor of a call is on the same GPU (the session's device is compared at the call)."""
+    found = {t.device for t in tensors.values() if t is not None}
+    if len(found) > 1 or any(d.type != "cuda" for d in found):
+        raise ValueError("tensors of one call are on " + ", ".join(sorted(f"{k}: {t.device}" for k, t in tensors.items()
+                                                                          if t is not None)))
+    return found.pop()
+
+
+def _cells(dim, group_size):
+    return 1 if group_size == 0 else -(-dim // group_size)
+
+
+def _norm_params(struct, x, residual, weight, residual_out, output, eps):
+    p = abi.new(struct)
+    rows, dim = x.shape
+    p._device = _one_device(x=x, residual=residual, weight=weight, residual_out=residual_out, output=output)
+    p.input, p.input_stride = _rows(x, "x", rows, dim)
+    p.residual, p.residual_stride = _rows(residual, "residual", rows, dim)
+    p.weight = _flat(weight, "weight", (dim,))
+    p.residual_out, p.residual_out_stride = _rows(residual_out, "residual_out", rows, dim)
+    p.output, p.output_stride = _rows(output, "output", rows, dim)
+    p.rows, p.dim, p.eps = rows, dim, eps
+    return p
+
+
+def add_rms_norm_params(x, residual, weight, residual_out, output, *, eps):
+    """RoostAmdAddRmsNormParams: output = RMS norm of x + residual, residual_out = x + residual. residual and residual_out
+    may be None, or x or the residual itself (in place)."""
+    p = _norm_params(abi.AddRmsNormParams, x, residual, weight, residual_out, output, eps)
+    p._keep = (x, residual, weight, residual_out, output)
+    return p
+
+
+def add_rms_norm_quant_params(x, residual, weight, residual_out, output, scales, *, eps, group_size=0):
+    """RoostAmdAddRmsNormQuantParams: the same with output in float8_e4m3fn and scales [rows, cells of a row] f32."""
+    p = _norm_params(abi.AddRmsNormQuantParams, x, residual, weight, residual_out, output, eps)
+    _one_device(output=output, scales=scales)
+    p.scales, p.group_size = _flat(scales, "scales", (p.rows, _cells(p.dim, group_size))), group_size
+    p._keep = (x, residual, weight, residual_out, output, scales)
+    return p
+
+
+def silu_mul_quant_params(gate, up, output, scales, *, group_size=0):
+    """RoostAmdSiluMulQuantParams: silu(gate) * up in float8_e4m3fn with scales [rows, cells of a row] f32; gate and up
+    may be the halves of one fused projection."""
+    p = abi.new(abi.SiluMulQuantParams)
+    rows, dim = gate.shape
+    p._device = _one_device(gate=gate, up=up, output=output, scales=scales)
+    p.gate, p.gate_stride = _rows(gate, "gate", rows, dim)
+    p.up, p.up_stride = _rows(up, "up", rows, dim, (gate.dtype,))
+    p.output, p.output_stride = _rows(output, "output", rows, dim)
+    p.scales = _flat(scales, "scales", (rows, _cells(dim, group_size)))
+    p.rows, p.dim, p.group_size = rows, dim, group_size
+    p._keep = (gate, up, output, scales)
+    return p
+
+
+def gemm_lora_params(x, weight, lora_a, lora_b, lora_scale, lora_slots, cu_seqlens, output, *, ranks=None, x_scale=None,
+                     w_scale=None, addend=None):
+    """RoostAmdGemmLoraParams: output = x weight^T + each sequence's adapter + addend. x [tokens, in_dim]; weight
+    [out_dim, in_dim] or None; lora_a [adapters, max_rank, in_dim], lora_b [adapters, out_dim, max_rank] and lora_slots
+    [batch], or None; cu_seqlens [batch + 1]; x_scale [tokens] and w_scale [out_dim] with float8_e4m3fn rows."""
+    torch = _torch()
+    p = abi.new(abi.GemmLoraParams)
+    tokens, in_dim = x.shape
+    out_dim = output.shape[1]
+    batch = cu_seqlens.shape[0] - 1
+    adapters, max_rank = (0, 0) if lora_a is None else lora_a.shape[:2]
+    p._device = _one_device(x=x, weight=weight, lora_a=lora_a, lora_b=lora_b, lora_scale=lora_scale, lora_slots=lora_slots,
+                            cu_seqlens=cu_seqlens, output=output, ranks=ranks, x_scale=x_scale, w_scale=w_scale, addend=addend)
+    p.x, p.x_stride = _rows(x, "x", tokens, in_dim)
+    p.x_scale = _flat(x_scale, "x_scale", (tokens,), torch.float32)
+    p.weight = _flat(weight, "weight", (out_dim, in_dim), x.dtype)
+    p.w_scale = _flat(w_scale, "w_scale", (out_dim,), torch.float32)
+    p.lora_a = _flat(lora_a, "lora_a", (adapters, max_rank, in_dim))
+    p.lora_b = _flat(lora_b, "lora_b", (adapters, out_dim, max_rank))
+    p.lora_scale = _flat(lora_scale, "lora_scale", (adapters,), torch.float32)
+    p.ranks = _flat(ranks, "ranks", (adapters,), torch.int32)
+    p.lora_slots = _flat(lora_slots, "lora_slots", (batch,), torch.int32)
+    p.cu_seqlens = _flat(cu_seqlens, "cu_seqlens", (batch + 1,), torch.int32)
+    p.addend, p.addend_stride = _rows(addend, "addend", tokens, out_dim)
+    p.output, p.output_stride = _rows(output, "output", tokens, out_dim)
+    p.tokens, p.batch, p.in_dim, p.out_dim, p.adapters, p.max_rank = tokens, batch, in_dim, out_dim, adapters, max_rank
+    p._keep = (x, weight, lora_a, lora_b, lora_scale, lora_slots, cu_seqlens, output, ranks, x_scale, w_scale, addend)
+    return p
+
+
+def _extension(session: OpSession, name: str, fn, params, *more) -> None:
+    if params._device != session.device:
+        raise ValueError(f"{name}: tensors on {params._device}, session on {session.device}")
+    status = fn(session.ctx, C.addressof(params), *more, session.stream_handle)
+    if status != abi.OK:
+        raise KernelError(name, status, session.lib.last_error())
+
+
+def add_rms_norm(session: OpSession, params) -> None:
+    """roost_amd_add_rms_norm_run on the session's stream."""
+    _extension(session, "add_rms_norm", session.lib.dll.roost_amd_add_rms_norm_run, params)
+
+
+def add_rms_norm_quant(session: OpSession, params) -> None:
+    """roost_amd_add_rms_norm_quant_run on the session's stream."""
+    _extension(session, "add_rms_norm_quant", session.lib.dll.roost_amd_add_rms_norm_quant_run, params)
+
+
+def silu_mul_quant(session: OpSession, params) -> None:
+    """roost_amd_silu_mul_quant_run on the session's stream."""
+    _extension(session, "silu_mul_quant", session.lib.dll.roost_amd_silu_mul_quant_run, params)
+
+
+def gemm_lora_workspace(session: OpSession, params, key=0) -> abi.Workspace:
+    """A workspace that roost_amd_gemm_lora_run of these params takes, kept by the session under `key` (grown when it
+    does not fit). Calls on one stream may share it; calls that overlap on the GPU may not."""
+    sizes = abi.new(abi.WorkspaceSizes)
+    status = session.lib.dll.roost_amd_gemm_lora_workspace(session.ctx, C.addressof(params), C.addressof(sizes))
+    if status != abi.OK:
+        raise KernelError("gemm_lora workspace", status, session.lib.last_error())
+    return session.workspace_of(("gemm_lora", key), sizes)[3]
+
+
+def gemm_lora(session: OpSession, params, ws: Optional[abi.Workspace] = None, key=0) -> None:
+    """roost_amd_gemm_lora_run on the session's stream, in `ws` or the session's workspace under `key`."""
+    if ws is None:
+        ws = gemm_lora_workspace(session, params, key)
+    _extension(session, "gemm_lora", session.lib.dll.roost_amd_gemm_lora_run, params, C.addressof(ws))
 
 
 def gated_rms_norm(session: OpSession, *args, **kwargs) -> None:

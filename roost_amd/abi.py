@@ -19,7 +19,7 @@ STATUS_NAMES = ["OK", "INVALID_ARGUMENT", "UNSUPPORTED", "CUDA_ERROR", "INTERNAL
 
 # Element types
 DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_F64 = 1, 2, 3, 4
-DTYPE_U8, DTYPE_I32, DTYPE_I64 = 8, 10, 12
+DTYPE_F8E4M3, DTYPE_U8, DTYPE_I32, DTYPE_I64 = 5, 8, 10, 12
 
 # Layouts
 LAYOUT_ROW_MAJOR, LAYOUT_PAGED_NHD, LAYOUT_PAGED_HND = 0, 2, 3
@@ -149,6 +149,37 @@ class QkvQkNormRopeCacheWriteParams(C.Structure):
                 ("page_size", C.c_uint32), ("eps", C.c_float), ("theta", C.c_float), ("reserved0", C.c_uint32)]
 
 
+class AddRmsNormParams(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32), ("input", DeviceSpan), ("residual", DeviceSpan),
+                ("weight", DeviceSpan), ("residual_out", DeviceSpan), ("output", DeviceSpan), ("rows", C.c_uint32),
+                ("dim", C.c_uint32), ("input_stride", C.c_uint32), ("residual_stride", C.c_uint32),
+                ("residual_out_stride", C.c_uint32), ("output_stride", C.c_uint32), ("eps", C.c_float),
+                ("reserved0", C.c_uint32)]
+
+
+class AddRmsNormQuantParams(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32), ("input", DeviceSpan), ("residual", DeviceSpan),
+                ("weight", DeviceSpan), ("residual_out", DeviceSpan), ("output", DeviceSpan), ("scales", DeviceSpan),
+                ("rows", C.c_uint32), ("dim", C.c_uint32), ("input_stride", C.c_uint32), ("residual_stride", C.c_uint32),
+                ("residual_out_stride", C.c_uint32), ("output_stride", C.c_uint32), ("eps", C.c_float),
+                ("group_size", C.c_uint32)]
+
+
+class SiluMulQuantParams(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32), ("gate", DeviceSpan), ("up", DeviceSpan),
+                ("output", DeviceSpan), ("scales", DeviceSpan), ("rows", C.c_uint32), ("dim", C.c_uint32),
+                ("gate_stride", C.c_uint32), ("up_stride", C.c_uint32), ("output_stride", C.c_uint32),
+                ("group_size", C.c_uint32)]
+
+
+class GemmLoraParams(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32)] + [
+        (name, DeviceSpan) for name in ("x", "x_scale", "weight", "w_scale", "lora_a", "lora_b", "lora_scale", "ranks",
+                                        "lora_slots", "cu_seqlens", "addend", "output")] + [
+        (name, C.c_uint32) for name in ("tokens", "batch", "in_dim", "out_dim", "adapters", "max_rank", "x_stride",
+                                        "addend_stride", "output_stride", "reserved0")]
+
+
 class SigmoidMulParams(C.Structure):
     _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32), ("input", DeviceSpan), ("gate", DeviceSpan),
                 ("output", DeviceSpan), ("rows", C.c_uint32), ("dim", C.c_uint32)]
@@ -238,7 +269,10 @@ ALL_STRUCTS = {
 }
 
 # Records of this library with no counterpart in the reference's C header (so not in its layout fixture).
-EXTENSION_STRUCTS = {"RoostQkvQkNormRopeCacheWriteParams": QkvQkNormRopeCacheWriteParams}
+EXTENSION_STRUCTS = {"RoostQkvQkNormRopeCacheWriteParams": QkvQkNormRopeCacheWriteParams,
+                     "RoostAmdAddRmsNormParams": AddRmsNormParams,
+                     "RoostAmdAddRmsNormQuantParams": AddRmsNormQuantParams,
+                     "RoostAmdSiluMulQuantParams": SiluMulQuantParams, "RoostAmdGemmLoraParams": GemmLoraParams}
 
 
 def new(struct_type):

@@ -19,6 +19,22 @@ struct RoostContext {
   uint32_t compute_units;
 };
 
+namespace roost {
+
+// A launch goes to the current device: refused where that is not the context's (no check without a visible device).
+inline Gate& OnDevice(Gate& gate, const RoostContext* ctx) {
+  int device = 0;
+  if (!gate.ok()) return gate;
+  if (hipGetDevice(&device) != hipSuccess) {
+    (void)hipGetLastError();
+    return gate;
+  }
+  return gate.Expect(device == ctx->device, ROOST_STATUS_INVALID_ARGUMENT,
+                     "the context belongs to device %d, device %d is current", ctx->device, device);
+}
+
+}  // namespace roost
+
 // ---- Device-side helpers -------------------------------------------------------------------------------------------
 
 namespace roost_dev {

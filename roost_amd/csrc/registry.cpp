@@ -53,6 +53,18 @@ static_assert(sizeof(RoostQkvQkNormRopeCacheWriteParams) == 232 &&
                   offsetof(RoostQkvQkNormRopeCacheWriteParams, tokens) == 200 &&
                   offsetof(RoostQkvQkNormRopeCacheWriteParams, theta) == 224,
               "RoostQkvQkNormRopeCacheWriteParams layout");
+static_assert(sizeof(RoostAmdAddRmsNormParams) == 160 && offsetof(RoostAmdAddRmsNormParams, rows) == 128 &&
+                  offsetof(RoostAmdAddRmsNormParams, eps) == 152,
+              "RoostAmdAddRmsNormParams layout");
+static_assert(sizeof(RoostAmdAddRmsNormQuantParams) == 184 && offsetof(RoostAmdAddRmsNormQuantParams, rows) == 152 &&
+                  offsetof(RoostAmdAddRmsNormQuantParams, group_size) == 180,
+              "RoostAmdAddRmsNormQuantParams layout");
+static_assert(sizeof(RoostAmdSiluMulQuantParams) == 128 && offsetof(RoostAmdSiluMulQuantParams, rows) == 104 &&
+                  offsetof(RoostAmdSiluMulQuantParams, group_size) == 124,
+              "RoostAmdSiluMulQuantParams layout");
+static_assert(sizeof(RoostAmdGemmLoraParams) == 336 && offsetof(RoostAmdGemmLoraParams, output) == 272 &&
+                  offsetof(RoostAmdGemmLoraParams, tokens) == 296 && offsetof(RoostAmdGemmLoraParams, reserved0) == 332,
+              "RoostAmdGemmLoraParams layout");
 static_assert(sizeof(RoostRecurrentStateCopyParams) == 72 && offsetof(RoostRecurrentStateCopyParams, slot_bytes) == 56,
               "RoostRecurrentStateCopyParams layout");
 static_assert(sizeof(RoostRecurrentStateSnapshotParams) == 96 &&

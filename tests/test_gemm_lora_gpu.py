@@ -1,0 +1,199 @@
+"""GemmLora on the GPU through the C ABI, against its definition in 64 bits; the bounds are derived in fused_cases.py."""
+import pytest
+import torch
+
+import roost_amd
+from fused_cases import BF16, F32, F8, Lora
+
+pytestmark = pytest.mark.gpu
+
+
+def _run(session, c, key=0, **kw):
+    roost_amd.gemm_lora(session, c.params(**kw), key=key)
+    torch.cuda.synchronize()
+
+
+CASES = {
+    "one token": dict(lens=[1], slots=[2], in_dim=1024, out_dim=6144),
+    "one token, one output": dict(lens=[1], slots=[0], in_dim=16, out_dim=1, adapters=1, max_rank=8),
+    "one token, no adapter": dict(lens=[1], slots=[-1], in_dim=256, out_dim=100),
+    "no adapters at all": dict(lens=[5, 9], slots=[0, 0], in_dim=264, out_dim=77, adapters=0, max_rank=0),
+    "ragged": dict(lens=[5, 0, 33, 1, 0, 18], slots=[1, 0, 3, -1, 2, 1], in_dim=520, out_dim=613, ranks=[16, 3, 0, 9]),
+    "decode": dict(lens=[1] * 61, slots=[(7 * i) % 25 - 1 for i in range(61)], in_dim=1024, out_dim=640, adapters=24,
+                   max_rank=32, ranks=[1 + (5 * i) % 32 for i in range(24)], pad=3),
+    "decode, 300 rows": dict(lens=[1] * 300, slots=[i % 5 - 1 for i in range(300)], in_dim=256, out_dim=200),
+    "one adapter for all": dict(lens=[1] * 70, slots=[1] * 70, in_dim=512, out_dim=96),
+    "slots outside the pool": dict(lens=[3, 3, 3], slots=[99, -7, 2], in_dim=128, out_dim=64),
+    "mixed step": dict(lens=[1] * 48 + [200, 131], slots=[i % 4 for i in range(50)], in_dim=2048, out_dim=1024, addend=BF16),
+    "prompt": dict(lens=[777], slots=[3], in_dim=1024, out_dim=1027, max_rank=64, ranks=[64, 64, 64, 57]),
+    "prompts": dict(lens=[500, 3, 421], slots=[0, 1, 2], in_dim=1088, out_dim=515, max_rank=128, out=F32),
+    "f32": dict(lens=[1, 40, 7], slots=[1, 0, -1], in_dim=516, out_dim=333, x=F32, out=F32, ranks=[16, 5, 2, 1]),
+    "f32, many rows": dict(lens=[150, 170], slots=[1, 0], in_dim=260, out_dim=300, x=F32, out=F32, addend=F32),
+    "8 bits, one token": dict(lens=[1], slots=[1], in_dim=1024, out_dim=800, x=F8),
+    "8 bits": dict(lens=[30, 1, 1, 60], slots=[1, -1, 2, 0], in_dim=528, out_dim=275, x=F8, ranks=[16, 4, 1, 0], pad=5),
+    "8 bits, prompts": dict(lens=[300, 290], slots=[1, 2], in_dim=1040, out_dim=520, x=F8, addend=BF16),
+    "adapters alone": dict(lens=[1, 90, 17], slots=[1, -1, 0], in_dim=640, out_dim=321, shared=False, addend=BF16, pad=2),
+    "adapters alone, no addend": dict(lens=[4, 60], slots=[1, -1], in_dim=640, out_dim=88, shared=False),
+    "adapters alone, 8 bits": dict(lens=[200, 55], slots=[3, 1], in_dim=640, out_dim=328, shared=False, addend=BF16, x=F8),
+    "strided rows": dict(lens=[20, 21], slots=[0, 3], in_dim=384, out_dim=101, x_gap=40, y_gap=3, addend=BF16),
+    "strided prompts": dict(lens=[280, 41], slots=[0, 3], in_dim=384, out_dim=258, x_gap=40, y_gap=6, addend=F32),
+    "f32 addend, f32 output": dict(lens=[9, 200], slots=[0, 3], in_dim=384, out_dim=128, addend=F32, out=F32),
+}
+
+
+@pytest.mark.parametrize("name", CASES)
+def test_gemm_lora(session, name):
+    c = Lora(len(name), **CASES[name])
+    _run(session, c)
+    c.check(name)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 400])
+@pytest.mark.parametrize("x", [BF16, F8])
+def test_numbers_of_rows(session, tokens, x):
+    """Around every tile and wavefront border, in sequences of 1 to 40 rows."""
+    lens, left = [], tokens
+    while left:
+        lens.append(min(left, 1 + (7 * len(lens)) % 40))
+        left -= lens[-1]
+    c = Lora(tokens, lens, [i % 6 - 1 for i in range(len(lens))], in_dim=272, out_dim=136, adapters=5, x=x, pad=1)
+    _run(session, c)
+    c.check(f"{tokens} rows")
+
+
+@pytest.mark.parametrize("out_dim", [1, 3, 4, 15, 16, 17, 63, 64, 65, 127, 129, 255, 257])
+@pytest.mark.parametrize("lens", [[3, 4], [150, 130]])
+def test_numbers_of_outputs(session, out_dim, lens):
+    c = Lora(out_dim, lens, [0, 1], in_dim=200, out_dim=out_dim)
+    _run(session, c)
+    c.check(f"{out_dim} outputs")
+
+
+@pytest.mark.parametrize("in_dim", [8, 24, 56, 64, 72, 120, 136, 1000])
+@pytest.mark.parametrize("lens", [[3, 4], [150, 130]])
+def test_inner_lengths(session, in_dim, lens):
+    c = Lora(in_dim, lens, [0, 1], in_dim=in_dim, out_dim=70)
+    _run(session, c)
+    c.check(f"inner length {in_dim}")
+
+
+@pytest.mark.parametrize("max_rank", [8, 24, 40, 64, 72, 120, 128])
+@pytest.mark.parametrize("lens", [[3, 1, 4], [150, 31, 130]])
+def test_ranks(session, max_rank, lens):
+    c = Lora(max_rank, lens, [0, 1, 2], in_dim=192, out_dim=80, adapters=3, max_rank=max_rank,
+             ranks=[max_rank, max_rank - 7, max_rank // 2 + 1])
+    _run(session, c)
+    c.check(f"pool rank {max_rank}")
+
+
+@pytest.mark.parametrize("lens", [[1] * 20, [150, 31, 130]])
+def test_one_adapter_never_reaches_another_sequence(session, lens):
+    """A broken adapter (NaN, infinities) leaves every other sequence's rows as they are without it, bit for bit; so does
+    what the pool holds past an adapter's rank."""
+    slots = [i % 3 for i in range(len(lens))]
+    c = Lora(5, lens, slots, in_dim=256, out_dim=144, adapters=3, ranks=[16, 11, 5])
+    _run(session, c)
+    clean = c.y.clone()
+    for pool, at in ((c.lora_a, (1, slice(None))), (c.lora_b, (1, slice(None)))):
+        kept = pool.clone()
+        pool[at] = float("nan")
+        pool[1, :3] = float("inf")
+        _run(session, c)
+        row = 0
+        for n, s in zip(lens, slots):
+            mine = c.y[row:row + n]
+            assert torch.isnan(mine).all() if s == 1 else torch.equal(mine, clean[row:row + n])
+            row += n
+        pool.copy_(kept)
+    c.lora_a[1, 11:] = float("nan")
+    c.lora_a[2, 5:] = float("inf")
+    c.lora_b[1, :, 11:] = float("nan")
+    c.lora_b[2, :, 5:] = float("inf")
+    _run(session, c)
+    assert torch.equal(c.y, clean)
+
+
+@pytest.mark.parametrize("lens", [[4] * 10, [130, 128]])
+def test_rows_of_no_sequence_may_hold_anything(session, lens):
+    c = Lora(6, lens, [i % 3 for i in range(len(lens))], in_dim=256, out_dim=144, adapters=3, pad=9)
+    c.x[sum(lens):] = float("nan")
+    _run(session, c)
+    c.check("NaN behind the last sequence")
+
+
+@pytest.mark.parametrize("lens,x", [([1] * 9, BF16), ([300], BF16), ([7, 3], F32), ([200, 90], F8)])
+def test_in_place_addend(session, lens, x):
+    out = F32 if x == F32 else BF16
+    c = Lora(7, lens, [i % 3 for i in range(len(lens))], in_dim=256, out_dim=144, adapters=3, x=x, out=out, addend=out)
+    _run(session, c)
+    want = c.y.clone()
+    c.y = c.addend
+    _run(session, c)
+    assert torch.equal(c.y, want)
+
+
+@pytest.mark.parametrize("lens", [[1] * 40, [260, 300]])
+def test_same_bits_every_time(session, lens):
+    c = Lora(8, lens, [i % 3 for i in range(len(lens))], in_dim=2048, out_dim=272, adapters=3)
+    _run(session, c)
+    first = c.y.clone()
+    for _ in range(3):
+        c.y.copy_(c.before)
+        _run(session, c)
+        assert torch.equal(c.y, first)
+
+
+def test_two_sessions_at_once(session):
+    """Calls on two streams with a workspace each."""
+    cases = [Lora(20 + i, [70, 1, 30], [0, 1, 2], in_dim=1024, out_dim=520) for i in range(2)]
+    sessions = [roost_amd.OpSession(session.lib, device=0, stream=torch.cuda.Stream()) for _ in range(2)]
+    params = [c.params() for c in cases]
+    spaces = [roost_amd.gemm_lora_workspace(s, p) for s, p in zip(sessions, params)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, p, w in zip(sessions, params, spaces):
+            roost_amd.gemm_lora(s, p, w)
+    torch.cuda.synchronize()
+    for i, c in enumerate(cases):
+        c.check(f"stream {i}")
+    for s in sessions:
+        s.close()
+
+
+@pytest.mark.parametrize("lens", [[1] * 30, [200, 140]])
+def test_graph_replays(session, lens):
+    """Captured once, replayed with other rows, lengths and adapters in the same buffers and eager calls in between."""
+    c = Lora(30, lens, [i % 4 for i in range(len(lens))], in_dim=512, out_dim=260, pad=4)
+    stream = torch.cuda.Stream()
+    s = roost_amd.OpSession(session.lib, device=0, stream=stream)
+    p = c.params()
+    ws = roost_amd.gemm_lora_workspace(s, p)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        roost_amd.gemm_lora(s, p, ws)
+    for k in range(4):
+        other = Lora(40 + k, lens, [(i + k) % 5 - 1 for i in range(len(lens))], in_dim=512, out_dim=260, pad=4)
+        if k == 2:  # a shorter last sequence, more rows behind it
+            other.lens = lens[:-1] + [max(lens[-1] - 1, 0)]
+            other.cu[-1] -= 1
+        for name in ("x", "cu", "slots_d", "y"):
+            getattr(c, name).copy_(getattr(other, name))
+        c.lens, c.slots, c.before = other.lens, other.slots, c.y.clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(f"replay {k}")
+        got = c.y.clone()
+        c.y.copy_(c.before)
+        _run(session, c)
+        assert torch.equal(got, c.y)
+    s.close()
+
+
+def test_large_offsets(session):
+    """A weight and a pool whose elements pass 2^31 bytes."""
+    c = Lora(50, [2, 17], [130, 3], in_dim=16384, out_dim=70000, adapters=131, max_rank=8)
+    assert c.weight.numel() * 2 > 1 << 31
+    _run(session, c)
+    c.check("long offsets")
