@@ -27,10 +27,20 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
 struct E4m3 {
   uint8_t bits;
 };
+// The same rows multiplied as bf16 (an exact conversion, in registers). The e4m3 matrix instructions keep fewer bits of their
+// inner sums: over 4,096 products of random codes they are 5e-5 of the result off, bf16's 4e-7. That is far below a bf16
+// output's rounding (2e-3) and far above an f32 output's, which therefore takes this form.
+struct E4m3AsBf16 {
+  uint8_t bits;
+};
+template <typename E>
+constexpr bool kIsE4m3 = std::is_same_v<E, E4m3> || std::is_same_v<E, E4m3AsBf16>;
 
 // The adapters' type beside rows of type E.
 template <typename E>
@@ -83,6 +93,20 @@ __device__ __forceinline__ uint32_t RankOf(const LoraArgs& g, int32_t slot) {
 
 // ---- Fragments -------------------------------------------------------------------------------------------------------
 
+// Eight e4m3 elements as eight bf16 (exact: e4m3 has three mantissa bits and a smaller exponent range).
+__device__ __forceinline__ bf16x8_t Bf16OfE4m3(uint32_t q0, uint32_t q1) {
+  u32x4_t v;
+  const uint32_t q[2] = {q0, q1};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(q[i]), false);
+    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(q[i]), true);
+    v[2 * i] = PackBf16Rne(lo[0], lo[1]);
+    v[2 * i + 1] = PackBf16Rne(hi[0], hi[1]);
+  }
+  return __builtin_bit_cast(bf16x8_t, v);
+}
+
 // acc += (16 rows) x (16 rows)^T over the 64 bytes that one piece a lane covers.
 template <typename E>
 __device__ __forceinline__ f32x4_t Mma16(u32x4_t a, u32x4_t b, f32x4_t acc) {
@@ -95,7 +119,7 @@ __device__ __forceinline__ f32x4_t Mma16(u32x4_t a, u32x4_t b, f32x4_t acc) {
       acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), acc, 0, 0, 0);
     }
     return acc;
-  } else {
+  } else if constexpr (std::is_same_v<E, E4m3>) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const u32x2_t pa = {a[2 * i], a[2 * i + 1]}, pb = {b[2 * i], b[2 * i + 1]};
@@ -103,172 +127,579 @@ __device__ __forceinline__ f32x4_t Mma16(u32x4_t a, u32x4_t b, f32x4_t acc) {
                                                        0);
     }
     return acc;
-  }
-}
-
-// The piece at byte `at` of a row of `bytes` bytes, zero past its end.
-__device__ __forceinline__ u32x4_t Piece(const void* row, uint32_t at, uint32_t bytes) {
-  u32x4_t v = {0, 0, 0, 0};
-  if (at < bytes) v = *reinterpret_cast<const u32x4_t*>(static_cast<const unsigned char*>(row) + at);
-  return v;
-}
-
-// Eight e4m3 elements as eight bf16 (exact: e4m3 has three mantissa bits and a smaller exponent range).
-__device__ __forceinline__ u32x4_t Bf16OfE4m3(u32x2_t q) {
-  u32x4_t v;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(q[i]), false);
-    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(q[i]), true);
-    v[2 * i] = PackBf16Rne(lo[0], lo[1]);
-    v[2 * i + 1] = PackBf16Rne(hi[0], hi[1]);
+    for (int i = 0; i < 2; ++i) {
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Bf16OfE4m3(a[2 * i], a[2 * i + 1]), Bf16OfE4m3(b[2 * i], b[2 * i + 1]),
+                                                    acc, 0, 0, 0);
+    }
+    return acc;
   }
-  return v;
+}
+
+// acc += (32 rows) x (32 rows)^T over the 64 bytes that two pieces a lane cover: lane l holds row l % 32, its pieces are two
+// of the four of those bytes (lanes 0 to 31 the first and third, the others the second and fourth).
+template <typename E>
+__device__ __forceinline__ f32x16_t Mma32(const u32x4_t (&a)[2], const u32x4_t (&b)[2], f32x16_t acc) {
+  if constexpr (std::is_same_v<E, E4m3>) {
+    const i32x8_t pa = {(int)a[0][0], (int)a[0][1], (int)a[0][2], (int)a[0][3], (int)a[1][0], (int)a[1][1], (int)a[1][2], (int)a[1][3]};
+    const i32x8_t pb = {(int)b[0][0], (int)b[0][1], (int)b[0][2], (int)b[0][3], (int)b[1][0], (int)b[1][1], (int)b[1][2], (int)b[1][3]};
+    // Block scales of 2^0 (biased exponent 127).
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pa, pb, acc, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if constexpr (std::is_same_v<E, uint16_t>) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[q]), __builtin_bit_cast(bf16x8_t, b[q]),
+                                                      acc, 0, 0, 0);
+      } else if constexpr (std::is_same_v<E, float>) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[q][i]), __uint_as_float(b[q][i]), acc, 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Bf16OfE4m3(a[q][2 * i], a[q][2 * i + 1]),
+                                                        Bf16OfE4m3(b[q][2 * i], b[q][2 * i + 1]), acc, 0, 0, 0);
+        }
+      }
+    }
+    return acc;
+  }
+}
+
+// The piece at byte `at` of a row; with kTail, zero past the row's `bytes` bytes (the load itself then repeats the first).
+template <bool kTail>
+__device__ __forceinline__ u32x4_t Piece(const void* row, uint32_t at, uint32_t bytes) {
+  const bool inside = !kTail || at < bytes;
+  const u32x4_t v = *reinterpret_cast<const u32x4_t*>(static_cast<const unsigned char*>(row) + (inside ? at : 0));
+  return inside ? v : u32x4_t{0, 0, 0, 0};
 }
 
 // ---- The low-rank rows -------------------------------------------------------------------------------------------------
 
-// Workgroup (i, j, z): rows 16 i .. + 15, ranks 16 j .. + 15, every gridDim.z-th run of rows with one adapter among them.
-// Four wavefronts take alternate 64-byte runs of the inner dimension and join their sums through LDS.
-template <typename E>
-__global__ void __launch_bounds__(256) ShrinkKernel(LoraArgs g) {
+// Workgroup (i, j, z): rows 16 kT i .. + 16 kT - 1, ranks 16 kR j .. + 16 kR - 1, every gridDim.z-th run of rows with one
+// adapter among them. The wavefronts take alternate 64-byte runs of the adapter's rows and join their sums through LDS.
+template <typename E, int kT, int kR>
+__global__ void __launch_bounds__(512) ShrinkKernel(LoraArgs g) {
   using Low = LowOf<E>;
-  __shared__ int32_t slot[16];
-  __shared__ f32x4_t part[3][64];
-  const uint32_t t0 = 16 * blockIdx.x, r0 = 16 * blockIdx.y;
+  constexpr int kWaves = 8, kRows = 16 * kT;
+  constexpr uint32_t kXBytes = kIsE4m3<E> ? 8 : 16;  // of a row of x beside 16 of the adapter's
+  __shared__ int32_t slot[kRows];
+  __shared__ f32x4_t part[kWaves][kT * kR][64];
+  const uint32_t t0 = kRows * blockIdx.x, r0 = 16 * kR * blockIdx.y;
   const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  FillSlots(g, t0, 16, slot);
+  FillSlots(g, t0, kRows, slot);
   __syncthreads();
-  const uint32_t low_bytes = g.in_dim * sizeof(Low);
-  const uint32_t t = min(t0 + lane % 16, g.tokens - 1);
-  const E* x = static_cast<const E*>(g.x) + t * g.x_stride;
+  const uint32_t bytes = g.in_dim * sizeof(Low);
+  const unsigned char* x[kT];
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
+    x[t] = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.x) + min(t0 + 16 * t + lane % 16, g.tokens - 1) * g.x_stride);
+  }
   uint32_t run = 0;
-  for (uint32_t i = 0, next; i < 16; i = next) {
+  for (uint32_t i = 0, next; i < kRows; i = next) {
     const int32_t s = slot[i];
-    for (next = i + 1; next < 16 && slot[next] == s; ++next) {}
+    for (next = i + 1; next < kRows && slot[next] == s; ++next) {}
     const uint32_t rank = RankOf(g, s);
     if (r0 >= rank || run++ % gridDim.z != blockIdx.z) continue;
-    const Low* a = static_cast<const Low*>(g.a) +
-                   (static_cast<uint64_t>(s) * g.max_rank + min(r0 + lane % 16, rank - 1)) * g.in_dim;
-    f32x4_t acc = {0, 0, 0, 0};
-    for (uint32_t base = 64 * wave; base < low_bytes; base += 256) {
-      const uint32_t at = base + 16 * (lane / 16);
-      const u32x4_t pa = Piece(a, at, low_bytes);
-      u32x4_t px;
-      if constexpr (std::is_same_v<E, E4m3>) {
-        u32x2_t q = {0, 0};
-        if (at < low_bytes) q = *reinterpret_cast<const u32x2_t*>(reinterpret_cast<const unsigned char*>(x) + at / 2);
-        px = Bf16OfE4m3(q);
-      } else {
-        px = Piece(x, at, low_bytes);
-      }
-      acc = Mma16<Low>(pa, px, acc);
+    const unsigned char* a[kR];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {  // ranks past the adapter's repeat its last; what they give is not stored
+      a[r] = reinterpret_cast<const unsigned char*>(
+          static_cast<const Low*>(g.a) + (static_cast<uint64_t>(s) * g.max_rank + min(r0 + 16 * r + lane % 16, rank - 1)) * g.in_dim);
     }
-    if (wave > 0) part[wave - 1][lane] = acc;
-    __syncthreads();
-    if (wave == 0) {
+    f32x4_t acc[kT][kR];
 #pragma unroll
-      for (int w = 0; w < 3; ++w) acc += part[w][lane];
-      const uint32_t row = lane % 16;
-      float scale = g.lora_scale != nullptr ? g.lora_scale[s] : 1.0f;
-      if (row >= i && row < next) {
-        if (g.x_scale != nullptr) scale *= g.x_scale[t0 + row];
+    for (int t = 0; t < kT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t r = r0 + 4 * (lane / 16) + e;
-          if (r < rank) g.u[static_cast<uint64_t>(t0 + row) * g.max_rank + r] = acc[e] * scale;
+      for (int r = 0; r < kR; ++r) acc[t][r] = f32x4_t{0, 0, 0, 0};
+    }
+    const auto step = [&](uint32_t base, auto tail) {
+      constexpr bool kTail = decltype(tail)::value;
+      const uint32_t at = base + 16 * (lane / 16);
+      u32x4_t pa[kR], px[kT];
+#pragma unroll
+      for (int r = 0; r < kR; ++r) pa[r] = Piece<kTail>(a[r], at, bytes);
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        if constexpr (kIsE4m3<E>) {
+          const bool inside = !kTail || at < bytes;
+          const u32x2_t q = *reinterpret_cast<const u32x2_t*>(x[t] + (inside ? at / 16 * kXBytes : 0));
+          px[t] = inside ? __builtin_bit_cast(u32x4_t, Bf16OfE4m3(q[0], q[1])) : u32x4_t{0, 0, 0, 0};
+        } else {
+          px[t] = Piece<kTail>(x[t], at, bytes);
         }
       }
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+#pragma unroll
+        for (int r = 0; r < kR; ++r) acc[t][r] = Mma16<Low>(pa[r], px[t], acc[t][r]);
+      }
+    };
+    const uint32_t full = bytes / 64 * 64;
+    uint32_t base = 64 * wave;
+#pragma unroll 4
+    for (; base < full; base += 64 * kWaves) step(base, std::false_type{});
+    if (base < bytes) step(base, std::true_type{});
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) part[wave][t * kR + r][lane] = acc[t][r];
+    }
+    __syncthreads();
+    for (uint32_t item = threadIdx.x; item < kT * kR * 64; item += 64 * kWaves) {
+      const uint32_t tile = item / 64, l = item % 64;
+      const uint32_t row = 16 * (tile / kR) + l % 16, first = r0 + 16 * (tile % kR) + 4 * (l / 16);
+      if (row < i || row >= next || first >= rank) continue;
+      f32x4_t v = part[0][tile][l];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) v += part[w][tile][l];
+      float scale = g.lora_scale != nullptr ? g.lora_scale[s] : 1.0f;
+      if constexpr (kIsE4m3<E>) scale *= g.x_scale[t0 + row];
+      // max_rank is a multiple of 8: the four are the row's own, those past the adapter's rank unused.
+      *reinterpret_cast<f32x4_t*>(g.u + static_cast<uint64_t>(t0 + row) * g.max_rank + first) = v * scale;
     }
     __syncthreads();
   }
+}
+
+// ---- After the product -----------------------------------------------------------------------------------------------------
+
+// Words of a 16-byte piece whose elements from `left` on are zeroed (left may be anything; 0 or less zeroes all).
+template <typename Low>
+__device__ __forceinline__ u32x4_t First(u32x4_t v, int32_t left) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(Low) == 4) {
+      if (i >= left) v[i] = 0;
+    } else {
+      v[i] = 2 * i + 1 < left ? v[i] : 2 * i < left ? v[i] & 0xFFFFu : 0;
+    }
+  }
+  return v;
+}
+template <typename Low>
+__device__ __forceinline__ float Element(u32x4_t v, int i) {
+  if constexpr (sizeof(Low) == 4) {
+    return __uint_as_float(v[i]);
+  } else {
+    return i % 2 ? Bf16HiToF32(v[i / 2]) : Bf16LoToF32(v[i / 2]);
+  }
+}
+
+// v += B_slot[n .. n + 3, :rank] u_t, element by element; outputs past the last repeat it.
+template <typename Low>
+__device__ __forceinline__ void AddLowRank(const LoraArgs& g, uint32_t t, uint32_t n, int32_t slot, uint32_t rank, f32x4_t& v) {
+  constexpr int kPer = 16 / sizeof(Low);
+  const float* u = g.u + static_cast<uint64_t>(t) * g.max_rank;
+  const Low* b = static_cast<const Low*>(g.b) + static_cast<uint64_t>(slot) * g.out_dim * g.max_rank;
+  const Low* row[4];
+#pragma unroll
+  for (uint32_t e = 0; e < 4; ++e) row[e] = b + static_cast<uint64_t>(min(n + e, g.out_dim - 1)) * g.max_rank;
+  for (uint32_t r = 0; r < rank; r += kPer) {
+    const auto left = static_cast<int32_t>(rank - r);
+    float ur[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer / 4; ++i) {
+      const f32x4_t q = *reinterpret_cast<const f32x4_t*>(u + r + 4 * i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ur[4 * i + j] = 4 * i + j < left ? q[j] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const u32x4_t q = First<Low>(*reinterpret_cast<const u32x4_t*>(row[e] + r), left);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[e] = fmaf(ur[i], Element<Low>(q, i), v[e]);
+    }
+  }
+}
+
+// Four consecutive elements of a row at `at`, which may be aligned to an element only.
+typedef uint32_t Bf16x4 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float F32x4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Adds the addend and stores outputs n .. n + 3 of row t.
+__device__ __forceinline__ void Store(const LoraArgs& g, uint32_t t, uint32_t n, f32x4_t v) {
+  const uint64_t at = t * g.y_stride + n, from = t * g.addend_stride + n;
+  if (g.out_dim - n >= 4) {
+    if (g.addend != nullptr) {
+      if (g.addend_f32) {
+        v += *reinterpret_cast<const F32x4*>(static_cast<const float*>(g.addend) + from);
+      } else {
+        const Bf16x4 q = *reinterpret_cast<const Bf16x4*>(static_cast<const uint16_t*>(g.addend) + from);
+        v += f32x4_t{Bf16LoToF32(q[0]), Bf16HiToF32(q[0]), Bf16LoToF32(q[1]), Bf16HiToF32(q[1])};
+      }
+    }
+    if (g.y_f32) {
+      *reinterpret_cast<F32x4*>(static_cast<float*>(g.y) + at) = v;
+    } else {
+      *reinterpret_cast<Bf16x4*>(static_cast<uint16_t*>(g.y) + at) = Bf16x4{PackBf16Rne(v[0], v[1]), PackBf16Rne(v[2], v[3])};
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < 3; ++e) {
+    if (e < g.out_dim - n) {
+      float one = v[e];
+      if (g.addend != nullptr) {
+        one += LoadF(g.addend, g.addend_f32 ? ROOST_DTYPE_F32 : ROOST_DTYPE_BF16, static_cast<int64_t>(from + e));
+      }
+      if (g.y_f32) {
+        static_cast<float*>(g.y)[at + e] = one;
+      } else {
+        static_cast<uint16_t*>(g.y)[at + e] = static_cast<uint16_t>(PackBf16Rne(one, 0.0f));
+      }
+    }
+  }
+}
+
+// The scales of e4m3 rows and weights, on outputs n .. n + 3 of row t.
+__device__ __forceinline__ f32x4_t Rescaled(const LoraArgs& g, float x_scale, uint32_t n, f32x4_t v) {
+#pragma unroll
+  for (uint32_t e = 0; e < 4; ++e) v[e] *= x_scale * g.w_scale[min(n + e, g.out_dim - 1)];
+  return v;
 }
 
 // ---- The product, straight from memory -----------------------------------------------------------------------------------
 
-// Adds the adapter, the addend and stores four consecutive outputs of one row.
-template <typename E>
-__device__ __forceinline__ void Finish(const LoraArgs& g, uint32_t t, uint32_t n, int32_t slot, f32x4_t v) {
-  using Low = LowOf<E>;
-  const uint32_t left = g.out_dim - n;  // outputs from n on
-  if constexpr (std::is_same_v<E, E4m3>) {
-    const float xs = g.x_scale[t];
+// Workgroup (i, j): outputs 16 kN i .. + 16 kN - 1 of rows 16 kT j .. + 16 kT - 1. The wavefronts take alternate 256-byte runs
+// of the inner dimension and join their sums through LDS.
+template <typename E, int kN, int kT>
+__global__ void __launch_bounds__(512) ProductKernel(LoraArgs g) {
+  constexpr int kWaves = 8, kPieces = 4;
+  __shared__ int32_t slot[16 * kT];
+  __shared__ f32x4_t part[kWaves][kN * kT][64];
+  const uint32_t n0 = 16 * kN * blockIdx.x, t0 = 16 * kT * blockIdx.y;
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  FillSlots(g, t0, 16 * kT, slot);
+  const uint32_t bytes = g.in_dim * sizeof(E);
+  f32x4_t acc[kN][kT];
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-      if (g.w != nullptr && e < left) v[e] *= xs * g.w_scale[n + e];
-    }
+  for (int n = 0; n < kN; ++n) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) acc[n][t] = f32x4_t{0, 0, 0, 0};
   }
-  const uint32_t rank = RankOf(g, slot);
-  const float* u = g.u + static_cast<uint64_t>(t) * g.max_rank;
-  for (uint32_t r = 0; r < rank; ++r) {
-    const float ur = u[r];
+  if (g.w != nullptr) {
+    const E* w[kN];
+    const E* x[kT];
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-      if (e < left) {
-        const uint64_t at = (static_cast<uint64_t>(slot) * g.out_dim + n + e) * g.max_rank + r;
-        float b;
-        if constexpr (sizeof(Low) == 2) {
-          b = Bf16ToF32(static_cast<const uint16_t*>(g.b)[at]);
-        } else {
-          b = static_cast<const float*>(g.b)[at];
+    for (int n = 0; n < kN; ++n) {
+      w[n] = static_cast<const E*>(g.w) + static_cast<uint64_t>(min(n0 + 16 * n + lane % 16, g.out_dim - 1)) * g.in_dim;
+    }
+#pragma unroll
+    for (int t = 0; t < kT; ++t) x[t] = static_cast<const E*>(g.x) + min(t0 + 16 * t + lane % 16, g.tokens - 1) * g.x_stride;
+    const auto step = [&](uint32_t base, auto tail) {
+      constexpr bool kTail = decltype(tail)::value;
+      u32x4_t pw[kN][kPieces], px[kT][kPieces];
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const uint32_t at = base + 64 * p + 16 * (lane / 16);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) pw[n][p] = Piece<kTail>(w[n], at, bytes);
+#pragma unroll
+        for (int t = 0; t < kT; ++t) px[t][p] = Piece<kTail>(x[t], at, bytes);
+      }
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+          for (int t = 0; t < kT; ++t) acc[n][t] = Mma16<E>(pw[n][p], px[t][p], acc[n][t]);
         }
-        v[e] = fmaf(ur, b, v[e]);
+      }
+    };
+    const uint32_t full = bytes / (64 * kPieces) * (64 * kPieces);
+    uint32_t base = 64 * kPieces * wave;
+    for (; base < full; base += 64 * kPieces * kWaves) step(base, std::false_type{});
+    if (base < bytes) step(base, std::true_type{});
+  }
+#pragma unroll
+  for (int n = 0; n < kN; ++n) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) part[wave][n * kT + t][lane] = acc[n][t];
+  }
+  __syncthreads();
+  for (uint32_t item = threadIdx.x; item < 64 * kN * kT; item += 64 * kWaves) {
+    const uint32_t tile = item / 64, l = item % 64;
+    const uint32_t row = 16 * (tile % kT) + l % 16, n = n0 + 16 * (tile / kT) + 4 * (l / 16);
+    const int32_t s = slot[row];
+    if (s == kNoRow || n >= g.out_dim) continue;
+    f32x4_t v = part[0][tile][l];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += part[w][tile][l];
+    if constexpr (kIsE4m3<E>) {
+      if (g.w != nullptr) v = Rescaled(g, g.x_scale[t0 + row], n, v);
+    }
+    AddLowRank<LowOf<E>>(g, t0 + row, n, s, RankOf(g, s), v);
+    Store(g, t0 + row, n, v);
+  }
+}
+
+// ---- The product by tiles ------------------------------------------------------------------------------------------------
+//
+// One workgroup: 32 kN kWN outputs x 32 kT kWT rows, its wavefronts in a kWN x kWT grid of 32 kN x 32 kT each, kept in
+// accumulators. 128 bytes of the inner dimension at a time are copied from memory straight into LDS (global_load_lds, no
+// registers), kStages - 1 steps ahead of the one being multiplied. A row's eight 16-byte pieces lie in LDS at piece p ^ (row % 8), so
+// that the 8 lanes one LDS cycle serves, 8 neighbouring rows at one piece, read 8 different bank groups; the copy writes LDS
+// in lane order, so it is the lanes' source addresses that are permuted.
+
+constexpr uint32_t kStepBytes = 128;
+
+__device__ const u32x4_t kZeroPiece = {0, 0, 0, 0};
+
+// 16 bytes a lane from memory to LDS: lane l's land at lds + 16 l. No register is written; the caller waits (WaitStep).
+__device__ __forceinline__ void Copy16(const void* base, uint32_t off, uint32_t lds) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(off), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void Copy16(const void* at, uint32_t lds) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(at), "s"(lds) : "memory");
+}
+
+// Every copy but this wavefront's last kLeft has landed, its own LDS reads have returned, and then every wavefront's.
+template <int kLeft>
+__device__ __forceinline__ void WaitStep() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
+}
+
+// Runs of one adapter among 32 rows that are multiplied on the matrix instructions, each over all 32 rows.
+constexpr int kRunsByMatrix = 4;
+
+// add(n, B_slot[out .. + 31, :rank] u) for the 32 kN outputs from n0 on and the 32 rows of the wavefront's lanes (lane l's is
+// `token`): D layout of the 32 x 32 instructions, lane l's values in column l % 32. A bf16 pool takes u in bf16 parts: one,
+// or where the output is f32 three, which hold all of its 24 bits.
+template <typename Low, int kN, typename F>
+__device__ __forceinline__ void AddRun(const LoraArgs& g, uint32_t token, uint32_t n0, int32_t slot, uint32_t rank, bool mine,
+                                       uint32_t lane, F&& add) {
+  constexpr uint32_t kPer = 16 / sizeof(Low);
+  f32x16_t d[kN];
+#pragma unroll
+  for (int n = 0; n < kN; ++n) d[n] = f32x16_t{};
+  const float* u = g.u + static_cast<uint64_t>(token) * g.max_rank;
+  const Low* b = static_cast<const Low*>(g.b) + static_cast<uint64_t>(slot) * g.out_dim * g.max_rank;
+  for (uint32_t r0 = 0; r0 < rank; r0 += 2 * kPer) {
+    const uint32_t r = r0 + kPer * (lane / 32);
+    const auto left = static_cast<int32_t>(rank) - static_cast<int32_t>(r);
+    const uint32_t at = left > 0 ? r : 0;
+    float ur[kPer];
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; i += 4) {
+      const f32x4_t q = *reinterpret_cast<const f32x4_t*>(u + at + i);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) ur[i + j] = mine && static_cast<int32_t>(i + j) < left ? q[j] : 0.0f;
+    }
+    u32x4_t pb[kN];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const uint32_t out = min(n0 + 32 * n + lane % 32, g.out_dim - 1);
+      pb[n] = First<Low>(*reinterpret_cast<const u32x4_t*>(b + static_cast<uint64_t>(out) * g.max_rank + at), left);
+    }
+    if constexpr (sizeof(Low) == 4) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(pb[n][i]), ur[i], d[n], 0, 0, 0);
+      }
+    } else {
+      for (int part = 0; part < (g.y_f32 ? 3 : 1); ++part) {
+        u32x4_t pu;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pu[i] = PackBf16Rne(ur[2 * i], ur[2 * i + 1]);
+          ur[2 * i] -= Bf16LoToF32(pu[i]);
+          ur[2 * i + 1] -= Bf16HiToF32(pu[i]);
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, pb[n]), __builtin_bit_cast(bf16x8_t, pu),
+                                                         d[n], 0, 0, 0);
+        }
       }
     }
   }
 #pragma unroll
-  for (uint32_t e = 0; e < 4; ++e) {
-    if (e >= left) continue;
-    if (g.addend != nullptr) {
-      v[e] += LoadF(g.addend, g.addend_f32 ? ROOST_DTYPE_F32 : ROOST_DTYPE_BF16,
-                    static_cast<int64_t>(t * g.addend_stride + n + e));
-    }
-    const uint64_t at = t * g.y_stride + n + e;
-    if (g.y_f32) {
-      static_cast<float*>(g.y)[at] = v[e];
-    } else {
-      static_cast<uint16_t*>(g.y)[at] = F32ToBf16(v[e]);
-    }
-  }
+  for (int n = 0; n < kN; ++n) add(n, d[n]);
 }
 
-// Workgroup (i, j): outputs 16 i .. + 15 of rows 16 kT j .. + 16 kT - 1. Four wavefronts take alternate 64-byte runs of the
-// inner dimension and join their sums through LDS.
-template <typename E, int kT>
-__global__ void __launch_bounds__(256) ProductKernel(LoraArgs g) {
-  __shared__ int32_t slot[16 * kT];
-  __shared__ f32x4_t part[4][kT][64];
-  const uint32_t n0 = 16 * blockIdx.x, t0 = 16 * kT * blockIdx.y;
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  FillSlots(g, t0, 16 * kT, slot);
-  const uint32_t bytes = g.in_dim * sizeof(E);
-  f32x4_t acc[kT];
+template <typename E, int kN, int kT, int kWN, int kWT, int kStages>
+__global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles) {
+  constexpr int kWaves = kWN * kWT;
+  constexpr int kRowsN = 32 * kN * kWN, kRowsT = 32 * kT * kWT;
+  constexpr int kCopiesN = kRowsN / (8 * kWaves), kCopiesT = kRowsT / (8 * kWaves);  // of 8 rows, by each wavefront
+  constexpr uint32_t kStage = (kRowsN + kRowsT) * kStepBytes;
+  static_assert(kCopiesN * 8 * kWaves == kRowsN && kCopiesT * 8 * kWaves == kRowsT, "every wavefront copies whole rows");
+  __shared__ __align__(16) unsigned char lds[kStages * kStage];
+  __shared__ int32_t slot[kRowsT];
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+
+  // Workgroups go to the 8 XCDs in turn; each XCD takes one run of the tiles, ordered in blocks of kBlockT rows of tiles, so
+  // that the tiles in flight on an XCD share weight and token rows in its L2.
+  constexpr uint32_t kXcds = 8, kBlockT = 8;
+  const uint32_t tiles = n_tiles * t_tiles;
+  const uint32_t per_xcd = (tiles + kXcds - 1) / kXcds;
+  const uint32_t at = (blockIdx.x % kXcds) * per_xcd + blockIdx.x / kXcds;
+  if (blockIdx.x / kXcds >= per_xcd || at >= tiles) return;
+  const uint32_t block = at / (kBlockT * n_tiles);
+  const uint32_t block_rows = min(kBlockT, t_tiles - block * kBlockT);
+  const uint32_t in_block = at - block * kBlockT * n_tiles;
+  const uint32_t t0 = (block * kBlockT + in_block % block_rows) * kRowsT;
+  const uint32_t n0 = (in_block / block_rows) * kRowsN;
+
+  FillSlots(g, t0, kRowsT, slot);
+
+  f32x16_t acc[kN][kT];
 #pragma unroll
-  for (int i = 0; i < kT; ++i) acc[i] = f32x4_t{0, 0, 0, 0};
+  for (int n = 0; n < kN; ++n) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) acc[n][t] = f32x16_t{};
+  }
+  const uint32_t wn = (wave % kWN) * 32 * kN, wt = (wave / kWN) * 32 * kT;  // this wavefront's corner of the tile
+
   if (g.w != nullptr) {
-    const E* w = static_cast<const E*>(g.w) + static_cast<uint64_t>(min(n0 + lane % 16, g.out_dim - 1)) * g.in_dim;
-    const E* x[kT];
+    const uint32_t bytes = g.in_dim * sizeof(E);
+    const uint64_t x_bytes = g.x_stride * sizeof(E);
+    const uint32_t steps = (bytes + kStepBytes - 1) / kStepBytes, full = bytes / kStepBytes;
+    const auto* w_base = static_cast<const unsigned char*>(g.w) + static_cast<uint64_t>(n0) * bytes;
+    const auto* x_base = static_cast<const unsigned char*>(g.x) + t0 * x_bytes;
+    // Rows past the last output or token repeat the last one; what they give is not stored.
+    uint32_t off_n[kCopiesN], off_t[kCopiesT];
+    const uint32_t piece = 16 * ((lane % 8) ^ (lane / 8));
 #pragma unroll
-    for (int i = 0; i < kT; ++i) x[i] = static_cast<const E*>(g.x) + min(t0 + 16 * i + lane % 16, g.tokens - 1) * g.x_stride;
-    for (uint32_t base = 64 * wave; base < bytes; base += 256) {
-      const uint32_t at = base + 16 * (lane / 16);
-      const u32x4_t pw = Piece(w, at, bytes);
+    for (int i = 0; i < kCopiesN; ++i) {
+      off_n[i] = min(8 * (wave + kWaves * i) + lane / 8, g.out_dim - 1 - n0) * bytes + piece;
+    }
 #pragma unroll
-      for (int i = 0; i < kT; ++i) acc[i] = Mma16<E>(pw, Piece(x[i], at, bytes), acc[i]);
+    for (int i = 0; i < kCopiesT; ++i) {
+      off_t[i] = min(8 * (wave + kWaves * i) + lane / 8, g.tokens - 1 - t0) * static_cast<uint32_t>(x_bytes) + piece;
+    }
+    const auto lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
+    const auto copy = [&](uint32_t step) {
+      const uint32_t to = lds0 + (step % kStages) * kStage + 1024 * wave;
+      const uint32_t from = step * kStepBytes;
+      if (step < full) {
+#pragma unroll
+        for (int i = 0; i < kCopiesN; ++i) Copy16(w_base + from, off_n[i], to + 1024 * kWaves * i);
+#pragma unroll
+        for (int i = 0; i < kCopiesT; ++i) Copy16(x_base + from, off_t[i], to + kRowsN * kStepBytes + 1024 * kWaves * i);
+      } else {  // the last, partial step: pieces past the row's end are zeros
+        const bool inside = from + piece < bytes;
+#pragma unroll
+        for (int i = 0; i < kCopiesN; ++i) {
+          Copy16(inside ? w_base + from + off_n[i] : reinterpret_cast<const unsigned char*>(&kZeroPiece),
+                 to + 1024 * kWaves * i);
+        }
+#pragma unroll
+        for (int i = 0; i < kCopiesT; ++i) {
+          Copy16(inside ? x_base + from + off_t[i] : reinterpret_cast<const unsigned char*>(&kZeroPiece),
+                 to + kRowsN * kStepBytes + 1024 * kWaves * i);
+        }
+      }
+    };
+    constexpr int kCopies = kCopiesN + kCopiesT;
+#pragma unroll
+    for (uint32_t s = 0; s + 1 < kStages; ++s) {
+      if (s < steps) copy(s);
+    }
+    uint32_t at_piece[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) at_piece[p] = (lane % 32) * kStepBytes + 16 * ((2 * p + lane / 32) ^ (lane % 8));
+    for (uint32_t step = 0; step < steps; ++step) {
+      // The copies of this step have landed once at most those of the kStages - 2 steps after it are in flight.
+      if (kStages > 2 && step + kStages - 2 < steps) {
+        WaitStep<(kStages - 2) * kCopies>();
+      } else {
+        WaitStep<0>();
+      }
+      if (step + kStages - 1 < steps) copy(step + kStages - 1);  // into the buffer that the step before has left
+      const unsigned char* from = lds + (step % kStages) * kStage;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        u32x4_t fn[kN][2], ft[kT][2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int n = 0; n < kN; ++n) {
+            fn[n][q] = *reinterpret_cast<const u32x4_t*>(from + (wn + 32 * n) * kStepBytes + at_piece[2 * half + q]);
+          }
+#pragma unroll
+          for (int t = 0; t < kT; ++t) {
+            ft[t][q] = *reinterpret_cast<const u32x4_t*>(from + (kRowsN + wt + 32 * t) * kStepBytes + at_piece[2 * half + q]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+          for (int t = 0; t < kT; ++t) acc[n][t] = Mma32<E>(fn[n], ft[t], acc[n][t]);
+        }
+      }
     }
   }
+  __syncthreads();  // the slots, where there was no product
+
+  // acc[n][t], register i, lane l: row wt + 32 t + l % 32, output wn + 32 n + 8 (i / 4) + 4 (l / 32) + i % 4.
+  using Low = LowOf<E>;
 #pragma unroll
-  for (int i = 0; i < kT; ++i) part[wave][i][lane] = acc[i];
-  __syncthreads();
-  for (uint32_t item = threadIdx.x; item < 64 * kT; item += 256) {
-    const uint32_t i = item / 64, l = item % 64;
-    const uint32_t row = 16 * i + l % 16, n = n0 + 4 * (l / 16);
+  for (int t = 0; t < kT; ++t) {
+    const uint32_t row = wt + 32 * t + lane % 32, token = t0 + row;
     const int32_t s = slot[row];
-    if (s == kNoRow || n >= g.out_dim) continue;
-    f32x4_t v = part[0][i][l];
+    const auto out_of = [&](int n, int q) { return n0 + wn + 32 * n + 8 * q + 4 * (lane / 32); };
+    const auto quad = [&](int n, int q) {
+      return f32x4_t{acc[n][t][4 * q], acc[n][t][4 * q + 1], acc[n][t][4 * q + 2], acc[n][t][4 * q + 3]};
+    };
+    const auto put = [&](int n, int q, f32x4_t v) {
 #pragma unroll
-    for (int w = 1; w < 4; ++w) v += part[w][i][l];
-    Finish<E>(g, t0 + row, n, s, v);
+      for (int e = 0; e < 4; ++e) acc[n][t][4 * q + e] = v[e];
+    };
+    if constexpr (kIsE4m3<E>) {
+      if (g.w != nullptr) {
+        const float xs = g.x_scale[min(token, g.tokens - 1)];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) put(n, q, Rescaled(g, xs, out_of(n, q), quad(n, q)));
+        }
+      }
+    }
+    // Runs of rows with one adapter among these 32. A few are multiplied run by run, each result kept by its own rows only;
+    // many (one-token sequences) element by element.
+    const int32_t before = __shfl_up(s, 1);
+    uint64_t starts = __ballot(lane < 32 && s >= 0 && (lane == 0 || before != s));
+    if (__popcll(starts) <= kRunsByMatrix) {
+      while (starts != 0) {
+        const int first = __builtin_ctzll(starts);
+        starts &= starts - 1;
+        const int32_t a = __builtin_amdgcn_readlane(s, first);
+        AddRun<Low, kN>(g, min(token, g.tokens - 1), n0 + wn, a, RankOf(g, a), s == a, lane, [&](int n, const f32x16_t& d) {
+          if (s == a) acc[n][t] += d;
+        });
+        // Another run of the same adapter among these rows is done with it.
+        starts &= ~__ballot(s == a);
+      }
+    } else if (s >= 0) {
+      const uint32_t rank = RankOf(g, s);
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4_t v = quad(n, q);
+          AddLowRank<Low>(g, token, out_of(n, q), s, rank, v);
+          put(n, q, v);
+        }
+      }
+    }
+    if (s == kNoRow) continue;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (out_of(n, q) < g.out_dim) Store(g, token, out_of(n, q), quad(n, q));
+      }
+    }
   }
 }
 
@@ -315,6 +746,8 @@ RoostStatus Admit(const RoostAmdGemmLoraParams& p, bool for_run) {
   gate.Expect(p.in_dim * es % 16 == 0 && x_stride * es % 16 == 0, ROOST_STATUS_UNSUPPORTED,
               "in_dim = %u, x_stride = %llu: rows of %s must be multiples of 16 bytes", p.in_dim,
               static_cast<unsigned long long>(x_stride), roost::Describe(e).name)
+      .Expect(x_stride <= 1u << 20, ROOST_STATUS_UNSUPPORTED, "x_stride = %llu; built for up to 1,048,576",
+              static_cast<unsigned long long>(x_stride))
       .Expect(x_stride >= p.in_dim && y_stride >= p.out_dim && add_stride >= p.out_dim, ROOST_STATUS_INVALID_ARGUMENT,
               "a row stride (x %llu, output %llu, addend %llu) is below its row's width",
               static_cast<unsigned long long>(x_stride), static_cast<unsigned long long>(y_stride),
@@ -385,19 +818,49 @@ uint64_t WorkspaceBytes(const RoostAmdGemmLoraParams& p) {
 
 // ---- Launch --------------------------------------------------------------------------------------------------------------
 
+template <typename E, int kT, int kR>
+void LaunchShrink(const LoraArgs& g, hipStream_t stream) {
+  const uint32_t runs = std::min(std::max(g.batch, 1u), 16u);
+  const dim3 grid(roost::CeilDiv(g.tokens, 16 * kT), roost::CeilDiv(g.max_rank, 16 * kR), kT == 1 ? runs : std::min(runs, 2u));
+  hipLaunchKernelGGL((ShrinkKernel<E, kT, kR>), grid, dim3(512), 0, stream, g);
+}
+template <typename E, int kT>
+void LaunchShrinkOfRows(const LoraArgs& g, hipStream_t stream) {
+  if (g.max_rank <= 16) return LaunchShrink<E, kT, 1>(g, stream);
+  if (g.max_rank <= 32) return LaunchShrink<E, kT, 2>(g, stream);
+  return LaunchShrink<E, kT, 4>(g, stream);
+}
+
+template <typename E, int kN, int kT>
+void LaunchProduct(const LoraArgs& g, hipStream_t stream) {
+  const dim3 grid(roost::CeilDiv(g.out_dim, 16 * kN), roost::CeilDiv(g.tokens, 16 * kT));
+  hipLaunchKernelGGL((ProductKernel<E, kN, kT>), grid, dim3(512), 0, stream, g);
+}
+
+template <typename E, int kN, int kT, int kWN, int kWT, int kStages>
+void LaunchTiles(const LoraArgs& g, hipStream_t stream) {
+  const auto n_tiles = static_cast<uint32_t>(roost::CeilDiv(g.out_dim, 32 * kN * kWN));
+  const auto t_tiles = static_cast<uint32_t>(roost::CeilDiv(g.tokens, 32 * kT * kWT));
+  const auto grid = static_cast<uint32_t>(roost::RoundUp(n_tiles * t_tiles, 8));
+  hipLaunchKernelGGL((TileKernel<E, kN, kT, kWN, kWT, kStages>), dim3(grid), dim3(64 * kWN * kWT), 0, stream, g, n_tiles, t_tiles);
+}
+
 template <typename E>
 void LaunchAll(const LoraArgs& g, hipStream_t stream) {
   if (g.a != nullptr) {
-    const dim3 grid(roost::CeilDiv(g.tokens, 16), roost::CeilDiv(g.max_rank, 16), std::min(std::max(g.batch, 1u), 16u));
-    hipLaunchKernelGGL(ShrinkKernel<E>, grid, dim3(256), 0, stream, g);
+    if (g.tokens / g.batch >= 64) {
+      LaunchShrinkOfRows<E, 4>(g, stream);
+    } else {
+      LaunchShrinkOfRows<E, 1>(g, stream);
+    }
   }
-  const auto product = [&](auto t) {
-    constexpr int kT = decltype(t)::value;
-    hipLaunchKernelGGL((ProductKernel<E, kT>), dim3(roost::CeilDiv(g.out_dim, 16), roost::CeilDiv(g.tokens, 16 * kT)),
-                       dim3(256), 0, stream, g);
-  };
-  if (g.tokens <= 16) return product(std::integral_constant<int, 1>{});
-  return product(std::integral_constant<int, 4>{});
+  if (g.tokens <= 16) return LaunchProduct<E, 1, 1>(g, stream);
+  if (g.tokens <= 32) return LaunchProduct<E, 1, 2>(g, stream);
+  if (g.tokens <= 64) return LaunchProduct<E, 2, 4>(g, stream);
+  const uint64_t large = roost::CeilDiv(g.out_dim, 256) * roost::CeilDiv(g.tokens, 256);
+  if (large >= 128) return LaunchTiles<E, 2, 4, 4, 2, 2>(g, stream);
+  if (roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(g.tokens, 128) >= 128) return LaunchTiles<E, 2, 2, 2, 2, 4>(g, stream);
+  return LaunchTiles<E, 1, 1, 2, 2, 4>(g, stream);
 }
 
 }  // namespace
@@ -453,6 +916,8 @@ extern "C" ROOST_API RoostStatus roost_amd_gemm_lora_run(RoostContext* ctx, cons
       LaunchAll<float>(g, s);
     } else if (p.x.dtype == ROOST_DTYPE_BF16) {
       LaunchAll<uint16_t>(g, s);
+    } else if (g.y_f32) {
+      LaunchAll<E4m3AsBf16>(g, s);
     } else {
       LaunchAll<E4m3>(g, s);
     }
