@@ -59,7 +59,10 @@ struct LoraArgs {
   const int32_t* cu;
   const void* addend;
   void* y;
-  float* u;  // [tokens, max_rank]
+  float* u;         // [tokens, max_rank]
+  uint16_t* u_bf16;  // the same in bf16 parts that add up to it, `parts` arrays one after another (bf16 adapters)
+  uint64_t u_part;   // elements of one
+  uint32_t parts;
   uint64_t x_stride, addend_stride, y_stride;  // elements
   uint32_t tokens, batch, in_dim, out_dim, adapters, max_rank;
   uint32_t addend_f32, y_f32;
@@ -70,18 +73,32 @@ struct LoraArgs {
 constexpr int32_t kNoRow = -2;      // the row belongs to no sequence
 constexpr int32_t kNoAdapter = -1;
 
-// slot[i] for rows t0 .. t0 + n - 1, by the whole workgroup; a barrier must follow.
+// slot[i] for rows t0 .. t0 + n - 1, by the whole workgroup; a barrier must follow. A lane writes a short sequence's rows
+// itself; a long one's are written by its wavefront.
 __device__ __forceinline__ void FillSlots(const LoraArgs& g, uint32_t t0, uint32_t n, int32_t* slot) {
+  constexpr int32_t kShort = 4;
   for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) slot[i] = kNoRow;
   __syncthreads();
-  const auto first = static_cast<int64_t>(t0);
-  const int64_t last = min(first + n, static_cast<int64_t>(g.tokens));
-  for (uint32_t b = threadIdx.x; b < g.batch; b += blockDim.x) {
-    const int64_t lo = max(static_cast<int64_t>(g.cu[b]), first), hi = min(static_cast<int64_t>(g.cu[b + 1]), last);
-    if (lo >= hi) continue;
-    int32_t s = g.a != nullptr ? g.slots[b] : kNoAdapter;
-    if (s < 0 || static_cast<uint32_t>(s) >= g.adapters) s = kNoAdapter;
-    for (int64_t t = lo; t < hi; ++t) slot[t - first] = s;
+  const auto rows = static_cast<int32_t>(min(n, g.tokens - t0));
+  for (uint32_t first = threadIdx.x / 64 * 64; first < g.batch; first += blockDim.x) {
+    const uint32_t b = first + threadIdx.x % 64;
+    int32_t lo = 0, hi = 0, s = kNoAdapter;
+    if (b < g.batch) {
+      const auto start = static_cast<int64_t>(t0);
+      lo = static_cast<int32_t>(min(max(g.cu[b] - start, int64_t{0}), int64_t{rows}));
+      hi = static_cast<int32_t>(min(max(g.cu[b + 1] - start, int64_t{0}), int64_t{rows}));
+      if (lo < hi && g.a != nullptr) s = g.slots[b];
+      if (s < 0 || static_cast<uint32_t>(s) >= g.adapters) s = kNoAdapter;
+    }
+    if (hi - lo <= kShort) {
+      for (int32_t t = lo; t < hi; ++t) slot[t] = s;
+    }
+    for (uint64_t left = __ballot(hi - lo > kShort); left != 0; left &= left - 1) {
+      const int l = __builtin_ctzll(left);
+      const int32_t from = __builtin_amdgcn_readlane(lo, l), to = __builtin_amdgcn_readlane(hi, l);
+      const int32_t its = __builtin_amdgcn_readlane(s, l);
+      for (int32_t t = from + static_cast<int32_t>(threadIdx.x % 64); t < to; t += 64) slot[t] = its;
+    }
   }
 }
 
@@ -137,33 +154,30 @@ __device__ __forceinline__ f32x4_t Mma16(u32x4_t a, u32x4_t b, f32x4_t acc) {
   }
 }
 
-// acc += (32 rows) x (32 rows)^T over the 64 bytes that two pieces a lane cover: lane l holds row l % 32, its pieces are two
-// of the four of those bytes (lanes 0 to 31 the first and third, the others the second and fourth).
+// The operand of Mma32: one piece, or two (e4m3).
 template <typename E>
-__device__ __forceinline__ f32x16_t Mma32(const u32x4_t (&a)[2], const u32x4_t (&b)[2], f32x16_t acc) {
+using FragOf = std::conditional_t<std::is_same_v<E, E4m3>, i32x8_t, u32x4_t>;
+
+// acc += (32 rows) x (32 rows)^T over the 32 bytes that one piece a lane covers, or 64 bytes and two pieces (e4m3): lane l
+// holds row l % 32, lanes 0 to 31 one half of the bytes, the others the other.
+template <typename E>
+__device__ __forceinline__ f32x16_t Mma32(FragOf<E> a, FragOf<E> b, f32x16_t acc) {
   if constexpr (std::is_same_v<E, E4m3>) {
-    const i32x8_t pa = {(int)a[0][0], (int)a[0][1], (int)a[0][2], (int)a[0][3], (int)a[1][0], (int)a[1][1], (int)a[1][2], (int)a[1][3]};
-    const i32x8_t pb = {(int)b[0][0], (int)b[0][1], (int)b[0][2], (int)b[0][3], (int)b[1][0], (int)b[1][1], (int)b[1][2], (int)b[1][3]};
     // Block scales of 2^0 (biased exponent 127).
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(pa, pb, acc, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+  } else if constexpr (std::is_same_v<E, uint16_t>) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), acc, 0, 0, 0);
+  } else if constexpr (std::is_same_v<E, float>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), acc, 0, 0, 0);
+    }
+    return acc;
   } else {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if constexpr (std::is_same_v<E, uint16_t>) {
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[q]), __builtin_bit_cast(bf16x8_t, b[q]),
-                                                      acc, 0, 0, 0);
-      } else if constexpr (std::is_same_v<E, float>) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[q][i]), __uint_as_float(b[q][i]), acc, 0, 0, 0);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Bf16OfE4m3(a[q][2 * i], a[q][2 * i + 1]),
-                                                        Bf16OfE4m3(b[q][2 * i], b[q][2 * i + 1]), acc, 0, 0, 0);
-        }
-      }
+    for (int i = 0; i < 2; ++i) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Bf16OfE4m3(a[2 * i], a[2 * i + 1]), Bf16OfE4m3(b[2 * i], b[2 * i + 1]),
+                                                    acc, 0, 0, 0);
     }
     return acc;
   }
@@ -240,7 +254,6 @@ __global__ void __launch_bounds__(512) ShrinkKernel(LoraArgs g) {
     };
     const uint32_t full = bytes / 64 * 64;
     uint32_t base = 64 * wave;
-#pragma unroll 4
     for (; base < full; base += 64 * kWaves) step(base, std::false_type{});
     if (base < bytes) step(base, std::true_type{});
 #pragma unroll
@@ -259,7 +272,16 @@ __global__ void __launch_bounds__(512) ShrinkKernel(LoraArgs g) {
       float scale = g.lora_scale != nullptr ? g.lora_scale[s] : 1.0f;
       if constexpr (kIsE4m3<E>) scale *= g.x_scale[t0 + row];
       // max_rank is a multiple of 8: the four are the row's own, those past the adapter's rank unused.
-      *reinterpret_cast<f32x4_t*>(g.u + static_cast<uint64_t>(t0 + row) * g.max_rank + first) = v * scale;
+      const uint64_t at = static_cast<uint64_t>(t0 + row) * g.max_rank + first;
+      v *= scale;
+      *reinterpret_cast<f32x4_t*>(g.u + at) = v;
+      if constexpr (sizeof(Low) == 2) {
+        for (uint32_t p = 0; p < g.parts; ++p) {
+          const u32x2_t w = {PackBf16Rne(v[0], v[1]), PackBf16Rne(v[2], v[3])};
+          *reinterpret_cast<u32x2_t*>(g.u_bf16 + p * g.u_part + at) = w;
+          v -= f32x4_t{Bf16LoToF32(w[0]), Bf16HiToF32(w[0]), Bf16LoToF32(w[1]), Bf16HiToF32(w[1])};
+        }
+      }
     }
     __syncthreads();
   }
@@ -316,9 +338,21 @@ __device__ __forceinline__ void AddLowRank(const LoraArgs& g, uint32_t t, uint32
   }
 }
 
-// Four consecutive elements of a row at `at`, which may be aligned to an element only.
+// Consecutive elements of a row at an address that may be aligned to an element only.
 typedef uint32_t Bf16x4 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t Bf16x8 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float F32x4 __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ float AddendOne(const LoraArgs& g, uint64_t at) {
+  return LoadF(g.addend, g.addend_f32 ? ROOST_DTYPE_F32 : ROOST_DTYPE_BF16, static_cast<int64_t>(at));
+}
+__device__ __forceinline__ void StoreOne(const LoraArgs& g, uint64_t at, float v) {
+  if (g.y_f32) {
+    static_cast<float*>(g.y)[at] = v;
+  } else {
+    static_cast<uint16_t*>(g.y)[at] = static_cast<uint16_t>(PackBf16Rne(v, 0.0f));
+  }
+}
 
 // Adds the addend and stores outputs n .. n + 3 of row t.
 __device__ __forceinline__ void Store(const LoraArgs& g, uint32_t t, uint32_t n, f32x4_t v) {
@@ -341,17 +375,7 @@ __device__ __forceinline__ void Store(const LoraArgs& g, uint32_t t, uint32_t n,
   }
 #pragma unroll
   for (uint32_t e = 0; e < 3; ++e) {
-    if (e < g.out_dim - n) {
-      float one = v[e];
-      if (g.addend != nullptr) {
-        one += LoadF(g.addend, g.addend_f32 ? ROOST_DTYPE_F32 : ROOST_DTYPE_BF16, static_cast<int64_t>(from + e));
-      }
-      if (g.y_f32) {
-        static_cast<float*>(g.y)[at + e] = one;
-      } else {
-        static_cast<uint16_t*>(g.y)[at + e] = static_cast<uint16_t>(PackBf16Rne(one, 0.0f));
-      }
-    }
+    if (e < g.out_dim - n) StoreOne(g, at + e, v[e] + (g.addend != nullptr ? AddendOne(g, from + e) : 0.0f));
   }
 }
 
@@ -441,13 +465,11 @@ __global__ void __launch_bounds__(512) ProductKernel(LoraArgs g) {
 //
 // One workgroup: 32 kN kWN outputs x 32 kT kWT rows, its wavefronts in a kWN x kWT grid of 32 kN x 32 kT each, kept in
 // accumulators. 128 bytes of the inner dimension at a time are copied from memory straight into LDS (global_load_lds, no
-// registers), kStages - 1 steps ahead of the one being multiplied. A row's eight 16-byte pieces lie in LDS at piece p ^ (row % 8), so
-// that the 8 lanes one LDS cycle serves, 8 neighbouring rows at one piece, read 8 different bank groups; the copy writes LDS
-// in lane order, so it is the lanes' source addresses that are permuted.
+// registers), kStages steps ahead. A row's eight 16-byte pieces lie in LDS at piece
+// p ^ (row / 2 % 8): 32 rows of 128 bytes read at one piece are then free of bank conflicts (with p ^ (row % 8) each read takes half
+// as long again). The copy writes LDS in lane order, so it is the lanes' source addresses that are permuted.
 
 constexpr uint32_t kStepBytes = 128;
-
-__device__ const u32x4_t kZeroPiece = {0, 0, 0, 0};
 
 // 16 bytes a lane from memory to LDS: lane l's land at lds + 16 l. No register is written; the caller waits (WaitStep).
 __device__ __forceinline__ void Copy16(const void* base, uint32_t off, uint32_t lds) {
@@ -455,76 +477,18 @@ __device__ __forceinline__ void Copy16(const void* base, uint32_t off, uint32_t 
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(m0) : "v"(off), "s"(base), "s"(lds) : "memory");
 }
-__device__ __forceinline__ void Copy16(const void* at, uint32_t lds) {
-  uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0) : "v"(at), "s"(lds) : "memory");
-}
-
 // Every copy but this wavefront's last kLeft has landed, its own LDS reads have returned, and then every wavefront's.
 template <int kLeft>
 __device__ __forceinline__ void WaitStep() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
 
-// Runs of one adapter among 32 rows that are multiplied on the matrix instructions, each over all 32 rows.
-constexpr int kRunsByMatrix = 4;
+// This wavefront's LDS writes are visible to its own lanes' reads after it, and no access moves across.
+__device__ __forceinline__ void WaveSync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// add(n, B_slot[out .. + 31, :rank] u) for the 32 kN outputs from n0 on and the 32 rows of the wavefront's lanes (lane l's is
-// `token`): D layout of the 32 x 32 instructions, lane l's values in column l % 32. A bf16 pool takes u in bf16 parts: one,
-// or where the output is f32 three, which hold all of its 24 bits.
-template <typename Low, int kN, typename F>
-__device__ __forceinline__ void AddRun(const LoraArgs& g, uint32_t token, uint32_t n0, int32_t slot, uint32_t rank, bool mine,
-                                       uint32_t lane, F&& add) {
-  constexpr uint32_t kPer = 16 / sizeof(Low);
-  f32x16_t d[kN];
-#pragma unroll
-  for (int n = 0; n < kN; ++n) d[n] = f32x16_t{};
-  const float* u = g.u + static_cast<uint64_t>(token) * g.max_rank;
-  const Low* b = static_cast<const Low*>(g.b) + static_cast<uint64_t>(slot) * g.out_dim * g.max_rank;
-  for (uint32_t r0 = 0; r0 < rank; r0 += 2 * kPer) {
-    const uint32_t r = r0 + kPer * (lane / 32);
-    const auto left = static_cast<int32_t>(rank) - static_cast<int32_t>(r);
-    const uint32_t at = left > 0 ? r : 0;
-    float ur[kPer];
-#pragma unroll
-    for (uint32_t i = 0; i < kPer; i += 4) {
-      const f32x4_t q = *reinterpret_cast<const f32x4_t*>(u + at + i);
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) ur[i + j] = mine && static_cast<int32_t>(i + j) < left ? q[j] : 0.0f;
-    }
-    u32x4_t pb[kN];
-#pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      const uint32_t out = min(n0 + 32 * n + lane % 32, g.out_dim - 1);
-      pb[n] = First<Low>(*reinterpret_cast<const u32x4_t*>(b + static_cast<uint64_t>(out) * g.max_rank + at), left);
-    }
-    if constexpr (sizeof(Low) == 4) {
-#pragma unroll
-      for (int n = 0; n < kN; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(pb[n][i]), ur[i], d[n], 0, 0, 0);
-      }
-    } else {
-      for (int part = 0; part < (g.y_f32 ? 3 : 1); ++part) {
-        u32x4_t pu;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pu[i] = PackBf16Rne(ur[2 * i], ur[2 * i + 1]);
-          ur[2 * i] -= Bf16LoToF32(pu[i]);
-          ur[2 * i + 1] -= Bf16HiToF32(pu[i]);
-        }
-#pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          d[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, pb[n]), __builtin_bit_cast(bf16x8_t, pu),
-                                                         d[n], 0, 0, 0);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int n = 0; n < kN; ++n) add(n, d[n]);
-}
+// Runs of rows with one adapter that a 32 x 32 tile a wavefront takes step by step; more (one-token sequences) are added element
+// by element.
+constexpr uint32_t kRunsBySteps = 4;
 
 template <typename E, int kN, int kT, int kWN, int kWT, int kStages>
 __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles) {
@@ -532,9 +496,13 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
   constexpr int kRowsN = 32 * kN * kWN, kRowsT = 32 * kT * kWT;
   constexpr int kCopiesN = kRowsN / (8 * kWaves), kCopiesT = kRowsT / (8 * kWaves);  // of 8 rows, by each wavefront
   constexpr uint32_t kStage = (kRowsN + kRowsT) * kStepBytes;
+  static_assert(kWaves % 2 == 0 && kRowsN % 16 == 0, "the permutation of a wavefront's copies is the same for each");
   static_assert(kCopiesN * 8 * kWaves == kRowsN && kCopiesT * 8 * kWaves == kRowsT, "every wavefront copies whole rows");
   __shared__ __align__(16) unsigned char lds[kStages * kStage];
   __shared__ int32_t slot[kRowsT];
+  __shared__ int32_t run_start[kRowsT + 1];  // the rows where the adapter changes
+  __shared__ uint32_t run_count;
+  __shared__ __align__(16) float w_scale[kIsE4m3<E> ? kRowsN : 4];
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 
   // Workgroups go to the 8 XCDs in turn; each XCD takes one run of the tiles, ordered in blocks of kBlockT rows of tiles, so
@@ -550,8 +518,6 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
   const uint32_t t0 = (block * kBlockT + in_block % block_rows) * kRowsT;
   const uint32_t n0 = (in_block / block_rows) * kRowsN;
 
-  FillSlots(g, t0, kRowsT, slot);
-
   f32x16_t acc[kN][kT];
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
@@ -560,146 +526,338 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
   }
   const uint32_t wn = (wave % kWN) * 32 * kN, wt = (wave / kWN) * 32 * kT;  // this wavefront's corner of the tile
 
-  if (g.w != nullptr) {
-    const uint32_t bytes = g.in_dim * sizeof(E);
-    const uint64_t x_bytes = g.x_stride * sizeof(E);
-    const uint32_t steps = (bytes + kStepBytes - 1) / kStepBytes, full = bytes / kStepBytes;
-    const auto* w_base = static_cast<const unsigned char*>(g.w) + static_cast<uint64_t>(n0) * bytes;
-    const auto* x_base = static_cast<const unsigned char*>(g.x) + t0 * x_bytes;
-    // Rows past the last output or token repeat the last one; what they give is not stored.
-    uint32_t off_n[kCopiesN], off_t[kCopiesT];
-    const uint32_t piece = 16 * ((lane % 8) ^ (lane / 8));
+  // The copies. Rows past the last output or token repeat the last one; what they give is not stored.
+  using Low = LowOf<E>;
+  const uint32_t bytes = g.in_dim * sizeof(E);
+  const uint64_t x_bytes = g.x_stride * sizeof(E);
+  const uint32_t full = g.w != nullptr ? bytes / kStepBytes : 0;
+  const uint32_t steps = g.w != nullptr ? (bytes + kStepBytes - 1) / kStepBytes : 0;
+  const auto* w_base = static_cast<const unsigned char*>(g.w) + static_cast<uint64_t>(n0) * bytes;
+  const auto* x_base = static_cast<const unsigned char*>(g.x) + t0 * x_bytes;
+  const uint32_t last_n = g.out_dim - 1 - n0, last_t = g.tokens - 1 - t0;
+  const uint32_t piece = 16 * ((lane % 8) ^ (4 * (wave % 2) + lane / 16));  // rows 8 (wave + kWaves i) + lane / 8
+  uint32_t off_n[kCopiesN], off_t[kCopiesT];
 #pragma unroll
-    for (int i = 0; i < kCopiesN; ++i) {
-      off_n[i] = min(8 * (wave + kWaves * i) + lane / 8, g.out_dim - 1 - n0) * bytes + piece;
+  for (int i = 0; i < kCopiesN; ++i) off_n[i] = min(8 * (wave + kWaves * i) + lane / 8, last_n) * bytes + piece;
+#pragma unroll
+  for (int i = 0; i < kCopiesT; ++i) {
+    off_t[i] = min(8 * (wave + kWaves * i) + lane / 8, last_t) * static_cast<uint32_t>(x_bytes) + piece;
+  }
+  const auto lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
+  const auto zero = [&](uint32_t stage) {  // this lane's pieces of a stage
+#pragma unroll
+    for (int i = 0; i < kCopiesN + kCopiesT; ++i) {
+      *reinterpret_cast<u32x4_t*>(lds + stage * kStage + 1024 * (wave + kWaves * i) + 16 * lane) = u32x4_t{0, 0, 0, 0};
     }
+  };
+  const auto copy = [&](uint32_t step) {
+    const uint32_t to_n = lds0 + (step % kStages) * kStage + 1024 * wave, to_t = to_n + kRowsN * kStepBytes;
+    const uint32_t from = step * kStepBytes;
+    if (step < full) {
 #pragma unroll
-    for (int i = 0; i < kCopiesT; ++i) {
-      off_t[i] = min(8 * (wave + kWaves * i) + lane / 8, g.tokens - 1 - t0) * static_cast<uint32_t>(x_bytes) + piece;
+      for (int i = 0; i < kCopiesN; ++i) Copy16(w_base + from, off_n[i], to_n + 1024 * kWaves * i);
+#pragma unroll
+      for (int i = 0; i < kCopiesT; ++i) Copy16(x_base + from, off_t[i], to_t + 1024 * kWaves * i);
+    } else if (from + piece < bytes) {
+#pragma unroll
+      for (int i = 0; i < kCopiesN; ++i) Copy16(w_base + from, off_n[i], to_n + 1024 * kWaves * i);
+#pragma unroll
+      for (int i = 0; i < kCopiesT; ++i) Copy16(x_base + from, off_t[i], to_t + 1024 * kWaves * i);
+    } else {  // the last, partial step: pieces past the row's end are zeros
+      zero(step % kStages);
     }
-    const auto lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
-    const auto copy = [&](uint32_t step) {
-      const uint32_t to = lds0 + (step % kStages) * kStage + 1024 * wave;
-      const uint32_t from = step * kStepBytes;
-      if (step < full) {
+  };
 #pragma unroll
-        for (int i = 0; i < kCopiesN; ++i) Copy16(w_base + from, off_n[i], to + 1024 * kWaves * i);
+  for (uint32_t i = 0; i < kStages; ++i) {
+    if (i < steps) copy(i);
+  }
+  FillSlots(g, t0, kRowsT, slot);
+  if constexpr (kIsE4m3<E>) {
+    if (g.w != nullptr) {
+      for (uint32_t i = threadIdx.x; i < kRowsN; i += 64 * kWaves) w_scale[i] = g.w_scale[min(n0 + i, g.out_dim - 1)];
+    }
+  }
+  __syncthreads();
+  if (wave == 0) {
+    uint32_t count = 0;
+    for (uint32_t i = lane; i < kRowsT; i += 64) {
+      const uint64_t starts = __ballot(i == 0 || slot[i] != slot[i - 1]);
+      if (starts >> lane & 1) run_start[count + __popcll(starts & ((uint64_t{1} << lane) - 1))] = i;
+      count += __popcll(starts);
+    }
+    if (lane == 0) {
+      run_start[count] = kRowsT;
+      run_count = count;
+    }
+  }
+
+  // A step is consumed in kPhases phases of kPieces pieces a lane, each in kHalves parts of the wavefront's rows; the
+  // operands are read from LDS one part ahead of the products that use them. The last part waits for the next step's
+  // copies, reads its first operands and refills the buffer that every wavefront has then read, all under its own products.
+  uint32_t at_piece[4];
 #pragma unroll
-        for (int i = 0; i < kCopiesT; ++i) Copy16(x_base + from, off_t[i], to + kRowsN * kStepBytes + 1024 * kWaves * i);
-      } else {  // the last, partial step: pieces past the row's end are zeros
-        const bool inside = from + piece < bytes;
-#pragma unroll
-        for (int i = 0; i < kCopiesN; ++i) {
-          Copy16(inside ? w_base + from + off_n[i] : reinterpret_cast<const unsigned char*>(&kZeroPiece),
-                 to + 1024 * kWaves * i);
-        }
-#pragma unroll
-        for (int i = 0; i < kCopiesT; ++i) {
-          Copy16(inside ? x_base + from + off_t[i] : reinterpret_cast<const unsigned char*>(&kZeroPiece),
-                 to + kRowsN * kStepBytes + 1024 * kWaves * i);
-        }
+  for (int p = 0; p < 4; ++p) at_piece[p] = (lane % 32) * kStepBytes + 16 * ((2 * p + lane / 32) ^ (lane / 2 % 8));
+  constexpr int kCopies = kCopiesN + kCopiesT;
+  if (steps > 0) {
+    constexpr int kPieces = std::is_same_v<E, E4m3> ? 2 : 1, kPhases = 4 / kPieces;
+    // e4m3 operands take twice the registers, so half of the rows at a time.
+    constexpr int kHalves = kPieces == 2 && kT > 1 ? 2 : 1, kHalfT = kT / kHalves, kParts = kPhases * kHalves;
+    FragOf<E> fn[2][kN], ft[2][kHalfT];
+    const auto load = [&](const unsigned char* rows, int phase) -> FragOf<E> {
+      if constexpr (kPieces == 2) {
+        const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(rows + at_piece[2 * phase]);
+        const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(rows + at_piece[2 * phase + 1]);
+        return __builtin_bit_cast(i32x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      } else {
+        return *reinterpret_cast<const u32x4_t*>(rows + at_piece[phase]);
       }
     };
-    constexpr int kCopies = kCopiesN + kCopiesT;
+    const auto read = [&](const unsigned char* from, int part) {
+      const int phase = part / kHalves, half = part % kHalves;
 #pragma unroll
-    for (uint32_t s = 0; s + 1 < kStages; ++s) {
-      if (s < steps) copy(s);
-    }
-    uint32_t at_piece[4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) at_piece[p] = (lane % 32) * kStepBytes + 16 * ((2 * p + lane / 32) ^ (lane % 8));
-    for (uint32_t step = 0; step < steps; ++step) {
-      // The copies of this step have landed once at most those of the kStages - 2 steps after it are in flight.
-      if (kStages > 2 && step + kStages - 2 < steps) {
-        WaitStep<(kStages - 2) * kCopies>();
-      } else {
-        WaitStep<0>();
+      for (int n = 0; n < kN; ++n) {
+        if (half == 0) fn[phase % 2][n] = load(from + (wn + 32 * n) * kStepBytes, phase);
       }
-      if (step + kStages - 1 < steps) copy(step + kStages - 1);  // into the buffer that the step before has left
+#pragma unroll
+      for (int t = 0; t < kHalfT; ++t) {
+        ft[part % 2][t] = load(from + (kRowsN + wt + 32 * (half * kHalfT + t)) * kStepBytes, phase);
+      }
+    };
+    if (steps >= kStages) {
+      WaitStep<(kStages - 1) * kCopies>();
+    } else {
+      WaitStep<0>();
+    }
+    read(lds, 0);
+#pragma unroll 1
+    for (uint32_t step = 0; step < steps; ++step) {
       const unsigned char* from = lds + (step % kStages) * kStage;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        u32x4_t fn[kN][2], ft[kT][2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-#pragma unroll
-          for (int n = 0; n < kN; ++n) {
-            fn[n][q] = *reinterpret_cast<const u32x4_t*>(from + (wn + 32 * n) * kStepBytes + at_piece[2 * half + q]);
+      for (int part = 0; part < kParts; ++part) {
+        if (part + 1 < kParts) {
+          read(from, part + 1);
+        } else if (step + 1 < steps) {
+          // Of the kStages steps whose copies are out, the next one's are to have landed.
+          if (kStages > 2 && step + kStages - 1 < steps) {
+            WaitStep<(kStages - 2) * kCopies>();
+          } else {
+            WaitStep<0>();
           }
-#pragma unroll
-          for (int t = 0; t < kT; ++t) {
-            ft[t][q] = *reinterpret_cast<const u32x4_t*>(from + (kRowsN + wt + 32 * t) * kStepBytes + at_piece[2 * half + q]);
-          }
+          read(lds + ((step + 1) % kStages) * kStage, 0);
+          if (step + kStages < steps) copy(step + kStages);
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
 #pragma unroll
-          for (int t = 0; t < kT; ++t) acc[n][t] = Mma32<E>(fn[n], ft[t], acc[n][t]);
+          for (int t = 0; t < kHalfT; ++t) {
+            f32x16_t& sum = acc[n][(part % kHalves) * kHalfT + t];
+            sum = Mma32<E>(fn[part / kHalves % 2][n], ft[part % 2][t], sum);
+            // Keeps the products of a part between its reads and the next part's.
+            if constexpr (kN * kT >= 8) asm volatile("" : "+v"(sum));
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  __syncthreads();  // the stages are free, the runs known
+
+  // The adapters, one run of rows after the other, by the same steps: 128 bytes of the ranks of the adapter's outputs and of the
+  // low-rank rows. A row takes only its own run's sums, so that no adapter's values, whatever they are, reach another's rows.
+  // acc[n][t], register i, lane l: row wt + 32 t + l % 32, output wn + 32 n + 8 (i / 4) + 4 (l / 32) + i % 4.
+  if constexpr (kIsE4m3<E>) {
+    if (g.w != nullptr) {
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const float xs = g.x_scale[t0 + min(wt + 32 * t + lane % 32, last_t)];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4_t ws = *reinterpret_cast<const f32x4_t*>(w_scale + wn + 32 * n + 8 * q + 4 * (lane / 32));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[n][t][4 * q + e] *= xs * ws[e];
+          }
         }
       }
     }
   }
-  __syncthreads();  // the slots, where there was no product
-
-  // acc[n][t], register i, lane l: row wt + 32 t + l % 32, output wn + 32 n + 8 (i / 4) + 4 (l / 32) + i % 4.
-  using Low = LowOf<E>;
-#pragma unroll
-  for (int t = 0; t < kT; ++t) {
-    const uint32_t row = wt + 32 * t + lane % 32, token = t0 + row;
-    const int32_t s = slot[row];
-    const auto out_of = [&](int n, int q) { return n0 + wn + 32 * n + 8 * q + 4 * (lane / 32); };
-    const auto quad = [&](int n, int q) {
-      return f32x4_t{acc[n][t][4 * q], acc[n][t][4 * q + 1], acc[n][t][4 * q + 2], acc[n][t][4 * q + 3]};
+  const uint32_t runs = __builtin_amdgcn_readfirstlane(g.a != nullptr ? run_count : 0);
+  if (kN * kT > 1 || runs <= kRunsBySteps) {
+    constexpr int kPer = 16 / sizeof(Low);
+    const uint32_t row_bytes = g.max_rank * sizeof(Low);
+    const uint32_t parts = sizeof(Low) == 2 ? g.parts : 1;
+    // A place in the list of steps: run, part of the low-rank rows, first byte of their ranks.
+    struct Place {
+      uint32_t run, part, from;
+      int32_t slot;
+      uint32_t bytes;  // of the run's ranks
     };
-    const auto put = [&](int n, int q, f32x4_t v) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][t][4 * q + e] = v[e];
+    const auto enter = [&](Place& p) {  // the next run with an adapter, from p.run on
+      for (; p.run < runs; ++p.run) {
+        p.slot = __builtin_amdgcn_readfirstlane(slot[run_start[p.run]]);
+        p.bytes = __builtin_amdgcn_readfirstlane(RankOf(g, p.slot)) * sizeof(Low);
+        if (p.bytes > 0) break;
+      }
+      p.part = p.from = 0;
     };
-    if constexpr (kIsE4m3<E>) {
-      if (g.w != nullptr) {
-        const float xs = g.x_scale[min(token, g.tokens - 1)];
+    const auto advance = [&](Place& p) {
+      p.from += kStepBytes;
+      if (p.from < p.bytes) return;
+      p.from = 0;
+      if (++p.part < parts) return;
+      ++p.run;
+      enter(p);
+    };
+    const auto copy_low = [&](const Place& p, uint32_t stage) {
+      const uint32_t to_n = lds0 + stage * kStage + 1024 * wave, to_t = to_n + kRowsN * kStepBytes;
+      const uint32_t at = p.from + piece;
+      if (at >= p.bytes) {
+        zero(stage);
+        return;
+      }
+      // A row of the pool is at most 512 bytes, so a tile's are within 32 bits of its first.
+      const auto* b_base = static_cast<const unsigned char*>(g.b) + (static_cast<uint64_t>(p.slot) * g.out_dim + n0) * row_bytes;
+      const auto* u_base = (sizeof(Low) == 2 ? reinterpret_cast<const unsigned char*>(g.u_bf16 + p.part * g.u_part)
+                                             : reinterpret_cast<const unsigned char*>(g.u)) + t0 * static_cast<uint64_t>(row_bytes);
+#pragma unroll
+      for (int i = 0; i < kCopiesN; ++i) {
+        Copy16(b_base, min(8 * (wave + kWaves * i) + lane / 8, last_n) * row_bytes + at, to_n + 1024 * kWaves * i);
+      }
+#pragma unroll
+      for (int i = 0; i < kCopiesT; ++i) {
+        Copy16(u_base, min(8 * (wave + kWaves * i) + lane / 8, last_t) * row_bytes + at, to_t + 1024 * kWaves * i);
+      }
+    };
+    Place next{}, now{};
+    enter(next);
+    now = next;
+    uint32_t step = 0;
+#pragma unroll 1
+    for (uint32_t i = 0; i + 1 < kStages && next.run < runs; ++i, advance(next)) copy_low(next, i);
+#pragma unroll 1
+    for (; now.run < runs; advance(now), ++step) {
+      WaitStep<0>();
+      if (next.run < runs) {
+        copy_low(next, (step + kStages - 1) % kStages);
+        advance(next);
+      }
+      const unsigned char* from = lds + (step % kStages) * kStage;
+      const auto lo = static_cast<uint32_t>(run_start[now.run]), hi = static_cast<uint32_t>(run_start[now.run + 1]);
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const uint32_t row = wt + 32 * t + lane % 32;
+        const bool mine = row >= lo && row < hi;
+        if (__ballot(mine) == 0) continue;
+        f32x16_t d[kN];
+#pragma unroll
+        for (int n = 0; n < kN; ++n) d[n] = f32x16_t{};
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const auto left = static_cast<int32_t>(now.bytes / sizeof(Low)) -
+                            static_cast<int32_t>(now.from / sizeof(Low) + kPer * (2 * p + lane / 32));
+          const u32x4_t fu =
+              First<Low>(*reinterpret_cast<const u32x4_t*>(from + at_piece[p] + (kRowsN + wt + 32 * t) * kStepBytes), left);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) {
+            const u32x4_t fb =
+                First<Low>(*reinterpret_cast<const u32x4_t*>(from + at_piece[p] + (wn + 32 * n) * kStepBytes), left);
+            d[n] = Mma32<Low>(fb, fu, d[n]);
+          }
+        }
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) put(n, q, Rescaled(g, xs, out_of(n, q), quad(n, q)));
+          for (int i = 0; i < 16; ++i) acc[n][t][i] += mine ? d[n][i] : 0.0f;
         }
       }
     }
-    // Runs of rows with one adapter among these 32. A few are multiplied run by run, each result kept by its own rows only;
-    // many (one-token sequences) element by element.
-    const int32_t before = __shfl_up(s, 1);
-    uint64_t starts = __ballot(lane < 32 && s >= 0 && (lane == 0 || before != s));
-    if (__popcll(starts) <= kRunsByMatrix) {
-      while (starts != 0) {
-        const int first = __builtin_ctzll(starts);
-        starts &= starts - 1;
-        const int32_t a = __builtin_amdgcn_readlane(s, first);
-        AddRun<Low, kN>(g, min(token, g.tokens - 1), n0 + wn, a, RankOf(g, a), s == a, lane, [&](int n, const f32x16_t& d) {
-          if (s == a) acc[n][t] += d;
-        });
-        // Another run of the same adapter among these rows is done with it.
-        starts &= ~__ballot(s == a);
-      }
-    } else if (s >= 0) {
-      const uint32_t rank = RankOf(g, s);
+    __syncthreads();
+  } else if constexpr (kN * kT == 1) {
+    const uint32_t token = t0 + min(wt + lane % 32, last_t);
+    const int32_t s = slot[wt + lane % 32];
+    const uint32_t rank = RankOf(g, s);
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
+    for (int q = 0; q < 4; ++q) {
+      f32x4_t v = {acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]};
+      AddLowRank<Low>(g, token, n0 + wn + 8 * q + 4 * (lane / 32), max(s, 0), rank, v);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          f32x4_t v = quad(n, q);
-          AddLowRank<Low>(g, token, out_of(n, q), s, rank, v);
-          put(n, q, v);
-        }
+      for (int e = 0; e < 4; ++e) acc[0][0][4 * q + e] = v[e];
+    }
+  }
+
+  // The sums go through LDS by 32 rows, each wavefront in a part of its own, and from there whole 128-byte runs of a row to a
+  // store. bf16 addends of all the rows are requested before the first is used (f32 ones of 32 rows, to save registers).
+  constexpr uint32_t kRowWords = 32 * kN + 4;  // 4 words of padding put 8 neighbouring rows on different banks
+  static_assert(kWaves * 32 * kRowWords * 4 <= kStages * kStage, "the wavefronts' parts fit the stages");
+  constexpr uint32_t kOctets = 4 * kN, kRowsAtOnce = 64 / kOctets, kTurns = 32 / kRowsAtOnce;
+  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kRowWords;
+  const uint32_t out = n0 + wn + 8 * (lane % kOctets);
+  const bool whole = out + 8 <= g.out_dim, part = out < g.out_dim && !whole;
+  u32x4_t early[kT][kTurns];
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
+#pragma unroll
+    for (uint32_t k = 0; k < kTurns; ++k) {
+      const uint32_t row = wt + 32 * t + kRowsAtOnce * k + lane / kOctets;
+      early[t][k] = u32x4_t{0, 0, 0, 0};
+      if (g.addend != nullptr && !g.addend_f32 && whole && slot[row] != kNoRow) {
+        early[t][k] = *reinterpret_cast<const Bf16x8*>(static_cast<const uint16_t*>(g.addend) + (t0 + row) * g.addend_stride + out);
       }
     }
-    if (s == kNoRow) continue;
+  }
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        if (out_of(n, q) < g.out_dim) Store(g, token, out_of(n, q), quad(n, q));
+        *reinterpret_cast<f32x4_t*>(mine + (lane % 32) * kRowWords + 32 * n + 8 * q + 4 * (lane / 32)) =
+            f32x4_t{acc[n][t][4 * q], acc[n][t][4 * q + 1], acc[n][t][4 * q + 2], acc[n][t][4 * q + 3]};
       }
     }
+    WaveSync();
+#pragma unroll
+    for (uint32_t k = 0; k < kTurns; ++k) {
+      const uint32_t row = kRowsAtOnce * k + lane / kOctets;
+      const float* from = mine + row * kRowWords + 8 * (lane % kOctets);
+      const bool live = slot[wt + 32 * t + row] != kNoRow;
+      const uint64_t token = t0 + wt + 32 * t + row;
+      if (whole && live) {
+        f32x4_t lo = *reinterpret_cast<const f32x4_t*>(from), hi = *reinterpret_cast<const f32x4_t*>(from + 4);
+        if (g.addend_f32) {
+          const auto* p = reinterpret_cast<const F32x4*>(static_cast<const float*>(g.addend) + token * g.addend_stride + out);
+          lo += p[0];
+          hi += p[1];
+        } else {
+          const u32x4_t w = early[t][k];
+          lo += f32x4_t{Bf16LoToF32(w[0]), Bf16HiToF32(w[0]), Bf16LoToF32(w[1]), Bf16HiToF32(w[1])};
+          hi += f32x4_t{Bf16LoToF32(w[2]), Bf16HiToF32(w[2]), Bf16LoToF32(w[3]), Bf16HiToF32(w[3])};
+        }
+        if (g.y_f32) {
+          auto* p = reinterpret_cast<F32x4*>(static_cast<float*>(g.y) + token * g.y_stride + out);
+          p[0] = lo;
+          p[1] = hi;
+        } else {
+          *reinterpret_cast<Bf16x8*>(static_cast<uint16_t*>(g.y) + token * g.y_stride + out) =
+              Bf16x8{PackBf16Rne(lo[0], lo[1]), PackBf16Rne(lo[2], lo[3]), PackBf16Rne(hi[0], hi[1]), PackBf16Rne(hi[2], hi[3])};
+        }
+      }
+    }
+    if (part) {  // the last outputs of rows that do not end with a whole eight
+#pragma unroll 1
+      for (uint32_t row = lane / kOctets; row < 32; row += kRowsAtOnce) {
+        const uint64_t token = t0 + wt + 32 * t + row;
+        if (slot[wt + 32 * t + row] == kNoRow) continue;
+#pragma unroll 1
+        for (uint32_t e = 0; e < g.out_dim - out; ++e) {
+          const float add = g.addend != nullptr ? AddendOne(g, token * g.addend_stride + out + e) : 0.0f;
+          StoreOne(g, token * g.y_stride + out + e, mine[row * kRowWords + 8 * (lane % kOctets) + e] + add);
+        }
+      }
+    }
+    WaveSync();
   }
 }
 
@@ -812,8 +970,16 @@ RoostStatus Admit(const RoostAmdGemmLoraParams& p, bool for_run) {
   return gate.status();
 }
 
+// The low-rank rows in f32, then, beside bf16 adapters, in bf16: one rounding under a bf16 output, three parts, which hold all
+// 24 bits, under an f32 one.
+uint64_t LowRankElements(const RoostAmdGemmLoraParams& p) {
+  return p.lora_a.address == nullptr ? 0 : roost::RoundUp(static_cast<uint64_t>(p.tokens) * p.max_rank, 64);
+}
+uint32_t LowRankParts(const RoostAmdGemmLoraParams& p) {
+  return p.x.dtype == ROOST_DTYPE_F32 ? 0 : p.output.dtype == ROOST_DTYPE_F32 ? 3 : 1;
+}
 uint64_t WorkspaceBytes(const RoostAmdGemmLoraParams& p) {
-  return p.lora_a.address == nullptr ? 0 : static_cast<uint64_t>(p.tokens) * p.max_rank * sizeof(float);
+  return LowRankElements(p) * (sizeof(float) + LowRankParts(p) * sizeof(uint16_t));
 }
 
 // ---- Launch --------------------------------------------------------------------------------------------------------------
@@ -906,6 +1072,9 @@ extern "C" ROOST_API RoostStatus roost_amd_gemm_lora_run(RoostContext* ctx, cons
     g.cu = static_cast<const int32_t*>(p.cu_seqlens.address);
     g.addend = p.addend.address, g.y = p.output.address;
     g.u = ws != nullptr ? static_cast<float*>(ws->device) : nullptr;
+    g.u_part = LowRankElements(p);
+    g.u_bf16 = reinterpret_cast<uint16_t*>(g.u + g.u_part);
+    g.parts = LowRankParts(p);
     g.x_stride = Stride(p.x_stride, p.in_dim), g.addend_stride = Stride(p.addend_stride, p.out_dim);
     g.y_stride = Stride(p.output_stride, p.out_dim);
     g.tokens = p.tokens, g.batch = p.batch, g.in_dim = p.in_dim, g.out_dim = p.out_dim, g.adapters = p.adapters;
