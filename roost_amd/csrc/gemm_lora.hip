@@ -73,39 +73,56 @@ struct LoraArgs {
 constexpr int32_t kNoRow = -2;      // the row belongs to no sequence
 constexpr int32_t kNoAdapter = -1;
 
-// slot[i] for rows t0 .. t0 + n - 1, by the whole workgroup; a barrier must follow. A lane writes a short sequence's rows
-// itself; a long one's are written by its wavefront.
-__device__ __forceinline__ void FillSlots(const LoraArgs& g, uint32_t t0, uint32_t n, int32_t* slot) {
-  constexpr int32_t kShort = 4;
-  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) slot[i] = kNoRow;
-  __syncthreads();
-  const auto rows = static_cast<int32_t>(min(n, g.tokens - t0));
-  for (uint32_t first = threadIdx.x / 64 * 64; first < g.batch; first += blockDim.x) {
-    const uint32_t b = first + threadIdx.x % 64;
-    int32_t lo = 0, hi = 0, s = kNoAdapter;
-    if (b < g.batch) {
-      const auto start = static_cast<int64_t>(t0);
-      lo = static_cast<int32_t>(min(max(g.cu[b] - start, int64_t{0}), int64_t{rows}));
-      hi = static_cast<int32_t>(min(max(g.cu[b + 1] - start, int64_t{0}), int64_t{rows}));
-      if (lo < hi && g.a != nullptr) s = g.slots[b];
-      if (s < 0 || static_cast<uint32_t>(s) >= g.adapters) s = kNoAdapter;
-    }
-    if (hi - lo <= kShort) {
-      for (int32_t t = lo; t < hi; ++t) slot[t] = s;
-    }
-    for (uint64_t left = __ballot(hi - lo > kShort); left != 0; left &= left - 1) {
-      const int l = __builtin_ctzll(left);
-      const int32_t from = __builtin_amdgcn_readlane(lo, l), to = __builtin_amdgcn_readlane(hi, l);
-      const int32_t its = __builtin_amdgcn_readlane(s, l);
-      for (int32_t t = from + static_cast<int32_t>(threadIdx.x % 64); t < to; t += 64) slot[t] = its;
-    }
-  }
-}
-
 __device__ __forceinline__ uint32_t RankOf(const LoraArgs& g, int32_t slot) {
   if (slot < 0) return 0;
   if (g.ranks == nullptr) return g.max_rank;
   return static_cast<uint32_t>(min(max(g.ranks[slot], 0), static_cast<int32_t>(g.max_rank)));
+}
+
+// A sequence's first row, the next one's and its adapter, as stored.
+struct Sequence {
+  int32_t from, to, slot;
+};
+__device__ __forceinline__ Sequence SequenceOf(const LoraArgs& g, uint32_t b) {
+  return Sequence{g.cu[b], g.cu[b + 1], g.a != nullptr ? g.slots[b] : kNoAdapter};
+}
+
+// slot[i] of each lane's sequence's rows, by whole wavefronts (rows t0 .. t0 + n - 1 of the call are slot[0 ..]): a lane writes a short sequence's itself, a long one's are
+// written by its wavefront.
+__device__ __forceinline__ void PutSlots(const LoraArgs& g, Sequence q, uint32_t t0, uint32_t n, int32_t* slot) {
+  constexpr int32_t kShort = 4;
+  const int64_t rows = min(n, g.tokens - t0), start = t0;
+  const auto lo = static_cast<int32_t>(min(max(q.from - start, int64_t{0}), rows));
+  const auto hi = static_cast<int32_t>(min(max(q.to - start, int64_t{0}), rows));
+  const int32_t s = q.slot < 0 || static_cast<uint32_t>(q.slot) >= g.adapters ? kNoAdapter : q.slot;
+  if (hi - lo <= kShort) {
+    for (int32_t t = lo; t < hi; ++t) slot[t] = s;
+  }
+  for (uint64_t left = __ballot(hi - lo > kShort); left != 0; left &= left - 1) {
+    const int l = __builtin_ctzll(left);
+    const int32_t from = __builtin_amdgcn_readlane(lo, l), to = __builtin_amdgcn_readlane(hi, l);
+    const int32_t its = __builtin_amdgcn_readlane(s, l);
+    for (int32_t t = from + static_cast<int32_t>(threadIdx.x % 64); t < to; t += 64) slot[t] = its;
+  }
+}
+
+// slot[i] for rows t0 .. t0 + n - 1, by the whole workgroup, in two halves: the first sequences' loads are issued by
+// BeginSlots, which the caller puts before its own, and used by EndSlots; a barrier must follow that.
+__device__ __forceinline__ Sequence BeginSlots(const LoraArgs& g, uint32_t n, int32_t* slot) {
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) slot[i] = kNoRow;
+  return SequenceOf(g, min(threadIdx.x, g.batch - 1));
+}
+__device__ __forceinline__ void EndSlots(const LoraArgs& g, Sequence first, uint32_t t0, uint32_t n, int32_t* slot) {
+  const Sequence none = {0, 0, kNoAdapter};
+  __syncthreads();
+  PutSlots(g, threadIdx.x < g.batch ? first : none, t0, n, slot);
+  for (uint32_t b = blockDim.x + threadIdx.x / 64 * 64; b < g.batch; b += blockDim.x) {
+    const uint32_t its = b + threadIdx.x % 64;
+    PutSlots(g, its < g.batch ? SequenceOf(g, its) : none, t0, n, slot);
+  }
+}
+__device__ __forceinline__ void FillSlots(const LoraArgs& g, uint32_t t0, uint32_t n, int32_t* slot) {
+  EndSlots(g, BeginSlots(g, n, slot), t0, n, slot);
 }
 
 // ---- Fragments -------------------------------------------------------------------------------------------------------
@@ -183,46 +200,139 @@ __device__ __forceinline__ f32x16_t Mma32(FragOf<E> a, FragOf<E> b, f32x16_t acc
   }
 }
 
-// The piece at byte `at` of a row; with kTail, zero past the row's `bytes` bytes (the load itself then repeats the first).
-template <bool kTail>
-__device__ __forceinline__ u32x4_t Piece(const void* row, uint32_t at, uint32_t bytes) {
-  const bool inside = !kTail || at < bytes;
-  const u32x4_t v = *reinterpret_cast<const u32x4_t*>(static_cast<const unsigned char*>(row) + (inside ? at : 0));
-  return inside ? v : u32x4_t{0, 0, 0, 0};
+// ---- Copies to LDS -------------------------------------------------------------------------------------------------------
+//
+// Rows are brought in by 128 bytes of the inner dimension, eight rows an instruction, each row's eight pieces from eight
+// neighbouring lanes. Loading the fragments themselves, 16 rows at a time with neighbouring lanes in different rows, costs one
+// address cycle a lane instead of one for each four: 30 us instead of 15 for a decode product of 64 x 6,144 over 4,096.
+
+constexpr uint32_t kStepBytes = 128;
+
+// 16 bytes a lane from memory to LDS: lane l's land at lds + 16 l. No register is written; the caller waits.
+__device__ __forceinline__ void Copy16(const void* base, uint32_t off, uint32_t lds) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(off), "s"(base), "s"(lds) : "memory");
+}
+
+__device__ __forceinline__ uint32_t LdsAddress(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const unsigned char*)p));
+}
+
+// A wavefront's own rows on their way through LDS: kA rows from one base and kB from another, kStages steps at a time. The first
+// rows' steps are kSub times as long as the others' and stand as kSub rows each: first all the rows' first 128 bytes, then
+// their second. Piece p of row r lies at p ^ (r % 8), so that the 16 rows of a fragment at one piece are free of bank conflicts; the copy writes LDS in
+// lane order, so it is the lanes' source addresses that are permuted. Nothing but this wavefront waits for it.
+template <int kA, int kB, int kSub, int kStages>
+struct RowStream {
+  static_assert(kA % (8 * kSub) == 0 && kB % 8 == 0, "eight rows an instruction");
+  static constexpr int kCopies = (kA + kB) / 8;
+  static constexpr uint32_t kStage = (kA + kB) * kStepBytes, kBytes = kStages * kStage;
+
+  const unsigned char *base_a, *base_b;  // the same in every lane
+  uint32_t off_a[kA / 8], off_b[kB / 8];  // of this lane's rows 8 i + lane / 8, from their base
+  unsigned char* lds;                     // kBytes
+  uint32_t bytes;                         // of a row
+  uint32_t piece;                         // this lane's, in its rows
+
+  __device__ __forceinline__ void Copy(uint32_t at, uint32_t stage) const {
+    unsigned char* to = lds + stage * kStage;
+    const uint32_t to_lds = LdsAddress(to);
+    if (at + kStepBytes <= bytes) {
+#pragma unroll
+      for (int i = 0; i < kA / 8; ++i) Copy16(base_a + at * kSub, off_a[i], to_lds + 1024 * i);
+#pragma unroll
+      for (int i = 0; i < kB / 8; ++i) Copy16(base_b + at, off_b[i], to_lds + 128 * kA + 1024 * i);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {  // the last, partial step: pieces past the rows' end are zeros
+      const bool a = i < kA / 8;
+      const uint32_t half = a ? 8 * i / (kA / kSub) : 0;
+      if (a ? at * kSub + half * kStepBytes + piece < bytes * kSub : at + piece < bytes) {
+        if (a) {
+          Copy16(base_a + at * kSub, off_a[a ? i : 0], to_lds + 1024 * i);
+        } else {
+          Copy16(base_b + at, off_b[a ? 0 : i - kA / 8], to_lds + 1024 * i);
+        }
+      } else {
+        *reinterpret_cast<u32x4_t*>(to + 1024 * i + 16 * (threadIdx.x % 64)) = u32x4_t{0, 0, 0, 0};
+      }
+    }
+  }
+
+  // use(stage) for the steps first, first + stride, .. (in bytes) of the rows; it is to have read what it needs of the stage
+  // into registers when it returns.
+  template <typename U>
+  __device__ __forceinline__ void Run(uint32_t first, uint32_t stride, U&& use) const {
+    const uint32_t steps = first < bytes ? (bytes - first + stride - 1) / stride : 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kStages; ++i) {
+      if (i < steps) Copy(first + i * stride, i);
+    }
+    uint32_t stage = 0;
+#pragma unroll 1
+    for (uint32_t i = 0; i < steps; ++i) {
+      if (i + kStages <= steps) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 1) * kCopies) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      }
+      use(lds + stage * kStage, [&] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + kStages < steps) Copy(first + (i + kStages) * stride, stage);
+      });
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+  }
+};
+
+// The piece of a row in a stage.
+__device__ __forceinline__ u32x4_t StagePiece(const unsigned char* stage, uint32_t row, uint32_t piece) {
+  return *reinterpret_cast<const u32x4_t*>(stage + row * kStepBytes + 16 * (piece ^ (row % 8)));
 }
 
 // ---- The low-rank rows -------------------------------------------------------------------------------------------------
 
 // Workgroup (i, j, z): rows 16 kT i .. + 16 kT - 1, ranks 16 kR j .. + 16 kR - 1, every gridDim.z-th run of rows with one
-// adapter among them. The wavefronts take alternate 64-byte runs of the adapter's rows and join their sums through LDS.
-template <typename E, int kT, int kR>
-__global__ void __launch_bounds__(512) ShrinkKernel(LoraArgs g) {
+// adapter among them. The wavefronts take alternate steps of the inner dimension and join their sums through LDS. A step is
+// 128 bytes of the rows; e4m3 rows meet twice as many bytes of the adapter's, which stand as two rows each.
+template <typename E, int kT, int kR, int kStages>
+__global__ void __launch_bounds__(256) ShrinkKernel(LoraArgs g) {
   using Low = LowOf<E>;
-  constexpr int kWaves = 8, kRows = 16 * kT;
-  constexpr uint32_t kXBytes = kIsE4m3<E> ? 8 : 16;  // of a row of x beside 16 of the adapter's
+  constexpr int kWaves = 4, kRows = 16 * kT, kSub = sizeof(Low) / sizeof(E);
+  using Stream = RowStream<16 * kR * kSub, kRows, kSub, kStages>;
+  static_assert(kWaves * Stream::kBytes >= kWaves * kT * kR * 64 * sizeof(f32x4_t), "the sums fit where the rows were");
+  __shared__ __align__(16) unsigned char lds[kWaves * Stream::kBytes];
   __shared__ int32_t slot[kRows];
-  __shared__ f32x4_t part[kWaves][kT * kR][64];
   const uint32_t t0 = kRows * blockIdx.x, r0 = 16 * kR * blockIdx.y;
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   FillSlots(g, t0, kRows, slot);
   __syncthreads();
-  const uint32_t bytes = g.in_dim * sizeof(Low);
-  const unsigned char* x[kT];
+  Stream rows;
+  rows.lds = lds + wave * Stream::kBytes;
+  rows.bytes = g.in_dim * sizeof(E);
+  rows.piece = 16 * ((lane % 8) ^ (lane / 8));
+  rows.base_b = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.x) + t0 * g.x_stride);
 #pragma unroll
-  for (int t = 0; t < kT; ++t) {
-    x[t] = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.x) + min(t0 + 16 * t + lane % 16, g.tokens - 1) * g.x_stride);
+  for (int i = 0; i < kRows / 8; ++i) {
+    rows.off_b[i] = min(8 * i + lane / 8, g.tokens - 1 - t0) * static_cast<uint32_t>(g.x_stride * sizeof(E)) + rows.piece;
   }
+  auto* part = reinterpret_cast<f32x4_t(*)[kT * kR][64]>(lds);
   uint32_t run = 0;
   for (uint32_t i = 0, next; i < kRows; i = next) {
-    const int32_t s = slot[i];
+    const int32_t s = __builtin_amdgcn_readfirstlane(slot[i]);
     for (next = i + 1; next < kRows && slot[next] == s; ++next) {}
-    const uint32_t rank = RankOf(g, s);
-    if (r0 >= rank || run++ % gridDim.z != blockIdx.z) continue;
-    const unsigned char* a[kR];
+    if (s < 0 || run++ % gridDim.z != blockIdx.z) continue;  // before its rank is looked up
+    const uint32_t rank = __builtin_amdgcn_readfirstlane(RankOf(g, s));
+    if (r0 >= rank) continue;
+    // Ranks past the adapter's repeat its last; what they give is not stored.
+    rows.base_a = reinterpret_cast<const unsigned char*>(static_cast<const Low*>(g.a) +
+                                                         (static_cast<uint64_t>(s) * g.max_rank + r0) * g.in_dim);
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {  // ranks past the adapter's repeat its last; what they give is not stored
-      a[r] = reinterpret_cast<const unsigned char*>(
-          static_cast<const Low*>(g.a) + (static_cast<uint64_t>(s) * g.max_rank + min(r0 + 16 * r + lane % 16, rank - 1)) * g.in_dim);
+    for (int k = 0; k < 2 * kR * kSub; ++k) {
+      const uint32_t row = 8 * k + lane / 8, of = row % (16 * kR), half = row / (16 * kR);
+      rows.off_a[k] = min(of, rank - 1 - r0) * static_cast<uint32_t>(g.in_dim * sizeof(Low)) + rows.piece + half * kStepBytes;
     }
     f32x4_t acc[kT][kR];
 #pragma unroll
@@ -230,32 +340,37 @@ __global__ void __launch_bounds__(512) ShrinkKernel(LoraArgs g) {
 #pragma unroll
       for (int r = 0; r < kR; ++r) acc[t][r] = f32x4_t{0, 0, 0, 0};
     }
-    const auto step = [&](uint32_t base, auto tail) {
-      constexpr bool kTail = decltype(tail)::value;
-      const uint32_t at = base + 16 * (lane / 16);
-      u32x4_t pa[kR], px[kT];
+    rows.Run(kStepBytes * wave, kStepBytes * kWaves, [&](const unsigned char* stage, auto&& done) {
+      u32x4_t a[2 * kSub][kR], x[2 * kSub][kT];
 #pragma unroll
-      for (int r = 0; r < kR; ++r) pa[r] = Piece<kTail>(a[r], at, bytes);
+      for (int p = 0; p < 2 * kSub; ++p) {
 #pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        if constexpr (kIsE4m3<E>) {
-          const bool inside = !kTail || at < bytes;
-          const u32x2_t q = *reinterpret_cast<const u32x2_t*>(x[t] + (inside ? at / 16 * kXBytes : 0));
-          px[t] = inside ? __builtin_bit_cast(u32x4_t, Bf16OfE4m3(q[0], q[1])) : u32x4_t{0, 0, 0, 0};
-        } else {
-          px[t] = Piece<kTail>(x[t], at, bytes);
+        for (int r = 0; r < kR; ++r) a[p][r] = StagePiece(stage, 16 * kR * (p / 2) + 16 * r + lane % 16, 4 * (p % 2) + lane / 16);
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          const uint32_t row = 16 * t + lane % 16;
+          if constexpr (kSub == 1) {
+            x[p][t] = StagePiece(stage, 16 * kR + row, 4 * p + lane / 16);
+          } else {
+            const uint32_t eighth = 4 * p + lane / 16;  // 8 bytes of the row's 128
+            const auto* from = stage + (16 * kR * kSub + row) * kStepBytes + 16 * ((eighth / 2) ^ (row % 8)) + 8 * (eighth % 2);
+            const u32x2_t q = *reinterpret_cast<const u32x2_t*>(from);
+            x[p][t] = u32x4_t{q[0], q[1], 0, 0};
+          }
         }
       }
+      done();
 #pragma unroll
-      for (int t = 0; t < kT; ++t) {
+      for (int p = 0; p < 2 * kSub; ++p) {
 #pragma unroll
-        for (int r = 0; r < kR; ++r) acc[t][r] = Mma16<Low>(pa[r], px[t], acc[t][r]);
+        for (int t = 0; t < kT; ++t) {
+          const u32x4_t px = kSub == 1 ? x[p][t] : __builtin_bit_cast(u32x4_t, Bf16OfE4m3(x[p][t][0], x[p][t][1]));
+#pragma unroll
+          for (int r = 0; r < kR; ++r) acc[t][r] = Mma16<Low>(a[p][r], px, acc[t][r]);
+        }
       }
-    };
-    const uint32_t full = bytes / 64 * 64;
-    uint32_t base = 64 * wave;
-    for (; base < full; base += 64 * kWaves) step(base, std::false_type{});
-    if (base < bytes) step(base, std::true_type{});
+    });
+    __syncthreads();
 #pragma unroll
     for (int t = 0; t < kT; ++t) {
 #pragma unroll
@@ -320,20 +435,30 @@ __device__ __forceinline__ void AddLowRank(const LoraArgs& g, uint32_t t, uint32
   const Low* row[4];
 #pragma unroll
   for (uint32_t e = 0; e < 4; ++e) row[e] = b + static_cast<uint64_t>(min(n + e, g.out_dim - 1)) * g.max_rank;
-  for (uint32_t r = 0; r < rank; r += kPer) {
-    const auto left = static_cast<int32_t>(rank - r);
-    float ur[kPer];
+  constexpr int kAhead = 2;  // pieces requested together
+#pragma unroll 1
+  for (uint32_t r0 = 0; r0 < rank; r0 += kAhead * kPer) {
+    f32x4_t ur[kAhead][kPer / 4];
+    u32x4_t br[kAhead][4];
 #pragma unroll
-    for (int i = 0; i < kPer / 4; ++i) {
-      const f32x4_t q = *reinterpret_cast<const f32x4_t*>(u + r + 4 * i);
+    for (int k = 0; k < kAhead; ++k) {
+      const uint32_t r = r0 + k * kPer, at = r < rank ? r : 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ur[4 * i + j] = 4 * i + j < left ? q[j] : 0.0f;
+      for (int i = 0; i < kPer / 4; ++i) ur[k][i] = *reinterpret_cast<const f32x4_t*>(u + at + 4 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) br[k][e] = *reinterpret_cast<const u32x4_t*>(row[e] + at);
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const u32x4_t q = First<Low>(*reinterpret_cast<const u32x4_t*>(row[e] + r), left);
+    for (int k = 0; k < kAhead; ++k) {
+      const auto left = static_cast<int32_t>(rank) - static_cast<int32_t>(r0 + k * kPer);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) v[e] = fmaf(ur[i], Element<Low>(q, i), v[e]);
+      for (int i = 0; i < kPer; ++i) ur[k][i / 4][i % 4] = i < left ? ur[k][i / 4][i % 4] : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const u32x4_t q = First<Low>(br[k][e], left);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[e] = fmaf(ur[k][i / 4][i % 4], Element<Low>(q, i), v[e]);
+      }
     }
   }
 }
@@ -386,19 +511,90 @@ __device__ __forceinline__ f32x4_t Rescaled(const LoraArgs& g, float x_scale, ui
   return v;
 }
 
-// ---- The product, straight from memory -----------------------------------------------------------------------------------
+// ---- The product of few rows ---------------------------------------------------------------------------------------------
 
-// Workgroup (i, j): outputs 16 kN i .. + 16 kN - 1 of rows 16 kT j .. + 16 kT - 1. The wavefronts take alternate 256-byte runs
-// of the inner dimension and join their sums through LDS.
-template <typename E, int kN, int kT>
-__global__ void __launch_bounds__(512) ProductKernel(LoraArgs g) {
-  constexpr int kWaves = 8, kPieces = 4;
+// v += B u for one 16 x 16 tile, lane l holding outputs n + 4 (l / 16) .. + 3 of the row `token` with adapter s (l % 16): the
+// adapters among the 16 rows in turn, kAhead of them requested together, each result kept by its own rows only.
+template <typename Low>
+__device__ __forceinline__ void AddLowRankTile(const LoraArgs& g, uint32_t token, int32_t s, uint32_t n, uint32_t lane, f32x4_t& v) {
+  constexpr int kAhead = 8;
+  constexpr uint32_t kPer = 16 / sizeof(Low);
+  uint64_t left = __ballot(lane < 16 && s >= 0);
+  if (left == 0) return;
+  const uint32_t its_rank = RankOf(g, s);
+  const uint32_t out = min(n + lane % 16, g.out_dim - 1);
+  const float* u = g.u + static_cast<uint64_t>(token) * g.max_rank;
+  while (left != 0) {
+    int32_t slots[kAhead];
+    uint32_t ranks[kAhead];
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int at = left != 0 ? __builtin_ctzll(left) : 0;
+      slots[k] = left != 0 ? __builtin_amdgcn_readlane(s, at) : kNoAdapter;
+      ranks[k] = left != 0 ? __builtin_amdgcn_readlane(its_rank, at) : 0;
+      left &= ~__ballot(s == slots[k]);
+      most = max(most, ranks[k]);
+    }
+    f32x4_t sum[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) sum[k] = f32x4_t{0, 0, 0, 0};
+#pragma unroll 1
+    for (uint32_t r0 = 0; r0 < most; r0 += 4 * kPer) {
+      const uint32_t r = r0 + kPer * (lane / 16);
+      u32x4_t b[kAhead];
+      f32x4_t ur[kPer / 4];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        b[k] = u32x4_t{0, 0, 0, 0};
+        if (r < ranks[k]) {
+          b[k] = *reinterpret_cast<const u32x4_t*>(static_cast<const Low*>(g.b) +
+                                                   (static_cast<uint64_t>(slots[k]) * g.out_dim + out) * g.max_rank + r);
+        }
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < kPer / 4; ++i) {
+        ur[i] = r < its_rank ? *reinterpret_cast<const f32x4_t*>(u + r + 4 * i) : f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) ur[i][j] = r + 4 * i + j < its_rank ? ur[i][j] : 0.0f;
+      }
+      for (uint32_t part = 0; part < (sizeof(Low) == 2 ? g.parts : 1); ++part) {
+        u32x4_t pu;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (sizeof(Low) == 2) {
+            pu[i] = PackBf16Rne(ur[i / 2][2 * i % 4], ur[i / 2][2 * i % 4 + 1]);
+            ur[i / 2][2 * i % 4] -= Bf16LoToF32(pu[i]);
+            ur[i / 2][2 * i % 4 + 1] -= Bf16HiToF32(pu[i]);
+          } else {
+            pu[i] = __float_as_uint(ur[0][i]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const auto rest = static_cast<int32_t>(ranks[k]) - static_cast<int32_t>(r);
+          sum[k] = Mma16<Low>(First<Low>(b[k], rest), pu, sum[k]);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (s >= 0 && s == slots[k]) v += sum[k];
+    }
+  }
+}
+
+// Workgroup (i, j): outputs 16 kN i .. + 16 kN - 1 of rows 16 kT j .. + 16 kT - 1. The wavefronts take alternate steps of the
+// inner dimension and join their sums through LDS.
+template <typename E, int kN, int kT, int kWaves, int kStages>
+__global__ void __launch_bounds__(64 * kWaves) ProductKernel(LoraArgs g) {
+  using Stream = RowStream<16 * kN, 16 * kT, 1, kStages>;
+  static_assert(Stream::kBytes >= kN * kT * 64 * sizeof(f32x4_t), "the sums fit where the rows were");
+  __shared__ __align__(16) unsigned char lds[kWaves * Stream::kBytes];
   __shared__ int32_t slot[16 * kT];
-  __shared__ f32x4_t part[kWaves][kN * kT][64];
   const uint32_t n0 = 16 * kN * blockIdx.x, t0 = 16 * kT * blockIdx.y;
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  FillSlots(g, t0, 16 * kT, slot);
-  const uint32_t bytes = g.in_dim * sizeof(E);
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const Sequence first = BeginSlots(g, 16 * kT, slot);
   f32x4_t acc[kN][kT];
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
@@ -406,58 +602,60 @@ __global__ void __launch_bounds__(512) ProductKernel(LoraArgs g) {
     for (int t = 0; t < kT; ++t) acc[n][t] = f32x4_t{0, 0, 0, 0};
   }
   if (g.w != nullptr) {
-    const E* w[kN];
-    const E* x[kT];
+    Stream rows;
+    rows.lds = lds + wave * Stream::kBytes;
+    rows.bytes = g.in_dim * sizeof(E);
+    rows.piece = 16 * ((lane % 8) ^ (lane / 8));
+    rows.base_a = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.w) + static_cast<uint64_t>(n0) * g.in_dim);
+    rows.base_b = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.x) + t0 * g.x_stride);
+    // Rows past the last output or token repeat the last one; what they give is not stored.
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      w[n] = static_cast<const E*>(g.w) + static_cast<uint64_t>(min(n0 + 16 * n + lane % 16, g.out_dim - 1)) * g.in_dim;
+    for (int i = 0; i < 2 * kN; ++i) rows.off_a[i] = min(8 * i + lane / 8, g.out_dim - 1 - n0) * rows.bytes + rows.piece;
+#pragma unroll
+    for (int i = 0; i < 2 * kT; ++i) {
+      rows.off_b[i] = min(8 * i + lane / 8, g.tokens - 1 - t0) * static_cast<uint32_t>(g.x_stride * sizeof(E)) + rows.piece;
     }
+    rows.Run(kStepBytes * wave, kStepBytes * kWaves, [&](const unsigned char* stage, auto&& done) {
+      u32x4_t w[2][kN], x[2][kT];
 #pragma unroll
-    for (int t = 0; t < kT; ++t) x[t] = static_cast<const E*>(g.x) + min(t0 + 16 * t + lane % 16, g.tokens - 1) * g.x_stride;
-    const auto step = [&](uint32_t base, auto tail) {
-      constexpr bool kTail = decltype(tail)::value;
-      u32x4_t pw[kN][kPieces], px[kT][kPieces];
+      for (int p = 0; p < 2; ++p) {
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p) {
-        const uint32_t at = base + 64 * p + 16 * (lane / 16);
+        for (int n = 0; n < kN; ++n) w[p][n] = StagePiece(stage, 16 * n + lane % 16, 4 * p + lane / 16);
 #pragma unroll
-        for (int n = 0; n < kN; ++n) pw[n][p] = Piece<kTail>(w[n], at, bytes);
-#pragma unroll
-        for (int t = 0; t < kT; ++t) px[t][p] = Piece<kTail>(x[t], at, bytes);
+        for (int t = 0; t < kT; ++t) x[p][t] = StagePiece(stage, 16 * kN + 16 * t + lane % 16, 4 * p + lane / 16);
       }
+      done();
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p) {
+      for (int p = 0; p < 2; ++p) {
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
 #pragma unroll
-          for (int t = 0; t < kT; ++t) acc[n][t] = Mma16<E>(pw[n][p], px[t][p], acc[n][t]);
+          for (int t = 0; t < kT; ++t) acc[n][t] = Mma16<E>(w[p][n], x[p][t], acc[n][t]);
         }
       }
-    };
-    const uint32_t full = bytes / (64 * kPieces) * (64 * kPieces);
-    uint32_t base = 64 * kPieces * wave;
-    for (; base < full; base += 64 * kPieces * kWaves) step(base, std::false_type{});
-    if (base < bytes) step(base, std::true_type{});
+    });
   }
+  EndSlots(g, first, t0, 16 * kT, slot);
+  __syncthreads();
+  auto* part = reinterpret_cast<f32x4_t(*)[kN * kT][64]>(lds);
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
 #pragma unroll
     for (int t = 0; t < kT; ++t) part[wave][n * kT + t][lane] = acc[n][t];
   }
   __syncthreads();
-  for (uint32_t item = threadIdx.x; item < 64 * kN * kT; item += 64 * kWaves) {
-    const uint32_t tile = item / 64, l = item % 64;
-    const uint32_t row = 16 * (tile % kT) + l % 16, n = n0 + 16 * (tile / kT) + 4 * (l / 16);
+#pragma unroll 1
+  for (uint32_t tile = wave; tile < kN * kT; tile += kWaves) {
+    const uint32_t row = 16 * (tile % kT) + lane % 16, n_tile = n0 + 16 * (tile / kT), n = n_tile + 4 * (lane / 16);
     const int32_t s = slot[row];
-    if (s == kNoRow || n >= g.out_dim) continue;
-    f32x4_t v = part[0][tile][l];
+    f32x4_t v = part[0][tile][lane];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) v += part[w][tile][l];
+    for (int w = 1; w < kWaves; ++w) v += part[w][tile][lane];
     if constexpr (kIsE4m3<E>) {
-      if (g.w != nullptr) v = Rescaled(g, g.x_scale[t0 + row], n, v);
+      if (g.w != nullptr) v = Rescaled(g, g.x_scale[min(t0 + row, g.tokens - 1)], n, v);
     }
-    AddLowRank<LowOf<E>>(g, t0 + row, n, s, RankOf(g, s), v);
-    Store(g, t0 + row, n, v);
+    AddLowRankTile<LowOf<E>>(g, min(t0 + row, g.tokens - 1), s, n_tile, lane, v);
+    if (s != kNoRow && n < g.out_dim) Store(g, t0 + row, n, v);
   }
 }
 
@@ -469,14 +667,6 @@ __global__ void __launch_bounds__(512) ProductKernel(LoraArgs g) {
 // p ^ (row / 2 % 8): 32 rows of 128 bytes read at one piece are then free of bank conflicts (with p ^ (row % 8) each read takes half
 // as long again). The copy writes LDS in lane order, so it is the lanes' source addresses that are permuted.
 
-constexpr uint32_t kStepBytes = 128;
-
-// 16 bytes a lane from memory to LDS: lane l's land at lds + 16 l. No register is written; the caller waits (WaitStep).
-__device__ __forceinline__ void Copy16(const void* base, uint32_t off, uint32_t lds) {
-  uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0) : "v"(off), "s"(base), "s"(lds) : "memory");
-}
 // Every copy but this wavefront's last kLeft has landed, its own LDS reads have returned, and then every wavefront's.
 template <int kLeft>
 __device__ __forceinline__ void WaitStep() {
@@ -543,7 +733,7 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
   for (int i = 0; i < kCopiesT; ++i) {
     off_t[i] = min(8 * (wave + kWaves * i) + lane / 8, last_t) * static_cast<uint32_t>(x_bytes) + piece;
   }
-  const auto lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
+  const uint32_t lds0 = LdsAddress(lds);
   const auto zero = [&](uint32_t stage) {  // this lane's pieces of a stage
 #pragma unroll
     for (int i = 0; i < kCopiesN + kCopiesT; ++i) {
@@ -986,21 +1176,27 @@ uint64_t WorkspaceBytes(const RoostAmdGemmLoraParams& p) {
 
 template <typename E, int kT, int kR>
 void LaunchShrink(const LoraArgs& g, hipStream_t stream) {
+  // As many stages as four wavefronts' rows leave room for, up to four.
+  constexpr int kRowBytes = 4 * kStepBytes * (16 * kT + 16 * kR * static_cast<int>(sizeof(LowOf<E>) / sizeof(E)));
+  constexpr int kStages = std::min(4, 150 * 1024 / kRowBytes);
+  static_assert(kStages >= 2, "a step on its way while one is multiplied");
   const uint32_t runs = std::min(std::max(g.batch, 1u), 16u);
   const dim3 grid(roost::CeilDiv(g.tokens, 16 * kT), roost::CeilDiv(g.max_rank, 16 * kR), kT == 1 ? runs : std::min(runs, 2u));
-  hipLaunchKernelGGL((ShrinkKernel<E, kT, kR>), grid, dim3(512), 0, stream, g);
+  hipLaunchKernelGGL((ShrinkKernel<E, kT, kR, kStages>), grid, dim3(256), 0, stream, g);
 }
 template <typename E, int kT>
 void LaunchShrinkOfRows(const LoraArgs& g, hipStream_t stream) {
   if (g.max_rank <= 16) return LaunchShrink<E, kT, 1>(g, stream);
-  if (g.max_rank <= 32) return LaunchShrink<E, kT, 2>(g, stream);
-  return LaunchShrink<E, kT, 4>(g, stream);
+  if constexpr (!kIsE4m3<E>) {
+    if (g.max_rank > 32) return LaunchShrink<E, kT, 4>(g, stream);
+  }
+  return LaunchShrink<E, kT, 2>(g, stream);
 }
 
-template <typename E, int kN, int kT>
+template <typename E, int kN, int kT, int kWaves, int kStages>
 void LaunchProduct(const LoraArgs& g, hipStream_t stream) {
   const dim3 grid(roost::CeilDiv(g.out_dim, 16 * kN), roost::CeilDiv(g.tokens, 16 * kT));
-  hipLaunchKernelGGL((ProductKernel<E, kN, kT>), grid, dim3(512), 0, stream, g);
+  hipLaunchKernelGGL((ProductKernel<E, kN, kT, kWaves, kStages>), grid, dim3(64 * kWaves), 0, stream, g);
 }
 
 template <typename E, int kN, int kT, int kWN, int kWT, int kStages>
@@ -1020,9 +1216,9 @@ void LaunchAll(const LoraArgs& g, hipStream_t stream) {
       LaunchShrinkOfRows<E, 1>(g, stream);
     }
   }
-  if (g.tokens <= 16) return LaunchProduct<E, 1, 1>(g, stream);
-  if (g.tokens <= 32) return LaunchProduct<E, 1, 2>(g, stream);
-  if (g.tokens <= 64) return LaunchProduct<E, 2, 4>(g, stream);
+  if (g.tokens <= 16) return LaunchProduct<E, 1, 1, 8, 2>(g, stream);
+  if (g.tokens <= 32) return LaunchProduct<E, 1, 2, 4, 4>(g, stream);
+  if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 3>(g, stream);
   const uint64_t large = roost::CeilDiv(g.out_dim, 256) * roost::CeilDiv(g.tokens, 256);
   if (large >= 128) return LaunchTiles<E, 2, 4, 4, 2, 2>(g, stream);
   if (roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(g.tokens, 128) >= 128) return LaunchTiles<E, 2, 2, 2, 2, 4>(g, stream);
