@@ -68,6 +68,9 @@ struct LoraArgs {
   uint32_t addend_f32, y_f32;
 };
 
+// This wavefront's LDS writes are visible to its own lanes' reads after it, and no access moves across.
+__device__ __forceinline__ void WaveSync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // ---- Which adapter a row has ---------------------------------------------------------------------------------------
 
 constexpr int32_t kNoRow = -2;      // the row belongs to no sequence
@@ -106,23 +109,19 @@ __device__ __forceinline__ void PutSlots(const LoraArgs& g, Sequence q, uint32_t
   }
 }
 
-// slot[i] for rows t0 .. t0 + n - 1, by the whole workgroup, in two halves: the first sequences' loads are issued by
-// BeginSlots, which the caller puts before its own, and used by EndSlots; a barrier must follow that.
-__device__ __forceinline__ Sequence BeginSlots(const LoraArgs& g, uint32_t n, int32_t* slot) {
-  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) slot[i] = kNoRow;
-  return SequenceOf(g, min(threadIdx.x, g.batch - 1));
-}
-__device__ __forceinline__ void EndSlots(const LoraArgs& g, Sequence first, uint32_t t0, uint32_t n, int32_t* slot) {
+// slot[i] for rows t0 .. t0 + n - 1, by the `count` wavefronts from `first` on; a barrier must follow.
+__device__ __forceinline__ void FillSlotsBy(const LoraArgs& g, uint32_t t0, uint32_t n, uint32_t first, uint32_t count,
+                                            int32_t* slot) {
   const Sequence none = {0, 0, kNoAdapter};
-  __syncthreads();
-  PutSlots(g, threadIdx.x < g.batch ? first : none, t0, n, slot);
-  for (uint32_t b = blockDim.x + threadIdx.x / 64 * 64; b < g.batch; b += blockDim.x) {
+  for (uint32_t b = (threadIdx.x / 64 - first) * 64; b < g.batch; b += 64 * count) {
     const uint32_t its = b + threadIdx.x % 64;
     PutSlots(g, its < g.batch ? SequenceOf(g, its) : none, t0, n, slot);
   }
 }
 __device__ __forceinline__ void FillSlots(const LoraArgs& g, uint32_t t0, uint32_t n, int32_t* slot) {
-  EndSlots(g, BeginSlots(g, n, slot), t0, n, slot);
+  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) slot[i] = kNoRow;
+  __syncthreads();
+  FillSlotsBy(g, t0, n, 0, blockDim.x / 64, slot);
 }
 
 // ---- Fragments -------------------------------------------------------------------------------------------------------
@@ -208,6 +207,14 @@ __device__ __forceinline__ f32x16_t Mma32(FragOf<E> a, FragOf<E> b, f32x16_t acc
 
 constexpr uint32_t kStepBytes = 128;
 
+// An address that is the same in every lane, in scalar registers whatever the compiler can prove of it.
+__device__ __forceinline__ const unsigned char* Uniform(const unsigned char* p) {
+  const auto a = reinterpret_cast<uint64_t>(p);
+  const uint64_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
+  const uint64_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
+  return reinterpret_cast<const unsigned char*>(hi << 32 | (lo & 0xFFFFFFFFu));
+}
+
 // 16 bytes a lane from memory to LDS: lane l's land at lds + 16 l. No register is written; the caller waits.
 __device__ __forceinline__ void Copy16(const void* base, uint32_t off, uint32_t lds) {
   uint32_t m0;
@@ -237,12 +244,13 @@ struct RowStream {
 
   __device__ __forceinline__ void Copy(uint32_t at, uint32_t stage) const {
     unsigned char* to = lds + stage * kStage;
-    const uint32_t to_lds = LdsAddress(to);
+    const uint32_t to_lds = __builtin_amdgcn_readfirstlane(LdsAddress(to));
+    const unsigned char *from_a = Uniform(base_a + at * kSub), *from_b = Uniform(base_b + at);
     if (at + kStepBytes <= bytes) {
 #pragma unroll
-      for (int i = 0; i < kA / 8; ++i) Copy16(base_a + at * kSub, off_a[i], to_lds + 1024 * i);
+      for (int i = 0; i < kA / 8; ++i) Copy16(from_a, off_a[i], to_lds + 1024 * i);
 #pragma unroll
-      for (int i = 0; i < kB / 8; ++i) Copy16(base_b + at, off_b[i], to_lds + 128 * kA + 1024 * i);
+      for (int i = 0; i < kB / 8; ++i) Copy16(from_b, off_b[i], to_lds + 128 * kA + 1024 * i);
       return;
     }
 #pragma unroll
@@ -251,9 +259,9 @@ struct RowStream {
       const uint32_t half = a ? 8 * i / (kA / kSub) : 0;
       if (a ? at * kSub + half * kStepBytes + piece < bytes * kSub : at + piece < bytes) {
         if (a) {
-          Copy16(base_a + at * kSub, off_a[a ? i : 0], to_lds + 1024 * i);
+          Copy16(from_a, off_a[a ? i : 0], to_lds + 1024 * i);
         } else {
-          Copy16(base_b + at, off_b[a ? 0 : i - kA / 8], to_lds + 1024 * i);
+          Copy16(from_b, off_b[a ? 0 : i - kA / 8], to_lds + 1024 * i);
         }
       } else {
         *reinterpret_cast<u32x4_t*>(to + 1024 * i + 16 * (threadIdx.x % 64)) = u32x4_t{0, 0, 0, 0};
@@ -297,10 +305,11 @@ __device__ __forceinline__ u32x4_t StagePiece(const unsigned char* stage, uint32
 // Workgroup (i, j, z): rows 16 kT i .. + 16 kT - 1, ranks 16 kR j .. + 16 kR - 1, every gridDim.z-th run of rows with one
 // adapter among them. The wavefronts take alternate steps of the inner dimension and join their sums through LDS. A step is
 // 128 bytes of the rows; e4m3 rows meet twice as many bytes of the adapter's, which stand as two rows each.
-template <typename E, int kT, int kR, int kStages>
-__global__ void __launch_bounds__(256) ShrinkKernel(LoraArgs g) {
+template <typename E, int kT, int kR, int kWaves, int kStages>
+__global__ void __launch_bounds__(64 * kWaves) ShrinkKernel(LoraArgs g) {
   using Low = LowOf<E>;
-  constexpr int kWaves = 4, kRows = 16 * kT, kSub = sizeof(Low) / sizeof(E);
+  constexpr int kRows = 16 * kT, kSub = sizeof(Low) / sizeof(E);
+  static_assert(kRows <= 64, "a wavefront sees where the adapter changes");
   using Stream = RowStream<16 * kR * kSub, kRows, kSub, kStages>;
   static_assert(kWaves * Stream::kBytes >= kWaves * kT * kR * 64 * sizeof(f32x4_t), "the sums fit where the rows were");
   __shared__ __align__(16) unsigned char lds[kWaves * Stream::kBytes];
@@ -319,11 +328,15 @@ __global__ void __launch_bounds__(256) ShrinkKernel(LoraArgs g) {
     rows.off_b[i] = min(8 * i + lane / 8, g.tokens - 1 - t0) * static_cast<uint32_t>(g.x_stride * sizeof(E)) + rows.piece;
   }
   auto* part = reinterpret_cast<f32x4_t(*)[kT * kR][64]>(lds);
-  uint32_t run = 0;
-  for (uint32_t i = 0, next; i < kRows; i = next) {
-    const int32_t s = __builtin_amdgcn_readfirstlane(slot[i]);
-    for (next = i + 1; next < kRows && slot[next] == s; ++next) {}
-    if (s < 0 || run++ % gridDim.z != blockIdx.z) continue;  // before its rank is looked up
+  const int32_t own = slot[lane % kRows], before = __shfl_up(own, 1);
+  const uint64_t ends = __ballot(lane < kRows && (lane == 0 || own != before)) >> 1;  // bit i - 1: a run starts at row i
+  uint64_t starts = __ballot(lane < kRows && own >= 0 && (lane == 0 || own != before));
+  for (uint32_t run = 0; starts != 0; ++run, starts &= starts - 1) {
+    if (run % gridDim.z != blockIdx.z) continue;
+    const uint32_t i = __builtin_ctzll(starts);
+    const uint64_t later = ends >> i;
+    const uint32_t next = later != 0 ? i + 1 + __builtin_ctzll(later) : kRows;
+    const int32_t s = __builtin_amdgcn_readlane(own, i);
     const uint32_t rank = __builtin_amdgcn_readfirstlane(RankOf(g, s));
     if (r0 >= rank) continue;
     // Ranks past the adapter's repeat its last; what they give is not stored.
@@ -584,24 +597,42 @@ __device__ __forceinline__ void AddLowRankTile(const LoraArgs& g, uint32_t token
   }
 }
 
-// Workgroup (i, j): outputs 16 kN i .. + 16 kN - 1 of rows 16 kT j .. + 16 kT - 1. The wavefronts take alternate steps of the
-// inner dimension and join their sums through LDS.
-template <typename E, int kN, int kT, int kWaves, int kStages>
-__global__ void __launch_bounds__(64 * kWaves) ProductKernel(LoraArgs g) {
+// Workgroup (i, j): outputs 16 kN i .. + 16 kN - 1 of rows 16 kT j .. + 16 kT - 1. kWaves wavefronts take alternate steps of the
+// inner dimension; beside them kLow others find the rows' adapters and compute their outputs, which has as long a chain of
+// loads (sequence, adapter, rank, its rows) as the product but moves little. All join their sums through LDS.
+template <typename E, int kN, int kT, int kWaves, int kLow, int kStages>
+__global__ void __launch_bounds__(64 * (kWaves + kLow)) ProductKernel(LoraArgs g) {
   using Stream = RowStream<16 * kN, 16 * kT, 1, kStages>;
-  static_assert(Stream::kBytes >= kN * kT * 64 * sizeof(f32x4_t), "the sums fit where the rows were");
+  constexpr int kTiles = kN * kT;
+  static_assert(Stream::kBytes >= kTiles * 64 * sizeof(f32x4_t), "the sums fit where the rows were");
   __shared__ __align__(16) unsigned char lds[kWaves * Stream::kBytes];
-  __shared__ int32_t slot[16 * kT];
+  __shared__ f32x4_t low[kTiles][64];
+  __shared__ int32_t slot[kLow][16 * kT];
   const uint32_t n0 = 16 * kN * blockIdx.x, t0 = 16 * kT * blockIdx.y;
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const Sequence first = BeginSlots(g, 16 * kT, slot);
+  // Each wavefront with adapters to compute finds all the rows' by itself, in a table of its own, so that none waits for another.
+  if (wave >= kWaves) {
+    int32_t* mine = slot[wave - kWaves];
+    for (uint32_t i = lane; i < 16 * kT; i += 64) mine[i] = kNoRow;
+    WaveSync();
+    FillSlotsBy(g, t0, 16 * kT, wave, 1, mine);
+    WaveSync();
+  }
   f32x4_t acc[kN][kT];
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
 #pragma unroll
     for (int t = 0; t < kT; ++t) acc[n][t] = f32x4_t{0, 0, 0, 0};
   }
-  if (g.w != nullptr) {
+  if (wave >= kWaves) {
+#pragma unroll 1
+    for (uint32_t tile = wave - kWaves; tile < kTiles; tile += kLow) {
+      const uint32_t row = 16 * (tile % kT) + lane % 16;
+      f32x4_t v = {0, 0, 0, 0};
+      AddLowRankTile<LowOf<E>>(g, min(t0 + row, g.tokens - 1), slot[wave - kWaves][row], n0 + 16 * (tile / kT), lane, v);
+      low[tile][lane] = v;
+    }
+  } else if (g.w != nullptr) {
     Stream rows;
     rows.lds = lds + wave * Stream::kBytes;
     rows.bytes = g.in_dim * sizeof(E);
@@ -635,27 +666,28 @@ __global__ void __launch_bounds__(64 * kWaves) ProductKernel(LoraArgs g) {
       }
     });
   }
-  EndSlots(g, first, t0, 16 * kT, slot);
   __syncthreads();
-  auto* part = reinterpret_cast<f32x4_t(*)[kN * kT][64]>(lds);
+  auto* part = reinterpret_cast<f32x4_t(*)[kTiles][64]>(lds);
+  if (wave < kWaves) {
 #pragma unroll
-  for (int n = 0; n < kN; ++n) {
+    for (int n = 0; n < kN; ++n) {
 #pragma unroll
-    for (int t = 0; t < kT; ++t) part[wave][n * kT + t][lane] = acc[n][t];
+      for (int t = 0; t < kT; ++t) part[wave][n * kT + t][lane] = acc[n][t];
+    }
   }
   __syncthreads();
+  // Lane l of a tile holds outputs 4 (l / 16) .. + 3 of row l % 16.
 #pragma unroll 1
-  for (uint32_t tile = wave; tile < kN * kT; tile += kWaves) {
-    const uint32_t row = 16 * (tile % kT) + lane % 16, n_tile = n0 + 16 * (tile / kT), n = n_tile + 4 * (lane / 16);
-    const int32_t s = slot[row];
+  for (uint32_t tile = wave; tile < kTiles; tile += kWaves + kLow) {
+    const uint32_t row = 16 * (tile % kT) + lane % 16, n = n0 + 16 * (tile / kT) + 4 * (lane / 16);
+    if (slot[0][row] == kNoRow || n >= g.out_dim) continue;
     f32x4_t v = part[0][tile][lane];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) v += part[w][tile][lane];
     if constexpr (kIsE4m3<E>) {
-      if (g.w != nullptr) v = Rescaled(g, g.x_scale[min(t0 + row, g.tokens - 1)], n, v);
+      if (g.w != nullptr) v = Rescaled(g, g.x_scale[t0 + row], n, v);
     }
-    AddLowRankTile<LowOf<E>>(g, min(t0 + row, g.tokens - 1), s, n_tile, lane, v);
-    if (s != kNoRow && n < g.out_dim) Store(g, t0 + row, n, v);
+    Store(g, t0 + row, n, v + low[tile][lane]);
   }
 }
 
@@ -672,9 +704,6 @@ template <int kLeft>
 __device__ __forceinline__ void WaitStep() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
-
-// This wavefront's LDS writes are visible to its own lanes' reads after it, and no access moves across.
-__device__ __forceinline__ void WaveSync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // Runs of rows with one adapter that a 32 x 32 tile a wavefront takes step by step; more (one-token sequences) are added element
 // by element.
@@ -1176,13 +1205,14 @@ uint64_t WorkspaceBytes(const RoostAmdGemmLoraParams& p) {
 
 template <typename E, int kT, int kR>
 void LaunchShrink(const LoraArgs& g, hipStream_t stream) {
-  // As many stages as four wavefronts' rows leave room for, up to four.
-  constexpr int kRowBytes = 4 * kStepBytes * (16 * kT + 16 * kR * static_cast<int>(sizeof(LowOf<E>) / sizeof(E)));
-  constexpr int kStages = std::min(4, 150 * 1024 / kRowBytes);
+  // Eight wavefronts where three stages of theirs fit, then as many stages as there is room for, up to four.
+  constexpr int kStepRows = 16 * kT + 16 * kR * static_cast<int>(sizeof(LowOf<E>) / sizeof(E)), kRoom = 150 * 1024;
+  constexpr int kWaves = 8 * 3 * kStepRows * static_cast<int>(kStepBytes) <= kRoom ? 8 : 4;
+  constexpr int kStages = std::min(4, kRoom / (kWaves * kStepRows * static_cast<int>(kStepBytes)));
   static_assert(kStages >= 2, "a step on its way while one is multiplied");
   const uint32_t runs = std::min(std::max(g.batch, 1u), 16u);
   const dim3 grid(roost::CeilDiv(g.tokens, 16 * kT), roost::CeilDiv(g.max_rank, 16 * kR), kT == 1 ? runs : std::min(runs, 2u));
-  hipLaunchKernelGGL((ShrinkKernel<E, kT, kR, kStages>), grid, dim3(256), 0, stream, g);
+  hipLaunchKernelGGL((ShrinkKernel<E, kT, kR, kWaves, kStages>), grid, dim3(64 * kWaves), 0, stream, g);
 }
 template <typename E, int kT>
 void LaunchShrinkOfRows(const LoraArgs& g, hipStream_t stream) {
@@ -1193,10 +1223,10 @@ void LaunchShrinkOfRows(const LoraArgs& g, hipStream_t stream) {
   return LaunchShrink<E, kT, 2>(g, stream);
 }
 
-template <typename E, int kN, int kT, int kWaves, int kStages>
+template <typename E, int kN, int kT, int kWaves, int kLow, int kStages>
 void LaunchProduct(const LoraArgs& g, hipStream_t stream) {
   const dim3 grid(roost::CeilDiv(g.out_dim, 16 * kN), roost::CeilDiv(g.tokens, 16 * kT));
-  hipLaunchKernelGGL((ProductKernel<E, kN, kT, kWaves, kStages>), grid, dim3(64 * kWaves), 0, stream, g);
+  hipLaunchKernelGGL((ProductKernel<E, kN, kT, kWaves, kLow, kStages>), grid, dim3(64 * (kWaves + kLow)), 0, stream, g);
 }
 
 template <typename E, int kN, int kT, int kWN, int kWT, int kStages>
@@ -1216,9 +1246,9 @@ void LaunchAll(const LoraArgs& g, hipStream_t stream) {
       LaunchShrinkOfRows<E, 1>(g, stream);
     }
   }
-  if (g.tokens <= 16) return LaunchProduct<E, 1, 1, 8, 2>(g, stream);
-  if (g.tokens <= 32) return LaunchProduct<E, 1, 2, 4, 4>(g, stream);
-  if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 3>(g, stream);
+  if (g.tokens <= 16) return LaunchProduct<E, 1, 1, 8, 1, 2>(g, stream);
+  if (g.tokens <= 32) return LaunchProduct<E, 1, 2, 4, 2, 4>(g, stream);
+  if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 4, 3>(g, stream);
   const uint64_t large = roost::CeilDiv(g.out_dim, 256) * roost::CeilDiv(g.tokens, 256);
   if (large >= 128) return LaunchTiles<E, 2, 4, 4, 2, 2>(g, stream);
   if (roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(g.tokens, 128) >= 128) return LaunchTiles<E, 2, 2, 2, 2, 4>(g, stream);
