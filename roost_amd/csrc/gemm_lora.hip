@@ -526,73 +526,64 @@ __device__ __forceinline__ f32x4_t Rescaled(const LoraArgs& g, float x_scale, ui
 
 // ---- The product of few rows ---------------------------------------------------------------------------------------------
 
-// v += B u for one 16 x 16 tile, lane l holding outputs n + 4 (l / 16) .. + 3 of the row `token` with adapter s (l % 16): the
-// adapters among the 16 rows in turn, kAhead of them requested together, each result kept by its own rows only.
+// v += B u for one 16 x 16 tile, lane l holding outputs n + 4 (l / 16) .. + 3 of the row `token` with adapter s (l % 16). The rows
+// of all the adapters among the 16 are requested together, before the ranks that say how much of them counts are known; each
+// adapter's product is kept by its own rows only.
 template <typename Low>
 __device__ __forceinline__ void AddLowRankTile(const LoraArgs& g, uint32_t token, int32_t s, uint32_t n, uint32_t lane, f32x4_t& v) {
-  constexpr int kAhead = 8;
   constexpr uint32_t kPer = 16 / sizeof(Low);
-  uint64_t left = __ballot(lane < 16 && s >= 0);
-  if (left == 0) return;
+  if (__ballot(s >= 0) == 0) return;
   const uint32_t its_rank = RankOf(g, s);
+  int32_t at[16];  // a row of the k-th adapter
+  int count = 0;
+  uint64_t left = __ballot(lane < 16 && s >= 0);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    at[k] = left != 0 ? __builtin_ctzll(left) : 0;
+    count += left != 0;
+    left &= ~__ballot(s == __builtin_amdgcn_readlane(s, at[k]));
+  }
   const uint32_t out = min(n + lane % 16, g.out_dim - 1);
   const float* u = g.u + static_cast<uint64_t>(token) * g.max_rank;
-  while (left != 0) {
-    int32_t slots[kAhead];
-    uint32_t ranks[kAhead];
-    uint32_t most = 0;
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int at = left != 0 ? __builtin_ctzll(left) : 0;
-      slots[k] = left != 0 ? __builtin_amdgcn_readlane(s, at) : kNoAdapter;
-      ranks[k] = left != 0 ? __builtin_amdgcn_readlane(its_rank, at) : 0;
-      left &= ~__ballot(s == slots[k]);
-      most = max(most, ranks[k]);
-    }
-    f32x4_t sum[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) sum[k] = f32x4_t{0, 0, 0, 0};
 #pragma unroll 1
-    for (uint32_t r0 = 0; r0 < most; r0 += 4 * kPer) {
-      const uint32_t r = r0 + kPer * (lane / 16);
-      u32x4_t b[kAhead];
-      f32x4_t ur[kPer / 4];
+  for (uint32_t r0 = 0; r0 < g.max_rank; r0 += 4 * kPer) {
+    if (r0 > 0 && __ballot(its_rank > r0) == 0) break;
+    const uint32_t r = r0 + kPer * (lane / 16), from = r < g.max_rank ? r : 0;
+    f32x4_t ur[kPer / 4];
+    u32x4_t b[16];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        b[k] = u32x4_t{0, 0, 0, 0};
-        if (r < ranks[k]) {
-          b[k] = *reinterpret_cast<const u32x4_t*>(static_cast<const Low*>(g.b) +
-                                                   (static_cast<uint64_t>(slots[k]) * g.out_dim + out) * g.max_rank + r);
-        }
-      }
+    for (uint32_t i = 0; i < kPer / 4; ++i) ur[i] = *reinterpret_cast<const f32x4_t*>(u + from + 4 * i);
 #pragma unroll
-      for (uint32_t i = 0; i < kPer / 4; ++i) {
-        ur[i] = r < its_rank ? *reinterpret_cast<const f32x4_t*>(u + r + 4 * i) : f32x4_t{0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) ur[i][j] = r + 4 * i + j < its_rank ? ur[i][j] : 0.0f;
-      }
-      for (uint32_t part = 0; part < (sizeof(Low) == 2 ? g.parts : 1); ++part) {
-        u32x4_t pu;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (sizeof(Low) == 2) {
-            pu[i] = PackBf16Rne(ur[i / 2][2 * i % 4], ur[i / 2][2 * i % 4 + 1]);
-            ur[i / 2][2 * i % 4] -= Bf16LoToF32(pu[i]);
-            ur[i / 2][2 * i % 4 + 1] -= Bf16HiToF32(pu[i]);
-          } else {
-            pu[i] = __float_as_uint(ur[0][i]);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          const auto rest = static_cast<int32_t>(ranks[k]) - static_cast<int32_t>(r);
-          sum[k] = Mma16<Low>(First<Low>(b[k], rest), pu, sum[k]);
-        }
+    for (int k = 0; k < 16; ++k) {
+      if (k < count) {
+        const auto slot = static_cast<uint64_t>(__builtin_amdgcn_readlane(s, at[k]));
+        b[k] = *reinterpret_cast<const u32x4_t*>(static_cast<const Low*>(g.b) + (slot * g.out_dim + out) * g.max_rank + from);
       }
     }
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (s >= 0 && s == slots[k]) v += sum[k];
+    for (uint32_t i = 0; i < kPer; ++i) ur[i / 4][i % 4] = r + i < its_rank ? ur[i / 4][i % 4] : 0.0f;
+    const uint32_t parts = sizeof(Low) == 2 ? g.parts : 1;
+#pragma unroll 1
+    for (uint32_t part = 0; part < parts; ++part) {
+      u32x4_t pu;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(Low) == 2) {
+          pu[i] = PackBf16Rne(ur[i / 2][2 * i % 4], ur[i / 2][2 * i % 4 + 1]);
+          ur[i / 2][2 * i % 4] -= Bf16LoToF32(pu[i]);
+          ur[i / 2][2 * i % 4 + 1] -= Bf16HiToF32(pu[i]);
+        } else {
+          pu[i] = __float_as_uint(ur[0][i]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        if (k < count) {
+          const auto rest = static_cast<int32_t>(__builtin_amdgcn_readlane(its_rank, at[k])) - static_cast<int32_t>(r);
+          const f32x4_t d = Mma16<Low>(First<Low>(b[k], rest), pu, f32x4_t{0, 0, 0, 0});
+          if (s == static_cast<int32_t>(__builtin_amdgcn_readlane(s, at[k]))) v += d;
+        }
+      }
     }
   }
 }
@@ -1248,7 +1239,7 @@ void LaunchAll(const LoraArgs& g, hipStream_t stream) {
   }
   if (g.tokens <= 16) return LaunchProduct<E, 1, 1, 8, 1, 2>(g, stream);
   if (g.tokens <= 32) return LaunchProduct<E, 1, 2, 4, 2, 4>(g, stream);
-  if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 4, 3>(g, stream);
+  if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
   const uint64_t large = roost::CeilDiv(g.out_dim, 256) * roost::CeilDiv(g.tokens, 256);
   if (large >= 128) return LaunchTiles<E, 2, 4, 4, 2, 2>(g, stream);
   if (roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(g.tokens, 128) >= 128) return LaunchTiles<E, 2, 2, 2, 2, 4>(g, stream);
