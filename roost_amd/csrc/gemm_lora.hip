@@ -302,116 +302,151 @@ __device__ __forceinline__ u32x4_t StagePiece(const unsigned char* stage, uint32
 
 // ---- The low-rank rows -------------------------------------------------------------------------------------------------
 
-// Workgroup (i, j, z): rows 16 kT i .. + 16 kT - 1, ranks 16 kR j .. + 16 kR - 1, every gridDim.z-th run of rows with one
-// adapter among them. The wavefronts take alternate steps of the inner dimension and join their sums through LDS. A step is
-// 128 bytes of the rows; e4m3 rows meet twice as many bytes of the adapter's, which stand as two rows each.
+// Rows [from, to) of the sequence with adapter `slot`.
+struct RowRange {
+  uint32_t from, to;
+  int32_t slot;
+};
+
+// The `at`-th piece of the batch, where every sequence is cut at the multiples of kRows: at most tokens / kRows + batch of them.
+// By the whole workgroup, a lane a sequence: the pieces before each are a prefix sum over the workgroup. Empty past the last.
+template <int kRows>
+__device__ __forceinline__ RowRange PieceOf(const LoraArgs& g, uint32_t at) {
+  __shared__ uint32_t sums[16];
+  __shared__ RowRange found;
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+  if (threadIdx.x == 0) found = RowRange{0, 0, kNoAdapter};
+  uint32_t before = 0;
+  for (uint32_t first = 0; first < g.batch; first += blockDim.x) {
+    const uint32_t b = first + threadIdx.x;
+    const Sequence q = SequenceOf(g, min(b, g.batch - 1));
+    const auto most = static_cast<int32_t>(g.tokens);
+    const auto lo = static_cast<uint32_t>(min(max(q.from, 0), most)), hi = static_cast<uint32_t>(min(max(q.to, 0), most));
+    const uint32_t pieces = b < g.batch && hi > lo ? (hi - 1) / kRows - lo / kRows + 1 : 0;
+    uint32_t sum = pieces;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t other = __shfl_up(sum, d);
+      if (lane >= static_cast<uint32_t>(d)) sum += other;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = sum;
+    __syncthreads();
+    uint32_t start = before + sum - pieces;
+    for (uint32_t w = 0; w < waves; ++w) {
+      if (w < wave) start += sums[w];
+      before += sums[w];
+    }
+    if (at >= start && at < start + pieces) {
+      const uint32_t block = lo / kRows + (at - start);
+      found = RowRange{max(lo, block * kRows), min(hi, (block + 1) * kRows), q.slot};
+    }
+    if (at < before) break;
+  }
+  __syncthreads();
+  RowRange r = found;
+  if (r.slot < 0 || static_cast<uint32_t>(r.slot) >= g.adapters) r.slot = kNoAdapter;
+  return r;
+}
+
+// Workgroup (i, j): the i-th piece of the batch (rows of one sequence within kRows = 16 kT), ranks 16 kR j .. + 16 kR - 1. The
+// wavefronts take alternate steps of the inner dimension and join their sums through LDS. A step is 128 bytes of the rows;
+// e4m3 rows meet twice as many bytes of the adapter's, which stand as two rows each.
 template <typename E, int kT, int kR, int kWaves, int kStages>
 __global__ void __launch_bounds__(64 * kWaves) ShrinkKernel(LoraArgs g) {
   using Low = LowOf<E>;
   constexpr int kRows = 16 * kT, kSub = sizeof(Low) / sizeof(E);
-  static_assert(kRows <= 64, "a wavefront sees where the adapter changes");
   using Stream = RowStream<16 * kR * kSub, kRows, kSub, kStages>;
   static_assert(kWaves * Stream::kBytes >= kWaves * kT * kR * 64 * sizeof(f32x4_t), "the sums fit where the rows were");
   __shared__ __align__(16) unsigned char lds[kWaves * Stream::kBytes];
-  __shared__ int32_t slot[kRows];
-  const uint32_t t0 = kRows * blockIdx.x, r0 = 16 * kR * blockIdx.y;
+  const uint32_t r0 = 16 * kR * blockIdx.y;
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  FillSlots(g, t0, kRows, slot);
-  __syncthreads();
+  const RowRange range = PieceOf<kRows>(g, blockIdx.x);
+  const int32_t s = __builtin_amdgcn_readfirstlane(range.slot);
+  const uint32_t from = __builtin_amdgcn_readfirstlane(range.from), to = __builtin_amdgcn_readfirstlane(range.to);
+  const uint32_t rank = __builtin_amdgcn_readfirstlane(RankOf(g, s));
+  if (from >= to || r0 >= rank) return;
   Stream rows;
   rows.lds = lds + wave * Stream::kBytes;
   rows.bytes = g.in_dim * sizeof(E);
   rows.piece = 16 * ((lane % 8) ^ (lane / 8));
-  rows.base_b = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.x) + t0 * g.x_stride);
+  rows.base_b = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.x) + from * g.x_stride);
+  // Rows past the piece's and ranks past the adapter's repeat the last; what they give is not stored.
 #pragma unroll
   for (int i = 0; i < kRows / 8; ++i) {
-    rows.off_b[i] = min(8 * i + lane / 8, g.tokens - 1 - t0) * static_cast<uint32_t>(g.x_stride * sizeof(E)) + rows.piece;
+    rows.off_b[i] = min(8 * i + lane / 8, to - 1 - from) * static_cast<uint32_t>(g.x_stride * sizeof(E)) + rows.piece;
   }
+  rows.base_a = reinterpret_cast<const unsigned char*>(static_cast<const Low*>(g.a) +
+                                                       (static_cast<uint64_t>(s) * g.max_rank + r0) * g.in_dim);
+#pragma unroll
+  for (int k = 0; k < 2 * kR * kSub; ++k) {
+    const uint32_t row = 8 * k + lane / 8, of = row % (16 * kR), half = row / (16 * kR);
+    rows.off_a[k] = min(of, rank - 1 - r0) * static_cast<uint32_t>(g.in_dim * sizeof(Low)) + rows.piece + half * kStepBytes;
+  }
+  f32x4_t acc[kT][kR];
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
+#pragma unroll
+    for (int r = 0; r < kR; ++r) acc[t][r] = f32x4_t{0, 0, 0, 0};
+  }
+  rows.Run(kStepBytes * wave, kStepBytes * kWaves, [&](const unsigned char* stage, auto&& done) {
+    u32x4_t a[2 * kSub][kR], x[2 * kSub][kT];
+#pragma unroll
+    for (int p = 0; p < 2 * kSub; ++p) {
+#pragma unroll
+      for (int r = 0; r < kR; ++r) a[p][r] = StagePiece(stage, 16 * kR * (p / 2) + 16 * r + lane % 16, 4 * (p % 2) + lane / 16);
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const uint32_t row = 16 * t + lane % 16;
+        if constexpr (kSub == 1) {
+          x[p][t] = StagePiece(stage, 16 * kR + row, 4 * p + lane / 16);
+        } else {
+          const uint32_t eighth = 4 * p + lane / 16;  // 8 bytes of the row's 128
+          const auto* from = stage + (16 * kR * kSub + row) * kStepBytes + 16 * ((eighth / 2) ^ (row % 8)) + 8 * (eighth % 2);
+          const u32x2_t q = *reinterpret_cast<const u32x2_t*>(from);
+          x[p][t] = u32x4_t{q[0], q[1], 0, 0};
+        }
+      }
+    }
+    done();
+#pragma unroll
+    for (int p = 0; p < 2 * kSub; ++p) {
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const u32x4_t px = kSub == 1 ? x[p][t] : __builtin_bit_cast(u32x4_t, Bf16OfE4m3(x[p][t][0], x[p][t][1]));
+#pragma unroll
+        for (int r = 0; r < kR; ++r) acc[t][r] = Mma16<Low>(a[p][r], px, acc[t][r]);
+      }
+    }
+  });
   auto* part = reinterpret_cast<f32x4_t(*)[kT * kR][64]>(lds);
-  const int32_t own = slot[lane % kRows], before = __shfl_up(own, 1);
-  const uint64_t ends = __ballot(lane < kRows && (lane == 0 || own != before)) >> 1;  // bit i - 1: a run starts at row i
-  uint64_t starts = __ballot(lane < kRows && own >= 0 && (lane == 0 || own != before));
-  for (uint32_t run = 0; starts != 0; ++run, starts &= starts - 1) {
-    if (run % gridDim.z != blockIdx.z) continue;
-    const uint32_t i = __builtin_ctzll(starts);
-    const uint64_t later = ends >> i;
-    const uint32_t next = later != 0 ? i + 1 + __builtin_ctzll(later) : kRows;
-    const int32_t s = __builtin_amdgcn_readlane(own, i);
-    const uint32_t rank = __builtin_amdgcn_readfirstlane(RankOf(g, s));
-    if (r0 >= rank) continue;
-    // Ranks past the adapter's repeat its last; what they give is not stored.
-    rows.base_a = reinterpret_cast<const unsigned char*>(static_cast<const Low*>(g.a) +
-                                                         (static_cast<uint64_t>(s) * g.max_rank + r0) * g.in_dim);
+  __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2 * kR * kSub; ++k) {
-      const uint32_t row = 8 * k + lane / 8, of = row % (16 * kR), half = row / (16 * kR);
-      rows.off_a[k] = min(of, rank - 1 - r0) * static_cast<uint32_t>(g.in_dim * sizeof(Low)) + rows.piece + half * kStepBytes;
-    }
-    f32x4_t acc[kT][kR];
+  for (int t = 0; t < kT; ++t) {
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
+    for (int r = 0; r < kR; ++r) part[wave][t * kR + r][lane] = acc[t][r];
+  }
+  __syncthreads();
+  for (uint32_t item = threadIdx.x; item < kT * kR * 64; item += 64 * kWaves) {
+    const uint32_t tile = item / 64, l = item % 64;
+    const uint32_t row = from + 16 * (tile / kR) + l % 16, first = r0 + 16 * (tile % kR) + 4 * (l / 16);
+    if (row >= to || first >= rank) continue;
+    f32x4_t v = part[0][tile][l];
 #pragma unroll
-      for (int r = 0; r < kR; ++r) acc[t][r] = f32x4_t{0, 0, 0, 0};
-    }
-    rows.Run(kStepBytes * wave, kStepBytes * kWaves, [&](const unsigned char* stage, auto&& done) {
-      u32x4_t a[2 * kSub][kR], x[2 * kSub][kT];
-#pragma unroll
-      for (int p = 0; p < 2 * kSub; ++p) {
-#pragma unroll
-        for (int r = 0; r < kR; ++r) a[p][r] = StagePiece(stage, 16 * kR * (p / 2) + 16 * r + lane % 16, 4 * (p % 2) + lane / 16);
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-          const uint32_t row = 16 * t + lane % 16;
-          if constexpr (kSub == 1) {
-            x[p][t] = StagePiece(stage, 16 * kR + row, 4 * p + lane / 16);
-          } else {
-            const uint32_t eighth = 4 * p + lane / 16;  // 8 bytes of the row's 128
-            const auto* from = stage + (16 * kR * kSub + row) * kStepBytes + 16 * ((eighth / 2) ^ (row % 8)) + 8 * (eighth % 2);
-            const u32x2_t q = *reinterpret_cast<const u32x2_t*>(from);
-            x[p][t] = u32x4_t{q[0], q[1], 0, 0};
-          }
-        }
-      }
-      done();
-#pragma unroll
-      for (int p = 0; p < 2 * kSub; ++p) {
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-          const u32x4_t px = kSub == 1 ? x[p][t] : __builtin_bit_cast(u32x4_t, Bf16OfE4m3(x[p][t][0], x[p][t][1]));
-#pragma unroll
-          for (int r = 0; r < kR; ++r) acc[t][r] = Mma16<Low>(a[p][r], px, acc[t][r]);
-        }
-      }
-    });
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < kT; ++t) {
-#pragma unroll
-      for (int r = 0; r < kR; ++r) part[wave][t * kR + r][lane] = acc[t][r];
-    }
-    __syncthreads();
-    for (uint32_t item = threadIdx.x; item < kT * kR * 64; item += 64 * kWaves) {
-      const uint32_t tile = item / 64, l = item % 64;
-      const uint32_t row = 16 * (tile / kR) + l % 16, first = r0 + 16 * (tile % kR) + 4 * (l / 16);
-      if (row < i || row >= next || first >= rank) continue;
-      f32x4_t v = part[0][tile][l];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) v += part[w][tile][l];
-      float scale = g.lora_scale != nullptr ? g.lora_scale[s] : 1.0f;
-      if constexpr (kIsE4m3<E>) scale *= g.x_scale[t0 + row];
-      // max_rank is a multiple of 8: the four are the row's own, those past the adapter's rank unused.
-      const uint64_t at = static_cast<uint64_t>(t0 + row) * g.max_rank + first;
-      v *= scale;
-      *reinterpret_cast<f32x4_t*>(g.u + at) = v;
-      if constexpr (sizeof(Low) == 2) {
-        for (uint32_t p = 0; p < g.parts; ++p) {
-          const u32x2_t w = {PackBf16Rne(v[0], v[1]), PackBf16Rne(v[2], v[3])};
-          *reinterpret_cast<u32x2_t*>(g.u_bf16 + p * g.u_part + at) = w;
-          v -= f32x4_t{Bf16LoToF32(w[0]), Bf16HiToF32(w[0]), Bf16LoToF32(w[1]), Bf16HiToF32(w[1])};
-        }
+    for (int w = 1; w < kWaves; ++w) v += part[w][tile][l];
+    float scale = g.lora_scale != nullptr ? g.lora_scale[s] : 1.0f;
+    if constexpr (kIsE4m3<E>) scale *= g.x_scale[row];
+    // max_rank is a multiple of 8: the four are the row's own, those past the adapter's rank unused.
+    const uint64_t at = static_cast<uint64_t>(row) * g.max_rank + first;
+    v *= scale;
+    *reinterpret_cast<f32x4_t*>(g.u + at) = v;
+    if constexpr (sizeof(Low) == 2) {
+      for (uint32_t p = 0; p < g.parts; ++p) {
+        const u32x2_t w = {PackBf16Rne(v[0], v[1]), PackBf16Rne(v[2], v[3])};
+        *reinterpret_cast<u32x2_t*>(g.u_bf16 + p * g.u_part + at) = w;
+        v -= f32x4_t{Bf16LoToF32(w[0]), Bf16HiToF32(w[0]), Bf16LoToF32(w[1]), Bf16HiToF32(w[1])};
       }
     }
-    __syncthreads();
   }
 }
 
@@ -854,8 +889,11 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
             WaitStep<0>();
           }
           read(lds + ((step + 1) % kStages) * kStage, 0);
-          if (step + kStages < steps) copy(step + kStages);
+          if (step + kStages >= full && step + kStages < steps) copy(step + kStages);
         }
+        // The next stage's copies go out one after each of the last part's products.
+        const bool refill = part + 1 == kParts && step + kStages < full;
+        const uint32_t to = lds0 + (step % kStages) * kStage + 1024 * wave, ahead = (step + kStages) * kStepBytes;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
@@ -865,6 +903,16 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
             sum = Mma32<E>(fn[part / kHalves % 2][n], ft[part % 2][t], sum);
             // Keeps the products of a part between its reads and the next part's.
             if constexpr (kN * kT >= 8) asm volatile("" : "+v"(sum));
+            constexpr int kEach = (kCopies + kN * kHalfT - 1) / (kN * kHalfT);  // copies after each product
+#pragma unroll
+            for (int c = (n * kHalfT + t) * kEach; c < (n * kHalfT + t + 1) * kEach && c < kCopies; ++c) {
+              if (!refill) continue;
+              if (c < kCopiesN) {
+                Copy16(w_base + ahead, off_n[c < kCopiesN ? c : 0], to + 1024 * kWaves * c);
+              } else {
+                Copy16(x_base + ahead, off_t[c < kCopiesN ? 0 : c - kCopiesN], to + 1024 * kWaves * c);
+              }
+            }
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -1201,8 +1249,7 @@ void LaunchShrink(const LoraArgs& g, hipStream_t stream) {
   constexpr int kWaves = 8 * 3 * kStepRows * static_cast<int>(kStepBytes) <= kRoom ? 8 : 4;
   constexpr int kStages = std::min(4, kRoom / (kWaves * kStepRows * static_cast<int>(kStepBytes)));
   static_assert(kStages >= 2, "a step on its way while one is multiplied");
-  const uint32_t runs = std::min(std::max(g.batch, 1u), 16u);
-  const dim3 grid(roost::CeilDiv(g.tokens, 16 * kT), roost::CeilDiv(g.max_rank, 16 * kR), kT == 1 ? runs : std::min(runs, 2u));
+  const dim3 grid(roost::CeilDiv(g.tokens, 16 * kT) + g.batch, roost::CeilDiv(g.max_rank, 16 * kR));
   hipLaunchKernelGGL((ShrinkKernel<E, kT, kR, kWaves, kStages>), grid, dim3(64 * kWaves), 0, stream, g);
 }
 template <typename E, int kT>
