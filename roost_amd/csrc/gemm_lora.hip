@@ -561,12 +561,14 @@ __device__ __forceinline__ f32x4_t Rescaled(const LoraArgs& g, float x_scale, ui
 
 // ---- The product of few rows ---------------------------------------------------------------------------------------------
 
-// v += B u for one 16 x 16 tile, lane l holding outputs n + 4 (l / 16) .. + 3 of the row `token` with adapter s (l % 16). The rows
-// of all the adapters among the 16 are requested together, before the ranks that say how much of them counts are known; each
-// adapter's product is kept by its own rows only.
-template <typename Low>
-__device__ __forceinline__ void AddLowRankTile(const LoraArgs& g, uint32_t token, int32_t s, uint32_t n, uint32_t lane, f32x4_t& v) {
+// v[m] += B u for kM 16 x 16 tiles side by side, lane l holding outputs n + 16 m + 4 (l / 16) .. + 3 of the row `token` with adapter
+// s (l % 16). The rows of the adapters among the 16 are requested sixteen at a time, before the ranks that say how much of them
+// counts are known; each adapter's product is kept by its own rows only.
+template <typename Low, int kM>
+__device__ __forceinline__ void AddLowRankTiles(const LoraArgs& g, uint32_t token, int32_t s, uint32_t n, uint32_t lane,
+                                                f32x4_t (&v)[kM]) {
   constexpr uint32_t kPer = 16 / sizeof(Low);
+  constexpr int kTogether = kM > 2 ? 4 : 16 / kM;
   if (__ballot(s >= 0) == 0) return;
   const uint32_t its_rank = RankOf(g, s);
   int32_t at[16];  // a row of the k-th adapter
@@ -578,86 +580,102 @@ __device__ __forceinline__ void AddLowRankTile(const LoraArgs& g, uint32_t token
     count += left != 0;
     left &= ~__ballot(s == __builtin_amdgcn_readlane(s, at[k]));
   }
-  const uint32_t out = min(n + lane % 16, g.out_dim - 1);
+  uint32_t out[kM];
+#pragma unroll
+  for (int m = 0; m < kM; ++m) out[m] = min(n + 16 * m + lane % 16, g.out_dim - 1);
   const float* u = g.u + static_cast<uint64_t>(token) * g.max_rank;
 #pragma unroll 1
   for (uint32_t r0 = 0; r0 < g.max_rank; r0 += 4 * kPer) {
     if (r0 > 0 && __ballot(its_rank > r0) == 0) break;
     const uint32_t r = r0 + kPer * (lane / 16), from = r < g.max_rank ? r : 0;
-    f32x4_t ur[kPer / 4];
-    u32x4_t b[16];
+    f32x4_t all[kPer / 4];
 #pragma unroll
-    for (uint32_t i = 0; i < kPer / 4; ++i) ur[i] = *reinterpret_cast<const f32x4_t*>(u + from + 4 * i);
+    for (uint32_t i = 0; i < kPer / 4; ++i) all[i] = *reinterpret_cast<const f32x4_t*>(u + from + 4 * i);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      if (k < count) {
-        const auto slot = static_cast<uint64_t>(__builtin_amdgcn_readlane(s, at[k]));
-        b[k] = *reinterpret_cast<const u32x4_t*>(static_cast<const Low*>(g.b) + (slot * g.out_dim + out) * g.max_rank + from);
-      }
-    }
+    for (int k0 = 0; k0 < 16; k0 += kTogether) {
+      if (k0 >= count) break;
+      u32x4_t b[kTogether][kM];
 #pragma unroll
-    for (uint32_t i = 0; i < kPer; ++i) ur[i / 4][i % 4] = r + i < its_rank ? ur[i / 4][i % 4] : 0.0f;
-    const uint32_t parts = sizeof(Low) == 2 ? g.parts : 1;
-#pragma unroll 1
-    for (uint32_t part = 0; part < parts; ++part) {
-      u32x4_t pu;
+      for (int k = 0; k < kTogether; ++k) {
+        if (k0 + k < count) {
+          const auto slot = static_cast<uint64_t>(__builtin_amdgcn_readlane(s, at[k0 + k]));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(Low) == 2) {
-          pu[i] = PackBf16Rne(ur[i / 2][2 * i % 4], ur[i / 2][2 * i % 4 + 1]);
-          ur[i / 2][2 * i % 4] -= Bf16LoToF32(pu[i]);
-          ur[i / 2][2 * i % 4 + 1] -= Bf16HiToF32(pu[i]);
-        } else {
-          pu[i] = __float_as_uint(ur[0][i]);
+          for (int m = 0; m < kM; ++m) {
+            b[k][m] = *reinterpret_cast<const u32x4_t*>(static_cast<const Low*>(g.b) + (slot * g.out_dim + out[m]) * g.max_rank +
+                                                        from);
+          }
         }
       }
+      f32x4_t ur[kPer / 4];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        if (k < count) {
-          const auto rest = static_cast<int32_t>(__builtin_amdgcn_readlane(its_rank, at[k])) - static_cast<int32_t>(r);
-          const f32x4_t d = Mma16<Low>(First<Low>(b[k], rest), pu, f32x4_t{0, 0, 0, 0});
-          if (s == static_cast<int32_t>(__builtin_amdgcn_readlane(s, at[k]))) v += d;
+      for (uint32_t i = 0; i < kPer; ++i) ur[i / 4][i % 4] = r + i < its_rank ? all[i / 4][i % 4] : 0.0f;
+      const uint32_t parts = sizeof(Low) == 2 ? g.parts : 1;
+#pragma unroll 1
+      for (uint32_t part = 0; part < parts; ++part) {
+        u32x4_t pu;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (sizeof(Low) == 2) {
+            pu[i] = PackBf16Rne(ur[i / 2][2 * i % 4], ur[i / 2][2 * i % 4 + 1]);
+            ur[i / 2][2 * i % 4] -= Bf16LoToF32(pu[i]);
+            ur[i / 2][2 * i % 4 + 1] -= Bf16HiToF32(pu[i]);
+          } else {
+            pu[i] = __float_as_uint(ur[0][i]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) {
+          if (k0 + k < count) {
+            const auto rest = static_cast<int32_t>(__builtin_amdgcn_readlane(its_rank, at[k0 + k])) - static_cast<int32_t>(r);
+            const bool its = s == static_cast<int32_t>(__builtin_amdgcn_readlane(s, at[k0 + k]));
+#pragma unroll
+            for (int m = 0; m < kM; ++m) {
+              const f32x4_t d = Mma16<Low>(First<Low>(b[k][m], rest), pu, f32x4_t{0, 0, 0, 0});
+              if (its) v[m] += d;
+            }
+          }
         }
       }
     }
   }
 }
 
-// Workgroup (i, j): outputs 16 kN i .. + 16 kN - 1 of rows 16 kT j .. + 16 kT - 1. kWaves wavefronts take alternate steps of the
+// A workgroup: 16 kN outputs of 16 kT rows. kWaves wavefronts take alternate steps of the
 // inner dimension; beside them kLow others find the rows' adapters and compute their outputs, which has as long a chain of
 // loads (sequence, adapter, rank, its rows) as the product but moves little. All join their sums through LDS.
 template <typename E, int kN, int kT, int kWaves, int kLow, int kStages>
-__global__ void __launch_bounds__(64 * (kWaves + kLow)) ProductKernel(LoraArgs g) {
+__global__ void __launch_bounds__(64 * (kWaves + kLow)) ProductKernel(LoraArgs g, uint32_t n_tiles) {
   using Stream = RowStream<16 * kN, 16 * kT, 1, kStages>;
   constexpr int kTiles = kN * kT;
-  static_assert(Stream::kBytes >= kTiles * 64 * sizeof(f32x4_t), "the sums fit where the rows were");
+  constexpr int kM = kTiles / kLow;  // tiles of outputs by each wavefront with adapters, of 16 rows
+  static_assert(kLow % kT == 0 && kM * kLow == kTiles, "as many for each");
+  static_assert(kWaves * Stream::kBytes >= (kWaves + 1) * kTiles * 64 * sizeof(f32x4_t), "the sums fit where the rows were");
   __shared__ __align__(16) unsigned char lds[kWaves * Stream::kBytes];
-  __shared__ f32x4_t low[kTiles][64];
-  __shared__ int32_t slot[kLow][16 * kT];
-  const uint32_t n0 = 16 * kN * blockIdx.x, t0 = 16 * kT * blockIdx.y;
+  __shared__ int32_t slot[kLow][16];
+  // Workgroups go to the 8 XCDs in turn; each XCD takes one run of the tiles, so that those next to each other in memory are read
+  // through one L2.
+  const uint32_t tiles = gridDim.x, xcd = blockIdx.x % 8;
+  const uint32_t at = xcd * (tiles / 8) + min(xcd, tiles % 8) + blockIdx.x / 8;
+  const uint32_t n0 = 16 * kN * (at % n_tiles), t0 = 16 * kT * (at / n_tiles);
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  // Each wavefront with adapters to compute finds all the rows' by itself, in a table of its own, so that none waits for another.
-  if (wave >= kWaves) {
-    int32_t* mine = slot[wave - kWaves];
-    for (uint32_t i = lane; i < 16 * kT; i += 64) mine[i] = kNoRow;
-    WaveSync();
-    FillSlotsBy(g, t0, 16 * kT, wave, 1, mine);
-    WaveSync();
-  }
   f32x4_t acc[kN][kT];
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
 #pragma unroll
     for (int t = 0; t < kT; ++t) acc[n][t] = f32x4_t{0, 0, 0, 0};
   }
+  f32x4_t low[kM];
+  const uint32_t low_t = (wave - kWaves) % kT, low_n = (wave - kWaves) / kT * kM;
   if (wave >= kWaves) {
-#pragma unroll 1
-    for (uint32_t tile = wave - kWaves; tile < kTiles; tile += kLow) {
-      const uint32_t row = 16 * (tile % kT) + lane % 16;
-      f32x4_t v = {0, 0, 0, 0};
-      AddLowRankTile<LowOf<E>>(g, min(t0 + row, g.tokens - 1), slot[wave - kWaves][row], n0 + 16 * (tile / kT), lane, v);
-      low[tile][lane] = v;
-    }
+    // Each finds its rows' adapters by itself, in a table of its own, so that none waits for another.
+    int32_t* mine = slot[wave - kWaves];
+    if (lane < 16) mine[lane] = kNoRow;
+    WaveSync();
+    FillSlotsBy(g, t0 + 16 * low_t, 16, wave, 1, mine);
+    WaveSync();
+#pragma unroll
+    for (int m = 0; m < kM; ++m) low[m] = f32x4_t{0, 0, 0, 0};
+    AddLowRankTiles<LowOf<E>, kM>(g, min(t0 + 16 * low_t + lane % 16, g.tokens - 1), mine[lane % 16], n0 + 16 * low_n, lane, low);
   } else if (g.w != nullptr) {
     Stream rows;
     rows.lds = lds + wave * Stream::kBytes;
@@ -700,20 +718,23 @@ __global__ void __launch_bounds__(64 * (kWaves + kLow)) ProductKernel(LoraArgs g
 #pragma unroll
       for (int t = 0; t < kT; ++t) part[wave][n * kT + t][lane] = acc[n][t];
     }
+  } else {
+#pragma unroll
+    for (int m = 0; m < kM; ++m) part[kWaves][(low_n + m) * kT + low_t][lane] = low[m];
   }
   __syncthreads();
   // Lane l of a tile holds outputs 4 (l / 16) .. + 3 of row l % 16.
 #pragma unroll 1
   for (uint32_t tile = wave; tile < kTiles; tile += kWaves + kLow) {
     const uint32_t row = 16 * (tile % kT) + lane % 16, n = n0 + 16 * (tile / kT) + 4 * (lane / 16);
-    if (slot[0][row] == kNoRow || n >= g.out_dim) continue;
+    if (slot[tile % kT][lane % 16] == kNoRow || n >= g.out_dim) continue;
     f32x4_t v = part[0][tile][lane];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) v += part[w][tile][lane];
     if constexpr (kIsE4m3<E>) {
       if (g.w != nullptr) v = Rescaled(g, g.x_scale[t0 + row], n, v);
     }
-    Store(g, t0 + row, n, v + low[tile][lane]);
+    Store(g, t0 + row, n, v + part[kWaves][tile][lane]);
   }
 }
 
@@ -941,6 +962,27 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
       }
     }
   }
+  // Below, a lane stores 8 outputs of a row; the addends of whole eights are loaded ahead: before the adapters where there are
+  // registers for it, else after them.
+  constexpr uint32_t kOctets = 4 * kN, kRowsAtOnce = 64 / kOctets, kTurns = 32 / kRowsAtOnce;
+  constexpr bool kEarly = kN * kT <= 4;
+  const uint32_t out = n0 + wn + 8 * (lane % kOctets);
+  const bool whole = out + 8 <= g.out_dim, part = out < g.out_dim && !whole;
+  u32x4_t early[kT][kTurns];
+  const auto load_addends = [&] {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+#pragma unroll
+      for (uint32_t k = 0; k < kTurns; ++k) {
+        const uint32_t row = wt + 32 * t + kRowsAtOnce * k + lane / kOctets;
+        early[t][k] = u32x4_t{0, 0, 0, 0};
+        if (g.addend != nullptr && !g.addend_f32 && whole && slot[row] != kNoRow) {
+          early[t][k] = *reinterpret_cast<const Bf16x8*>(static_cast<const uint16_t*>(g.addend) + (t0 + row) * g.addend_stride + out);
+        }
+      }
+    }
+  };
+  if (kEarly) load_addends();
   const uint32_t runs = __builtin_amdgcn_readfirstlane(g.a != nullptr ? run_count : 0);
   if (kN * kT > 1 || runs <= kRunsBySteps) {
     constexpr int kPer = 16 / sizeof(Low);
@@ -996,10 +1038,16 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
     for (uint32_t i = 0; i + 1 < kStages && next.run < runs; ++i, advance(next)) copy_low(next, i);
 #pragma unroll 1
     for (; now.run < runs; advance(now), ++step) {
-      WaitStep<0>();
-      if (next.run < runs) {
-        copy_low(next, (step + kStages - 1) % kStages);
-        advance(next);
+      if constexpr (kStages == 1) {
+        __syncthreads();  // the step before is read
+        copy_low(now, 0);
+        WaitStep<0>();
+      } else {
+        WaitStep<0>();
+        if (next.run < runs) {
+          copy_low(next, (step + kStages - 1) % kStages);
+          advance(next);
+        }
       }
       const unsigned char* from = lds + (step % kStages) * kStage;
       const auto lo = static_cast<uint32_t>(run_start[now.run]), hi = static_cast<uint32_t>(run_start[now.run + 1]);
@@ -1049,22 +1097,8 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
   // store. bf16 addends of all the rows are requested before the first is used (f32 ones of 32 rows, to save registers).
   constexpr uint32_t kRowWords = 32 * kN + 4;  // 4 words of padding put 8 neighbouring rows on different banks
   static_assert(kWaves * 32 * kRowWords * 4 <= kStages * kStage, "the wavefronts' parts fit the stages");
-  constexpr uint32_t kOctets = 4 * kN, kRowsAtOnce = 64 / kOctets, kTurns = 32 / kRowsAtOnce;
   float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kRowWords;
-  const uint32_t out = n0 + wn + 8 * (lane % kOctets);
-  const bool whole = out + 8 <= g.out_dim, part = out < g.out_dim && !whole;
-  u32x4_t early[kT][kTurns];
-#pragma unroll
-  for (int t = 0; t < kT; ++t) {
-#pragma unroll
-    for (uint32_t k = 0; k < kTurns; ++k) {
-      const uint32_t row = wt + 32 * t + kRowsAtOnce * k + lane / kOctets;
-      early[t][k] = u32x4_t{0, 0, 0, 0};
-      if (g.addend != nullptr && !g.addend_f32 && whole && slot[row] != kNoRow) {
-        early[t][k] = *reinterpret_cast<const Bf16x8*>(static_cast<const uint16_t*>(g.addend) + (t0 + row) * g.addend_stride + out);
-      }
-    }
-  }
+  if (!kEarly) load_addends();
 #pragma unroll
   for (int t = 0; t < kT; ++t) {
 #pragma unroll
@@ -1263,8 +1297,9 @@ void LaunchShrinkOfRows(const LoraArgs& g, hipStream_t stream) {
 
 template <typename E, int kN, int kT, int kWaves, int kLow, int kStages>
 void LaunchProduct(const LoraArgs& g, hipStream_t stream) {
-  const dim3 grid(roost::CeilDiv(g.out_dim, 16 * kN), roost::CeilDiv(g.tokens, 16 * kT));
-  hipLaunchKernelGGL((ProductKernel<E, kN, kT, kWaves, kLow, kStages>), grid, dim3(64 * (kWaves + kLow)), 0, stream, g);
+  const auto n_tiles = static_cast<uint32_t>(roost::CeilDiv(g.out_dim, 16 * kN));
+  const auto grid = static_cast<uint32_t>(n_tiles * roost::CeilDiv(g.tokens, 16 * kT));
+  hipLaunchKernelGGL((ProductKernel<E, kN, kT, kWaves, kLow, kStages>), dim3(grid), dim3(64 * (kWaves + kLow)), 0, stream, g, n_tiles);
 }
 
 template <typename E, int kN, int kT, int kWN, int kWT, int kStages>
@@ -1278,7 +1313,7 @@ void LaunchTiles(const LoraArgs& g, hipStream_t stream) {
 template <typename E>
 void LaunchAll(const LoraArgs& g, hipStream_t stream) {
   if (g.a != nullptr) {
-    if (g.tokens / g.batch >= 64) {
+    if (g.tokens / g.batch >= 64 && g.tokens >= 6144) {
       LaunchShrinkOfRows<E, 4>(g, stream);
     } else {
       LaunchShrinkOfRows<E, 1>(g, stream);
@@ -1286,9 +1321,11 @@ void LaunchAll(const LoraArgs& g, hipStream_t stream) {
   }
   if (g.tokens <= 16) return LaunchProduct<E, 1, 1, 8, 1, 2>(g, stream);
   if (g.tokens <= 32) return LaunchProduct<E, 1, 2, 4, 2, 4>(g, stream);
-  if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
+  if (roost::CeilDiv(g.out_dim, 32) * roost::CeilDiv(g.tokens, 64) <= 256) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
+  if (roost::CeilDiv(g.out_dim, 80) * roost::CeilDiv(g.tokens, 64) <= 256) return LaunchProduct<E, 5, 4, 4, 4, 2>(g, stream);
+  if (g.w == nullptr) return LaunchTiles<E, 1, 2, 2, 1, 1>(g, stream);
   const uint64_t large = roost::CeilDiv(g.out_dim, 256) * roost::CeilDiv(g.tokens, 256);
-  if (large >= 128) return LaunchTiles<E, 2, 4, 4, 2, 2>(g, stream);
+  if (large >= 160) return LaunchTiles<E, 2, 4, 4, 2, 2>(g, stream);
   if (roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(g.tokens, 128) >= 128) return LaunchTiles<E, 2, 2, 2, 2, 4>(g, stream);
   return LaunchTiles<E, 1, 1, 2, 2, 4>(g, stream);
 }
