@@ -422,14 +422,16 @@ bool ScalesClash(const RoostDeviceSpan& scales, uint64_t count, std::initializer
 
 // ---- Launch --------------------------------------------------------------------------------------------------------------
 
-// Vectors a thread holds and threads of a row's workgroup.
+// Vectors a thread holds and threads of a row's workgroup: one vector a thread as long as the row's threads fit a workgroup, for
+// more of a row's wavefronts hide more of each other's waits. Against 2 and 4 a thread: 8,192 rows of 4,096 bf16 onto f32 70.9
+// and 75.9 us, 64 rows of 4,096 to e4m3 4.1 and 5.0 us, 6,007 rows of 5,000 to e4m3 by groups 49 and 58 us (4 a thread).
 struct Shape {
   int per_thread;
   uint32_t threads;
 };
 Shape ShapeOf(uint32_t dim) {
   const uint64_t vectors = roost::CeilDiv(dim, 8);
-  const int v = vectors <= 256 ? 1 : vectors <= 512 ? 2 : 4;
+  const int v = vectors <= kMaxThreads ? 1 : vectors <= 2 * kMaxThreads ? 2 : 4;
   return Shape{v, static_cast<uint32_t>(roost::RoundUp(roost::CeilDiv(vectors, v), 64))};
 }
 
