@@ -349,6 +349,41 @@ __device__ __forceinline__ RowRange PieceOf(const LoraArgs& g, uint32_t at) {
   return r;
 }
 
+// acc += one step of a RowStream's rows: kRows of the input (fewer than 16 kT stand for the others too) times 16 kR of an adapter's.
+template <typename E, int kT, int kR, int kRows, typename Done>
+__device__ __forceinline__ void ShrinkStep(const unsigned char* stage, uint32_t lane, Done&& done, f32x4_t (&acc)[kT][kR]) {
+  using Low = LowOf<E>;
+  constexpr int kSub = sizeof(Low) / sizeof(E);
+  u32x4_t a[2 * kSub][kR], x[2 * kSub][kT];
+#pragma unroll
+  for (int p = 0; p < 2 * kSub; ++p) {
+#pragma unroll
+    for (int r = 0; r < kR; ++r) a[p][r] = StagePiece(stage, 16 * kR * (p / 2) + 16 * r + lane % 16, 4 * (p % 2) + lane / 16);
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const uint32_t row = (16 * t + lane % 16) % kRows;
+      if constexpr (kSub == 1) {
+        x[p][t] = StagePiece(stage, 16 * kR + row, 4 * p + lane / 16);
+      } else {
+        const uint32_t eighth = 4 * p + lane / 16;  // 8 bytes of the row's 128
+        const auto* from = stage + (16 * kR * kSub + row) * kStepBytes + 16 * ((eighth / 2) ^ (row % 8)) + 8 * (eighth % 2);
+        const u32x2_t q = *reinterpret_cast<const u32x2_t*>(from);
+        x[p][t] = u32x4_t{q[0], q[1], 0, 0};
+      }
+    }
+  }
+  done();
+#pragma unroll
+  for (int p = 0; p < 2 * kSub; ++p) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const u32x4_t px = kSub == 1 ? x[p][t] : __builtin_bit_cast(u32x4_t, Bf16OfE4m3(x[p][t][0], x[p][t][1]));
+#pragma unroll
+      for (int r = 0; r < kR; ++r) acc[t][r] = Mma16<Low>(a[p][r], px, acc[t][r]);
+    }
+  }
+}
+
 // Workgroup (i, j): the i-th piece of the batch (rows of one sequence within kRows = 16 kT), ranks 16 kR j .. + 16 kR - 1. The
 // wavefronts take alternate steps of the inner dimension and join their sums through LDS. A step is 128 bytes of the rows;
 // e4m3 rows meet twice as many bytes of the adapter's, which stand as two rows each.
@@ -389,36 +424,8 @@ __global__ void __launch_bounds__(64 * kWaves) ShrinkKernel(LoraArgs g) {
 #pragma unroll
     for (int r = 0; r < kR; ++r) acc[t][r] = f32x4_t{0, 0, 0, 0};
   }
-  rows.Run(kStepBytes * wave, kStepBytes * kWaves, [&](const unsigned char* stage, auto&& done) {
-    u32x4_t a[2 * kSub][kR], x[2 * kSub][kT];
-#pragma unroll
-    for (int p = 0; p < 2 * kSub; ++p) {
-#pragma unroll
-      for (int r = 0; r < kR; ++r) a[p][r] = StagePiece(stage, 16 * kR * (p / 2) + 16 * r + lane % 16, 4 * (p % 2) + lane / 16);
-#pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        const uint32_t row = 16 * t + lane % 16;
-        if constexpr (kSub == 1) {
-          x[p][t] = StagePiece(stage, 16 * kR + row, 4 * p + lane / 16);
-        } else {
-          const uint32_t eighth = 4 * p + lane / 16;  // 8 bytes of the row's 128
-          const auto* from = stage + (16 * kR * kSub + row) * kStepBytes + 16 * ((eighth / 2) ^ (row % 8)) + 8 * (eighth % 2);
-          const u32x2_t q = *reinterpret_cast<const u32x2_t*>(from);
-          x[p][t] = u32x4_t{q[0], q[1], 0, 0};
-        }
-      }
-    }
-    done();
-#pragma unroll
-    for (int p = 0; p < 2 * kSub; ++p) {
-#pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        const u32x4_t px = kSub == 1 ? x[p][t] : __builtin_bit_cast(u32x4_t, Bf16OfE4m3(x[p][t][0], x[p][t][1]));
-#pragma unroll
-        for (int r = 0; r < kR; ++r) acc[t][r] = Mma16<Low>(a[p][r], px, acc[t][r]);
-      }
-    }
-  });
+  rows.Run(kStepBytes * wave, kStepBytes * kWaves,
+           [&](const unsigned char* stage, auto&& done) { ShrinkStep<E, kT, kR, kRows>(stage, lane, done, acc); });
   auto* part = reinterpret_cast<f32x4_t(*)[kT * kR][64]>(lds);
   __syncthreads();
 #pragma unroll
@@ -561,6 +568,24 @@ __device__ __forceinline__ f32x4_t Rescaled(const LoraArgs& g, float x_scale, ui
 
 // ---- The product of few rows ---------------------------------------------------------------------------------------------
 
+// A piece of low-rank rows for the adapters' type: fp32 as it is; bf16 rounded to nearest, what that leaves staying in ur for the
+// next part.
+template <typename Low>
+__device__ __forceinline__ u32x4_t NextPart(f32x4_t (&ur)[4 / sizeof(Low)]) {
+  u32x4_t pu;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(Low) == 2) {
+      pu[i] = PackBf16Rne(ur[i / 2][2 * i % 4], ur[i / 2][2 * i % 4 + 1]);
+      ur[i / 2][2 * i % 4] -= Bf16LoToF32(pu[i]);
+      ur[i / 2][2 * i % 4 + 1] -= Bf16HiToF32(pu[i]);
+    } else {
+      pu[i] = __float_as_uint(ur[0][i]);
+    }
+  }
+  return pu;
+}
+
 // v[m] += B u for kM 16 x 16 tiles side by side, lane l holding outputs n + 16 m + 4 (l / 16) .. + 3 of the row `token` with adapter
 // s (l % 16). The rows of the adapters among the 16 are requested sixteen at a time, before the ranks that say how much of them
 // counts are known; each adapter's product is kept by its own rows only.
@@ -612,17 +637,7 @@ __device__ __forceinline__ void AddLowRankTiles(const LoraArgs& g, uint32_t toke
       const uint32_t parts = sizeof(Low) == 2 ? g.parts : 1;
 #pragma unroll 1
       for (uint32_t part = 0; part < parts; ++part) {
-        u32x4_t pu;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (sizeof(Low) == 2) {
-            pu[i] = PackBf16Rne(ur[i / 2][2 * i % 4], ur[i / 2][2 * i % 4 + 1]);
-            ur[i / 2][2 * i % 4] -= Bf16LoToF32(pu[i]);
-            ur[i / 2][2 * i % 4 + 1] -= Bf16HiToF32(pu[i]);
-          } else {
-            pu[i] = __float_as_uint(ur[0][i]);
-          }
-        }
+        const u32x4_t pu = NextPart<Low>(ur);
 #pragma unroll
         for (int k = 0; k < kTogether; ++k) {
           if (k0 + k < count) {
@@ -736,6 +751,150 @@ __global__ void __launch_bounds__(64 * (kWaves + kLow)) ProductKernel(LoraArgs g
     }
     Store(g, t0 + row, n, v + part[kWaves][tile][lane]);
   }
+}
+
+// ---- One or two short sequences -------------------------------------------------------------------------------------------
+//
+// A chat's single token waits for nothing but latency, so its low-rank rows are not a launch of their own: every workgroup computes
+// them all again for its 16 outputs, by wavefronts beside the product's, from rows that the other workgroups read as well. That
+// holds for kFewRows rows and, over all sequences, kFewRanks ranks. Against two launches, one row, rank 16: 1024 to 6144 channels
+// 6.7 and 12.7 us, 4096 to 6144 15.7 and 19.7 us, 4096 to 14336 30.5 and 31.6 us, 14336 to 4096 32.5 and 37.9 us.
+constexpr uint32_t kFewRows = 8, kFewRanks = 16;
+
+template <typename E>
+__global__ void __launch_bounds__(64 * 12) FewRowsKernel(LoraArgs g) {
+  using Low = LowOf<E>;
+  constexpr int kWaves = 8, kSide = 4, kSub = sizeof(Low) / sizeof(E);
+  constexpr uint32_t kPer = 16 / sizeof(Low);
+  using Main = RowStream<16, kFewRows, 1, 2>;
+  using Side = RowStream<16 * kSub, kFewRows, kSub, 2>;
+  __shared__ __align__(16) unsigned char lds[kWaves * Main::kBytes + kSide * Side::kBytes];
+  __shared__ __align__(16) float u[16][kFewRanks];  // [row][rank]
+  const uint32_t tiles = gridDim.x, xcd = blockIdx.x % 8;
+  const uint32_t n0 = 16 * (xcd * (tiles / 8) + min(xcd, tiles % 8) + blockIdx.x / 8);
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t piece = 16 * ((lane % 8) ^ (lane / 8));
+  const uint32_t x_row = min(lane / 8, g.tokens - 1) * static_cast<uint32_t>(g.x_stride * sizeof(E)) + piece;
+  const auto* x = static_cast<const unsigned char*>(g.x);
+
+  // Of the last wavefront, which joins the sums, and requested before the rows that it sums: the sequences' adapters, their rows of
+  // B (of output n0 + lane % 16), and row t's sequence and scales.
+  const uint32_t t = lane % 16;
+  int32_t slot[2] = {kNoAdapter, kNoAdapter}, its = kNoRow;
+  uint32_t rank[2] = {};
+  u32x4_t b[2] = {};
+  float scale = 1.0f, x_scale = 1.0f;
+  f32x4_t acc[1][1] = {{f32x4_t{0, 0, 0, 0}}};
+  if (wave >= kWaves) {
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      if (i < g.batch) slot[i] = g.slots[i];
+      if (slot[i] < 0 || static_cast<uint32_t>(slot[i]) >= g.adapters) slot[i] = kNoAdapter;
+    }
+    Side rows;
+    rows.lds = lds + kWaves * Main::kBytes + (wave - kWaves) * Side::kBytes;
+    rows.bytes = g.in_dim * sizeof(E);
+    rows.piece = piece;
+    rows.base_a = static_cast<const unsigned char*>(g.a);
+    rows.base_b = x;
+    rows.off_b[0] = x_row;
+#pragma unroll
+    for (int k = 0; k < 2 * kSub; ++k) {
+      // Row j: rank j % max_rank of sequence j / max_rank; those of no adapter repeat the first row, and their sums are not kept.
+      const uint32_t row = 8 * k + lane / 8, j = row % 16, half = row / 16, i = j / g.max_rank;
+      const int32_t its = i == 0 ? slot[0] : i == 1 ? slot[1] : kNoAdapter;
+      const uint32_t of = its >= 0 ? static_cast<uint32_t>(its) * g.max_rank + j % g.max_rank : 0;
+      rows.off_a[k] = of * static_cast<uint32_t>(g.in_dim * sizeof(Low)) + piece + half * kStepBytes;
+    }
+    if (wave == kWaves + kSide - 1) {
+      const uint32_t out = min(n0 + lane % 16, g.out_dim - 1), j = kPer * (lane / 16);
+      if constexpr (kIsE4m3<E>) x_scale = g.x_scale[min(t, g.tokens - 1)];
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        rank[i] = RankOf(g, slot[i]);
+        if (i < g.batch && t < g.tokens && static_cast<int32_t>(t) >= g.cu[i] && static_cast<int32_t>(t) < g.cu[i + 1]) {
+          its = i;
+          scale = g.lora_scale != nullptr && slot[i] >= 0 ? g.lora_scale[slot[i]] : 1.0f;
+        }
+        if (slot[i] >= 0 && j < kFewRanks && j / g.max_rank == i) {
+          const uint64_t row = static_cast<uint64_t>(slot[i]) * g.out_dim + out;
+          b[i] = *reinterpret_cast<const u32x4_t*>(static_cast<const Low*>(g.b) + row * g.max_rank + j % g.max_rank);
+        }
+      }
+    }
+    if (slot[0] >= 0 || slot[1] >= 0) {
+      rows.Run(kStepBytes * (wave - kWaves), kStepBytes * kSide,
+               [&](const unsigned char* stage, auto&& done) { ShrinkStep<E, 1, 1, kFewRows>(stage, lane, done, acc); });
+    }
+  } else if (g.w != nullptr) {
+    Main rows;
+    rows.lds = lds + wave * Main::kBytes;
+    rows.bytes = g.in_dim * sizeof(E);
+    rows.piece = piece;
+    rows.base_a = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.w) + static_cast<uint64_t>(n0) * g.in_dim);
+    rows.base_b = x;
+    rows.off_b[0] = x_row;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) rows.off_a[i] = min(8 * i + lane / 8, g.out_dim - 1 - n0) * rows.bytes + piece;
+    rows.Run(kStepBytes * wave, kStepBytes * kWaves, [&](const unsigned char* stage, auto&& done) {
+      u32x4_t w[2], v[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        w[p] = StagePiece(stage, lane % 16, 4 * p + lane / 16);
+        v[p] = StagePiece(stage, 16 + lane % kFewRows, 4 * p + lane / 16);
+      }
+      done();
+#pragma unroll
+      for (int p = 0; p < 2; ++p) acc[0][0] = Mma16<E>(w[p], v[p], acc[0][0]);
+    });
+  }
+  auto* part = reinterpret_cast<f32x4_t(*)[64]>(lds);
+  __syncthreads();
+  part[wave][lane] = acc[0][0];
+  __syncthreads();
+  if (wave != kWaves + kSide - 1) return;
+
+  // Lane l: row t = l % 16, outputs (of the product) or ranks (of the low-rank rows) 4 (l / 16) .. + 3.
+  const uint32_t first = 4 * (lane / 16);
+  f32x4_t low = part[kWaves][lane];
+#pragma unroll
+  for (int i = 1; i < kSide; ++i) low += part[kWaves + i][lane];
+  if constexpr (kIsE4m3<E>) scale *= x_scale;
+  const uint32_t of = first / g.max_rank;  // the sequence of these four ranks
+  const uint32_t its_rank = its == 0 ? rank[0] : its == 1 ? rank[1] : 0;
+#pragma unroll
+  for (uint32_t e = 0; e < 4; ++e) {
+    const bool kept = static_cast<int32_t>(of) == its && first + e - of * g.max_rank < its_rank;
+    u[t][first + e] = kept ? low[e] * scale : 0.0f;
+  }
+  WaveSync();
+  const uint32_t j = kPer * (lane / 16);
+  f32x4_t ur[kPer / 4] = {};
+  if (j < kFewRanks) {
+#pragma unroll
+    for (uint32_t i = 0; i < kPer / 4; ++i) ur[i] = *reinterpret_cast<const f32x4_t*>(&u[t][j + 4 * i]);
+  }
+  f32x4_t v = {0, 0, 0, 0};
+  const uint32_t parts = sizeof(Low) == 2 ? g.parts : 1;
+#pragma unroll 1
+  for (uint32_t p = 0; p < parts; ++p) {
+    const u32x4_t pu = NextPart<Low>(ur);
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      const auto left = static_cast<int32_t>(rank[i] + i * g.max_rank) - static_cast<int32_t>(j);
+      const f32x4_t d = Mma16<Low>(First<Low>(b[i], left), pu, f32x4_t{0, 0, 0, 0});
+      if (its == static_cast<int32_t>(i)) v += d;
+    }
+  }
+  const uint32_t n = n0 + first;
+  if (its == kNoRow || n >= g.out_dim) return;
+  f32x4_t sum = part[0][lane];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) sum += part[w][lane];
+  if constexpr (kIsE4m3<E>) {
+    if (g.w != nullptr) sum = Rescaled(g, x_scale, n, sum);
+  }
+  Store(g, t, n, sum + v);
 }
 
 // ---- The product by tiles ------------------------------------------------------------------------------------------------
@@ -1312,6 +1471,11 @@ void LaunchTiles(const LoraArgs& g, hipStream_t stream) {
 
 template <typename E>
 void LaunchAll(const LoraArgs& g, hipStream_t stream) {
+  const uint64_t a_bytes = static_cast<uint64_t>(g.adapters) * g.max_rank * g.in_dim * sizeof(LowOf<E>);
+  if (g.a != nullptr && g.tokens <= kFewRows && static_cast<uint64_t>(g.batch) * g.max_rank <= kFewRanks && a_bytes < (1ull << 31)) {
+    hipLaunchKernelGGL((FewRowsKernel<E>), dim3(roost::CeilDiv(g.out_dim, 16)), dim3(64 * 12), 0, stream, g);
+    return;
+  }
   if (g.a != nullptr) {
     if (g.tokens / g.batch >= 64 && g.tokens >= 6144) {
       LaunchShrinkOfRows<E, 4>(g, stream);
