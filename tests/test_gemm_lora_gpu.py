@@ -197,3 +197,160 @@ def test_large_offsets(session):
     assert c.weight.numel() * 2 > 1 << 31
     _run(session, c)
     c.check("long offsets")
+
+
+TYPES = [(BF16, BF16), (BF16, F32), (F32, F32), (F8, BF16), (F8, F32)]
+
+
+# Sequences that share one launch with their low-rank rows: up to 8 rows, up to 16 ranks over all sequences; and one row more.
+@pytest.mark.parametrize("x,out", TYPES)
+@pytest.mark.parametrize("lens,max_rank", [([1], 16), ([8], 16), ([9], 16), ([1], 8), ([3, 5], 8), ([0, 4], 8), ([2, 0], 8),
+                                           ([1, 1], 8), ([1], 24), ([2, 2, 2], 8)])
+def test_few_rows(session, lens, max_rank, x, out):
+    for k, (in_dim, out_dim, pad) in enumerate([(1024, 613, 0), (48, 16, 2), (1040, 5, 1)]):
+        pad = min(pad, max(0, 8 - sum(lens)))
+        slots = [(k + 2 * i) % 5 - 1 for i in range(len(lens))]
+        c = Lora(60 + k, lens, slots, in_dim=in_dim, out_dim=out_dim, adapters=4, max_rank=max_rank,
+                 ranks=[max_rank, 3, 0, 1 + max_rank // 2], x=x, out=out, addend=[None, BF16, F32][k], pad=pad,
+                 x_gap=[0, 16, 32][k], y_gap=[0, 1, 3][k])
+        _run(session, c)
+        c.check(f"{lens} rows, inner length {in_dim}")
+
+
+@pytest.mark.parametrize("x", [BF16, F32, F8])
+def test_few_rows_keep_apart(session, x):
+    """Of two sequences in one launch: NaN in one's adapter, rows or past its rank does not reach the other's rows."""
+    out = F32 if x == F32 else BF16
+    c = Lora(70, [3, 2], [1, 2], in_dim=640, out_dim=77, adapters=3, max_rank=8, ranks=[8, 6, 5], x=x, out=out, pad=1)
+    _run(session, c)
+    clean = c.y.clone()
+    c.lora_a[1, 6:] = c.lora_a[2, 5:] = c.lora_a[0] = float("nan")
+    c.lora_b[1, :, 6:] = c.lora_b[2, :, 5:] = c.lora_b[0] = float("inf")
+    _run(session, c)
+    assert torch.equal(c.y, clean)
+    c.lora_a[2, 0] = float("nan")
+    c.lora_b[2, :, 1] = float("-inf")
+    _run(session, c)
+    assert torch.equal(c.y[:3], clean[:3]) and torch.isnan(c.y[3:5]).all()
+    if x != F8:  # rows of NaN
+        c.x[4] = float("nan")
+        c.x[5] = float("nan")
+        _run(session, c)
+        assert torch.equal(c.y[:3], clean[:3]) and torch.equal(c.y[5:], clean[5:])
+
+
+def test_few_rows_replayed(session):
+    c = Lora(71, [1], [2], in_dim=1024, out_dim=640)
+    stream = torch.cuda.Stream()
+    s = roost_amd.OpSession(session.lib, device=0, stream=stream)
+    p = c.params()
+    ws = roost_amd.gemm_lora_workspace(s, p)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        roost_amd.gemm_lora(s, p, ws)
+    for k in range(4):
+        other = Lora(72 + k, [1], [k - 1], in_dim=1024, out_dim=640)
+        for name in ("x", "slots_d", "y"):
+            getattr(c, name).copy_(getattr(other, name))
+        c.slots, c.before = other.slots, c.y.clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(f"replay {k}")
+    s.close()
+
+
+def _lens(tokens, long):
+    """Sequences of one token to `long`, and empty ones."""
+    lens, left, k = [], tokens, 0
+    while left:
+        lens.append(min(left, [1, long, 1, 0, 3, long // 2, 17, 1][k % 8]))
+        left -= lens[-1]
+        k += 1
+    return lens
+
+
+# Rows x outputs that take each of the tilings of many rows, with sequences that start and end inside the tiles.
+@pytest.mark.parametrize("x,out", TYPES)
+@pytest.mark.parametrize("tokens,out_dim,long", [
+    (300, 2100, 90),    # 80 x 64
+    (130, 8300, 1),     # 80 x 64, a sequence a row
+    (300, 5001, 90),    # 64 x 64
+    (1020, 2100, 400),  # 128 x 128
+    (1100, 2100, 2),    # 128 x 128, a sequence a row or two
+    (2601, 4200, 900),  # 256 x 256
+    (2600, 4203, 4),    # 256 x 256, short sequences
+])
+def test_tilings(session, tokens, out_dim, long, x, out):
+    lens = _lens(tokens, long)
+    c = Lora(80, lens, [(5 * i) % 8 - 1 for i in range(len(lens))], in_dim=144, out_dim=out_dim, adapters=7, max_rank=40,
+             ranks=[40, 1, 16, 33, 0, 24, 39], x=x, out=out, pad=7)
+    _run(session, c)
+    c.check(f"{tokens} x {out_dim}")
+
+
+@pytest.mark.parametrize("x", [BF16, F32, F8])
+@pytest.mark.parametrize("tokens,out_dim,long", [(300, 5001, 90), (2600, 1100, 4), (4000, 640, 1500)])
+def test_tilings_of_adapters_alone(session, tokens, out_dim, long, x):
+    lens = _lens(tokens, long)
+    out = F32 if x == F32 else BF16
+    c = Lora(81, lens, [(5 * i) % 8 - 1 for i in range(len(lens))], in_dim=144, out_dim=out_dim, adapters=7, max_rank=128,
+             ranks=[128, 1, 16, 33, 0, 24, 97], x=x, out=out, shared=False, addend=out, pad=3)
+    _run(session, c)
+    c.check(f"{tokens} x {out_dim}")
+
+
+@pytest.mark.parametrize("x,out", TYPES)
+@pytest.mark.parametrize("max_rank", [16, 32, 128])
+def test_low_rank_rows_of_long_prompts(session, max_rank, x, out):
+    """Pieces of 64 rows of one sequence, from sequences that start and end anywhere."""
+    lens = [3001, 1, 0, 62, 2900, 300]
+    c = Lora(82, lens, [0, 1, 2, 3, 1, 2], in_dim=400, out_dim=72, max_rank=max_rank, ranks=[max_rank, max_rank - 1, 3, 9], x=x,
+             out=out, pad=2)
+    _run(session, c)
+    c.check(f"pool rank {max_rank}")
+
+
+@pytest.mark.parametrize("each", [1, 2])
+def test_more_sequences_than_a_workgroup_has_threads(session, each):
+    lens = [each] * 1300
+    lens[5] = lens[700] = 0
+    c = Lora(83, lens, [(3 * i) % 12 - 1 for i in range(1300)], in_dim=128, out_dim=96, adapters=11)
+    _run(session, c)
+    c.check(f"1300 sequences of {each}")
+
+
+@pytest.mark.parametrize("tokens", [6, 30, 300])
+def test_ranks_outside_the_pool(session, tokens):
+    """Ranks below zero count as none, above the pool's as the pool's."""
+    c = Lora(84, [tokens // 3] * 3, [0, 1, 2], in_dim=256, out_dim=100, adapters=3, ranks=[-5, 1 << 30, 7])
+    _run(session, c)
+    c.check("ranks")
+
+
+@pytest.mark.parametrize("lens", [[1], [2] * 20, [1000]])
+def test_two_graphs_that_share_a_workspace(session, lens):
+    """Replayed one after the other on one stream."""
+    cases = [Lora(85 + i, lens, [i + 1] * len(lens), in_dim=512, out_dim=260) for i in range(2)]
+    stream = torch.cuda.Stream()
+    s = roost_amd.OpSession(session.lib, device=0, stream=stream)
+    params = [c.params() for c in cases]
+    ws = roost_amd.gemm_lora_workspace(s, params[0])
+    torch.cuda.synchronize()
+    graphs = []
+    for p in params:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            roost_amd.gemm_lora(s, p, ws)
+    for _ in range(3):
+        for c in cases:
+            c.y.copy_(c.before)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for g in graphs:
+                g.replay()
+        torch.cuda.synchronize()
+        for c in cases:
+            c.check("replayed")
+    s.close()
