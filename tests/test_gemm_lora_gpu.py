@@ -281,6 +281,8 @@ def _lens(tokens, long):
     (1100, 2100, 2),    # 128 x 128, a sequence a row or two
     (2601, 4200, 900),  # 256 x 256
     (2600, 4203, 4),    # 256 x 256, short sequences
+    (4201, 4200, 700),  # 256 x 256 for 3,840 rows, 128 x 128 for the rest
+    (4200, 4203, 5),
 ])
 def test_tilings(session, tokens, out_dim, long, x, out):
     lens = _lens(tokens, long)
