@@ -228,6 +228,7 @@ class OpSession:
         self.stream = stream or torch.cuda.current_stream(self.device)
         self.ctx = self.lib.create_context(device)
         self._ws = {}  # (variant, key) -> [device tensor, pinned tensor, plan buffer, Workspace, event]
+        self._outgrown = []
 
     @property
     def stream_handle(self) -> int:
@@ -244,14 +245,18 @@ class OpSession:
     def _workspace(self, entry: Entry, params, key) -> abi.Workspace:
         return self.workspace_of((entry.variant_id, key), self.workspace_sizes(entry, params))
 
-    def workspace_of(self, key, sizes: abi.WorkspaceSizes) -> list:
-        """The buffers kept under `key`, allocated anew when they do not hold `sizes`."""
+    def workspace_of(self, key, sizes: abi.WorkspaceSizes, keep: bool = False) -> list:
+        """The buffers kept under `key`, allocated anew when they do not hold `sizes`. keep: the old ones stay allocated until
+        close(), for a captured graph may hold their addresses; each new one is at least twice as large."""
         torch = _torch()
         slot = self._ws.get(key)
         fits = slot is not None and slot[3].device_bytes >= sizes.device_bytes and \
             slot[3].pinned_host_bytes >= sizes.pinned_host_bytes and slot[3].plan_bytes >= sizes.plan_bytes
         if not fits:
             self.stream.synchronize()  # in-flight kernels may still read the old buffers
+            if keep and slot is not None:
+                self._outgrown.append(slot)
+                sizes.device_bytes = max(sizes.device_bytes, 2 * slot[3].device_bytes)
             dev = torch.empty(max(int(sizes.device_bytes), 1) + 256, dtype=torch.uint8, device=self.device)
             pinned = torch.empty(max(int(sizes.pinned_host_bytes), 1), dtype=torch.uint8, pin_memory=True)
             plan = C.create_string_buffer(max(int(sizes.plan_bytes), 1))
@@ -303,6 +308,7 @@ class OpSession:
             self.lib.destroy_context(self.ctx)
             self.ctx = None
             self._ws.clear()
+            self._outgrown.clear()
 
 
 # ---- op mirrors (CudaOps) ---------------------------------------------------------------------------------------------
@@ -694,13 +700,14 @@ def silu_mul_quant(session: OpSession, params) -> None:
 
 
 def gemm_lora_workspace(session: OpSession, params, key=0) -> abi.Workspace:
-    """A workspace that roost_amd_gemm_lora_run of these params takes, kept by the session under `key` (grown when it
-    does not fit). Calls on one stream may share it; calls that overlap on the GPU may not."""
+    """A workspace that roost_amd_gemm_lora_run of these params takes, kept by the session under `key`: a larger one when it
+    does not fit, beside which the old one stays valid until close(). Calls on one stream may share it; calls that overlap on
+    the GPU may not."""
     sizes = abi.new(abi.WorkspaceSizes)
     status = session.lib.dll.roost_amd_gemm_lora_workspace(session.ctx, C.addressof(params), C.addressof(sizes))
     if status != abi.OK:
         raise KernelError("gemm_lora workspace", status, session.lib.last_error())
-    return session.workspace_of(("gemm_lora", key), sizes)[3]
+    return session.workspace_of(("gemm_lora", key), sizes, keep=True)[3]
 
 
 def gemm_lora(session: OpSession, params, ws: Optional[abi.Workspace] = None, key=0) -> None:

@@ -1438,9 +1438,11 @@ uint64_t WorkspaceBytes(const RoostAmdGemmLoraParams& p) {
 
 template <typename E, int kT, int kR>
 void LaunchShrink(const LoraArgs& g, hipStream_t stream) {
-  // Eight wavefronts where three stages of theirs fit, then as many stages as there is room for, up to four.
-  constexpr int kStepRows = 16 * kT + 16 * kR * static_cast<int>(sizeof(LowOf<E>) / sizeof(E)), kRoom = 150 * 1024;
-  constexpr int kWaves = 8 * 3 * kStepRows * static_cast<int>(kStepBytes) <= kRoom ? 8 : 4;
+  // One tile: two workgroups share a CU's LDS. Else eight wavefronts where three stages of theirs fit, then as many stages as there
+  // is room for, up to four.
+  constexpr bool kOne = kT == 1 && kR == 1;
+  constexpr int kStepRows = 16 * kT + 16 * kR * static_cast<int>(sizeof(LowOf<E>) / sizeof(E)), kRoom = (kOne ? 75 : 150) * 1024;
+  constexpr int kWaves = 8 * (kOne ? 2 : 3) * kStepRows * static_cast<int>(kStepBytes) <= kRoom ? 8 : 4;
   constexpr int kStages = std::min(4, kRoom / (kWaves * kStepRows * static_cast<int>(kStepBytes)));
   static_assert(kStages >= 2, "a step on its way while one is multiplied");
   const dim3 grid(roost::CeilDiv(g.tokens, 16 * kT) + g.batch, roost::CeilDiv(g.max_rank, 16 * kR));

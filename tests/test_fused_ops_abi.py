@@ -218,3 +218,37 @@ def test_nothing_to_do(kernels, ctx):
         p = _lora()
         setattr(p, name, 0)
         assert _run_lora(kernels, ctx, p) == abi.OK
+
+
+def test_gemm_lora_row_limits(kernels, ctx):
+    """Strides past what a tile's 32-bit offsets reach are refused; neighbouring columns of one tensor are not."""
+    p = _lora()
+    p.x_stride, p.x = (1 << 20) + 8, _span(0x100000, 10 << 21, BF16)
+    assert _run_lora(kernels, ctx, p) == abi.UNSUPPORTED and "x_stride" in kernels.last_error()
+
+
+def test_python_checks():
+    """The mirrors refuse what the C records cannot carry before a record is made."""
+    import torch
+
+    import roost_amd
+
+    t = torch.zeros(4, 16)
+    assert roost_amd._rows(t[:, 2:10], "x", 4, 8)[1] == 16 and roost_amd._rows(t[:1, 2:10], "x", 1, 8)[1] == 8
+    assert roost_amd._rows(t[:0], "x", 0, 16)[0].length == 0 and roost_amd._rows(None, "x", 4, 16)[1] == 0
+    for bad, shape in ((t, (4, 8)), (t[0], (16, 1)), (t.T, (16, 4)), (t[:1].expand(4, 16), (4, 16)), (t[:, ::2], (4, 8))):
+        with pytest.raises(ValueError, match="x: "):
+            roost_amd._rows(bad, "x", *shape)
+    with pytest.raises(ValueError, match="not one of"):
+        roost_amd._rows(t, "up", 4, 16, (torch.bfloat16,))
+    assert roost_amd._flat(t, "w", (4, 16)).length == 64 and not roost_amd._flat(None, "w", (4, 16)).address
+    for bad, shape, dtype in ((t, (16, 4), None), (t[:, :8], (4, 8), None), (t, (4, 16), torch.int32)):
+        with pytest.raises(ValueError, match="w: "):
+            roost_amd._flat(bad, "w", shape, dtype)
+    cu, slots = torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="tensors of one call are on"):
+        roost_amd.gemm_lora_params(t, t, None, None, None, slots, cu, torch.zeros(4, 4))
+    with pytest.raises(ValueError, match="tensors of one call are on"):
+        roost_amd.add_rms_norm_params(t, None, t[0], None, t, eps=1e-6)
+    with pytest.raises(ValueError, match="tensors of one call are on"):
+        roost_amd.silu_mul_quant_params(t, t, t, t[:, :1])

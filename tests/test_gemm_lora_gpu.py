@@ -356,3 +356,38 @@ def test_two_graphs_that_share_a_workspace(session, lens):
         for c in cases:
             c.check("replayed")
     s.close()
+
+
+def test_a_graph_keeps_its_workspace_when_the_session_needs_a_larger_one(session):
+    c = Lora(90, [20, 30], [1, 2], in_dim=512, out_dim=260)
+    big = Lora(91, [2000], [1], in_dim=512, out_dim=64)
+    stream = torch.cuda.Stream()
+    s = roost_amd.OpSession(session.lib, device=0, stream=stream)
+    p, q = c.params(), big.params()
+    first = roost_amd.gemm_lora_workspace(s, p).device
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        roost_amd.gemm_lora(s, p)
+    roost_amd.gemm_lora(s, q)
+    torch.cuda.synchronize()
+    taken = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")  # what a freed workspace's memory would be given to
+    assert roost_amd.gemm_lora_workspace(s, p).device != first
+    assert not any(t.data_ptr() < first + 256 and first < t.data_ptr() + t.numel() for t in (taken, big.y, c.y))
+    for _ in range(2):
+        c.y.copy_(c.before)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check("replayed beside a larger workspace")
+    assert (taken == 0).all()
+    big.check("the larger call")
+    s.close()
+
+
+def test_other_sessions_device_is_refused(session):
+    c = Lora(92, [2], [1], in_dim=64, out_dim=16)
+    p = c.params()
+    p._device = torch.device("cuda", 1)
+    with pytest.raises(ValueError, match="session on"):
+        roost_amd.gemm_lora(session, p)
