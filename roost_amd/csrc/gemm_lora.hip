@@ -1492,10 +1492,17 @@ void LaunchAll(const LoraArgs& g, hipStream_t stream) {
       LaunchShrinkOfRows<E, 1>(g, stream);
     }
   }
-  if (g.tokens <= 16) return LaunchProduct<E, 1, 1, 8, 1, 2>(g, stream);
-  if (g.tokens <= 32) return LaunchProduct<E, 1, 2, 4, 2, 4>(g, stream);
-  if (roost::CeilDiv(g.out_dim, 32) * roost::CeilDiv(g.tokens, 64) <= 256) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
-  if (roost::CeilDiv(g.out_dim, 80) * roost::CeilDiv(g.tokens, 64) <= 256) return LaunchProduct<E, 5, 4, 4, 4, 2>(g, stream);
+  // Few rows: as many workgroups as outputs allow, up to one a CU; a second round costs more than wider tiles. 16 rows of 4096
+  // channels to 4096 and 6144: 16.7 and 22.4 us by 16 outputs a workgroup, 18.0 and 18.8 by 32; 32 rows 18.0 and 25.4, 20.0 and 21.1.
+  const bool wide = roost::CeilDiv(g.out_dim, 16) > kCus;
+  if (g.tokens <= 16) return wide ? LaunchProduct<E, 2, 1, 4, 2, 4>(g, stream) : LaunchProduct<E, 1, 1, 8, 1, 2>(g, stream);
+  if (g.tokens <= 32) return wide ? LaunchProduct<E, 2, 2, 4, 4, 4>(g, stream) : LaunchProduct<E, 1, 2, 4, 2, 4>(g, stream);
+  // More rows: the smallest tile whose workgroups are one round. From 4096 channels, in tiles of 32 outputs x 64 rows, 80 x 64 and
+  // 64 x 64 (below): 128 rows to 4096 28, 37 and 43 us; 256 rows to 4096 41, 35 and 43; 1,072 rows of 2048 to 1024 30, 20 and 28;
+  // 48 rows to 12288 38.5 and 37.
+  if (roost::CeilDiv(g.out_dim, 32) * roost::CeilDiv(g.tokens, 64) <= kCus) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
+  if (roost::CeilDiv(g.out_dim, 80) * roost::CeilDiv(g.tokens, 64) <= kCus) return LaunchProduct<E, 5, 4, 4, 4, 2>(g, stream);
+  if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
   if (g.w == nullptr) return LaunchTiles<E, 1, 2, 2, 1, 1>(g, 0, g.tokens, stream);
   const uint64_t across = roost::CeilDiv(g.out_dim, 256), large = across * roost::CeilDiv(g.tokens, 256);
   if (large >= 160) {

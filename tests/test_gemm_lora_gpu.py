@@ -274,6 +274,9 @@ def _lens(tokens, long):
 # Rows x outputs that take each of the tilings of many rows, with sequences that start and end inside the tiles.
 @pytest.mark.parametrize("x,out", TYPES)
 @pytest.mark.parametrize("tokens,out_dim,long", [
+    (13, 5001, 5),      # 32 outputs x 16 rows
+    (31, 5001, 9),      # 32 x 32
+    (40, 20500, 9),     # 32 x 64, more than one round
     (300, 2100, 90),    # 80 x 64
     (130, 8300, 1),     # 80 x 64, a sequence a row
     (300, 5001, 90),    # 64 x 64
