@@ -1504,21 +1504,24 @@ void LaunchAll(const LoraArgs& g, hipStream_t stream) {
   if (roost::CeilDiv(g.out_dim, 80) * roost::CeilDiv(g.tokens, 64) <= kCus) return LaunchProduct<E, 5, 4, 4, 4, 2>(g, stream);
   if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
   if (g.w == nullptr) return LaunchTiles<E, 1, 2, 2, 1, 1>(g, 0, g.tokens, stream);
-  const uint64_t across = roost::CeilDiv(g.out_dim, 256), large = across * roost::CeilDiv(g.tokens, 256);
+  // Tiles of many rows: a CU holds one workgroup of 256 x 256, 256 x 128 or 128 x 128, so they go in rounds of kCus, and a larger
+  // tile's round does more for its time. From 4096 channels, rank 32, in rounds of 256 x 256, of 128 x 128 and of 64 x 64 (two
+  // workgroups a CU): 6,000 rows to 2048 126, 153 us; 2,048 rows to 2048 - , 58, 76 us; of 256 x 128 and 128 x 128: 1,100 rows to
+  // 4096 75 and 95 us, 900 rows to 4096 (one round of either) 73 and 55 us.
+  const uint64_t across = roost::CeilDiv(g.out_dim, 256);
+  const auto medium = [&](uint64_t rows) { return roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(rows, 128); };
+  uint64_t done = 0;
+  const uint64_t large = across * roost::CeilDiv(g.tokens, 256);
   if (large >= 160) {
-    // A CU holds one such tile, so the tiles go in rounds of kCus. Where the last round is a short one, the rows past the rounds
-    // before it take small tiles instead, if those are one round. In bf16, 4096 to 4096 channels, rank 32: 4,400 rows 185 us against
-    // 225 in large tiles alone, 8,500 rows 302 against 340, 13,000 rows 427 against 462.
-    const uint64_t before = large > kCus ? (roost::CeilDiv(large, kCus) - 1) * kCus / across * 256 : 0;
-    const uint64_t small = roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(g.tokens - before, 128);
-    const auto end = before > 0 && small <= kCus ? static_cast<uint32_t>(before) : g.tokens;
-    LaunchTiles<E, 2, 4, 4, 2, 2>(g, 0, end, stream);
-    if (end < g.tokens) LaunchTiles<E, 2, 2, 2, 2, 4>(g, end, g.tokens, stream);
-    return;
+    // Where the last round is a short one, the rows past the rounds before it take smaller tiles instead, if those are one round.
+    // In bf16, 4096 to 4096 channels, rank 32: 4,400 rows 185 us against 225 in large tiles alone, 6,000 rows 220 against 235.
+    done = (roost::CeilDiv(large, kCus) - 1) * kCus / across * 256;
+    if (done == 0 || across * roost::CeilDiv(g.tokens - done, 128) > kCus) done = g.tokens;
+    LaunchTiles<E, 2, 4, 4, 2, 2>(g, 0, done, stream);
+    if (done == g.tokens) return;
   }
-  if (roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(g.tokens, 128) >= 128) {
-    return LaunchTiles<E, 2, 2, 2, 2, 4>(g, 0, g.tokens, stream);
-  }
+  if (medium(g.tokens - done) > kCus) return LaunchTiles<E, 2, 2, 4, 2, 3>(g, done, g.tokens, stream);
+  if (done > 0 || medium(g.tokens) >= 128) return LaunchTiles<E, 2, 2, 2, 2, 4>(g, done, g.tokens, stream);
   return LaunchTiles<E, 1, 1, 2, 2, 4>(g, 0, g.tokens, stream);
 }
 

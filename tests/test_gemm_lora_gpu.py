@@ -282,10 +282,13 @@ def _lens(tokens, long):
     (300, 5001, 90),    # 64 x 64
     (1020, 2100, 400),  # 128 x 128
     (1100, 2100, 2),    # 128 x 128, a sequence a row or two
+    (1500, 2901, 300),  # 256 x 128
+    (1500, 2900, 3),
     (2601, 4200, 900),  # 256 x 256
     (2600, 4203, 4),    # 256 x 256, short sequences
     (4201, 4200, 700),  # 256 x 256 for 3,840 rows, 128 x 128 for the rest
     (4200, 4203, 5),
+    (5201, 4200, 900),  # 256 x 256 for 3,840 rows, 256 x 128 for the rest
 ])
 def test_tilings(session, tokens, out_dim, long, x, out):
     lens = _lens(tokens, long)
