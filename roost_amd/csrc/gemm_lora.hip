@@ -1,16 +1,28 @@
-// GemmLora for gfx950: a projection shared by every sequence, with each sequence's own low-rank adapter and an addend on top.
+// GemmLora for gfx950: a projection shared by every sequence, with each sequence's own low-rank adapter and an addend on
+// top.
 //
 //   y_t = W x_t + scale_a B_a[:, :rank] (A_a[:rank] x_t) + addend_t,   a = the adapter of row t's sequence (or none)
 //
-// Two launches: ShrinkKernel leaves the low-rank rows u_t = scale_a A_a x_t in the workspace, then the product's kernel
-// adds B_a u_t to its own sums before they are stored, so the output is written once.
+// Launches: ShrinkKernel leaves the low-rank rows u_t = scale_a A_a x_t in the workspace, then the product's kernel adds
+// B_a u_t to its own sums before they are stored, so the output is written once. One or two short sequences take a single
+// launch (FewRowsKernel). Up to 64 rows, and where their tiles fill one round of the CUs, the wavefronts of a workgroup
+// split the inner dimension (ProductKernel: bound by the weight's bytes and by latency); more rows go by tiles (TileKernel:
+// bound by the matrix instructions). LaunchAll holds the rules between them, with what was measured on both sides.
 //
-// Operands: everything is moved in 16-byte pieces along the inner dimension (8 bf16, 4 f32 or 16 e4m3). A matrix-instruction
-// fragment of 16 rows is one piece a lane: lane l holds row l % 16, piece l / 16 of a 64-byte run. That is the operand layout
-// of v_mfma_f32_16x16x32_bf16 as it stands; for f32 (four v_mfma_f32_16x16x4_f32, one word of the piece each) and e4m3 (two
+// Sums are fp32. Low-rank rows are fp32 beside f32 adapters; beside bf16 ones the matrix instructions take them in bf16: rounded
+// once under a bf16 output (off by at most 2^-8 of each, as a bf16 tensor between two products would be), in three parts that
+// hold all 24 bits under an f32 output.
+//
+// Operands: everything is moved in 16-byte pieces along the inner dimension (8 bf16, 4 f32 or 16 e4m3), from memory
+// straight into LDS (global_load_lds, 8 rows of 128 bytes an instruction), and read from there as fragments: a load of a
+// fragment from memory touches 16 or 32 rows at once, which the address unit takes one after another (58 requests an
+// instruction were counted), while eight whole 128-byte lines are eight. A matrix-instruction fragment of 16 rows is one
+// piece a lane: lane l holds row l % 16, piece l / 16 of a 64-byte run. That is the operand layout of
+// v_mfma_f32_16x16x32_bf16 as it stands; for f32 (four v_mfma_f32_16x16x4_f32, one word of the piece each) and e4m3 (two
 // v_mfma_f32_16x16x32_fp8_fp8, 8 bytes each) the pieces visit the inner dimension in another order, the same for both
-// operands, so the sum is over the same products. Weight rows are the first operand and token rows the second: in the result
-// lane l holds token l % 16 and the four consecutive outputs 4 (l / 16) .. + 3.
+// operands, so the sum is over the same products. Weight rows are the first operand and token rows the second: in the
+// result lane l holds token l % 16 and the four consecutive outputs 4 (l / 16) .. + 3. The 32-row fragments of the tiles
+// are the same with 32 rows and two pieces.
 
 #include <type_traits>
 
@@ -34,9 +46,9 @@ typedef int i32x8_t __attribute__((ext_vector_type(8)));
 struct E4m3 {
   uint8_t bits;
 };
-// The same rows multiplied as bf16 (an exact conversion, in registers). The e4m3 matrix instructions keep fewer bits of their
-// inner sums: over 4,096 products of random codes they are 5e-5 of the result off, bf16's 4e-7. That is far below a bf16
-// output's rounding (2e-3) and far above an f32 output's, which therefore takes this form.
+// The same rows multiplied as bf16 (an exact conversion, in registers). The e4m3 matrix instructions keep fewer bits of
+// their inner sums: over 4,096 products of random codes they are 5e-5 of the result off, bf16's 4e-7. That is far below a
+// bf16 output's rounding (2e-3) and far above an f32 output's, which therefore takes this form.
 struct E4m3AsBf16 {
   uint8_t bits;
 };
@@ -91,8 +103,8 @@ __device__ __forceinline__ Sequence SequenceOf(const LoraArgs& g, uint32_t b) {
   return Sequence{g.cu[b], g.cu[b + 1], g.a != nullptr ? g.slots[b] : kNoAdapter};
 }
 
-// slot[i] of each lane's sequence's rows, by whole wavefronts (rows t0 .. t0 + n - 1 of the call are slot[0 ..]): a lane writes a short sequence's itself, a long one's are
-// written by its wavefront.
+// slot[i] of each lane's sequence's rows, by whole wavefronts (rows t0 .. t0 + n - 1 of the call are slot[0 ..]): a lane
+// writes a short sequence's itself, a long one's are written by its wavefront.
 __device__ __forceinline__ void PutSlots(const LoraArgs& g, Sequence q, uint32_t t0, uint32_t n, int32_t* slot) {
   constexpr int32_t kShort = 4;
   const int64_t rows = min(n, g.tokens - t0), start = t0;
@@ -183,7 +195,8 @@ __device__ __forceinline__ f32x16_t Mma32(FragOf<E> a, FragOf<E> b, f32x16_t acc
     // Block scales of 2^0 (biased exponent 127).
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 0, 0, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
   } else if constexpr (std::is_same_v<E, uint16_t>) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), acc, 0,
+                                                   0, 0);
   } else if constexpr (std::is_same_v<E, float>) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -203,8 +216,8 @@ __device__ __forceinline__ f32x16_t Mma32(FragOf<E> a, FragOf<E> b, f32x16_t acc
 // ---- Copies to LDS -------------------------------------------------------------------------------------------------------
 //
 // Rows are brought in by 128 bytes of the inner dimension, eight rows an instruction, each row's eight pieces from eight
-// neighbouring lanes. Loading the fragments themselves, 16 rows at a time with neighbouring lanes in different rows, costs one
-// address cycle a lane instead of one for each four: 30 us instead of 15 for a decode product of 64 x 6,144 over 4,096.
+// neighbouring lanes. Loading the fragments themselves, 16 rows at a time with neighbouring lanes in different rows, costs
+// one address cycle a lane instead of one for each four: 30 us instead of 15 for a decode product of 64 x 6,144 over 4,096.
 
 constexpr uint32_t kStepBytes = 128;
 
@@ -227,10 +240,11 @@ __device__ __forceinline__ uint32_t LdsAddress(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const unsigned char*)p));
 }
 
-// A wavefront's own rows on their way through LDS: kA rows from one base and kB from another, kStages steps at a time. The first
-// rows' steps are kSub times as long as the others' and stand as kSub rows each: first all the rows' first 128 bytes, then
-// their second. Piece p of row r lies at p ^ (r % 8), so that the 16 rows of a fragment at one piece are free of bank conflicts; the copy writes LDS in
-// lane order, so it is the lanes' source addresses that are permuted. Nothing but this wavefront waits for it.
+// A wavefront's own rows on their way through LDS: kA rows from one base and kB from another, kStages steps at a time. The
+// first rows' steps are kSub times as long as the others' and stand as kSub rows each: first all the rows' first 128 bytes,
+// then their second. Piece p of row r lies at p ^ (r % 8), so that the 16 rows of a fragment at one piece are free of bank
+// conflicts; the copy writes LDS in lane order, so it is the lanes' source addresses that are permuted. Nothing but this
+// wavefront waits for it.
 template <int kA, int kB, int kSub, int kStages>
 struct RowStream {
   static_assert(kA % (8 * kSub) == 0 && kB % 8 == 0, "eight rows an instruction");
@@ -270,8 +284,8 @@ struct RowStream {
     }
   }
 
-  // use(stage) for the steps first, first + stride, .. (in bytes) of the rows; it is to have read what it needs of the stage
-  // into registers when it returns.
+  // use(stage) for the steps first, first + stride, .. (in bytes) of the rows; it is to have read what it needs of the
+  // stage into registers when it returns.
   template <typename U>
   __device__ __forceinline__ void Run(uint32_t first, uint32_t stride, U&& use) const {
     const uint32_t steps = first < bytes ? (bytes - first + stride - 1) / stride : 0;
@@ -309,8 +323,9 @@ struct RowRange {
   int32_t slot;
 };
 
-// The `at`-th piece of the batch, where every sequence is cut at the multiples of kRows: at most tokens / kRows + batch of them.
-// By the whole workgroup, a lane a sequence: the pieces before each are a prefix sum over the workgroup. Empty past the last.
+// The `at`-th piece of the batch, where every sequence is cut at the multiples of kRows: at most tokens / kRows + batch of
+// them. By the whole workgroup, a lane a sequence: the pieces before each are a prefix sum over the workgroup. Empty past
+// the last.
 template <int kRows>
 __device__ __forceinline__ RowRange PieceOf(const LoraArgs& g, uint32_t at) {
   __shared__ uint32_t sums[16];
@@ -350,7 +365,8 @@ __device__ __forceinline__ RowRange PieceOf(const LoraArgs& g, uint32_t at) {
   return r;
 }
 
-// acc += one step of a RowStream's rows: kRows of the input (fewer than 16 kT stand for the others too) times 16 kR of an adapter's.
+// acc += one step of a RowStream's rows: kRows of the input (fewer than 16 kT stand for the others too) times 16 kR of an
+// adapter's.
 template <typename E, int kT, int kR, int kRows, typename Done>
 __device__ __forceinline__ void ShrinkStep(const unsigned char* stage, uint32_t lane, Done&& done, f32x4_t (&acc)[kT][kR]) {
   using Low = LowOf<E>;
@@ -385,9 +401,9 @@ __device__ __forceinline__ void ShrinkStep(const unsigned char* stage, uint32_t 
   }
 }
 
-// Workgroup (i, j): the i-th piece of the batch (rows of one sequence within kRows = 16 kT), ranks 16 kR j .. + 16 kR - 1. The
-// wavefronts take alternate steps of the inner dimension and join their sums through LDS. A step is 128 bytes of the rows;
-// e4m3 rows meet twice as many bytes of the adapter's, which stand as two rows each.
+// Workgroup (i, j): the i-th piece of the batch (rows of one sequence within kRows = 16 kT), ranks 16 kR j .. + 16 kR - 1.
+// The wavefronts take alternate steps of the inner dimension and join their sums through LDS. A step is 128 bytes of the
+// rows; e4m3 rows meet twice as many bytes of the adapter's, which stand as two rows each.
 template <typename E, int kT, int kR, int kWaves, int kStages>
 __global__ void __launch_bounds__(64 * kWaves) ShrinkKernel(LoraArgs g) {
   using Low = LowOf<E>;
@@ -569,8 +585,8 @@ __device__ __forceinline__ f32x4_t Rescaled(const LoraArgs& g, float x_scale, ui
 
 // ---- The product of few rows ---------------------------------------------------------------------------------------------
 
-// A piece of low-rank rows for the adapters' type: fp32 as it is; bf16 rounded to nearest, what that leaves staying in ur for the
-// next part.
+// A piece of low-rank rows for the adapters' type: fp32 as it is; bf16 rounded to nearest, what that leaves staying in ur
+// for the next part.
 template <typename Low>
 __device__ __forceinline__ u32x4_t NextPart(f32x4_t (&ur)[4 / sizeof(Low)]) {
   u32x4_t pu;
@@ -587,14 +603,14 @@ __device__ __forceinline__ u32x4_t NextPart(f32x4_t (&ur)[4 / sizeof(Low)]) {
   return pu;
 }
 
-// v[m] += B u for kM 16 x 16 tiles side by side, lane l holding outputs n + 16 m + 4 (l / 16) .. + 3 of the row `token` with adapter
-// s (l % 16). The rows of the adapters among the 16 are requested sixteen at a time, before the ranks that say how much of them
-// counts are known; each adapter's product is kept by its own rows only.
+// v[m] += B u for kM 16 x 16 tiles side by side, lane l holding outputs n + 16 m + 4 (l / 16) .. + 3 of the row `token`
+// with adapter s (l % 16). The rows of the adapters among the 16 are requested sixteen at a time, before the ranks that say
+// how much of them counts are known; each adapter's product is kept by its own rows only.
 template <typename Low, int kM>
 __device__ __forceinline__ void AddLowRankTiles(const LoraArgs& g, uint32_t token, int32_t s, uint32_t n, uint32_t lane,
                                                 f32x4_t (&v)[kM]) {
   constexpr uint32_t kPer = 16 / sizeof(Low);
-  constexpr int kTogether = kM > 2 ? 4 : 16 / kM;
+  constexpr int kTogether = kM == 1 ? 16 : 4;  // adapters whose rows are on their way, kM pieces each
   if (__ballot(s >= 0) == 0) return;
   const uint32_t its_rank = RankOf(g, s);
   int32_t at[16];  // a row of the k-th adapter
@@ -627,8 +643,8 @@ __device__ __forceinline__ void AddLowRankTiles(const LoraArgs& g, uint32_t toke
           const auto slot = static_cast<uint64_t>(__builtin_amdgcn_readlane(s, at[k0 + k]));
 #pragma unroll
           for (int m = 0; m < kM; ++m) {
-            b[k][m] = *reinterpret_cast<const u32x4_t*>(static_cast<const Low*>(g.b) + (slot * g.out_dim + out[m]) * g.max_rank +
-                                                        from);
+            const uint64_t at_row = (slot * g.out_dim + out[m]) * g.max_rank;
+            b[k][m] = *reinterpret_cast<const u32x4_t*>(static_cast<const Low*>(g.b) + at_row + from);
           }
         }
       }
@@ -656,6 +672,10 @@ __device__ __forceinline__ void AddLowRankTiles(const LoraArgs& g, uint32_t toke
   }
 }
 
+// Bound by the weight's bytes on their way from memory and by the latency of the first of them. 64 rows, 4096 to 6144 channels:
+// 14 us for 50 MB of weight (3.6 TB/s) and 32 KB of rows a step and CU out of L2; with the workgroups of an XCD on neighbouring
+// tiles, against 21 us with neighbours spread over the XCDs.
+//
 // A workgroup: 16 kN outputs of 16 kT rows. kWaves wavefronts take alternate steps of the
 // inner dimension; beside them kLow others find the rows' adapters and compute their outputs, which has as long a chain of
 // loads (sequence, adapter, rank, its rows) as the product but moves little. All join their sums through LDS.
@@ -668,8 +688,8 @@ __global__ void __launch_bounds__(64 * (kWaves + kLow)) ProductKernel(LoraArgs g
   static_assert(kWaves * Stream::kBytes >= (kWaves + 1) * kTiles * 64 * sizeof(f32x4_t), "the sums fit where the rows were");
   __shared__ __align__(16) unsigned char lds[kWaves * Stream::kBytes];
   __shared__ int32_t slot[kLow][16];
-  // Workgroups go to the 8 XCDs in turn; each XCD takes one run of the tiles, so that those next to each other in memory are read
-  // through one L2.
+  // Workgroups go to the 8 XCDs in turn; each XCD takes one run of the tiles, so that those next to each other in memory
+  // are read through one L2.
   const uint32_t tiles = gridDim.x, xcd = blockIdx.x % 8;
   const uint32_t at = xcd * (tiles / 8) + min(xcd, tiles % 8) + blockIdx.x / 8;
   const uint32_t n0 = 16 * kN * (at % n_tiles), t0 = 16 * kT * (at / n_tiles);
@@ -691,7 +711,8 @@ __global__ void __launch_bounds__(64 * (kWaves + kLow)) ProductKernel(LoraArgs g
     WaveSync();
 #pragma unroll
     for (int m = 0; m < kM; ++m) low[m] = f32x4_t{0, 0, 0, 0};
-    AddLowRankTiles<LowOf<E>, kM>(g, min(t0 + 16 * low_t + lane % 16, g.tokens - 1), mine[lane % 16], n0 + 16 * low_n, lane, low);
+    const uint32_t token = min(t0 + 16 * low_t + lane % 16, g.tokens - 1);
+    AddLowRankTiles<LowOf<E>, kM>(g, token, mine[lane % 16], n0 + 16 * low_n, lane, low);
   } else if (g.w != nullptr) {
     Stream rows;
     rows.lds = lds + wave * Stream::kBytes;
@@ -756,10 +777,11 @@ __global__ void __launch_bounds__(64 * (kWaves + kLow)) ProductKernel(LoraArgs g
 
 // ---- One or two short sequences -------------------------------------------------------------------------------------------
 //
-// A chat's single token waits for nothing but latency, so its low-rank rows are not a launch of their own: every workgroup computes
-// them all again for its 16 outputs, by wavefronts beside the product's, from rows that the other workgroups read as well. That
-// holds for kFewRows rows and, over all sequences, kFewRanks ranks. Against two launches, one row, rank 16: 1024 to 6144 channels
-// 6.7 and 12.7 us, 4096 to 6144 15.7 and 19.7 us, 4096 to 14336 30.5 and 31.6 us, 14336 to 4096 32.5 and 37.9 us.
+// A chat's single token waits for nothing but latency, so its low-rank rows are not a launch of their own: every workgroup
+// computes them all again for its 16 outputs, by wavefronts beside the product's, from rows that the other workgroups read
+// as well. That holds for kFewRows rows and, over all sequences, kFewRanks ranks. Against two launches, one row, rank 16:
+// 1024 to 6144 channels 6.7 and 12.7 us, 4096 to 6144 15.7 and 19.7 us, 4096 to 14336 30.5 and 31.6 us, 14336 to 4096 32.5
+// and 37.9 us.
 constexpr uint32_t kFewRows = 8, kFewRanks = 16;
 
 template <typename E>
@@ -778,8 +800,8 @@ __global__ void __launch_bounds__(64 * 12) FewRowsKernel(LoraArgs g) {
   const uint32_t x_row = min(lane / 8, g.tokens - 1) * static_cast<uint32_t>(g.x_stride * sizeof(E)) + piece;
   const auto* x = static_cast<const unsigned char*>(g.x);
 
-  // Of the last wavefront, which joins the sums, and requested before the rows that it sums: the sequences' adapters, their rows of
-  // B (of output n0 + lane % 16), and row t's sequence and scales.
+  // Of the last wavefront, which joins the sums, and requested before the rows that it sums: the sequences' adapters, their
+  // rows of B (of output n0 + lane % 16), and row t's sequence and scales.
   const uint32_t t = lane % 16;
   int32_t slot[2] = {kNoAdapter, kNoAdapter}, its = kNoRow;
   uint32_t rank[2] = {};
@@ -801,7 +823,8 @@ __global__ void __launch_bounds__(64 * 12) FewRowsKernel(LoraArgs g) {
     rows.off_b[0] = x_row;
 #pragma unroll
     for (int k = 0; k < 2 * kSub; ++k) {
-      // Row j: rank j % max_rank of sequence j / max_rank; those of no adapter repeat the first row, and their sums are not kept.
+      // Row j: rank j % max_rank of sequence j / max_rank; those of no adapter repeat the first row, and their sums are not
+      // kept.
       const uint32_t row = 8 * k + lane / 8, j = row % 16, half = row / 16, i = j / g.max_rank;
       const int32_t its = i == 0 ? slot[0] : i == 1 ? slot[1] : kNoAdapter;
       const uint32_t of = its >= 0 ? static_cast<uint32_t>(its) * g.max_rank + j % g.max_rank : 0;
@@ -902,9 +925,9 @@ __global__ void __launch_bounds__(64 * 12) FewRowsKernel(LoraArgs g) {
 //
 // One workgroup: 32 kN kWN outputs x 32 kT kWT rows, its wavefronts in a kWN x kWT grid of 32 kN x 32 kT each, kept in
 // accumulators. 128 bytes of the inner dimension at a time are copied from memory straight into LDS (global_load_lds, no
-// registers), kStages steps ahead. A row's eight 16-byte pieces lie in LDS at piece
-// p ^ (row / 2 % 8): 32 rows of 128 bytes read at one piece are then free of bank conflicts (with p ^ (row % 8) each read takes half
-// as long again). The copy writes LDS in lane order, so it is the lanes' source addresses that are permuted.
+// registers), kStages steps ahead. A row's eight 16-byte pieces lie in LDS at piece p ^ (row / 2 % 8): 32 rows of 128 bytes
+// read at one piece are then free of bank conflicts (with p ^ (row % 8) each read takes half as long again). The copy
+// writes LDS in lane order, so it is the lanes' source addresses that are permuted.
 
 // Every copy but this wavefront's last kLeft has landed, its own LDS reads have returned, and then every wavefront's.
 template <int kLeft>
@@ -912,12 +935,13 @@ __device__ __forceinline__ void WaitStep() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
 
-// Runs of rows with one adapter that a 32 x 32 tile a wavefront takes step by step; more (one-token sequences) are added element
-// by element.
+// Runs of rows with one adapter that a 32 x 32 tile a wavefront takes step by step; more (one-token sequences) are added
+// element by element.
 constexpr uint32_t kRunsBySteps = 4;
 
 template <typename E, int kN, int kT, int kWN, int kWT, int kStages>
-__global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles, uint32_t first) {
+__global__ void __launch_bounds__(64 * kWN * kWT, 1)
+TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles, uint32_t first) {
   constexpr int kWaves = kWN * kWT;
   constexpr int kRowsN = 32 * kN * kWN, kRowsT = 32 * kT * kWT;
   constexpr int kCopiesN = kRowsN / (8 * kWaves), kCopiesT = kRowsT / (8 * kWaves);  // of 8 rows, by each wavefront
@@ -931,8 +955,8 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
   __shared__ __align__(16) float w_scale[kIsE4m3<E> ? kRowsN : 4];
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 
-  // Workgroups go to the 8 XCDs in turn; each XCD takes one run of the tiles, ordered in blocks of kBlockT rows of tiles, so
-  // that the tiles in flight on an XCD share weight and token rows in its L2.
+  // Workgroups go to the 8 XCDs in turn; each XCD takes one run of the tiles, ordered in blocks of kBlockT rows of tiles,
+  // so that the tiles in flight on an XCD share weight and token rows in its L2.
   constexpr uint32_t kXcds = 8, kBlockT = 8;
   const uint32_t tiles = n_tiles * t_tiles;
   const uint32_t per_xcd = (tiles + kXcds - 1) / kXcds;
@@ -1102,9 +1126,10 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
   }
   __syncthreads();  // the stages are free, the runs known
 
-  // The adapters, one run of rows after the other, by the same steps: 128 bytes of the ranks of the adapter's outputs and of the
-  // low-rank rows. A row takes only its own run's sums, so that no adapter's values, whatever they are, reach another's rows.
-  // acc[n][t], register i, lane l: row wt + 32 t + l % 32, output wn + 32 n + 8 (i / 4) + 4 (l / 32) + i % 4.
+  // The adapters, one run of rows after the other, by the same steps: 128 bytes of the ranks of the adapter's outputs and
+  // of the low-rank rows. A row takes only its own run's sums, so that no adapter's values, whatever they are, reach
+  // another's rows. acc[n][t], register i, lane l: row wt + 32 t + l % 32, output wn + 32 n + 8 (i / 4) + 4 (l / 32) + i %
+  // 4.
   if constexpr (kIsE4m3<E>) {
     if (g.w != nullptr) {
 #pragma unroll
@@ -1122,8 +1147,8 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
       }
     }
   }
-  // Below, a lane stores 8 outputs of a row; the addends of whole eights are loaded ahead: before the adapters where there are
-  // registers for it, else after them.
+  // Below, a lane stores 8 outputs of a row; the addends of whole eights are loaded ahead: before the adapters where there
+  // are registers for it, else after them.
   constexpr uint32_t kOctets = 4 * kN, kRowsAtOnce = 64 / kOctets, kTurns = 32 / kRowsAtOnce;
   constexpr bool kEarly = kN * kT <= 4;
   const uint32_t out = n0 + wn + 8 * (lane % kOctets);
@@ -1137,7 +1162,8 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
         const uint32_t row = wt + 32 * t + kRowsAtOnce * k + lane / kOctets;
         early[t][k] = u32x4_t{0, 0, 0, 0};
         if (g.addend != nullptr && !g.addend_f32 && whole && slot[row] != kNoRow) {
-          early[t][k] = *reinterpret_cast<const Bf16x8*>(static_cast<const uint16_t*>(g.addend) + (t0 + row) * g.addend_stride + out);
+          const uint64_t at = (t0 + row) * g.addend_stride + out;
+          early[t][k] = *reinterpret_cast<const Bf16x8*>(static_cast<const uint16_t*>(g.addend) + at);
         }
       }
     }
@@ -1178,9 +1204,11 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
         return;
       }
       // A row of the pool is at most 512 bytes, so a tile's are within 32 bits of its first.
-      const auto* b_base = static_cast<const unsigned char*>(g.b) + (static_cast<uint64_t>(p.slot) * g.out_dim + n0) * row_bytes;
-      const auto* u_base = (sizeof(Low) == 2 ? reinterpret_cast<const unsigned char*>(g.u_bf16 + p.part * g.u_part)
-                                             : reinterpret_cast<const unsigned char*>(g.u)) + t0 * static_cast<uint64_t>(row_bytes);
+      const uint64_t b_row = static_cast<uint64_t>(p.slot) * g.out_dim + n0;
+      const auto* b_base = static_cast<const unsigned char*>(g.b) + b_row * row_bytes;
+      const auto* u_base = sizeof(Low) == 2 ? reinterpret_cast<const unsigned char*>(g.u_bf16 + p.part * g.u_part)
+                                            : reinterpret_cast<const unsigned char*>(g.u);
+      u_base += t0 * static_cast<uint64_t>(row_bytes);
 #pragma unroll
       for (int i = 0; i < kCopiesN; ++i) {
         Copy16(b_base, min(8 * (wave + kWaves * i) + lane / 8, last_n) * row_bytes + at, to_n + 1024 * kWaves * i);
@@ -1253,8 +1281,8 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
     }
   }
 
-  // The sums go through LDS by 32 rows, each wavefront in a part of its own, and from there whole 128-byte runs of a row to a
-  // store. bf16 addends of all the rows are requested before the first is used (f32 ones of 32 rows, to save registers).
+  // The sums go through LDS by 32 rows, each wavefront in a part of its own, and from there whole 128-byte runs of a row to
+  // a store. bf16 addends of all the rows are requested before the first is used (f32 ones of 32 rows, to save registers).
   constexpr uint32_t kRowWords = 32 * kN + 4;  // 4 words of padding put 8 neighbouring rows on different banks
   static_assert(kWaves * 32 * kRowWords * 4 <= kStages * kStage, "the wavefronts' parts fit the stages");
   float* mine = reinterpret_cast<float*>(lds) + wave * 32 * kRowWords;
@@ -1293,7 +1321,8 @@ __global__ void __launch_bounds__(64 * kWN * kWT, 1) TileKernel(LoraArgs g, uint
           p[1] = hi;
         } else {
           *reinterpret_cast<Bf16x8*>(static_cast<uint16_t*>(g.y) + token * g.y_stride + out) =
-              Bf16x8{PackBf16Rne(lo[0], lo[1]), PackBf16Rne(lo[2], lo[3]), PackBf16Rne(hi[0], hi[1]), PackBf16Rne(hi[2], hi[3])};
+              Bf16x8{PackBf16Rne(lo[0], lo[1]), PackBf16Rne(lo[2], lo[3]), PackBf16Rne(hi[0], hi[1]),
+                     PackBf16Rne(hi[2], hi[3])};
         }
       }
     }
@@ -1422,8 +1451,8 @@ RoostStatus Admit(const RoostAmdGemmLoraParams& p, bool for_run) {
   return gate.status();
 }
 
-// The low-rank rows in f32, then, beside bf16 adapters, in bf16: one rounding under a bf16 output, three parts, which hold all
-// 24 bits, under an f32 one.
+// The low-rank rows in f32, then, beside bf16 adapters, in bf16: one rounding under a bf16 output, three parts, which hold
+// all 24 bits, under an f32 one.
 uint64_t LowRankElements(const RoostAmdGemmLoraParams& p) {
   return p.lora_a.address == nullptr ? 0 : roost::RoundUp(static_cast<uint64_t>(p.tokens) * p.max_rank, 64);
 }
@@ -1438,10 +1467,11 @@ uint64_t WorkspaceBytes(const RoostAmdGemmLoraParams& p) {
 
 template <typename E, int kT, int kR>
 void LaunchShrink(const LoraArgs& g, hipStream_t stream) {
-  // One tile: two workgroups share a CU's LDS. Else eight wavefronts where three stages of theirs fit, then as many stages as there
-  // is room for, up to four.
+  // One tile: two workgroups share a CU's LDS. Else eight wavefronts where three stages of theirs fit, then as many stages
+  // as there is room for, up to four.
   constexpr bool kOne = kT == 1 && kR == 1;
-  constexpr int kStepRows = 16 * kT + 16 * kR * static_cast<int>(sizeof(LowOf<E>) / sizeof(E)), kRoom = (kOne ? 75 : 150) * 1024;
+  constexpr int kStepRows = 16 * kT + 16 * kR * static_cast<int>(sizeof(LowOf<E>) / sizeof(E));
+  constexpr int kRoom = (kOne ? 75 : 150) * 1024;
   constexpr int kWaves = 8 * (kOne ? 2 : 3) * kStepRows * static_cast<int>(kStepBytes) <= kRoom ? 8 : 4;
   constexpr int kStages = std::min(4, kRoom / (kWaves * kStepRows * static_cast<int>(kStepBytes)));
   static_assert(kStages >= 2, "a step on its way while one is multiplied");
@@ -1450,9 +1480,9 @@ void LaunchShrink(const LoraArgs& g, hipStream_t stream) {
 }
 template <typename E, int kT>
 void LaunchShrinkOfRows(const LoraArgs& g, hipStream_t stream) {
-  // Blocks of 16 ranks while all the workgroups have a CU of their own, else as wide as the pool's ranks, up to 32 or 64, so that
-  // the rows are read once. 64 one-token sequences of 4096 channels, rank 32: 17.8 us a call in blocks of 16, 18.7 of 32; 256 of
-  // them 24.9 and 22.5; 1,000 of rank 128: 186 in blocks of 16, 127 of 64.
+  // Blocks of 16 ranks while all the workgroups have a CU of their own, else as wide as the pool's ranks, up to 32 or 64,
+  // so that the rows are read once. 64 one-token sequences of 4096 channels, rank 32: 17.8 us a call in blocks of 16, 18.7
+  // of 32; 256 of them 24.9 and 22.5; 1,000 of rank 128: 186 in blocks of 16, 127 of 64.
   const uint64_t blocks = (roost::CeilDiv(g.tokens, 16 * kT) + g.batch) * roost::CeilDiv(g.max_rank, 16);
   if (g.max_rank <= 16 || (kT == 1 && blocks <= kCus)) return LaunchShrink<E, kT, 1>(g, stream);
   if constexpr (!kIsE4m3<E>) {
@@ -1465,7 +1495,8 @@ template <typename E, int kN, int kT, int kWaves, int kLow, int kStages>
 void LaunchProduct(const LoraArgs& g, hipStream_t stream) {
   const auto n_tiles = static_cast<uint32_t>(roost::CeilDiv(g.out_dim, 16 * kN));
   const auto grid = static_cast<uint32_t>(n_tiles * roost::CeilDiv(g.tokens, 16 * kT));
-  hipLaunchKernelGGL((ProductKernel<E, kN, kT, kWaves, kLow, kStages>), dim3(grid), dim3(64 * (kWaves + kLow)), 0, stream, g, n_tiles);
+  hipLaunchKernelGGL((ProductKernel<E, kN, kT, kWaves, kLow, kStages>), dim3(grid), dim3(64 * (kWaves + kLow)), 0, stream, g,
+                     n_tiles);
 }
 
 // Rows first .. end - 1.
@@ -1474,47 +1505,52 @@ void LaunchTiles(const LoraArgs& g, uint32_t first, uint32_t end, hipStream_t st
   const auto n_tiles = static_cast<uint32_t>(roost::CeilDiv(g.out_dim, 32 * kN * kWN));
   const auto t_tiles = static_cast<uint32_t>(roost::CeilDiv(end - first, 32 * kT * kWT));
   const auto grid = static_cast<uint32_t>(roost::RoundUp(n_tiles * t_tiles, 8));
-  hipLaunchKernelGGL((TileKernel<E, kN, kT, kWN, kWT, kStages>), dim3(grid), dim3(64 * kWN * kWT), 0, stream, g, n_tiles, t_tiles,
-                     first);
+  hipLaunchKernelGGL((TileKernel<E, kN, kT, kWN, kWT, kStages>), dim3(grid), dim3(64 * kWN * kWT), 0, stream, g, n_tiles,
+                     t_tiles, first);
 }
 
 template <typename E>
 void LaunchAll(const LoraArgs& g, hipStream_t stream) {
   const uint64_t a_bytes = static_cast<uint64_t>(g.adapters) * g.max_rank * g.in_dim * sizeof(LowOf<E>);
-  if (g.a != nullptr && g.tokens <= kFewRows && static_cast<uint64_t>(g.batch) * g.max_rank <= kFewRanks && a_bytes < (1ull << 31)) {
+  const uint64_t ranks = static_cast<uint64_t>(g.batch) * g.max_rank;
+  // (A lane's offset into the adapters is 32 bits there.)
+  if (g.a != nullptr && g.tokens <= kFewRows && ranks <= kFewRanks && a_bytes < (1ull << 31)) {
     hipLaunchKernelGGL((FewRowsKernel<E>), dim3(roost::CeilDiv(g.out_dim, 16)), dim3(64 * 12), 0, stream, g);
     return;
   }
   if (g.a != nullptr) {
+    // Pieces of 64 rows read an adapter a fourth as often as pieces of 16, but are a fourth as many: 4,480 bf16 rows of
+    // 4096 channels, rank 16, 17.4 and 15.6 us; 6,700 e4m3 rows, rank 32, 17.6 and 20.5 us.
     if (g.tokens / g.batch >= 64 && g.tokens >= 6144) {
       LaunchShrinkOfRows<E, 4>(g, stream);
     } else {
       LaunchShrinkOfRows<E, 1>(g, stream);
     }
   }
-  // Few rows: as many workgroups as outputs allow, up to one a CU; a second round costs more than wider tiles. 16 rows of 4096
-  // channels to 4096 and 6144: 16.7 and 22.4 us by 16 outputs a workgroup, 18.0 and 18.8 by 32; 32 rows 18.0 and 25.4, 20.0 and 21.1.
+  // Few rows: 16 outputs a workgroup while that is one workgroup a CU, else 32, for a second round costs more. 16 rows of 4096
+  // channels: to 4096 outputs 16.7 us by 16 and 18.0 by 32, to 6144 22.4 and 18.8; 32 rows: 18.0 and 20.0, 25.4 and 21.1.
   const bool wide = roost::CeilDiv(g.out_dim, 16) > kCus;
   if (g.tokens <= 16) return wide ? LaunchProduct<E, 2, 1, 4, 2, 4>(g, stream) : LaunchProduct<E, 1, 1, 8, 1, 2>(g, stream);
   if (g.tokens <= 32) return wide ? LaunchProduct<E, 2, 2, 4, 4, 4>(g, stream) : LaunchProduct<E, 1, 2, 4, 2, 4>(g, stream);
-  // More rows: the smallest tile whose workgroups are one round. From 4096 channels, in tiles of 32 outputs x 64 rows, 80 x 64 and
-  // 64 x 64 (below): 128 rows to 4096 28, 37 and 43 us; 256 rows to 4096 41, 35 and 43; 1,072 rows of 2048 to 1024 30, 20 and 28;
-  // 48 rows to 12288 38.5 and 37.
+  // More rows: the smallest tile whose workgroups are one round. In tiles of 32 outputs x 64 rows, of 80 x 64 and of 64 x 64 by
+  // TileKernel: 128 rows, 4096 to 4096, 28, 37 and 43 us; 256 rows 41, 35 and 43 us; 1,072 rows, 2048 to 1024, 30, 20 and 28 us.
   if (roost::CeilDiv(g.out_dim, 32) * roost::CeilDiv(g.tokens, 64) <= kCus) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
   if (roost::CeilDiv(g.out_dim, 80) * roost::CeilDiv(g.tokens, 64) <= kCus) return LaunchProduct<E, 5, 4, 4, 4, 2>(g, stream);
   if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
+  // The adapters alone move an addend and an output: small tiles, many to a CU (4,480 rows of 4096 outputs, rank 16: 26 us,
+  // by 256 x 256 36 us).
   if (g.w == nullptr) return LaunchTiles<E, 1, 2, 2, 1, 1>(g, 0, g.tokens, stream);
-  // Tiles of many rows: a CU holds one workgroup of 256 x 256, 256 x 128 or 128 x 128, so they go in rounds of kCus, and a larger
-  // tile's round does more for its time. From 4096 channels, rank 32, in rounds of 256 x 256, of 128 x 128 and of 64 x 64 (two
-  // workgroups a CU): 6,000 rows to 2048 126, 153 us; 2,048 rows to 2048 - , 58, 76 us; of 256 x 128 and 128 x 128: 1,100 rows to
-  // 4096 75 and 95 us, 900 rows to 4096 (one round of either) 73 and 55 us.
+  // Tiles of many rows: a CU holds one workgroup of 256 x 256, 256 x 128 or 128 x 128, so they go in rounds of kCus, and a
+  // larger tile's round does more for its time (4096 channels, bf16: about 116, 65 and 45 us). So the smallest tile with one
+  // round, and 256 x 256 from where 256 x 128 would take a second one. 900 rows to 4096: 256 x 128 73, 128 x 128 55, 64 x 64 73
+  // us; 1,100 rows to 4096: 75, 95 and 87 us; 6,000 rows to 2048: 256 x 256 126, 128 x 128 153 us.
   const uint64_t across = roost::CeilDiv(g.out_dim, 256);
   const auto medium = [&](uint64_t rows) { return roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(rows, 128); };
   uint64_t done = 0;
   const uint64_t large = across * roost::CeilDiv(g.tokens, 256);
   if (large >= 160) {
-    // Where the last round is a short one, the rows past the rounds before it take smaller tiles instead, if those are one round.
-    // In bf16, 4096 to 4096 channels, rank 32: 4,400 rows 185 us against 225 in large tiles alone, 6,000 rows 220 against 235.
+    // Where the last round is a short one, the rows past the rounds before it take smaller tiles instead, if those are one
+    // round: 4,400 rows to 4096 185 us against 225 in large tiles alone, 6,000 rows 220 against 235.
     done = (roost::CeilDiv(large, kCus) - 1) * kCus / across * 256;
     if (done == 0 || across * roost::CeilDiv(g.tokens - done, 128) > kCus) done = g.tokens;
     LaunchTiles<E, 2, 4, 4, 2, 2>(g, 0, done, stream);

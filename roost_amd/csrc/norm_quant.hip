@@ -2,16 +2,16 @@
 // and the MLP's activation, both optionally in 8 bits with scales.
 //
 // Per row, in fp32: s = x + residual (stored, rounded to the residual's type); y = s / sqrt(mean(s^2) + eps) * weight. The
-// 8-bit forms cut the row into cells (the whole row, or `group` columns): scale = max(max|y| / 448, 2^-126), code =
-// e4m3(y / scale). 448 is e4m3's largest value, so no code overflows; the floor keeps 1 / scale finite for a cell of
-// zeros. max|y| is taken over the bit patterns as integers, where a NaN is larger than every number, so a NaN reaches the
-// scale instead of being dropped by a float maximum.
+// 8-bit forms cut the row into cells (the whole row, or `group` columns): scale = max(max|y| / 448, 2^-126), code = e4m3(y
+// / scale). 448 is e4m3's largest value, so no code overflows; the floor keeps 1 / scale finite for a cell of zeros. max|y|
+// is taken over the bit patterns as integers, where a NaN is larger than every number, so a NaN reaches the scale instead
+// of being dropped by a float maximum.
 //
 // Design: pure memory traffic, so one pass: a workgroup holds one row in registers (kV vectors of 8 elements a thread,
-// thread t's vector v at column 8 (v * threads + t), so a wavefront reads 1 KB of consecutive bf16), all its loads requested
-// before the first is used, and everything after them (sum of squares, largest magnitude) is a reduction over registers.
-// Rows of odd widths or strides take the same path: gfx950 loads 16 bytes from any address that suits the element, and
-// only the last few columns of a row, fewer than 8, go one by one.
+// thread t's vector v at column 8 (v * threads + t), so a wavefront reads 1 KB of consecutive bf16), all its loads
+// requested before the first is used, and everything after them (sum of squares, largest magnitude) is a reduction over
+// registers. Rows of odd widths or strides take the same path: gfx950 loads 16 bytes from any address that suits the
+// element, and only the last few columns of a row, fewer than 8, go one by one.
 
 #include <initializer_list>
 #include <type_traits>
@@ -422,9 +422,10 @@ bool ScalesClash(const RoostDeviceSpan& scales, uint64_t count, std::initializer
 
 // ---- Launch --------------------------------------------------------------------------------------------------------------
 
-// Vectors a thread holds and threads of a row's workgroup: one vector a thread as long as the row's threads fit a workgroup, for
-// more of a row's wavefronts hide more of each other's waits. Against 2 and 4 a thread: 8,192 rows of 4,096 bf16 onto f32 70.9
-// and 75.9 us, 64 rows of 4,096 to e4m3 4.1 and 5.0 us, 6,007 rows of 5,000 to e4m3 by groups 49 and 58 us (4 a thread).
+// Vectors a thread holds and threads of a row's workgroup: one vector a thread as long as the row's threads fit a
+// workgroup, for more of a row's wavefronts hide more of each other's waits. Against 2 and 4 a thread: 8,192 rows of 4,096
+// bf16 onto f32 70.9 and 75.9 us, 64 rows of 4,096 to e4m3 4.1 and 5.0 us, 6,007 rows of 5,000 to e4m3 by groups 49 and 58
+// us (4 a thread).
 struct Shape {
   int per_thread;
   uint32_t threads;
