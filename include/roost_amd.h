@@ -281,12 +281,14 @@ ROOST_API RoostStatus roost_amd_silu_mul_quant_run(RoostContext* ctx, const void
  *     group_size 0): weight f8e4m3, a scale for each row of x and of weight, adapters bf16, output bf16 or f32.
  *   - weight NULL: the adapters alone, on top of the addend (a product that ran elsewhere) or alone.
  *   - lora_a NULL: no adapters (adapters = max_rank = 0; lora_slots, lora_b, lora_scale and ranks unused).
- *   - addend: bf16 or f32, may be exactly the output (same address, stride and type); any other overlap of the output is refused.
- * Sums are f32. In bf16 the low-rank rows A_a x are rounded to bf16 once where many rows are multiplied together.
- * x, weight, lora_a and lora_b are 16-byte aligned; in_dim and x_stride are multiples of 16 bytes; max_rank is a multiple of
- * 8 up to 128. cu_seqlens[0] = 0 and cu_seqlens does not go backwards (device data, not checked; a table that breaks this
- * leaves rows unwritten or gives them a neighbour's adapter, and reads and writes nothing outside the spans). The results
- * of a row may differ in rounding with the number of tokens of the call. */
+ *   - addend: bf16 or f32, may be exactly the output (same address, stride and type); any other overlap of the output is
+ *     refused.
+ * Sums are f32. Beside bf16 adapters the low-rank rows lora_scale[a] A_a x_t may be rounded to bf16 once under a bf16 output
+ * (off by at most 2^-8 of each); under an f32 output they keep 24 bits.
+ * x, weight, lora_a and lora_b are 16-byte aligned; in_dim and x_stride are multiples of 16 bytes and, like out_dim, at most
+ * 2^20 elements; tokens are below 2^20; max_rank is a multiple of 8 up to 128. cu_seqlens[0] = 0 and cu_seqlens does not go
+ * backwards (device data, not checked; a table that breaks this leaves the rows in question unwritten or undefined, and reads
+ * and writes nothing outside the spans). The results of a row may differ in rounding with the number of tokens of the call. */
 typedef struct RoostAmdGemmLoraParams {
   uint32_t struct_size;
   uint32_t abi_minor;
