@@ -205,7 +205,7 @@ ROOST_API RoostStatus roost_qkv_qk_norm_rope_cache_write_run(RoostContext* ctx, 
  * The norm takes the f32 sum, not the rounded residual_out; each output is rounded once. Without a residual (NULL
  * address) s = input; without a residual_out the sum is not stored. output and residual_out may each be exactly the
  * input or the residual (same address, stride and type); any other overlap is refused. A row's result does not depend on
- * the other rows of the call. dim <= 32768. */
+ * the other rows of the call. dim <= 32768; rows up to 4,194,303 of any width. */
 typedef struct RoostAmdAddRmsNormParams {
   uint32_t struct_size;
   uint32_t abi_minor;
@@ -253,7 +253,8 @@ typedef struct RoostAmdAddRmsNormQuantParams {
 ROOST_API RoostStatus roost_amd_add_rms_norm_quant_run(RoostContext* ctx, const void* params, void* stream);
 
 /* SiluMulQuant. y = gate * sigmoid(gate) * up in f32, then 8 bits and scales as AddRmsNormQuant's. gate and up may be the
- * halves of one fused projection (row strides); the outputs overlap nothing. dim <= 32768. */
+ * halves of one fused projection (row strides); the outputs overlap nothing. dim <= 32768;
+ * rows up to 4,194,303 of any width. */
 typedef struct RoostAmdSiluMulQuantParams {
   uint32_t struct_size;
   uint32_t abi_minor;

@@ -357,8 +357,25 @@ roost::Gate& RowSpan(roost::Gate& gate, const char* name, const RoostDeviceSpan&
   return gate.Tensor(name, s, dtype, need).Aligned(name, s.address, roost::ElementBytes(dtype));
 }
 
-roost::Gate& Width(roost::Gate& gate, uint32_t dim) {
-  return gate.Expect(dim > 0 && dim <= kMaxDim, ROOST_STATUS_UNSUPPORTED, "dim = %u; built for 1 to %u columns", dim, kMaxDim);
+// Vectors a thread holds and threads of a row's workgroup: one vector a thread as long as the row's threads fit a
+// workgroup, for more of a row's wavefronts hide more of each other's waits. Against 2 and 4 a thread: 8,192 rows of 4,096
+// bf16 onto f32 70.9 and 75.9 us, 64 rows of 4,096 to e4m3 4.1 and 5.0 us, 6,007 rows of 5,000 to e4m3 by groups 49 and 58
+// us (4 a thread).
+struct Shape {
+  int per_thread;
+  uint32_t threads;
+};
+Shape ShapeOf(uint32_t dim) {
+  const uint64_t vectors = roost::CeilDiv(dim, 8);
+  const int v = vectors <= kMaxThreads ? 1 : vectors <= 2 * kMaxThreads ? 2 : 4;
+  return Shape{v, static_cast<uint32_t>(roost::RoundUp(roost::CeilDiv(vectors, v), 64))};
+}
+
+roost::Gate& Size(roost::Gate& gate, uint32_t rows, uint32_t dim) {
+  gate.Expect(dim > 0 && dim <= kMaxDim, ROOST_STATUS_UNSUPPORTED, "dim = %u; built for 1 to %u columns", dim, kMaxDim);
+  if (!gate.ok()) return gate;
+  return gate.Expect(uint64_t{rows} * ShapeOf(dim).threads < 1ull << 32, ROOST_STATUS_UNSUPPORTED,
+                     "rows = %u of %u columns; a launch is below 2^32 threads, %u to a row", rows, dim, ShapeOf(dim).threads);
 }
 
 roost::Gate& Quant(roost::Gate& gate, const RoostDeviceSpan& y, const RoostDeviceSpan& scales, uint32_t rows, uint32_t dim,
@@ -380,7 +397,7 @@ QuantArgs MakeQuant(const RoostDeviceSpan& y, const RoostDeviceSpan& scales, uin
 // The rules the two norms share; `p` is either params struct.
 template <typename Params>
 void AdmitNorm(roost::Gate& gate, const Params& p, uint32_t out_type) {
-  Width(gate, p.dim)
+  Size(gate, p.rows, p.dim)
       .Expect(FloatType(p.input.dtype), ROOST_STATUS_UNSUPPORTED, "input is %s; built for bf16 and f32",
               roost::Describe(p.input.dtype).name)
       .Expect(FloatType(p.weight.dtype), ROOST_STATUS_UNSUPPORTED, "weight is %s; built for bf16 and f32",
@@ -421,20 +438,6 @@ bool ScalesClash(const RoostDeviceSpan& scales, uint64_t count, std::initializer
 }
 
 // ---- Launch --------------------------------------------------------------------------------------------------------------
-
-// Vectors a thread holds and threads of a row's workgroup: one vector a thread as long as the row's threads fit a
-// workgroup, for more of a row's wavefronts hide more of each other's waits. Against 2 and 4 a thread: 8,192 rows of 4,096
-// bf16 onto f32 70.9 and 75.9 us, 64 rows of 4,096 to e4m3 4.1 and 5.0 us, 6,007 rows of 5,000 to e4m3 by groups 49 and 58
-// us (4 a thread).
-struct Shape {
-  int per_thread;
-  uint32_t threads;
-};
-Shape ShapeOf(uint32_t dim) {
-  const uint64_t vectors = roost::CeilDiv(dim, 8);
-  const int v = vectors <= kMaxThreads ? 1 : vectors <= 2 * kMaxThreads ? 2 : 4;
-  return Shape{v, static_cast<uint32_t>(roost::RoundUp(roost::CeilDiv(vectors, v), 64))};
-}
 
 // Calls f with the number of vectors as a constant.
 template <typename F>
@@ -528,8 +531,9 @@ extern "C" ROOST_API RoostStatus roost_amd_silu_mul_quant_run(RoostContext* ctx,
   ROOST_GATE_RETURN(gate);
   const auto& p = *static_cast<const RoostAmdSiluMulQuantParams*>(params);
   return roost::CatchAll(kOp, [&]() -> RoostStatus {
-    Width(gate, p.dim).Expect(FloatType(p.gate.dtype), ROOST_STATUS_UNSUPPORTED, "gate is %s; built for bf16 and f32",
-                              roost::Describe(p.gate.dtype).name);
+    Size(gate, p.rows, p.dim)
+        .Expect(FloatType(p.gate.dtype), ROOST_STATUS_UNSUPPORTED, "gate is %s; built for bf16 and f32",
+                roost::Describe(p.gate.dtype).name);
     ROOST_GATE_RETURN(gate);
     RowSpan(gate, "gate", p.gate, p.gate.dtype, p.rows, p.dim, p.gate_stride);
     RowSpan(gate, "up", p.up, p.gate.dtype, p.rows, p.dim, p.up_stride);

@@ -252,3 +252,14 @@ def test_python_checks():
         roost_amd.add_rms_norm_params(t, None, t[0], None, t, eps=1e-6)
     with pytest.raises(ValueError, match="tensors of one call are on"):
         roost_amd.silu_mul_quant_params(t, t, t, t[:, :1])
+
+
+@pytest.mark.parametrize("rows,dim", [(1 << 26, 64), (1 << 26, 512), (1 << 22, 8192), (1 << 22, 32768)])
+def test_rows_of_a_launch(kernels, ctx, rows, dim):
+    """Every row has a workgroup; a launch of 2^32 threads is refused by its size, one row fewer by its spans' lengths."""
+    for struct, fn in ((abi.AddRmsNormParams, "add_rms_norm"), (abi.AddRmsNormQuantParams, "add_rms_norm_quant"),
+                       (abi.SiluMulQuantParams, "silu_mul_quant")):
+        for fewer, want in ((0, abi.UNSUPPORTED), (1, abi.INVALID_ARGUMENT)):
+            p = _silu() if fn == "silu_mul_quant" else _norm(struct)
+            p.rows, p.dim = rows - fewer, dim
+            assert getattr(kernels.dll, f"roost_amd_{fn}_run")(ctx, C.addressof(p), None) == want, kernels.last_error()
