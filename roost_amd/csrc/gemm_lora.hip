@@ -941,9 +941,8 @@ __device__ __forceinline__ void WaitStep() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
 
-// Runs of rows with one adapter that a 32 x 32 tile a wavefront takes step by step; more (one-token sequences) are added
-// element by element.
-constexpr uint32_t kRunsBySteps = 4;
+// Adapters that a tile of 64 x 64 takes step by step; more are added element by element.
+constexpr uint32_t kAdaptersBySteps = 4;
 
 template <typename E, int kN, int kT, int kWN, int kWT, int kStages>
 __global__ void __launch_bounds__(64 * kWN * kWT, 1)
@@ -956,8 +955,8 @@ TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles, uint32_t first) {
   static_assert(kCopiesN * 8 * kWaves == kRowsN && kCopiesT * 8 * kWaves == kRowsT, "every wavefront copies whole rows");
   __shared__ __align__(16) unsigned char lds[kStages * kStage];
   __shared__ int32_t slot[kRowsT];
-  __shared__ int32_t run_start[kRowsT + 1];  // the rows where the adapter changes
-  __shared__ uint32_t run_count;
+  __shared__ int32_t adapter[kRowsT];  // of the tile's rows, each once
+  __shared__ uint32_t adapter_rank[kRowsT], adapter_count;
   __shared__ __align__(16) float w_scale[kIsE4m3<E> ? kRowsN : 4];
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 
@@ -1034,17 +1033,24 @@ TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles, uint32_t first) {
     }
   }
   __syncthreads();
-  if (wave == 0) {
+  if (wave == 0 && g.a != nullptr) {
+    int32_t its[kRowsT / 64];
     uint32_t count = 0;
-    for (uint32_t i = lane; i < kRowsT; i += 64) {
-      const uint64_t starts = __ballot(i == 0 || slot[i] != slot[i - 1]);
-      if (starts >> lane & 1) run_start[count + __popcll(starts & ((uint64_t{1} << lane) - 1))] = i;
-      count += __popcll(starts);
+#pragma unroll
+    for (int c = 0; c < kRowsT / 64; ++c) its[c] = slot[64 * c + lane];
+#pragma unroll
+    for (int c = 0; c < kRowsT / 64; ++c) {
+      for (uint64_t left = __ballot(its[c] >= 0); left != 0; left = __ballot(its[c] >= 0)) {
+        const int32_t one = __builtin_amdgcn_readlane(its[c], __builtin_ctzll(left));
+        if (lane == 0) adapter[count] = one;
+        ++count;
+#pragma unroll
+        for (int k = c; k < kRowsT / 64; ++k) its[k] = its[k] == one ? kNoAdapter : its[k];
+      }
     }
-    if (lane == 0) {
-      run_start[count] = kRowsT;
-      run_count = count;
-    }
+    WaveSync();
+    for (uint32_t i = lane; i < count; i += 64) adapter_rank[i] = RankOf(g, adapter[i]);
+    if (lane == 0) adapter_count = count;
   }
 
   // A step is consumed in kPhases phases of kPieces pieces a lane, each in kHalves parts of the wavefront's rows; the
@@ -1130,12 +1136,11 @@ TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles, uint32_t first) {
       }
     }
   }
-  __syncthreads();  // the stages are free, the runs known
+  __syncthreads();  // the stages are free, the adapters known
 
-  // The adapters, one run of rows after the other, by the same steps: 128 bytes of the ranks of the adapter's outputs and
-  // of the low-rank rows. A row takes only its own run's sums, so that no adapter's values, whatever they are, reach
-  // another's rows. acc[n][t], register i, lane l: row wt + 32 t + l % 32, output wn + 32 n + 8 (i / 4) + 4 (l / 32) + i %
-  // 4.
+  // The adapters of the tile, one after the other, by the same steps: 128 bytes of the ranks of the adapter's outputs and of
+  // the low-rank rows. A row takes only its own adapter's sums, so that no adapter's values, whatever they are, reach
+  // another's rows. acc[n][t], register i, lane l: row wt + 32 t + l % 32, output wn + 32 n + 8 (i / 4) + 4 (l / 32) + i % 4.
   if constexpr (kIsE4m3<E>) {
     if (g.w != nullptr) {
 #pragma unroll
@@ -1175,21 +1180,21 @@ TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles, uint32_t first) {
     }
   };
   if (kEarly) load_addends();
-  const uint32_t runs = __builtin_amdgcn_readfirstlane(g.a != nullptr ? run_count : 0);
-  if (kN * kT > 1 || runs <= kRunsBySteps) {
+  const uint32_t count = __builtin_amdgcn_readfirstlane(g.a != nullptr ? adapter_count : 0);
+  if (kN * kT > 1 || count <= kAdaptersBySteps) {
     constexpr int kPer = 16 / sizeof(Low);
     const uint32_t row_bytes = g.max_rank * sizeof(Low);
     const uint32_t parts = sizeof(Low) == 2 ? g.parts : 1;
-    // A place in the list of steps: run, part of the low-rank rows, first byte of their ranks.
+    // A place in the list of steps: adapter, part of the low-rank rows, first byte of their ranks.
     struct Place {
-      uint32_t run, part, from;
+      uint32_t index, part, from;
       int32_t slot;
-      uint32_t bytes;  // of the run's ranks
+      uint32_t bytes;  // of the adapter's ranks
     };
-    const auto enter = [&](Place& p) {  // the next run with an adapter, from p.run on
-      for (; p.run < runs; ++p.run) {
-        p.slot = __builtin_amdgcn_readfirstlane(slot[run_start[p.run]]);
-        p.bytes = __builtin_amdgcn_readfirstlane(RankOf(g, p.slot)) * sizeof(Low);
+    const auto enter = [&](Place& p) {  // the next adapter with a rank, from p.index on
+      for (; p.index < count; ++p.index) {
+        p.slot = __builtin_amdgcn_readfirstlane(adapter[p.index]);
+        p.bytes = __builtin_amdgcn_readfirstlane(adapter_rank[p.index]) * sizeof(Low);
         if (p.bytes > 0) break;
       }
       p.part = p.from = 0;
@@ -1199,16 +1204,13 @@ TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles, uint32_t first) {
       if (p.from < p.bytes) return;
       p.from = 0;
       if (++p.part < parts) return;
-      ++p.run;
+      ++p.index;
       enter(p);
     };
     const auto copy_low = [&](const Place& p, uint32_t stage) {
       const uint32_t to_n = lds0 + stage * kStage + 1024 * wave, to_t = to_n + kRowsN * kStepBytes;
       const uint32_t at = p.from + piece;
-      if (at >= p.bytes) {
-        zero(stage);
-        return;
-      }
+      if (at >= p.bytes) return;  // what the stage holds there is not multiplied
       // A row of the pool is at most 512 bytes, so a tile's are within 32 bits of its first.
       const uint64_t b_row = static_cast<uint64_t>(p.slot) * g.out_dim + n0;
       const auto* b_base = static_cast<const unsigned char*>(g.b) + b_row * row_bytes;
@@ -1224,37 +1226,39 @@ TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles, uint32_t first) {
         Copy16(u_base, min(8 * (wave + kWaves * i) + lane / 8, last_t) * row_bytes + at, to_t + 1024 * kWaves * i);
       }
     };
+    int32_t row_slot[kT];
+#pragma unroll
+    for (int t = 0; t < kT; ++t) row_slot[t] = slot[wt + 32 * t + lane % 32];
     Place next{}, now{};
     enter(next);
     now = next;
     uint32_t step = 0;
 #pragma unroll 1
-    for (uint32_t i = 0; i + 1 < kStages && next.run < runs; ++i, advance(next)) copy_low(next, i);
+    for (uint32_t i = 0; i + 1 < kStages && next.index < count; ++i, advance(next)) copy_low(next, i);
 #pragma unroll 1
-    for (; now.run < runs; advance(now), ++step) {
+    for (; now.index < count; advance(now), ++step) {
       if constexpr (kStages == 1) {
         __syncthreads();  // the step before is read
         copy_low(now, 0);
         WaitStep<0>();
       } else {
         WaitStep<0>();
-        if (next.run < runs) {
+        if (next.index < count) {
           copy_low(next, (step + kStages - 1) % kStages);
           advance(next);
         }
       }
       const unsigned char* from = lds + (step % kStages) * kStage;
-      const auto lo = static_cast<uint32_t>(run_start[now.run]), hi = static_cast<uint32_t>(run_start[now.run + 1]);
 #pragma unroll
       for (int t = 0; t < kT; ++t) {
-        const uint32_t row = wt + 32 * t + lane % 32;
-        const bool mine = row >= lo && row < hi;
+        const bool mine = row_slot[t] == now.slot;
         if (__ballot(mine) == 0) continue;
         f32x16_t d[kN];
 #pragma unroll
         for (int n = 0; n < kN; ++n) d[n] = f32x16_t{};
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
+          if (now.from + 32 * p >= now.bytes) break;
           const auto left = static_cast<int32_t>(now.bytes / sizeof(Low)) -
                             static_cast<int32_t>(now.from / sizeof(Low) + kPer * (2 * p + lane / 32));
           const u32x4_t fu =
