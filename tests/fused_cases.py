@@ -17,6 +17,7 @@ BF16, F32, F8 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
 HALF = {BF16: 2.0 ** -8, F32: 2.0 ** -24}
 NORM, SILU = 2.0 ** -18, 2.0 ** -17
 ADD = 2.0 ** -23
+PRODUCTS = 2.0 ** -10
 
 
 def rounded_bound(y, dtype, more):
@@ -126,6 +127,7 @@ class Lora:
         y = torch.zeros((live, out_dim), dtype=torch.float64, device="cuda")
         size = torch.zeros_like(y)   # sums of magnitudes that f32 additions run over
         low = torch.zeros_like(y)    # those of the low-rank rows, which bf16 rounds once
+        cut = 0.0
         terms = x.shape[1] + self.max_rank + 16
         if self.weight is not None:
             w = self.weight.double()
@@ -133,6 +135,9 @@ class Lora:
                 w = w * self.w_scale.double()[:, None]
             y += x[:live] @ w.T
             size += x[:live].abs() @ w.abs().T
+            if self.x_scale is not None and self.y.dtype == BF16:
+                eights = [v.abs().reshape(v.shape[0], -1, 8).amax(2) for v in (x[:live], w)]
+                cut = PRODUCTS * (eights[0] @ eights[1].T)
         at = 0
         for n, a in zip(self.lens, self.slots):
             if n and self.lora_a is not None and 0 <= a < self.adapters:
@@ -148,7 +153,7 @@ class Lora:
         if self.addend is not None:
             y += self.addend[:live].double()
             size += self.addend[:live].double().abs()
-        more = terms * ADD * size
+        more = terms * ADD * size + cut
         if self.low == BF16:
             more = more + 2.0 ** -8 * (low + more)
         return y, rounded_bound(y, self.y.dtype, more)

@@ -397,3 +397,36 @@ def test_other_sessions_device_is_refused(session):
     p._device = torch.device("cuda", 1)
     with pytest.raises(ValueError, match="session on"):
         roost_amd.gemm_lora(session, p)
+
+
+# Tiles of many rows with one to many adapters each, of pool ranks that share a step of the ranks (up to 32 and 64 bytes of a row)
+# and that do not; the same adapters come again and again.
+@pytest.mark.parametrize("x,out", TYPES)
+@pytest.mark.parametrize("max_rank,adapters", [(8, 3), (8, 70), (16, 5), (16, 41), (24, 9), (32, 30), (64, 6)])
+@pytest.mark.parametrize("tokens,out_dim", [(100, 12200), (300, 5001), (1500, 2901)])
+def test_adapters_of_a_tile(session, tokens, out_dim, max_rank, adapters, x, out):
+    lens = _lens(tokens, 20)
+    c = Lora(86, lens, [(11 * i + i // 7) % (adapters + 1) - 1 for i in range(len(lens))], in_dim=80, out_dim=out_dim,
+             adapters=adapters, max_rank=max_rank, ranks=[(max_rank, 1, 5, 0, max_rank - 1, 8)[i % 6] for i in range(adapters)],
+             x=x, out=out, pad=2)
+    _run(session, c)
+    c.check(f"{adapters} adapters of rank {max_rank}")
+
+
+@pytest.mark.parametrize("max_rank", [8, 16, 32, 48])
+def test_adapters_of_a_tile_keep_apart(session, max_rank):
+    """One broken adapter among many that share a tile and a step, and what the pool holds past the others' ranks."""
+    lens = [1, 2] * 110
+    slots = [i % 7 for i in range(220)]
+    c = Lora(87, lens, slots, in_dim=128, out_dim=6000, adapters=7, max_rank=max_rank, ranks=[max_rank, 3, max_rank - 1, 0, 7, 8, 1])
+    _run(session, c)
+    clean = c.y.clone()
+    for a, r in enumerate(c.ranks_h):
+        c.lora_a[a, r:] = float("nan")
+        c.lora_b[a, :, r:] = float("inf")
+    c.lora_a[2] = float("nan")
+    c.lora_b[4] = float("inf")
+    _run(session, c)
+    rows = torch.tensor([s for n, s in zip(lens, slots) for _ in range(n)], device="cuda")
+    hit = (rows == 2) | (rows == 4)
+    assert torch.equal(c.y[~hit], clean[~hit]) and not torch.isfinite(c.y[hit]).any()
