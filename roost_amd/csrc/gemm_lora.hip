@@ -931,10 +931,10 @@ __global__ void __launch_bounds__(64 * 12) FewRowsKernel(LoraArgs g) {
 // read at one piece are then free of bank conflicts (with p ^ (row % 8) each read takes half as long again). The copy
 // writes LDS in lane order, so it is the lanes' source addresses that are permuted.
 //
-// Bound by the matrix instructions and what keeps them fed. 15,000 rows, 4096 to 4096 channels, bf16, rank 64: about 445 us of
-// 256 x 256 tiles, 1.14 PFLOP/s, where a plain library product of these sizes takes 356 us; 944 tiles are 3.7 rounds of the
+// Bound by the matrix instructions and what keeps them fed. 15,000 rows, 4096 to 4096 channels, bf16, rank 64: about 435 us of
+// 256 x 256 tiles, 1.16 PFLOP/s, where a plain library product of these sizes takes 356 us; 944 tiles are 3.7 rounds of the
 // CUs, the instructions and their LDS reads by themselves 365 us, the copies 60 and the last store 50 more. e4m3 rows, 6,700 x
-// 4096 x 12288, rank 32: 1.9 PFLOP/s.
+// 4096 x 12288, rank 32: 2.0 PFLOP/s.
 
 // Every copy but this wavefront's last kLeft has landed, its own LDS reads have returned, and then every wavefront's.
 template <int kLeft>
@@ -942,9 +942,10 @@ __device__ __forceinline__ void WaitStep() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLeft) : "memory");
 }
 
-// Adapters that a tile of 64 x 64 takes step by step; more are added element by element. 100 rows, 4096 to 12288, 16 adapters
-// a tile: 59 us by steps and 53 by elements, 64: 79 and 57.
-constexpr uint32_t kAdaptersBySteps = 4;
+// Adapters that a tile of 64 x 64 takes step by step; more are added element by element, whose time grows with the rank where
+// a step's does not. 100 rows, 4096 to 12288: 16 adapters of rank 16 59 us by steps and 53 by elements, 64 of them 79 and 57;
+// 16 of rank 64 71 and 90, 64 of them 104 and 107.
+__device__ __forceinline__ uint32_t AdaptersBySteps(uint32_t max_rank) { return max(4u, max_rank / 4); }
 
 template <typename E, int kN, int kT, int kWN, int kWT, int kStages>
 __global__ void __launch_bounds__(64 * kWN * kWT, 1)
@@ -1183,7 +1184,7 @@ TileKernel(LoraArgs g, uint32_t n_tiles, uint32_t t_tiles, uint32_t first) {
   };
   if (kEarly) load_addends();
   const uint32_t count = __builtin_amdgcn_readfirstlane(g.a != nullptr ? adapter_count : 0);
-  if (kN * kT > 1 || count <= kAdaptersBySteps) {
+  if (kN * kT > 1 || count <= AdaptersBySteps(g.max_rank)) {
     constexpr int kPer = 16 / sizeof(Low);
     const uint32_t row_bytes = g.max_rank * sizeof(Low);
     const uint32_t parts = sizeof(Low) == 2 ? g.parts : 1;
@@ -1549,7 +1550,7 @@ void LaunchAll(const LoraArgs& g, hipStream_t stream) {
   if (roost::CeilDiv(g.out_dim, 32) * roost::CeilDiv(g.tokens, 64) <= kCus) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
   if (roost::CeilDiv(g.out_dim, 80) * roost::CeilDiv(g.tokens, 64) <= kCus) return LaunchProduct<E, 5, 4, 4, 4, 2>(g, stream);
   if (g.tokens <= 64) return LaunchProduct<E, 2, 4, 4, 8, 3>(g, stream);
-  // The adapters alone move an addend and an output: small tiles, many to a CU (4,480 rows of 4096 outputs, rank 16: 26 us,
+  // The adapters alone move an addend and an output: small tiles, many to a CU (4,480 rows of 4096 outputs, rank 16: 22 us,
   // by 256 x 256 36 us).
   if (g.w == nullptr) return LaunchTiles<E, 1, 2, 2, 1, 1>(g, 0, g.tokens, stream);
   // Tiles of many rows: a CU holds one workgroup of 256 x 256, 256 x 128 or 128 x 128, so they go in rounds of kCus, and a
