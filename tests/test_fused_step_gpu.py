@@ -65,7 +65,8 @@ class Layer:
                 mapping.append(int(perm[self.indptr_h[s] + p // PAGE]) * PAGE + p % PAGE)
         self.positions, self.mapping = i32(positions + [0] * pad).cuda(), torch.tensor(mapping + [-1] * pad).cuda()
         e = lambda *s, dtype=BF16: torch.zeros(s, dtype=dtype, device="cuda")  # noqa: E731
-        self.residual, self.h, self.h8, self.h8_scale = self.residual0.clone(), e(t, DIM), e(t, DIM, dtype=F8), e(t, 1, dtype=F32)
+        self.residual, self.h = self.residual0.clone(), e(t, DIM)
+        self.h8, self.h8_scale = e(t, DIM, dtype=F8), e(t, 1, dtype=F32)
         self.qkv_y, self.q, self.attn = e(t, (HQ + 2 * HK) * HD), e(t, HQ, HD), e(t, HQ, HD)
         self.gate_up, self.act8, self.act8_scale = e(t, 2 * MLP), e(t, MLP, dtype=F8), e(t, 1, dtype=F32)
 
@@ -91,7 +92,8 @@ class Layer:
                 f(*args, **kw)
 
         # h = norm(residual + x), the residual in place
-        roost_amd.add_rms_norm(s, roost_amd.add_rms_norm_params(self.x, self.residual, self.norm1, self.residual, self.h, eps=EPS))
+        p = roost_amd.add_rms_norm_params(self.x, self.residual, self.norm1, self.residual, self.h, eps=EPS)
+        roost_amd.add_rms_norm(s, p)
         looked(self.check_norm, self.x, self.residual0)
         self.lora("qkv", self.qkv, self.h, self.qkv_y)
         looked(self.check_lora, "q/k/v", self.qkv, self.h, self.qkv_y)
@@ -134,7 +136,8 @@ class Layer:
         at = 0
         for s, (n, kv) in enumerate(zip(self.lens, self.kv_lens)):
             pages = self.indices[self.indptr_h[s]:self.indptr_h[s + 1]].long()
-            k, v = (c[pages].reshape(-1, HK, HD)[:kv].float().repeat_interleave(HQ // HK, 1) for c in (self.k_cache, self.v_cache))
+            k, v = (c[pages].reshape(-1, HK, HD)[:kv].float().repeat_interleave(HQ // HK, 1)
+                    for c in (self.k_cache, self.v_cache))
             q = self.q[at:at + n].float()
             score = (q[:, None] * k[None]).sum(-1) * HD ** -0.5  # [n, kv, heads]
             past = torch.arange(kv, device="cuda")[None] <= torch.arange(kv - n, kv, device="cuda")[:, None]
@@ -149,7 +152,8 @@ class Layer:
             self.q[:self.live], self.attn[:self.live], self.k_cache, self.v_cache, self.q_indptr, self.indptr, self.indices,
             self.last, q_indptr_host=self.q_indptr_h, kv_indptr_host=self.indptr_h, kv_last_page_len_host=self.last_h,
             batch=len(self.lens), q_heads=HQ, kv_heads=HK, head_dim=HD, page_size=PAGE)
-        self.attention_ws = self.session.prepare(self.session.lib.entry(roost_amd.ATTENTION_VARIANT), self.attention, key="step")
+        entry = self.session.lib.entry(roost_amd.ATTENTION_VARIANT)
+        self.attention_ws = self.session.prepare(entry, self.attention, key="step")
 
     @property
     def q_indptr(self):

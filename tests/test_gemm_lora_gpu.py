@@ -314,8 +314,8 @@ def test_tilings_of_adapters_alone(session, tokens, out_dim, long, x):
 def test_low_rank_rows_of_long_prompts(session, max_rank, x, out):
     """Pieces of 64 rows of one sequence, from sequences that start and end anywhere."""
     lens = [3001, 1, 0, 62, 2900, 300]
-    c = Lora(82, lens, [0, 1, 2, 3, 1, 2], in_dim=400, out_dim=72, max_rank=max_rank, ranks=[max_rank, max_rank - 1, 3, 9], x=x,
-             out=out, pad=2)
+    c = Lora(82, lens, [0, 1, 2, 3, 1, 2], in_dim=400, out_dim=72, max_rank=max_rank,
+             ranks=[max_rank, max_rank - 1, 3, 9], x=x, out=out, pad=2)
     _run(session, c)
     c.check(f"pool rank {max_rank}")
 
@@ -399,15 +399,15 @@ def test_other_sessions_device_is_refused(session):
         roost_amd.gemm_lora(session, p)
 
 
-# Tiles of many rows with one to many adapters each, of pool ranks that share a step of the ranks (up to 32 and 64 bytes of a row)
-# and that do not; the same adapters come again and again.
+# Tiles of many rows with few and many adapters each, which come again and again among their rows.
 @pytest.mark.parametrize("x,out", TYPES)
 @pytest.mark.parametrize("max_rank,adapters", [(8, 3), (8, 70), (16, 5), (16, 41), (24, 9), (32, 30), (64, 6)])
 @pytest.mark.parametrize("tokens,out_dim", [(100, 12200), (300, 5001), (1500, 2901)])
 def test_adapters_of_a_tile(session, tokens, out_dim, max_rank, adapters, x, out):
     lens = _lens(tokens, 20)
     c = Lora(86, lens, [(11 * i + i // 7) % (adapters + 1) - 1 for i in range(len(lens))], in_dim=80, out_dim=out_dim,
-             adapters=adapters, max_rank=max_rank, ranks=[(max_rank, 1, 5, 0, max_rank - 1, 8)[i % 6] for i in range(adapters)],
+             adapters=adapters, max_rank=max_rank,
+             ranks=[(max_rank, 1, 5, 0, max_rank - 1, 8)[i % 6] for i in range(adapters)],
              x=x, out=out, pad=2)
     _run(session, c)
     c.check(f"{adapters} adapters of rank {max_rank}")
@@ -415,10 +415,11 @@ def test_adapters_of_a_tile(session, tokens, out_dim, max_rank, adapters, x, out
 
 @pytest.mark.parametrize("max_rank", [8, 16, 32, 48])
 def test_adapters_of_a_tile_keep_apart(session, max_rank):
-    """One broken adapter among many that share a tile and a step, and what the pool holds past the others' ranks."""
+    """Broken adapters among others in a tile, and what the pool holds past the others' ranks."""
     lens = [1, 2] * 110
     slots = [i % 7 for i in range(220)]
-    c = Lora(87, lens, slots, in_dim=128, out_dim=6000, adapters=7, max_rank=max_rank, ranks=[max_rank, 3, max_rank - 1, 0, 7, 8, 1])
+    c = Lora(87, lens, slots, in_dim=128, out_dim=6000, adapters=7, max_rank=max_rank,
+             ranks=[max_rank, 3, max_rank - 1, 0, 7, 8, 1])
     _run(session, c)
     clean = c.y.clone()
     for a, r in enumerate(c.ranks_h):
