@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "row_steps.h"
 
 namespace {
 
@@ -220,7 +221,7 @@ __device__ __forceinline__ f32x16_t Mma32(FragOf<E> a, FragOf<E> b, f32x16_t acc
 // neighbouring lanes. Loading the fragments themselves, 16 rows at a time with neighbouring lanes in different rows, costs
 // one address cycle a lane instead of one for each four: 30 us instead of 15 for a decode product of 64 x 6,144 over 4,096.
 
-constexpr uint32_t kStepBytes = 128;
+using roost::kStepBytes;
 
 // An address that is the same in every lane, in scalar registers whatever the compiler can prove of it.
 __device__ __forceinline__ const unsigned char* Uniform(const unsigned char* p) {
@@ -262,7 +263,7 @@ struct RowStream {
     unsigned char* to = lds + stage * kStage;
     const uint32_t to_lds = __builtin_amdgcn_readfirstlane(LdsAddress(to));
     const unsigned char *from_a = Uniform(base_a + at * kSub), *from_b = Uniform(base_b + at);
-    if (at + kStepBytes <= bytes) {
+    if (roost::WholeStep(at, bytes)) {
 #pragma unroll
       for (int i = 0; i < kA / 8; ++i) Copy16(from_a, off_a[i], to_lds + 1024 * i);
 #pragma unroll
@@ -270,10 +271,10 @@ struct RowStream {
       return;
     }
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {  // the last, partial step: pieces past the rows' end are zeros
+    for (int i = 0; i < kCopies; ++i) {  // the last, partial step: pieces past the rows' end are zeros, and no copies
       const bool a = i < kA / 8;
       const uint32_t half = a ? 8 * i / (kA / kSub) : 0;
-      if (a ? at * kSub + half * kStepBytes + piece < bytes * kSub : at + piece < bytes) {
+      if (roost::CopiesPiece(at, half, piece, bytes, a ? kSub : 1)) {
         if (a) {
           Copy16(from_a, off_a[a ? i : 0], to_lds + 1024 * i);
         } else {
@@ -289,7 +290,7 @@ struct RowStream {
   // stage into registers when it returns.
   template <typename U>
   __device__ __forceinline__ void Run(uint32_t first, uint32_t stride, U&& use) const {
-    const uint32_t steps = first < bytes ? (bytes - first + stride - 1) / stride : 0;
+    const uint32_t steps = roost::StepsOf(first, stride, bytes), by_count = roost::StepsByCount(first, stride, bytes);
 #pragma unroll
     for (uint32_t i = 0; i < kStages; ++i) {
       if (i < steps) Copy(first + i * stride, i);
@@ -297,7 +298,7 @@ struct RowStream {
     uint32_t stage = 0;
 #pragma unroll 1
     for (uint32_t i = 0; i < steps; ++i) {
-      if (i + kStages <= steps) {
+      if (i + kStages <= by_count) {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 1) * kCopies) : "memory");
       } else {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(64 * kWaves) ShrinkKernel(LoraArgs g) {
   Stream rows;
   rows.lds = lds + wave * Stream::kBytes;
   rows.bytes = g.in_dim * sizeof(E);
-  rows.piece = 16 * ((lane % 8) ^ (lane / 8));
+  rows.piece = roost::PieceOfLane(lane);
   rows.base_b = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.x) + from * g.x_stride);
   // Rows past the piece's and ranks past the adapter's repeat the last; what they give is not stored.
 #pragma unroll
@@ -719,7 +720,7 @@ __global__ void __launch_bounds__(64 * (kWaves + kLow)) ProductKernel(LoraArgs g
     Stream rows;
     rows.lds = lds + wave * Stream::kBytes;
     rows.bytes = g.in_dim * sizeof(E);
-    rows.piece = 16 * ((lane % 8) ^ (lane / 8));
+    rows.piece = roost::PieceOfLane(lane);
     rows.base_a = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.w) + static_cast<uint64_t>(n0) * g.in_dim);
     rows.base_b = reinterpret_cast<const unsigned char*>(static_cast<const E*>(g.x) + t0 * g.x_stride);
     // Rows past the last output or token repeat the last one; what they give is not stored.
@@ -798,7 +799,7 @@ __global__ void __launch_bounds__(64 * 12) FewRowsKernel(LoraArgs g) {
   const uint32_t tiles = gridDim.x, xcd = blockIdx.x % 8;
   const uint32_t n0 = 16 * (xcd * (tiles / 8) + min(xcd, tiles % 8) + blockIdx.x / 8);
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint32_t piece = 16 * ((lane % 8) ^ (lane / 8));
+  const uint32_t piece = roost::PieceOfLane(lane);
   const uint32_t x_row = min(lane / 8, g.tokens - 1) * static_cast<uint32_t>(g.x_stride * sizeof(E)) + piece;
   const auto* x = static_cast<const unsigned char*>(g.x);
 
