@@ -106,10 +106,11 @@ __device__ __forceinline__ Sequence SequenceOf(const LoraArgs& g, uint32_t b) {
 }
 
 // slot[i] of each lane's sequence's rows, by whole wavefronts (rows t0 .. t0 + n - 1 of the call are slot[0 ..]): a lane
-// writes a short sequence's itself, a long one's are written by its wavefront.
+// writes a short sequence's itself, a long one's are written by its wavefront. The last tile may start part of itself past the
+// call's rows: there no row is anyone's, whatever the table says.
 __device__ __forceinline__ void PutSlots(const LoraArgs& g, Sequence q, uint32_t t0, uint32_t n, int32_t* slot) {
   constexpr int32_t kShort = 4;
-  const int64_t rows = min(n, g.tokens - t0), start = t0;
+  const int64_t rows = t0 < g.tokens ? min(n, g.tokens - t0) : 0, start = t0;
   const auto lo = static_cast<int32_t>(min(max(q.from - start, int64_t{0}), rows));
   const auto hi = static_cast<int32_t>(min(max(q.to - start, int64_t{0}), rows));
   const int32_t s = q.slot < 0 || static_cast<uint32_t>(q.slot) >= g.adapters ? kNoAdapter : q.slot;

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import fused_cases
 import roost_amd
 from fused_cases import BF16, F32, F8, Lora
 
@@ -431,3 +432,30 @@ def test_adapters_of_a_tile_keep_apart(session, max_rank):
     rows = torch.tensor([s for n, s in zip(lens, slots) for _ in range(n)], device="cuda")
     hit = (rows == 2) | (rows == 4)
     assert torch.equal(c.y[~hit], clean[~hit]) and not torch.isfinite(c.y[hit]).any()
+
+
+# Tables that the documentation rules out: past the call's rows, backwards, below zero. Each ends in what belongs to the call.
+# 33 to 65 rows and 300 by 80 outputs: tiles whose last rows start past the call's; the others: the tiles of many rows.
+@pytest.mark.parametrize("x,out", [(BF16, BF16), (F8, BF16), (F32, F32)])
+@pytest.mark.parametrize("tokens,out_dim", [(6, 40), (15, 40), (31, 300), (33, 40), (40, 9000), (65, 40), (300, 2100), (300, 5001),
+                                            (1020, 2100), (1500, 2901)])
+def test_a_broken_table_writes_nothing_behind_the_call(session, tokens, out_dim, x, out):
+    first = tokens // 3
+    c = Lora(93, [first, tokens - first], [1, 2], in_dim=144, out_dim=out_dim, max_rank=8, x=x, out=out, addend=out)
+    want, bound = c.want()
+    guard = 300  # rows behind the call's, in the same allocations
+    wide = {}
+    for name in ("y", "addend", "x_scale"):
+        t = getattr(c, name)
+        if t is not None:
+            wide[name] = torch.cat([t, torch.full((guard, *t.shape[1:]), 7.0, device="cuda").to(t.dtype)])
+            setattr(c, name, wide[name][:tokens])
+    big = (1 << 31) - 1
+    for table in ([0, first, tokens + 200], [0, first, big], [0, tokens + 200, tokens], [0, big, tokens], [-big, first, big],
+                  [0, first, -5], [tokens + 7, tokens + 9, big]):
+        c.cu.copy_(torch.tensor(table, dtype=torch.int32))
+        wide["y"][:tokens] = c.before
+        _run(session, c)
+        assert all((t[tokens:].float() == 7).all() for t in wide.values()), table
+        if table[0] <= 0 and table[1] == first:  # the first sequence is as it should be
+            fused_cases.assert_within(c.y[:first], want[:first], bound[:first], str(table))
