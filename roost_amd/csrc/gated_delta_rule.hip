@@ -980,10 +980,11 @@ __device__ __forceinline__ uint32_t LdsAddr(const void* p) {
 
 // global -> LDS copies (global_load_lds): lane l's bytes land at lds + size * l; lds must be wave-uniform. Issued from
 // inline assembly so that the compiler does not treat every later LDS access as waiting on them (it cannot tell which
-// LDS bytes they write); the scan waits for them itself, one chunk later. M0 carries the LDS address and is restored.
+// LDS bytes they write); the scan waits for them itself, one chunk later. M0 carries the LDS address and is restored; the copy
+// may read it one wait state after its write (s_nop), which the compiler does not see to inside an assembly block.
 __device__ __forceinline__ void Dma16(const void* g, uint32_t lds) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(g), "s"(lds));
 }
 // s_waitcnt vmcnt(0) alone (expcnt and lgkmcnt fields at their maxima).
@@ -1374,7 +1375,7 @@ struct Stage {
 // at lds + 16 l. M0 carries the LDS address and is restored.
 __device__ __forceinline__ void DmaS(const void* sbase, uint32_t voff, uint32_t lds) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(voff), "s"(sbase), "s"(lds));
 }
 
@@ -1383,7 +1384,7 @@ __device__ __forceinline__ void DmaS(const void* sbase, uint32_t voff, uint32_t 
 // 0.166 ms).
 __device__ __forceinline__ void DmaSNt(const void* sbase, uint32_t voff, uint32_t lds) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2 nt\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(voff), "s"(sbase), "s"(lds));
 }
 

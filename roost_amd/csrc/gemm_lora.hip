@@ -232,10 +232,11 @@ __device__ __forceinline__ const unsigned char* Uniform(const unsigned char* p) 
   return reinterpret_cast<const unsigned char*>(hi << 32 | (lo & 0xFFFFFFFFu));
 }
 
-// 16 bytes a lane from memory to LDS: lane l's land at lds + 16 l. No register is written; the caller waits.
+// 16 bytes a lane from memory to LDS: lane l's land at lds + 16 l. No register is written; the caller waits. The copy may read
+// M0 one wait state after its write (s_nop), which the compiler does not see to inside an assembly block.
 __device__ __forceinline__ void Copy16(const void* base, uint32_t off, uint32_t lds) {
   uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(m0) : "v"(off), "s"(base), "s"(lds) : "memory");
 }
 

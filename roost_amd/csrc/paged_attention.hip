@@ -2086,17 +2086,18 @@ __device__ __forceinline__ uint32_t LdsAddr(const void* p) {
 }
 
 // global -> LDS copy of 16 bytes per lane (lane l lands at lds + 16 l; lds wave-uniform), from inline assembly so that
-// the compiler does not make every later LDS access wait on it; the kernel waits for it itself. M0 is restored.
+// the compiler does not make every later LDS access wait on it; the kernel waits for it itself. M0 is restored; the copy may
+// read it one wait state after its write (s_nop), which the compiler does not see to inside an assembly block.
 __device__ __forceinline__ void Dma16(const void* g, uint32_t lds) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(g), "s"(lds));
 }
 
 // The same with a wave-uniform 64-bit base in SGPRs and a 32-bit per-lane byte offset.
 __device__ __forceinline__ void Dma16(const void* sbase, uint32_t voff, uint32_t lds) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(voff), "s"(sbase), "s"(lds));
 }
 
@@ -2105,7 +2106,7 @@ __device__ __forceinline__ void Dma16(const void* sbase, uint32_t voff, uint32_t
 template <int kOff>
 __device__ __forceinline__ void Dma16At(const void* sbase, uint32_t voff, uint32_t lds) {
   uint32_t save;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4\n\ts_mov_b32 m0, %0"
                : "=&s"(save) : "v"(voff), "s"(sbase), "s"(lds - kOff), "i"(kOff));
 }
 
