@@ -228,8 +228,8 @@ ROOST_API RoostStatus roost_amd_add_rms_norm_run(RoostContext* ctx, const void* 
 
 /* AddRmsNormQuant. AddRmsNorm with its output y in 8 bits (OCP e4m3) and a scale for each cell: a whole row
  * (group_size 0) or group_size consecutive columns of it (a power of two from 16 to 512; the last cell of a row may be
- * shorter). scale = max(max|y| / 448, 2^-126) over the cell's f32 values, code = y / scale rounded to nearest, ties to
- * even, so code * scale stands for y and a cell of zeros has zero codes. A cell that holds a NaN has a NaN scale and NaN
+ * shorter). scale = max(max|y| / 448, 2^-126) over the cell's f32 values, code = the f32 quotient y / scale rounded to
+ * nearest, ties to even, so code * scale stands for y and a cell of zeros has zero codes. A cell that holds a NaN has a NaN scale and NaN
  * codes; one that holds an infinity has an infinite scale, zero codes for its finite values and NaN codes for the others. */
 typedef struct RoostAmdAddRmsNormQuantParams {
   uint32_t struct_size;

@@ -159,6 +159,27 @@ def test_every_code_rounds_to_nearest_even(session):
     assert torch.equal(y.cpu().float()[0], vals.to(F8).float())
 
 
+@pytest.mark.parametrize("top", [1.0, 3.3, 447.9, 12345.678, 1e-3, 7e-30, 2.5e-36, 6e-36, 3e33])
+def test_codes_are_quotients_by_the_scale(session, top):
+    """At scales that are no powers of two: the f32 quotient of each value and the scale, rounded to nearest even, bit for bit.
+    Every e4m3 value and every midpoint between two of them times the scale, and the f32 neighbours of those; a
+    product by the scale's reciprocal gives some of them the other code."""
+    codes = torch.arange(127, dtype=torch.uint8).view(F8).float()
+    mids = (codes[:-1] + codes[1:]) / 2
+    near = torch.cat([codes, mids]) * (torch.tensor(top) / 448)
+    scale = (torch.tensor(top) / 448).clamp(min=2.0 ** -126)
+    near = torch.cat([near] + [torch.nextafter(near, near * k) for k in (0, 2)]).clamp(max=top)
+    vals = torch.cat([torch.tensor([top]), near, -near])
+    up = vals / 64  # silu(64) = 64 in f32
+    vals = up * 64
+    y = torch.empty((1, vals.numel()), device="cuda", dtype=F8)
+    scales = torch.empty((1, 1), device="cuda")
+    gate = torch.full_like(y, 64.0, dtype=F32)
+    roost_amd.silu_mul_quant(session, roost_amd.silu_mul_quant_params(gate, up.cuda()[None], y, scales))
+    assert scales.cpu().item() == scale.item()
+    assert torch.equal(y.cpu().float()[0], (vals / scale).to(F8).float())
+
+
 def test_graph_replays(session):
     """Captured once, replayed with other inputs and eager work in between."""
     xs, residual, weight = _norm_case(8, 40, 2000)
