@@ -31,3 +31,44 @@ def test_low_rank_rows_of_8_bit_rows(session, lens, max_rank, in_dim, out):
         for _ in range(2):
             _run(session, c)
             assert torch.equal(c.y, first)
+
+
+def _lens(tokens, long):
+    """Sequences of one token to `long`, and empty ones."""
+    lens, left, k = [], tokens, 0
+    while left:
+        lens.append(min(left, [1, long, 0, 5, long // 2, 30][k % 6]))
+        left -= lens[-1]
+        k += 1
+    return lens
+
+
+# Rows x outputs that take each of the tilings, with as many steps of 128 bytes as make its ring of stages come round twice and
+# more (by tiles: 2 to 4 stages; by wavefronts that split the steps: 4 or 8 of them and 2 to 4 stages each), the last of them
+# whole or cut. With a few adapters in each tile, whose steps follow in the same ring.
+@pytest.mark.parametrize("x,out", [(BF16, BF16), (BF16, F32), (F32, F32), (F8, BF16), (F8, F32)])
+@pytest.mark.parametrize("cut", [0, 16, 48, 80, 112])
+@pytest.mark.parametrize("tokens,out_dim,steps", [
+    (5, 300, 41),      # one launch
+    (13, 2100, 41),    # 16 outputs x 16 rows
+    (13, 5001, 41),    # 32 x 16
+    (31, 2100, 41),    # 16 x 32
+    (31, 5001, 41),    # 32 x 32
+    (63, 6100, 41),    # 32 x 64
+    (300, 2100, 41),   # 80 x 64
+    (300, 5001, 10),   # 64 x 64
+    (1020, 2100, 10),  # 128 x 128
+    (1500, 2901, 10),  # 256 x 128
+    (2601, 4200, 10),  # 256 x 256
+    (4201, 4200, 10),  # 256 x 256 and 128 x 128
+])
+def test_rings_come_round(session, tokens, out_dim, steps, cut, x, out):
+    size = torch.tensor([], dtype=x).element_size()
+    lens = [tokens] if tokens == 5 else _lens(tokens, 70)
+    c = Lora(steps + cut + tokens, lens, [(3 * i + 1) % 4 for i in range(len(lens))], in_dim=(128 * steps + cut) // size,
+             out_dim=out_dim, max_rank=16, ranks=[16, 9, 3, 16], x=x, out=out, pad=1)
+    _run(session, c)
+    c.check(f"{tokens} x {out_dim}, {128 * steps + cut} bytes")
+    first = c.y.clone()
+    _run(session, c)
+    assert torch.equal(c.y, first)
