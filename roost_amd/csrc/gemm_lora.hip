@@ -1559,12 +1559,13 @@ void LaunchAll(const LoraArgs& g, hipStream_t stream) {
   // Tiles of many rows: a CU holds one workgroup of 256 x 256, 256 x 128 or 128 x 128, so they go in rounds of kCus, and a
   // larger tile's round does more for its time (4096 channels, bf16: about 116, 65 and 45 us). So the smallest tile with one
   // round, and 256 x 256 from where 256 x 128 would take a second one. 900 rows to 4096: 128 x 128 55, 64 x 64 73 us; 1,100 rows
-  // to 4096: 256 x 128 75, 128 x 128 95, 64 x 64 87 us; 6,000 rows to 2048: 256 x 256 126, 128 x 128 153 us.
+  // to 4096: 256 x 128 75, 128 x 128 95, 64 x 64 87 us; 2,049 rows to 3,700 (255 of 256 x 128) 75, by 256 x 256 101 us; 2,304
+  // rows to 4096 (288) 112, by 256 x 256 86 us; e4m3 70 and 48; 6,000 rows to 2048: 256 x 256 126, 128 x 128 153 us.
   const uint64_t across = roost::CeilDiv(g.out_dim, 256);
   const auto medium = [&](uint64_t rows) { return roost::CeilDiv(g.out_dim, 128) * roost::CeilDiv(rows, 128); };
   uint64_t done = 0;
   const uint64_t large = across * roost::CeilDiv(g.tokens, 256);
-  if (large >= 160) {
+  if (across * roost::CeilDiv(g.tokens, 128) > kCus) {
     // Where the last round is a short one, the rows past the rounds before it take smaller tiles instead, if those are one
     // round: 4,400 rows to 4096 185 us against 225 in large tiles alone, 6,000 rows 220 against 235.
     done = (roost::CeilDiv(large, kCus) - 1) * kCus / across * 256;

@@ -459,3 +459,13 @@ def test_a_broken_table_writes_nothing_behind_the_call(session, tokens, out_dim,
         assert all((t[tokens:].float() == 7).all() for t in wide.values()), table
         if table[0] <= 0 and table[1] == first:  # the first sequence is as it should be
             fused_cases.assert_within(c.y[:first], want[:first], bound[:first], str(table))
+
+
+# Rows and outputs on both sides of where 256 x 128 tiles would take a second round of the CUs and 256 x 256 tiles begin.
+@pytest.mark.parametrize("x,out", [(BF16, BF16), (F8, BF16), (F32, F32)])
+@pytest.mark.parametrize("tokens,out_dim", [(2048, 4096), (2049, 4096), (2303, 4090), (2049, 3700), (384, 21700), (385, 21700)])
+def test_where_the_largest_tiles_begin(session, tokens, out_dim, x, out):
+    lens = _lens(tokens, 500)
+    c = Lora(94, lens, [(3 * i) % 5 - 1 for i in range(len(lens))], in_dim=208, out_dim=out_dim, ranks=[16, 5, 0, 9], x=x, out=out)
+    _run(session, c)
+    c.check(f"{tokens} x {out_dim}")
