@@ -35,7 +35,7 @@ using namespace roost_dev;
 
 constexpr char kOp[] = "gemm_lora";
 constexpr uint32_t kMaxRank = 128;
-constexpr uint32_t kCus = 256;
+constexpr uint32_t kCus = 256;  // of an MI355X that is one device; only which tiles are taken depends on it
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -1535,8 +1535,11 @@ void LaunchAll(const LoraArgs& g, hipStream_t stream) {
     return;
   }
   if (g.a != nullptr) {
-    // Pieces of 64 rows read an adapter a fourth as often as pieces of 16, but are a fourth as many: 4,480 bf16 rows of
-    // 4096 channels, rank 16, 17.4 and 15.6 us; 6,700 e4m3 rows, rank 32, 17.6 and 20.5 us.
+    // Pieces of 64 rows read an adapter a fourth as often as pieces of 16, but are a fourth as many. Four sequences of 4096
+    // channels to 64 outputs, by 16 and by 64, us a call: bf16, rank 16, 2,048 rows 17.7 and 20.6, 6,144 23.8 and 23.5, 15,000
+    // 51 and 50; rank 64 22.1 and 26.9, 33.5 and 28.7, 78 and 56; e4m3, rank 16, 15.2 and 17.8, 18.9 and 18.7, 34 and 30; rank
+    // 64 18.2 and 20.6, 31.9 and 25.5, 67 and 45. At 4,480 rows pieces of 64 already gain (rank 16 22.7 and 21.9, rank 64 32.7
+    // and 27.8): the border is on the safe side of where they are even.
     if (g.tokens / g.batch >= 64 && g.tokens >= 6144) {
       LaunchShrinkOfRows<E, 4>(g, stream);
     } else {

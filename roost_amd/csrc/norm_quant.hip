@@ -10,10 +10,11 @@
 // the scale instead of being dropped by a float maximum.
 //
 // Design: pure memory traffic, so one pass: a workgroup holds one row in registers (kV vectors of 8 elements a thread,
-// thread t's vector v at column 8 (v * threads + t), so a wavefront reads 1 KB of consecutive bf16), all its loads
-// requested before the first is used, and everything after them (sum of squares, largest magnitude) is a reduction over
-// registers. Rows of odd widths or strides take the same path: gfx950 loads 16 bytes from any address that suits the
-// element, and only the last few columns of a row, fewer than 8, go one by one.
+// thread t's vector v at column 8 (v * threads + t), so a wavefront reads 1 KB of consecutive bf16), and everything after
+// the loads (sum of squares, largest magnitude) is a reduction over registers. A thread's loads of f32 go out one behind
+// the other; a bf16 vector is awaited where the branch between whole and short vectors ends, and what hides that is the
+// row's other wavefronts. Rows of odd widths or strides take the same path: gfx950 loads 16 bytes from any address that
+// suits the element, and only the last few columns of a row, fewer than 8, go one by one.
 
 #include <initializer_list>
 #include <type_traits>
