@@ -602,8 +602,8 @@ def _exact_values(codes, scales):
     c = torch.stack((lo, hi), 3).reshape(*codes.shape[:2], -1)
     size, sign = c % 8, 1 - 2 * (c // 8)
     # e2m1: an exponent of two bits and a mantissa of one, no exponent below 1.
-    value = torch.where(size < 2, 0.5 * size, (1 + 0.5 * (size % 2)) * 2.0 ** (size // 2 - 1).double())
-    scale = 2.0 ** (scales.double() - 127)
+    value = torch.where(size < 2, 0.5 * size, (1 + 0.5 * (size % 2)) * torch.exp2((size // 2 - 1).double()))
+    scale = torch.exp2(scales.double() - 127)  # exact, which pow() is not
     return (sign * value * scale.transpose(1, 2).repeat_interleave(BLOCK, 2)).flatten(0, 1)
 
 
@@ -613,8 +613,8 @@ def _exact_f4(x, kept):
     top = cells.abs().amax(-1, keepdim=True)
     # The smallest power of two with top <= 7 * scale, within its range.
     e = torch.ceil(torch.log2(top.clamp(min=2.0 ** -140) / 7))
-    scale = 2.0 ** e.clamp(LOW - 127, HIGH - 127)
+    scale = torch.exp2(e.clamp(LOW - 127, HIGH - 127))
     r = cells.abs() / scale
-    step = 2.0 ** (torch.floor(torch.log2(r.clamp(min=1.0))).clamp(max=2.0) - 1)
+    step = torch.exp2(torch.floor(torch.log2(r.clamp(min=1.0))).clamp(max=2.0) - 1)
     y = (torch.round(r / step) * step).clamp(max=6.0) * scale * torch.sign(cells)  # round() takes ties to even
     return torch.where(kept[:, None, None], y.view(x.shape), 0.0)
