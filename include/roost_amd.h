@@ -325,6 +325,186 @@ ROOST_API RoostStatus roost_amd_gemm_lora_workspace(RoostContext* ctx, const voi
 ROOST_API RoostStatus roost_amd_gemm_lora_run(RoostContext* ctx, const void* params, const RoostWorkspace* ws,
                                               void* stream);
 
+/* ---- A KV cache held in 4 bits ----------------------------------------------------------------------------------------
+ * One layer's K and V in e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, two a byte, the lower dim in the low
+ * half) with one power-of-two scale for each 32 consecutive dims of a row: 4.25 bits a value. A scale byte b stands for
+ * 2^(b - 127), 7 <= b <= 252; 255 marks a block that held a NaN or an infinity, which reads as NaN. Calls of this section and
+ * of the next are reached by name, outside the registration table. Every run call may be captured into a HIP graph, allocates
+ * nothing, does not synchronise and is deterministic; the context's device must be current.
+ *
+ * Codes lie as [pages, kv_heads, page_size, head_dim / 2], scales as [pages, kv_heads, head_dim / 32, page_size] bytes: one
+ * head's part of a page is contiguous, and so are its tokens' scales of one block. head_dim is 64, 128 or 256, page_size a
+ * power of two from 16 to 1024, every address 16-byte aligned. `length` of k and v counts values (two a byte), of the scales
+ * bytes; a span may hold more than whole pages, and the pool has the pages that all four hold. */
+typedef struct RoostAmdCacheF4 {
+  RoostDeviceSpan k;        /* f4e2m1 [pages, kv_heads, page_size, head_dim] */
+  RoostDeviceSpan k_scales; /* u8 [pages, kv_heads, head_dim / 32, page_size] */
+  RoostDeviceSpan v;
+  RoostDeviceSpan v_scales;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+  uint32_t page_size;
+  uint32_t reserved0;
+} RoostAmdCacheF4;
+
+/* CacheWriteF4: token t's K and V rows into slot slot_mapping[t] = page * page_size + offset; a slot below 0 or past the pool
+ * skips the token. Per block of 32 dims with largest magnitude a: scale = the smallest power of two with a <= 7 scale, held to
+ * 2^-120 .. 2^125 (a block of zeros has 2^-120); code = x / scale rounded to nearest, ties to the even code, at most 6. So a
+ * value is off by at most one scale, half the grid's last step (two scales where a is above 7 * 2^125). Slots of one call
+ * differ; a slot named twice holds parts of both tokens' rows.
+ * CacheReadF4: the same record the other way, every value exactly (bf16 or f32); rows of a skipped token are left as they were.
+ * k and v are [tokens, kv_heads, head_dim], heads contiguous, tokens k_stride / v_stride elements apart (0 for contiguous
+ * rows): column views of one projection. They are 16-byte aligned and their strides multiples of 16 bytes; tokens are below
+ * 2^24. CacheReadF4's k and v overlap nothing. */
+typedef struct RoostAmdCacheF4Params {
+  uint32_t struct_size;
+  uint32_t abi_minor;
+  RoostDeviceSpan k; /* bf16, f16 (write only) or f32 */
+  RoostDeviceSpan v; /* k's type */
+  RoostAmdCacheF4 cache;
+  RoostDeviceSpan slot_mapping; /* [tokens] i64 */
+  uint32_t tokens;
+  uint32_t k_stride;
+  uint32_t v_stride;
+  uint32_t reserved0;
+} RoostAmdCacheF4Params;
+
+ROOST_API RoostStatus roost_amd_cache_write_f4_run(RoostContext* ctx, const void* params, void* stream);
+ROOST_API RoostStatus roost_amd_cache_read_f4_run(RoostContext* ctx, const void* params, void* stream);
+
+/* PagedAttentionF4: attention of a step's queries over such a cache, decode rows, prompt chunks and both in one call. Sequence
+ * b's queries are rows cu_seqlens[b] .. cu_seqlens[b + 1] of q and stand at its last positions: with n of them and `len` keys,
+ * query i is at position len - n + i and sees the keys up to it (all of them unless causal), from position - window_left on
+ * where window_left >= 0. Per query head h with KV head h / (q_heads / kv_heads):
+ *   s_j = sm_scale q . k_j, with logits_soft_cap > 0 then cap tanh(s_j / cap); p = softmax(s); out = sum_j p_j v_j;
+ *   lse = log2 sum_j exp(s_j).
+ * A query that sees no key has zero output and an lse of minus infinity. Rows of no sequence (behind cu_seqlens[batch], in a
+ * padded batch) are left as they were. Keys that a query does not see never reach it, NaN blocks included.
+ * Tables, all device data, so that one captured call serves steps of other lengths, in either of two forms:
+ *   - block_tables [table_rows, max_blocks] and kv_lens [table_rows], as the page calls below keep them; sequence b's row is
+ *     sequences[b], or b where sequences is NULL;
+ *   - kv_indptr [batch + 1], block_tables [.] and kv_lens [batch] as the plan region's kv_indptr, kv_indices and
+ *     kv_last_page_len; max_blocks, table_rows and sequences are 0.
+ * A page id outside the pool holds no keys; a row outside the tables has none; lengths are cut to the row's pages. Queries past
+ * the keys (n > len) see none; cu_seqlens[0] = 0 and cu_seqlens does not go backwards (else the rows in question are undefined
+ * or unwritten, and nothing outside the spans is read or written).
+ * max_q_len and max_kv_len are the largest n and len that the caller expects (0: unknown). They choose how the work is cut and
+ * bound nothing: longer sequences are computed too, only less evenly spread.
+ * Scores and sums are f32; each probability is rounded to bf16 once, in front of its product with v. q is 16-byte aligned, its
+ * token stride a multiple of 8; q_heads is a multiple of kv_heads, at most 32 to each; tokens are below 2^24. */
+typedef struct RoostAmdPagedAttentionF4Params {
+  uint32_t struct_size;
+  uint32_t abi_minor;
+  RoostDeviceSpan q;      /* bf16 [tokens, q_heads, head_dim], tokens q_stride apart (0: contiguous) */
+  RoostDeviceSpan output; /* bf16 [tokens, q_heads, head_dim] */
+  RoostDeviceSpan lse;    /* f32 [tokens, q_heads], or NULL */
+  RoostAmdCacheF4 cache;
+  RoostDeviceSpan cu_seqlens;   /* [batch + 1] i32 */
+  RoostDeviceSpan block_tables; /* i32 */
+  RoostDeviceSpan kv_lens;      /* i32 */
+  RoostDeviceSpan kv_indptr;    /* [batch + 1] i32, or NULL */
+  RoostDeviceSpan sequences;    /* [batch] i32, or NULL */
+  uint32_t batch;
+  uint32_t tokens;
+  uint32_t q_heads;
+  uint32_t q_stride;
+  uint32_t table_rows;
+  uint32_t max_blocks;
+  uint32_t max_q_len;
+  uint32_t max_kv_len;
+  float sm_scale;        /* 0 = 1/sqrt(head_dim) */
+  float logits_soft_cap; /* 0 = off */
+  int32_t window_left;   /* -1 = no sliding window */
+  uint32_t causal;
+} RoostAmdPagedAttentionF4Params;
+
+/* Device scratch of a call (partial results of sequences whose keys are split). Undefined before and after; a function of the
+ * record's numbers, not of its device data. */
+ROOST_API RoostStatus roost_amd_paged_attention_f4_workspace(RoostContext* ctx, const void* params,
+                                                             RoostWorkspaceSizes* sizes);
+ROOST_API RoostStatus roost_amd_paged_attention_f4_run(RoostContext* ctx, const void* params, const RoostWorkspace* ws,
+                                                       void* stream);
+
+/* ---- Pages of a cache ---------------------------------------------------------------------------------------------------
+ * Pools of any element type whose page p is page_bytes bytes at address + layer * layer_bytes + p * page_bytes, in each of
+ * `layers` layers. Addresses are 16-byte aligned, page_bytes and layer_bytes multiples of 16; pools do not overlap. */
+typedef struct RoostAmdPagePool {
+  void* address;
+  uint64_t page_bytes;
+  uint64_t layer_bytes;
+  uint32_t layers;
+  uint32_t reserved0;
+} RoostAmdPagePool;
+
+#define ROOST_AMD_MAX_PAGE_POOLS 16u
+
+/* CacheCopy: page pairs[i][0] to page pairs[i][1] in every layer of every pool, with the result of one pair after the other
+ * (RecurrentStateCopy's order). A pair that names a page outside the pools is skipped. Pairs that share no page with another
+ * as a destination run side by side; the others one after the other. count is at most 65,536. */
+typedef struct RoostAmdCacheCopyParams {
+  uint32_t struct_size;
+  uint32_t abi_minor;
+  const RoostAmdPagePool* pools; /* host memory, read during the call */
+  uint32_t pool_count;
+  uint32_t pages;
+  RoostDeviceSpan pairs; /* [count, 2] i32 */
+  uint32_t count;
+  uint32_t reserved0;
+} RoostAmdCacheCopyParams;
+
+/* Device scratch of a call of more than 1,024 pairs; zero bytes for others, which take a NULL workspace. */
+ROOST_API RoostStatus roost_amd_cache_copy_workspace(RoostContext* ctx, const void* params, RoostWorkspaceSizes* sizes);
+ROOST_API RoostStatus roost_amd_cache_copy_run(RoostContext* ctx, const void* params, const RoostWorkspace* ws, void* stream);
+
+/* Which pages the sequences hold, on the device: sequence s has lengths[s] tokens in the first ceil(lengths[s] / page_size)
+ * pages of its row of block_tables; refs[p] is how many rows hold page p, 0 for a free page. Whole pages may be shared; a last,
+ * partly filled page is its sequence's own, so that it can be written. The calls below keep to that, and read the state from
+ * before the call throughout: a request does not see what another of the same call did. Free pages are given in the order of
+ * the requests, lowest page first. Page ids outside the pool are left alone wherever a row holds them. */
+typedef struct RoostAmdCachePagesParams {
+  uint32_t struct_size;
+  uint32_t abi_minor;
+  const RoostAmdPagePool* pools; /* host memory, read during the call; fork and compact */
+  uint32_t pool_count;
+  uint32_t count;               /* requests, at most 1,024 */
+  RoostDeviceSpan block_tables; /* [sequences, max_blocks] i32 */
+  RoostDeviceSpan lengths;      /* [sequences] i32 */
+  RoostDeviceSpan refs;         /* [pages] i32 */
+  RoostDeviceSpan requests;     /* i32: fork [count, 2] (parent, child), grow and free [count] */
+  RoostDeviceSpan cu_seqlens;   /* grow: [count + 1] i32 */
+  RoostDeviceSpan slot_mapping; /* grow: [tokens] i64 */
+  RoostDeviceSpan status;       /* i32: fork and grow [count], or NULL; compact [1], or NULL */
+  uint32_t sequences;
+  uint32_t max_blocks;
+  uint32_t pages;               /* at most 4,194,304 */
+  uint32_t page_size;           /* a power of two */
+} RoostAmdCachePagesParams;
+
+/* Device scratch of fork, grow and compact: one size for all three, from `pages` alone. Undefined before and after. */
+ROOST_API RoostStatus roost_amd_cache_pages_workspace(RoostContext* ctx, const void* params, RoostWorkspaceSizes* sizes);
+
+/* CacheFork: the child gets its parent's length and pages: whole ones shared (refs + 1), a last partly filled one copied, in
+ * every layer of every pool, into a free page (refs 1). status 1. Status 0, nothing done: the parent is empty, the child is
+ * not, either is no sequence, an earlier request names the same child, or no free page is left for it. */
+ROOST_API RoostStatus roost_amd_cache_fork_run(RoostContext* ctx, const void* params, const RoostWorkspace* ws, void* stream);
+
+/* CacheGrow: sequence requests[i] gets room for cu_seqlens[i + 1] - cu_seqlens[i] more tokens: free pages (refs 1) at the end of
+ * its row, its new length, and slot_mapping[cu_seqlens[i] ..] = its new tokens' slots, as CacheWrite and CacheWriteF4 take
+ * them. status 1. Status 0 and slots of -1, nothing else done: no such sequence, one that an earlier request names, more tokens
+ * than its row holds, or fewer free pages left than this request and the earlier ones need. Entries of slot_mapping behind the
+ * last request's are left as they were; cu_seqlens[0] = 0 and cu_seqlens does not go backwards. */
+ROOST_API RoostStatus roost_amd_cache_grow_run(RoostContext* ctx, const void* params, const RoostWorkspace* ws, void* stream);
+
+/* CacheFree: sequence requests[i] ends: refs - 1 for each of its pages, their entries of its row -1, its length 0. Empty
+ * sequences, and numbers of no sequence, are skipped; naming one twice frees it once. */
+ROOST_API RoostStatus roost_amd_cache_free_run(RoostContext* ctx, const void* params, void* stream);
+
+/* CacheCompact: with `live` pages in use (refs above 0), the i-th used page from page `live` on moves to the i-th free page
+ * below it, in every layer of every pool, with its refs; the sequences' rows follow. Then pages 0 .. live - 1 are in use and
+ * the others free. status[0] = live. What the others hold stays. */
+ROOST_API RoostStatus roost_amd_cache_compact_run(RoostContext* ctx, const void* params, const RoostWorkspace* ws,
+                                                  void* stream);
+
 /* The plan region: the batch tables and slot mapping of one worker step, from its sequences. Replaces the worker's
  * PlanRegionWriter.Fill (reference src/Starlings.Roost.Worker/Eager/PlanRegionWriter.cs:19-64), which the reference runs
  * in C# on a host mirror of the region before one host-to-device copy. For sequence b (in order):

@@ -21,7 +21,7 @@ from __future__ import annotations
 import ctypes as C
 from dataclasses import dataclass
 from pathlib import Path
-from typing import Optional
+from typing import NamedTuple, Optional
 
 from . import abi
 
@@ -119,8 +119,14 @@ class KernelLibrary:
                      "roost_amd_gemm_lora_workspace"):
             getattr(self.dll, name).argtypes = [C.c_void_p] * 3
             getattr(self.dll, name).restype = C.c_int32
-        self.dll.roost_amd_gemm_lora_run.argtypes = [C.c_void_p] * 4
-        self.dll.roost_amd_gemm_lora_run.restype = C.c_int32
+        for name in ("roost_amd_cache_write_f4_run", "roost_amd_cache_read_f4_run", "roost_amd_paged_attention_f4_workspace",
+                     "roost_amd_cache_copy_workspace", "roost_amd_cache_free_run", "roost_amd_cache_pages_workspace"):
+            getattr(self.dll, name).argtypes = [C.c_void_p] * 3
+            getattr(self.dll, name).restype = C.c_int32
+        for name in ("roost_amd_gemm_lora_run", "roost_amd_paged_attention_f4_run", "roost_amd_cache_copy_run",
+                     "roost_amd_cache_fork_run", "roost_amd_cache_grow_run", "roost_amd_cache_compact_run"):
+            getattr(self.dll, name).argtypes = [C.c_void_p] * 4
+            getattr(self.dll, name).restype = C.c_int32
         self.dll.roost_amd_plan_region_from_step.argtypes = [C.c_void_p, C.c_uint64, C.POINTER(abi.StepTables)]
         self.dll.roost_amd_plan_region_from_step.restype = C.c_int32
         version = self.dll.roost_abi_version()
@@ -715,6 +721,268 @@ def gemm_lora(session: OpSession, params, ws: Optional[abi.Workspace] = None, ke
     if ws is None:
         ws = gemm_lora_workspace(session, params, key)
     _extension(session, "gemm_lora", session.lib.dll.roost_amd_gemm_lora_run, params, C.addressof(ws))
+
+
+# ---- a KV cache held in 4 bits, and the pages of a cache --------------------------------------------------------------------
+
+class CacheF4(NamedTuple):
+    """One layer's K and V in 4 bits, uint8 tensors: codes [pages, kv_heads, page_size, head_dim / 2] and scales
+    [pages, kv_heads, head_dim / 32, page_size]. Any tuple of the four will do."""
+    k: object
+    k_scales: object
+    v: object
+    v_scales: object
+
+
+def cache_f4(pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> CacheF4:
+    """A zeroed cache of `pages` pages."""
+    torch = _torch()
+    codes, scales = (pages, kv_heads, page_size, head_dim // 2), (pages, kv_heads, head_dim // 32, page_size)
+    return CacheF4(*(torch.zeros(s, dtype=torch.uint8, device=device) for s in (codes, scales, codes, scales)))
+
+
+def _of_cache(cache) -> dict:
+    return {f"cache {name}": t for name, t in zip(CacheF4._fields, cache)}
+
+
+def _cache_f4(cache) -> abi.CacheF4:
+    torch = _torch()
+    k, k_scales, v, v_scales = cache
+    if k.dim() != 4:
+        raise ValueError(f"cache: codes of shape {tuple(k.shape)}, not [pages, kv_heads, page_size, head_dim / 2]")
+    pages, kv_heads, page_size, half = k.shape
+    c = abi.CacheF4()
+    c.k = _flat(k, "cache k", k.shape, torch.uint8)
+    c.v = _flat(v, "cache v", k.shape, torch.uint8)
+    for s in (c.k, c.v):
+        s.length, s.dtype = 2 * s.length, abi.DTYPE_F4E2M1
+    c.k_scales = _flat(k_scales, "cache k_scales", (pages, kv_heads, half // 16, page_size), torch.uint8)
+    c.v_scales = _flat(v_scales, "cache v_scales", (pages, kv_heads, half // 16, page_size), torch.uint8)
+    c.kv_heads, c.head_dim, c.page_size = kv_heads, 2 * half, page_size
+    return c
+
+
+def _token_heads(t, name, tokens, heads, dim):
+    """(span, token stride) of a [tokens, heads, dim] tensor whose tokens are contiguous, any distance apart."""
+    if tuple(t.shape) != (tokens, heads, dim):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, not {(tokens, heads, dim)}")
+    if dim > 1 and t.stride(2) != 1 or heads > 1 and t.stride(1) != dim:
+        raise ValueError(f"{name}: strides {t.stride()}: a token's heads have to be contiguous")
+    stride = t.stride(0) if tokens > 1 else heads * dim
+    if stride < heads * dim:
+        raise ValueError(f"{name}: tokens are {stride} elements apart, below their {heads * dim} elements")
+    return span(t, length=0 if tokens == 0 else (tokens - 1) * stride + heads * dim), stride
+
+
+def cache_f4_params(k, v, cache, slot_mapping):
+    """RoostAmdCacheF4Params: k and v [tokens, kv_heads, head_dim] (column views of a projection will do), slot_mapping
+    [tokens] int64; of cache_write_f4, which reads k and v, and of cache_read_f4, which writes them."""
+    p = abi.new(abi.CacheF4Params)
+    p._device = _one_device(k=k, v=v, slot_mapping=slot_mapping, **_of_cache(cache))
+    p.cache = _cache_f4(cache)
+    tokens = k.shape[0]
+    p.k, p.k_stride = _token_heads(k, "k", tokens, p.cache.kv_heads, p.cache.head_dim)
+    p.v, p.v_stride = _token_heads(v, "v", tokens, p.cache.kv_heads, p.cache.head_dim)
+    p.slot_mapping = _flat(slot_mapping, "slot_mapping", (tokens,), _torch().int64)
+    p.tokens = tokens
+    p._keep = (k, v, tuple(cache), slot_mapping)
+    return p
+
+
+def cache_write_f4(session: OpSession, params) -> None:
+    """roost_amd_cache_write_f4_run on the session's stream."""
+    _extension(session, "cache_write_f4", session.lib.dll.roost_amd_cache_write_f4_run, params)
+
+
+def cache_read_f4(session: OpSession, params) -> None:
+    """roost_amd_cache_read_f4_run on the session's stream."""
+    _extension(session, "cache_read_f4", session.lib.dll.roost_amd_cache_read_f4_run, params)
+
+
+def paged_attention_f4_params(q, output, cache, cu_seqlens, *, block_tables=None, kv_lens=None, sequences=None, kv_indptr=None,
+                              kv_indices=None, kv_last_page_len=None, lse=None, max_q_len=0, max_kv_len=0, sm_scale=0.0,
+                              soft_cap=0.0, window_left=-1, causal=True):
+    """RoostAmdPagedAttentionF4Params: q and output [tokens, q_heads, head_dim], cu_seqlens [batch + 1]. The tables are either
+    block_tables [rows, max_blocks] with kv_lens [rows] and sequences [batch] (None: row b), or the plan region's kv_indptr,
+    kv_indices and kv_last_page_len. All int32 on the GPU; max_q_len and max_kv_len are what the caller expects at most."""
+    torch = _torch()
+    p = abi.new(abi.PagedAttentionF4Params)
+    dense = block_tables is not None
+    if dense != (kv_lens is not None) or dense == (kv_indptr is not None) or \
+            (kv_indptr is None) != (kv_indices is None) or (kv_indptr is None) != (kv_last_page_len is None) or \
+            (sequences is not None and not dense):
+        raise ValueError("tables: either block_tables and kv_lens (and sequences), or kv_indptr, kv_indices and kv_last_page_len")
+    p._device = _one_device(q=q, output=output, lse=lse, cu_seqlens=cu_seqlens, block_tables=block_tables, kv_lens=kv_lens,
+                            sequences=sequences, kv_indptr=kv_indptr, kv_indices=kv_indices,
+                            kv_last_page_len=kv_last_page_len, **_of_cache(cache))
+    p.cache = _cache_f4(cache)
+    tokens, q_heads, dim = q.shape
+    batch = cu_seqlens.shape[0] - 1
+    p.q, p.q_stride = _token_heads(q, "q", tokens, q_heads, p.cache.head_dim)
+    p.output = _flat(output, "output", (tokens, q_heads, dim))
+    p.lse = _flat(lse, "lse", (tokens, q_heads), torch.float32)
+    p.cu_seqlens = _flat(cu_seqlens, "cu_seqlens", (batch + 1,), torch.int32)
+    if dense:
+        rows, p.max_blocks = block_tables.shape
+        p.table_rows = rows
+        p.block_tables = _flat(block_tables, "block_tables", block_tables.shape, torch.int32)
+        p.kv_lens = _flat(kv_lens, "kv_lens", (rows,), torch.int32)
+        p.sequences = _flat(sequences, "sequences", (batch,), torch.int32)
+    else:
+        p.block_tables = _flat(kv_indices, "kv_indices", (kv_indices.numel(),), torch.int32)
+        p.kv_lens = _flat(kv_last_page_len, "kv_last_page_len", (batch,), torch.int32)
+        p.kv_indptr = _flat(kv_indptr, "kv_indptr", (batch + 1,), torch.int32)
+    p.batch, p.tokens, p.q_heads, p.max_q_len, p.max_kv_len = batch, tokens, q_heads, max_q_len, max_kv_len
+    p.sm_scale, p.logits_soft_cap, p.window_left, p.causal = sm_scale, soft_cap, window_left, int(causal)
+    p._keep = (q, output, lse, tuple(cache), cu_seqlens, block_tables, kv_lens, sequences, kv_indptr, kv_indices,
+               kv_last_page_len)
+    return p
+
+
+def _device_workspace(session: OpSession, name: str, fn, params, key) -> abi.Workspace:
+    sizes = abi.new(abi.WorkspaceSizes)
+    status = fn(session.ctx, C.addressof(params), C.addressof(sizes))
+    if status != abi.OK:
+        raise KernelError(f"{name} workspace", status, session.lib.last_error())
+    return session.workspace_of((name, key), sizes, keep=True)[3]
+
+
+def paged_attention_f4_workspace(session: OpSession, params, key=0) -> abi.Workspace:
+    """A workspace for paged_attention_f4 of these params, kept by the session under `key` as gemm_lora_workspace keeps its."""
+    return _device_workspace(session, "paged_attention_f4", session.lib.dll.roost_amd_paged_attention_f4_workspace, params, key)
+
+
+def paged_attention_f4(session: OpSession, params, ws: Optional[abi.Workspace] = None, key=0) -> None:
+    """roost_amd_paged_attention_f4_run on the session's stream, in `ws` or the session's workspace under `key`."""
+    if ws is None:
+        ws = paged_attention_f4_workspace(session, params, key)
+    _extension(session, "paged_attention_f4", session.lib.dll.roost_amd_paged_attention_f4_run, params, C.addressof(ws))
+
+
+def _pools(pools):
+    """(array of RoostAmdPagePool, pages) of tensors [layers, pages, ...] whose pages are contiguous."""
+    if not pools:
+        raise ValueError("pools: none given")
+    found = (abi.PagePool * len(pools))()
+    pages = pools[0].shape[1]
+    for i, t in enumerate(pools):
+        if t.dim() < 2 or t.shape[1] != pages:
+            raise ValueError(f"pool {i}: shape {tuple(t.shape)}, not [layers, {pages}, ...]")
+        size = t.element_size() * t[0, 0].numel() if t.numel() else 0
+        if t.numel() == 0 or not t[0].is_contiguous():
+            raise ValueError(f"pool {i}: shape {tuple(t.shape)}, strides {t.stride()}: a layer's pages have to be contiguous")
+        found[i].address, found[i].page_bytes, found[i].layers = t.data_ptr(), size, t.shape[0]
+        found[i].layer_bytes = t.stride(0) * t.element_size() if t.shape[0] > 1 else pages * size
+    return found, pages
+
+
+def cache_copy_params(pools, pairs):
+    """RoostAmdCacheCopyParams: pools are tensors [layers, pages, ...] of any type, pairs [count, 2] int32 (from, to)."""
+    p = abi.new(abi.CacheCopyParams)
+    p._device = _one_device(pairs=pairs, **{f"pool {i}": t for i, t in enumerate(pools)})
+    found, p.pages = _pools(pools)
+    p.pools, p.pool_count = C.addressof(found), len(found)
+    p.count = pairs.shape[0]
+    p.pairs = _flat(pairs, "pairs", (p.count, 2), _torch().int32)
+    p._keep = (tuple(pools), found, pairs)
+    return p
+
+
+def cache_copy_workspace(session: OpSession, params, key=0) -> abi.Workspace:
+    """A workspace for cache_copy of these params, kept by the session under `key`."""
+    return _device_workspace(session, "cache_copy", session.lib.dll.roost_amd_cache_copy_workspace, params, key)
+
+
+def cache_copy(session: OpSession, params, ws: Optional[abi.Workspace] = None, key=0) -> None:
+    """roost_amd_cache_copy_run on the session's stream, in `ws` or the session's workspace under `key`."""
+    if ws is None:
+        ws = cache_copy_workspace(session, params, key)
+    _extension(session, "cache_copy", session.lib.dll.roost_amd_cache_copy_run, params, C.addressof(ws))
+
+
+def _pages_params(pools, requests, block_tables, lengths, refs, page_size, columns, **more):
+    torch = _torch()
+    p = abi.new(abi.CachePagesParams)
+    p._device = _one_device(block_tables=block_tables, lengths=lengths, refs=refs, requests=requests, **more,
+                            **{f"pool {i}": t for i, t in enumerate(pools)})
+    found = None
+    if pools:
+        found, pages = _pools(pools)
+        if pages != refs.numel():
+            raise ValueError(f"pools of {pages} pages, refs of {refs.numel()}")
+        p.pools, p.pool_count = C.addressof(found), len(found)
+    p.sequences, p.max_blocks = block_tables.shape
+    p.pages, p.page_size = refs.numel(), page_size
+    p.block_tables = _flat(block_tables, "block_tables", block_tables.shape, torch.int32)
+    p.lengths = _flat(lengths, "lengths", (p.sequences,), torch.int32)
+    p.refs = _flat(refs, "refs", (p.pages,), torch.int32)
+    if requests is not None:
+        p.count = requests.shape[0]
+        p.requests = _flat(requests, "requests", (p.count, 2) if columns == 2 else (p.count,), torch.int32)
+    p._keep = (tuple(pools), found, requests, block_tables, lengths, refs, more)
+    return p
+
+
+def cache_fork_params(pools, pairs, status=None, *, block_tables, lengths, refs, page_size):
+    """RoostAmdCachePagesParams of cache_fork: pairs [count, 2] (parent, child), status [count] (or None), all int32;
+    block_tables [sequences, max_blocks], lengths [sequences] and refs [pages] are read and written."""
+    p = _pages_params(pools, pairs, block_tables, lengths, refs, page_size, 2, status=status)
+    p.status = _flat(status, "status", (p.count,), _torch().int32)
+    return p
+
+
+def cache_grow_params(sequences, cu_seqlens, slot_mapping, status=None, *, block_tables, lengths, refs, page_size):
+    """RoostAmdCachePagesParams of cache_grow: sequences [count] and cu_seqlens [count + 1] int32, slot_mapping [tokens] int64."""
+    torch = _torch()
+    p = _pages_params((), sequences, block_tables, lengths, refs, page_size, 1, cu_seqlens=cu_seqlens,
+                      slot_mapping=slot_mapping, status=status)
+    p.cu_seqlens = _flat(cu_seqlens, "cu_seqlens", (p.count + 1,), torch.int32)
+    p.slot_mapping = _flat(slot_mapping, "slot_mapping", (slot_mapping.numel(),), torch.int64)
+    p.status = _flat(status, "status", (p.count,), torch.int32)
+    return p
+
+
+def cache_free_params(sequences, *, block_tables, lengths, refs, page_size):
+    """RoostAmdCachePagesParams of cache_free: sequences [count] int32."""
+    return _pages_params((), sequences, block_tables, lengths, refs, page_size, 1)
+
+
+def cache_compact_params(pools, live=None, *, block_tables, lengths, refs, page_size):
+    """RoostAmdCachePagesParams of cache_compact; live [1] int32 receives the number of pages in use."""
+    p = _pages_params(pools, None, block_tables, lengths, refs, page_size, 0, live=live)
+    p.status = _flat(live, "live", (1,), _torch().int32)
+    return p
+
+
+def cache_pages_workspace(session: OpSession, params, key=0) -> abi.Workspace:
+    """A workspace for cache_fork, cache_grow and cache_compact over as many pages, kept by the session under `key`."""
+    return _device_workspace(session, "cache_pages", session.lib.dll.roost_amd_cache_pages_workspace, params, key)
+
+
+def _pages_call(session: OpSession, name: str, params, ws, key) -> None:
+    if ws is None:
+        ws = cache_pages_workspace(session, params, key)
+    _extension(session, name, getattr(session.lib.dll, f"roost_amd_{name}_run"), params, C.addressof(ws))
+
+
+def cache_fork(session: OpSession, params, ws: Optional[abi.Workspace] = None, key=0) -> None:
+    """roost_amd_cache_fork_run on the session's stream."""
+    _pages_call(session, "cache_fork", params, ws, key)
+
+
+def cache_grow(session: OpSession, params, ws: Optional[abi.Workspace] = None, key=0) -> None:
+    """roost_amd_cache_grow_run on the session's stream."""
+    _pages_call(session, "cache_grow", params, ws, key)
+
+
+def cache_free(session: OpSession, params) -> None:
+    """roost_amd_cache_free_run on the session's stream."""
+    _extension(session, "cache_free", session.lib.dll.roost_amd_cache_free_run, params)
+
+
+def cache_compact(session: OpSession, params, ws: Optional[abi.Workspace] = None, key=0) -> None:
+    """roost_amd_cache_compact_run on the session's stream."""
+    _pages_call(session, "cache_compact", params, ws, key)
 
 
 def gated_rms_norm(session: OpSession, *args, **kwargs) -> None:

@@ -20,6 +20,7 @@ STATUS_NAMES = ["OK", "INVALID_ARGUMENT", "UNSUPPORTED", "CUDA_ERROR", "INTERNAL
 # Element types
 DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_F64 = 1, 2, 3, 4
 DTYPE_F8E4M3, DTYPE_U8, DTYPE_I32, DTYPE_I64 = 5, 8, 10, 12
+DTYPE_F4E2M1 = 16
 
 # Layouts
 LAYOUT_ROW_MAJOR, LAYOUT_PAGED_NHD, LAYOUT_PAGED_HND = 0, 2, 3
@@ -180,6 +181,44 @@ class GemmLoraParams(C.Structure):
                                         "addend_stride", "output_stride", "reserved0")]
 
 
+class CacheF4(C.Structure):
+    _fields_ = [(name, DeviceSpan) for name in ("k", "k_scales", "v", "v_scales")] + [
+        (name, C.c_uint32) for name in ("kv_heads", "head_dim", "page_size", "reserved0")]
+
+
+class CacheF4Params(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32), ("k", DeviceSpan), ("v", DeviceSpan),
+                ("cache", CacheF4), ("slot_mapping", DeviceSpan), ("tokens", C.c_uint32), ("k_stride", C.c_uint32),
+                ("v_stride", C.c_uint32), ("reserved0", C.c_uint32)]
+
+
+class PagedAttentionF4Params(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32), ("q", DeviceSpan), ("output", DeviceSpan),
+                ("lse", DeviceSpan), ("cache", CacheF4)] + [
+        (name, DeviceSpan) for name in ("cu_seqlens", "block_tables", "kv_lens", "kv_indptr", "sequences")] + [
+        (name, C.c_uint32) for name in ("batch", "tokens", "q_heads", "q_stride", "table_rows", "max_blocks", "max_q_len",
+                                        "max_kv_len")] + [
+        ("sm_scale", C.c_float), ("logits_soft_cap", C.c_float), ("window_left", C.c_int32), ("causal", C.c_uint32)]
+
+
+class PagePool(C.Structure):
+    _fields_ = [("address", C.c_void_p), ("page_bytes", C.c_uint64), ("layer_bytes", C.c_uint64), ("layers", C.c_uint32),
+                ("reserved0", C.c_uint32)]
+
+
+class CacheCopyParams(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32), ("pools", C.c_void_p), ("pool_count", C.c_uint32),
+                ("pages", C.c_uint32), ("pairs", DeviceSpan), ("count", C.c_uint32), ("reserved0", C.c_uint32)]
+
+
+class CachePagesParams(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32), ("pools", C.c_void_p), ("pool_count", C.c_uint32),
+                ("count", C.c_uint32)] + [
+        (name, DeviceSpan) for name in ("block_tables", "lengths", "refs", "requests", "cu_seqlens", "slot_mapping",
+                                        "status")] + [
+        (name, C.c_uint32) for name in ("sequences", "max_blocks", "pages", "page_size")]
+
+
 class SigmoidMulParams(C.Structure):
     _fields_ = [("struct_size", C.c_uint32), ("abi_minor", C.c_uint32), ("input", DeviceSpan), ("gate", DeviceSpan),
                 ("output", DeviceSpan), ("rows", C.c_uint32), ("dim", C.c_uint32)]
@@ -272,7 +311,10 @@ ALL_STRUCTS = {
 EXTENSION_STRUCTS = {"RoostQkvQkNormRopeCacheWriteParams": QkvQkNormRopeCacheWriteParams,
                      "RoostAmdAddRmsNormParams": AddRmsNormParams,
                      "RoostAmdAddRmsNormQuantParams": AddRmsNormQuantParams,
-                     "RoostAmdSiluMulQuantParams": SiluMulQuantParams, "RoostAmdGemmLoraParams": GemmLoraParams}
+                     "RoostAmdSiluMulQuantParams": SiluMulQuantParams, "RoostAmdGemmLoraParams": GemmLoraParams,
+                     "RoostAmdCacheF4": CacheF4, "RoostAmdCacheF4Params": CacheF4Params,
+                     "RoostAmdPagedAttentionF4Params": PagedAttentionF4Params, "RoostAmdPagePool": PagePool,
+                     "RoostAmdCacheCopyParams": CacheCopyParams, "RoostAmdCachePagesParams": CachePagesParams}
 
 
 def new(struct_type):

@@ -20,7 +20,7 @@ BUILD = HERE / "_build"
 LIB_NAME = "libroost_kernels_gfx950.so"
 LIB_PATH = HERE / LIB_NAME
 SOURCES = ["registry.cpp", "cache_write.hip", "paged_attention.hip", "gated_delta_rule.hip", "gdn_layer.hip", "qk_rope.hip",
-           "plan_region.hip", "norm_quant.hip", "gemm_lora.hip"]
+           "plan_region.hip", "norm_quant.hip", "gemm_lora.hip", "cache_f4.hip", "cache_pages.hip", "paged_attention_f4.hip"]
 
 # Packed-FP32 instructions are kept out of every HIP object (the compiler would otherwise form v_pk_* from scalar
 # float code); the host pass of hipcc warns that it does not know the feature, which is harmless.

@@ -65,6 +65,14 @@ static_assert(sizeof(RoostAmdSiluMulQuantParams) == 128 && offsetof(RoostAmdSilu
 static_assert(sizeof(RoostAmdGemmLoraParams) == 336 && offsetof(RoostAmdGemmLoraParams, output) == 272 &&
                   offsetof(RoostAmdGemmLoraParams, tokens) == 296 && offsetof(RoostAmdGemmLoraParams, reserved0) == 332,
               "RoostAmdGemmLoraParams layout");
+static_assert(sizeof(RoostAmdCacheF4) == 112 && offsetof(RoostAmdCacheF4, kv_heads) == 96, "RoostAmdCacheF4 layout");
+static_assert(sizeof(RoostAmdCacheF4Params) == 208 && offsetof(RoostAmdCacheF4Params, tokens) == 192, "RoostAmdCacheF4Params layout");
+static_assert(sizeof(RoostAmdPagedAttentionF4Params) == 360 && offsetof(RoostAmdPagedAttentionF4Params, cu_seqlens) == 192 &&
+                  offsetof(RoostAmdPagedAttentionF4Params, sm_scale) == 344,
+              "RoostAmdPagedAttentionF4Params layout");
+static_assert(sizeof(RoostAmdPagePool) == 32 && sizeof(RoostAmdCacheCopyParams) == 56 && sizeof(RoostAmdCachePagesParams) == 208 &&
+                  offsetof(RoostAmdCachePagesParams, sequences) == 192,
+              "page records' layout");
 static_assert(sizeof(RoostRecurrentStateCopyParams) == 72 && offsetof(RoostRecurrentStateCopyParams, slot_bytes) == 56,
               "RoostRecurrentStateCopyParams layout");
 static_assert(sizeof(RoostRecurrentStateSnapshotParams) == 96 &&
