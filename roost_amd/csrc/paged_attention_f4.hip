@@ -21,10 +21,16 @@ constexpr float kGrow = 8.0f;           // the running maximum moves when a scor
 typedef float F4v __attribute__((ext_vector_type(4)));
 typedef uint32_t U2 __attribute__((ext_vector_type(2)));
 typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+typedef float F16v __attribute__((ext_vector_type(16)));
+typedef short I4h __attribute__((ext_vector_type(4)));
 typedef __bf16 B8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ F4v Mfma16(U4 a, U4 b, F4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(B8, a), __builtin_bit_cast(B8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ F16v Mfma32(U4 a, U4 b, F16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(B8, a), __builtin_bit_cast(B8, b), c, 0, 0, 0);
 }
 
 struct SoftCap {  // cap tanh(s / cap) in log2 units: capl - 2 capl / (1 + 2^(k y)), y the scaled score
@@ -51,6 +57,8 @@ struct Args {
   uint32_t splits, part;     // a sequence's keys in at most `splits` parts of `part`, the last one open-ended
   uint32_t short_tokens;     // sequences of at most so many tokens may be split
   uint32_t row_limit;        // the row kernel takes sequences of at most so many rows, the tile kernel the others
+  float *tile_o, *tile_ml;   // the tile kernel's partial rows, in at most tile_splits parts of its keys
+  uint32_t tile_splits;
 };
 
 // ---- A sequence ---------------------------------------------------------------------------------------------------------
@@ -443,36 +451,379 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
   }
 }
 
-// A split sequence's parts, in order. Block (rows of a KV head by fours, KV head, sequence), a wavefront a row.
+// ---- The tile kernel ----------------------------------------------------------------------------------------------------------
+// 32 kWaves rows of one sequence and KV head (rows are its tokens' query heads, token by token) against the keys that they see, 64
+// at a time: prompt chunks. Bound by the matrix instructions and, beside them, by LDS reads and the softmax.
+//
+// A tile's codes come through registers, a lane a block of 32 dims (16 bytes, one scale), and go to LDS as bf16 once for all
+// wavefronts: 64 conversions a lane and tile at head_dim 128 and 256 rows, where converting in each wavefront would take 192. Codes
+// of the next tile are under way during a tile's products; LDS holds two tiles, so there is one barrier a tile.
+//
+// v_mfma_f32_32x32x16_bf16, lane l = 32 g + m: A[m][8 g + j], B[8 g + j][m], result register v at [8 (v / 4) + 4 g + v % 4][m].
+//   S^T = K Q^T with 32 keys as A and the wavefront's 32 rows as B. A lane then holds, of its row, keys 4 g + i of each 8; the
+//   products O^T = V^T P^T contract the keys in that order, so p stays in its lane, and V^T's operand (dim m, four keys twice) is
+//   read from LDS by transposing reads.
+// LDS: K rows are padded by 16 bytes, so that 16 keys' reads of 16 bytes meet no bank twice; V's 64-byte chunks are swizzled by
+// the key, and their 16-byte pieces by the next bits of it, which does the same for the transposing reads of 8 keys x 64 bytes.
+
+constexpr int kTileKeys = 64;
+
+typedef __attribute__((address_space(3))) unsigned char LdsByte;
+
+__device__ __forceinline__ U2 LdsTranspose(const unsigned char* base, uint32_t off) {
+  auto* p = reinterpret_cast<__attribute__((address_space(3))) I4h*>(const_cast<LdsByte*>((const LdsByte*)base + off));
+  return __builtin_bit_cast(U2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
+}
+
 template <int D>
-__global__ void __launch_bounds__(256) RowMergeKernel(Args a) {
-  const Sequence s = SequenceOf(a, blockIdx.z);
-  const int32_t rows = s.count * static_cast<int32_t>(a.group);
-  const int32_t row = static_cast<int32_t>(blockIdx.x * 4 + threadIdx.x / 64);
-  if (row >= rows || rows > static_cast<int32_t>(a.row_limit) || s.count > static_cast<int32_t>(a.short_tokens)) return;
-  const uint32_t parts = PartsOf(a, FirstKey(a, s, 0), s.keys);
-  if (parts <= 1) return;
+struct TileLds {
+  static constexpr int kKeyRow = 2 * D + 16;
+  unsigned char k[2][kTileKeys * kKeyRow];
+  unsigned char v[2][kTileKeys * 2 * D];
+  uint32_t bad[3];                // groups of 16 keys without a page, of this tile, the next and the one after
+  uint32_t nan[3][kTileKeys];     // blocks of V that are NaN; only kept in a careful pass
+};
+
+// Where block `block`, piece `piece` (8 dims) of a key lies in LDS.
+template <int D>
+__device__ __forceinline__ uint32_t ValueAt(uint32_t key, uint32_t block, uint32_t piece) {
+  const uint32_t swap = D == 64 ? key >> 1 & 1 : key & 3;
+  return key * 2 * D + ((block ^ swap) * 64) + ((piece ^ (key >> 2 & 3)) * 16);
+}
+
+// Tile `rank` of all sequences' that have more rows than row_limit; a sequence's last tiles first, whose rows see most keys.
+// Every wavefront finds it by itself.
+__device__ __forceinline__ bool FindTile(const Args& a, uint32_t rank, uint32_t rows_a_tile, uint32_t& b, int32_t& tile) {
   const int lane = threadIdx.x & 63;
+  const int32_t most = static_cast<int32_t>(a.tokens);
+  for (uint32_t base = 0; base < a.batch; base += 64) {
+    uint32_t tiles = 0;
+    if (base + lane < a.batch) {
+      const int32_t first = min(max(a.cu[base + lane], 0), most);
+      const uint32_t rows = static_cast<uint32_t>(min(max(a.cu[base + lane + 1], first), most) - first) * a.group;
+      tiles = rows > a.row_limit ? (rows + rows_a_tile - 1) / rows_a_tile : 0;
+    }
+    uint32_t end = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = static_cast<uint32_t>(__shfl_up(static_cast<int>(end), d));
+      if (lane >= d) end += o;
+    }
+    const uint64_t here = __ballot(rank < end);
+    if (here != 0) {
+      const int at = __builtin_ctzll(here);
+      b = base + static_cast<uint32_t>(at);
+      tile = static_cast<int32_t>(__builtin_amdgcn_readlane(static_cast<int>(end), at)) - 1 - static_cast<int32_t>(rank);
+      return true;
+    }
+    rank -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(end), 63));
+  }
+  return false;
+}
+
+// A tile's keys, and their parts.
+struct TileKeys {
+  int32_t begin, end, part;
+  uint32_t parts;
+};
+__device__ __forceinline__ TileKeys KeysOfTile(const Args& a, const Sequence& s, int32_t tile, int32_t rows_a_tile) {
+  const int32_t group = static_cast<int32_t>(a.group);
+  const int32_t first = tile * rows_a_tile / group, last = min((tile * rows_a_tile + rows_a_tile - 1) / group, s.count - 1);
+  TileKeys k;
+  k.begin = FirstKey(a, s, first);
+  k.end = a.causal ? max(0, s.keys - s.count + last + 1) : s.keys;
+  const int32_t n = max(0, k.end - k.begin);
+  k.part = ((n + static_cast<int32_t>(a.tile_splits) - 1) / static_cast<int32_t>(a.tile_splits) + kTileKeys - 1) & ~(kTileKeys - 1);
+  k.parts = n == 0 ? 1 : static_cast<uint32_t>((n + k.part - 1) / k.part);
+  return k;
+}
+
+template <int D, int kWaves, bool kCap>
+__global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(Args a) {
+  constexpr int kThreads = 64 * kWaves, kRows = 32 * kWaves;
+  constexpr int kKs = D / 16, kDt = D / 32;
+  constexpr int kPieces = (4 * D + kThreads - 1) / kThreads;  // blocks of 32 codes that a lane stages
+  __shared__ __attribute__((aligned(16))) TileLds<D> lds;
+
+  const uint32_t head = blockIdx.x % a.cache.kv_heads, split = blockIdx.x / a.cache.kv_heads % a.tile_splits;
+  uint32_t b = 0;
+  int32_t tile = 0;
+  if (!FindTile(a, blockIdx.x / a.cache.kv_heads / a.tile_splits, kRows, b, tile)) return;
+  b = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b)));
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  const Sequence s = SequenceOf(a, b);
+  const TileKeys range = KeysOfTile(a, s, tile, kRows);
+  if (split >= range.parts) return;
+  const int32_t k0 = range.begin + static_cast<int32_t>(split) * range.part;
+  const int32_t k1 = min(range.end, k0 + range.part);
+  const int32_t tiles = k1 > k0 ? (k1 - k0 + kTileKeys - 1) / kTileKeys : 0;
+
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, g = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t group = static_cast<int32_t>(a.group), rows = s.count * group;
+  const int32_t r = tile * kRows + 32 * w + m;
+  const bool row_ok = r < rows;
+  const int32_t token = row_ok ? r / group : 0;
+  const uint32_t h = head * a.group + static_cast<uint32_t>(row_ok ? r - token * group : 0);
+  const int32_t before = s.keys - s.count;  // the first token's position
+  const int32_t pos = before + token;
+  // Positions of the wavefront's first and last row.
+  const int32_t low = before + (tile * kRows + 32 * w) / group;
+  const int32_t high = before + min((tile * kRows + 32 * w + 31) / group, s.count - 1);
+  const bool idle = tile * kRows + 32 * w >= rows;  // the wavefront has no row, and only stages
+  const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + h;
+
+  U4 q[kKs];
+  {
+    const uint16_t* qr = a.q + static_cast<uint64_t>(s.first + token) * a.q_stride + static_cast<uint64_t>(h) * D + 8 * g;
+#pragma unroll
+    for (int i = 0; i < kKs; ++i) {
+      const U4 x = *reinterpret_cast<const U4*>(qr + 16 * i);
+      q[i] = row_ok ? x : U4{0, 0, 0, 0};
+    }
+  }
+
+  // Staging: piece tid + i kThreads of [K, V] x 64 keys x blocks.
+  const uint32_t shift = a.cache.page_shift, in_page = (1u << shift) - 1;
+  const auto piece_of = [&](int i, bool& value, int32_t& key, uint32_t& block) {
+    const int p = tid + i * kThreads;
+    value = p >= 2 * D;
+    key = (p & (2 * D - 1)) / (D / 32);
+    block = static_cast<uint32_t>(p) & (D / 32 - 1);
+    return p < 4 * D;
+  };
+  int32_t ids[kPieces];
+  U4 codes[kPieces];
+  uint32_t scales[kPieces];
+  const auto load_ids = [&](int32_t t) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      bool value;
+      int32_t key;
+      uint32_t block;
+      ids[i] = -1;
+      if (!piece_of(i, value, key, block) || t >= tiles) continue;
+      const int32_t k = k0 + t * kTileKeys + key, entry = k >> shift;
+      if ((k & ~15) < k1 && entry < s.blocks) ids[i] = s.pages[entry];
+    }
+  };
+  const auto load_codes = [&](int32_t t) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      bool value;
+      int32_t key;
+      uint32_t block;
+      if (!piece_of(i, value, key, block)) continue;
+      if (static_cast<uint32_t>(ids[i]) >= a.cache.pages) ids[i] = -1;
+      const uint32_t within = static_cast<uint32_t>(k0 + t * kTileKeys + key) & in_page;
+      const uint64_t head_page = static_cast<uint64_t>(max(ids[i], 0)) * a.cache.kv_heads + head;
+      codes[i] = *reinterpret_cast<const U4*>((value ? a.cache.v : a.cache.k) + ((head_page << shift) + within) * (D / 2) + 16 * block);
+      scales[i] = (value ? a.cache.v_scales : a.cache.k_scales)[((head_page * (D / 32) + block) << shift) + within];
+      if (ids[i] < 0) scales[i] |= 0x100;  // no key
+    }
+  };
+  const auto store = [&](int32_t t, bool careful) {
+    const int slot = t % 3;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      bool value;
+      int32_t key;
+      uint32_t block;
+      if (!piece_of(i, value, key, block)) continue;
+      const bool none = (scales[i] & 0x100) != 0;
+      if (none && block == 0) atomicOr(&lds.bad[slot], 1u << (key / 16));
+      uint32_t byte = scales[i] & 0xFF;
+      if (value) {
+        if (none || k0 + t * kTileKeys + key >= k1) byte = 127;  // whatever lies there: finite, times p = 0
+        if (careful && byte > kF4ByteHigh) {
+          byte = 127;
+          atomicOr(&lds.nan[slot][key], 1u << block);
+        }
+      }
+      const float scale = F4Scale(byte);
+      unsigned char* const to = value ? lds.v[t & 1] : lds.k[t & 1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t c = codes[i][j];
+        const U4 x{FromF4<0>(c, scale), FromF4<1>(c, scale), FromF4<2>(c, scale), FromF4<3>(c, scale)};
+        const uint32_t off = value ? ValueAt<D>(key, block, j) : key * TileLds<D>::kKeyRow + 64 * block + 16 * j;
+        *reinterpret_cast<U4*>(to + off) = x;
+      }
+    }
+  };
+
+  F16v o[kDt];
+  float top, sum;
+  const auto pass = [&](bool careful) {
+    top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDt; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+    if (tid < 3) lds.bad[tid] = 0;
+    if (careful && tid < 64) lds.nan[0][tid] = lds.nan[1][tid] = lds.nan[2][tid] = 0;
+    __syncthreads();
+    if (tiles > 0) {
+      load_ids(0);
+      load_codes(0);
+      load_ids(1);
+      store(0, careful);
+    }
+    for (int32_t t = 0; t < tiles; ++t) {
+      __syncthreads();  // tile t is in LDS; nobody reads tile t - 1 any more
+      const int slot = t % 3, after = (t + 2) % 3;
+      if (tid == 0) lds.bad[after] = 0;
+      if (careful && tid < 64) lds.nan[after][tid] = 0;
+      if (t + 1 < tiles) {
+        load_codes(t + 1);
+        load_ids(t + 2);
+      }
+      const int32_t kb = k0 + t * kTileKeys;
+      if (!idle && !(a.causal && kb > high)) {
+        const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(lds.bad[slot])));
+        const bool mask = kb + kTileKeys > k1 || (a.causal && kb + kTileKeys - 1 > low) || bad != 0 ||
+                          (a.window >= 0 && kb < high - a.window);
+        const unsigned char* kt = lds.k[t & 1] + m * TileLds<D>::kKeyRow + 16 * g;
+        const unsigned char* vt = lds.v[t & 1];
+        // The transposing read of four keys x 16 dims by 16 lanes: lane 16 c + j addresses key j / 4, dims 4 (j % 4) of it.
+        const uint32_t j = lane & 15, key4 = 4 * g + j / 4, piece = 2 * (lane >> 4 & 1) + (j % 4) / 2;
+        uint32_t va[2];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) va[f] = ValueAt<D>(key4 + 8 * f, 0, piece) + 8 * (j & 1);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (a.causal && kb + 32 * half > high) break;
+          F16v sc;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sc[v] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kKs; ++i) {
+            sc = Mfma32(*reinterpret_cast<const U4*>(kt + 32 * half * TileLds<D>::kKeyRow + 32 * i), q[i], sc);
+          }
+          if constexpr (kCap) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sc[v] = Capped(sc[v] * a.scale_log2, a.cap);
+          }
+          if (mask) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              const int kk = 32 * half + 8 * (v / 4) + 4 * g + v % 4;
+              const int32_t key = kb + kk;
+              const bool off = (key >= k1) | ((a.causal != 0) & (key > pos)) | ((a.window >= 0) & (key < pos - a.window)) |
+                               ((bad >> (kk / 16) & 1) != 0);
+              sc[v] = off ? -INFINITY : sc[v];
+            }
+          }
+          const float scale = kCap ? 1.0f : a.scale_log2;
+          float mx = sc[0];
+#pragma unroll
+          for (int v = 1; v < 16; ++v) mx = fmaxf(mx, sc[v]);
+          mx *= scale;
+          if (__any(mx > top + kGrow)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float now = mx > top ? mx : top;
+            const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - now);
+            sum *= by;
+#pragma unroll
+            for (int d = 0; d < kDt; ++d)
+#pragma unroll
+              for (int v = 0; v < 16; ++v) o[d][v] *= by;
+            top = now;
+          }
+          const float base = top == -INFINITY ? 0.0f : top;
+          U4 p[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              y[e] = __builtin_amdgcn_exp2f(fmaf(sc[8 * c + e], scale, -base));
+              sum += y[e];
+            }
+            p[c] = U4{PackBf16Rne(y[0], y[1]), PackBf16Rne(y[2], y[3]), PackBf16Rne(y[4], y[5]), PackBf16Rne(y[6], y[7])};
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int d = 0; d < kDt; ++d) {
+              const uint32_t row = 16 * (2 * half + c) * 2 * D;
+              const U2 lo = LdsTranspose(vt, (va[0] ^ (64 * d)) + row), hi = LdsTranspose(vt, (va[1] ^ (64 * d)) + row);
+              o[d] = Mfma32(U4{lo[0], lo[1], hi[0], hi[1]}, p[c], o[d]);
+            }
+          }
+          if (careful) {
+            for (int kk = 32 * half; kk < 32 * half + 32; ++kk) {
+              const uint32_t blocks = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(lds.nan[slot][kk])));
+              if (blocks == 0) continue;
+              const int32_t key = kb + kk;
+              if ((a.causal && key > pos) || (a.window >= 0 && key < pos - a.window)) continue;
+#pragma unroll
+              for (int d = 0; d < kDt; ++d) {
+                if (blocks >> d & 1) {
+#pragma unroll
+                  for (int v = 0; v < 16; ++v) o[d][v] = NAN;
+                }
+              }
+            }
+          }
+        }
+      }
+      if (t + 1 < tiles) store(t + 1, careful);
+    }
+  };
+  pass(false);
+  bool nan = false;
+#pragma unroll
+  for (int d = 0; d < kDt; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) nan |= o[d][v] != o[d][v];
+  if (__syncthreads_or(nan)) pass(true);
+
+  sum += __shfl_xor(sum, 32);
+  if (!row_ok) return;
+  if (range.parts > 1) {
+    const uint64_t row = static_cast<uint64_t>(split) * a.tokens * a.q_heads + at;
+#pragma unroll
+    for (int d = 0; d < kDt; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        *reinterpret_cast<F4v*>(a.tile_o + row * D + 32 * d + 8 * i + 4 * g) =
+            F4v{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+      }
+    if (g == 0) a.tile_ml[2 * row] = top, a.tile_ml[2 * row + 1] = sum;
+    return;
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : NAN;
+#pragma unroll
+  for (int d = 0; d < kDt; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<U2*>(a.out + at * D + 32 * d + 8 * i + 4 * g) =
+          U2{PackBf16Rne(o[d][4 * i] * inv, o[d][4 * i + 1] * inv), PackBf16Rne(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv)};
+    }
+  if (a.lse != nullptr && g == 0) a.lse[at] = sum > 0.0f ? top + __builtin_amdgcn_logf(sum) : sum == sum ? -INFINITY : NAN;
+}
+
+// One row's parts, in order, by a wavefront. first: its first partial row, `step` rows between parts; at: its output row.
+template <int D>
+__device__ __forceinline__ void MergeRow(const Args& a, const float* part_o, const float* part_ml, uint64_t first, uint64_t step,
+                                         uint32_t parts, uint64_t at) {
   constexpr int kPer = D / 64;
-  const int32_t token = row / static_cast<int32_t>(a.group);
-  const uint32_t h = blockIdx.y * a.group + static_cast<uint32_t>(row - token * static_cast<int32_t>(a.group));
-  const uint64_t step = static_cast<uint64_t>(a.short_tokens) * a.q_heads;
-  const uint64_t first = static_cast<uint64_t>(blockIdx.z) * a.splits * step + static_cast<uint64_t>(token) * a.q_heads + h;
+  const int lane = threadIdx.x & 63;
   float big = -INFINITY;
-  for (uint32_t p = lane; p < parts; p += 64) big = fmaxf(big, a.part_ml[2 * (first + p * step)]);
+  for (uint32_t p = lane; p < parts; p += 64) big = fmaxf(big, part_ml[2 * (first + p * step)]);
 #pragma unroll
   for (int x = 32; x >= 1; x >>= 1) big = fmaxf(big, __shfl_xor(big, x));
   float total = 0.0f, y[kPer] = {};
   for (uint32_t p = 0; p < parts; ++p) {
-    const uint64_t at = first + p * step;
-    const float m = a.part_ml[2 * at];
+    const uint64_t row = first + p * step;
+    const float m = part_ml[2 * row];
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - big);
-    total += a.part_ml[2 * at + 1] * f;
+    total += part_ml[2 * row + 1] * f;
 #pragma unroll
-    for (int d = 0; d < kPer; ++d) y[d] += a.part_o[at * D + lane * kPer + d] * f;
+    for (int d = 0; d < kPer; ++d) y[d] += part_o[row * D + lane * kPer + d] * f;
   }
   const float inv = total > 0.0f ? 1.0f / total : total == total ? 0.0f : NAN;
-  const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + h;
 #pragma unroll
   for (int d = 0; d < kPer; ++d) a.out[at * D + lane * kPer + d] = static_cast<uint16_t>(PackBf16Rne(y[d] * inv, 0.0f));
   if (a.lse != nullptr && lane == 0) {
@@ -480,33 +831,95 @@ __global__ void __launch_bounds__(256) RowMergeKernel(Args a) {
   }
 }
 
+// Block (tile and KV head, rows by fours).
+template <int D, int kWaves>
+__global__ void __launch_bounds__(256) TileMergeKernel(Args a) {
+  const uint32_t head = blockIdx.x % a.cache.kv_heads;
+  uint32_t b = 0;
+  int32_t tile = 0;
+  if (!FindTile(a, blockIdx.x / a.cache.kv_heads, 32 * kWaves, b, tile)) return;
+  const Sequence s = SequenceOf(a, b);
+  const TileKeys range = KeysOfTile(a, s, tile, 32 * kWaves);
+  const int32_t group = static_cast<int32_t>(a.group);
+  const int32_t row = tile * 32 * kWaves + static_cast<int32_t>(blockIdx.y * 4 + threadIdx.x / 64);
+  if (range.parts <= 1 || row >= s.count * group) return;
+  const int32_t token = row / group;
+  const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + head * a.group + static_cast<uint32_t>(row - token * group);
+  MergeRow<D>(a, a.tile_o, a.tile_ml, at, static_cast<uint64_t>(a.tokens) * a.q_heads, range.parts, at);
+}
+
+// A split sequence's parts. Block (rows of a KV head by fours, KV head, sequence).
+template <int D>
+__global__ void __launch_bounds__(256) RowMergeKernel(Args a) {
+  const Sequence s = SequenceOf(a, blockIdx.z);
+  const int32_t group = static_cast<int32_t>(a.group), rows = s.count * group;
+  const int32_t row = static_cast<int32_t>(blockIdx.x * 4 + threadIdx.x / 64);
+  if (row >= rows || rows > static_cast<int32_t>(a.row_limit) || s.count > static_cast<int32_t>(a.short_tokens)) return;
+  const uint32_t parts = PartsOf(a, FirstKey(a, s, 0), s.keys);
+  if (parts <= 1) return;
+  const int32_t token = row / group;
+  const uint32_t h = blockIdx.y * a.group + static_cast<uint32_t>(row - token * group);
+  const uint64_t step = static_cast<uint64_t>(a.short_tokens) * a.q_heads;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.z) * a.splits * step + static_cast<uint64_t>(token) * a.q_heads + h;
+  MergeRow<D>(a, a.part_o, a.part_ml, first, step, parts, static_cast<uint64_t>(s.first + token) * a.q_heads + h);
+}
+
 // ---- Admission and launch --------------------------------------------------------------------------------------------------
 
+constexpr int TileWaves(uint32_t d) { return d == 256 ? 4 : 8; }
+
 struct Cut {
-  uint32_t tiles;         // of 16 rows in the row kernel
+  uint32_t row_tiles;     // of 16 rows in the row kernel
   uint32_t splits, part, short_tokens;
-  uint64_t rows;          // partial rows
+  uint64_t rows;          // its partial rows
+  bool by_row, by_tile;   // which kernels run
+  uint32_t row_limit;
+  uint32_t tiles, tile_splits;
+  uint64_t tile_rows;     // its partial rows
 };
 
 Cut CutOf(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
   Cut c{};
   const uint32_t group = p.q_heads / p.cache.kv_heads;
-  c.tiles = group > 16 ? 2 : 1;
-  c.short_tokens = 16 * c.tiles / group;
   const uint64_t most = p.kv_indptr.address != nullptr ? p.block_tables.length : p.max_blocks;
   uint64_t keys = p.max_kv_len ? p.max_kv_len : std::min<uint64_t>(most * p.cache.page_size, 16384);
-  if (p.window_left >= 0) keys = std::min<uint64_t>(keys, uint64_t{1} * p.window_left + 16 + c.short_tokens);
   keys = std::min<uint64_t>(std::max<uint64_t>(keys, 1), kMostKeys);
-  const uint64_t wanted = roost::CeilDiv(4 * cus, std::max<uint64_t>(1, uint64_t{p.batch} * p.cache.kv_heads));
-  const uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(wanted, roost::CeilDiv(keys, 128)));
-  c.part = static_cast<uint32_t>(roost::RoundUp(roost::CeilDiv(keys, splits), 64));
-  c.splits = static_cast<uint32_t>(roost::CeilDiv(keys, c.part));
-  c.rows = c.splits > 1 ? uint64_t{p.batch} * c.splits * c.short_tokens * p.q_heads : 0;
+  const auto seen = [&](uint64_t tokens) {
+    return p.window_left < 0 ? keys : std::min<uint64_t>(keys, uint64_t{1} * p.window_left + 16 + tokens);
+  };
+  // Which kernels: sequences of up to 16 rows (32 where a token alone has more than 16) go row by row, longer ones by tiles. One
+  // kernel is enough where no sequence is expected for the other; it then takes all, so an expectation that fails costs time only.
+  const uint64_t expected = uint64_t{p.max_q_len ? std::min(p.max_q_len, p.tokens) : p.tokens} * group;
+  c.row_tiles = group > 16 || (expected > 16 && expected <= 32) ? 2 : 1;
+  const uint32_t few = 16 * c.row_tiles;
+  c.short_tokens = few / group;
+  c.by_tile = expected > few;
+  c.by_row = !c.by_tile || p.batch > 1;
+  c.row_limit = !c.by_tile ? 0x7FFFFFFF : c.by_row ? few : 0;
+  if (c.by_row) {
+    const uint64_t wanted = roost::CeilDiv(4 * cus, std::max<uint64_t>(1, uint64_t{p.batch} * p.cache.kv_heads));
+    const uint64_t k = seen(c.short_tokens), splits = std::max<uint64_t>(1, std::min<uint64_t>(wanted, roost::CeilDiv(k, 128)));
+    c.part = static_cast<uint32_t>(roost::RoundUp(roost::CeilDiv(k, splits), 64));
+    c.splits = static_cast<uint32_t>(roost::CeilDiv(k, c.part));
+    c.rows = c.splits > 1 ? uint64_t{p.batch} * c.splits * c.short_tokens * p.q_heads : 0;
+  } else {
+    c.splits = 1, c.part = kMostKeys;
+  }
+  c.tile_splits = 1;
+  if (c.by_tile) {
+    const uint64_t rows = 32 * TileWaves(p.cache.head_dim), all = uint64_t{p.tokens} * group;
+    const uint64_t longer = std::min<uint64_t>(p.batch, all / (c.row_limit + 1));  // sequences that it can have
+    c.tiles = static_cast<uint32_t>(all / rows + longer);
+    const uint64_t groups = std::max<uint64_t>(1, roost::CeilDiv(all, rows) * p.cache.kv_heads);
+    if (4 * groups < 3 * cus) c.tile_splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(cus / groups, seen(p.tokens) / 512)));
+    c.tile_rows = c.tile_splits > 1 ? uint64_t{c.tile_splits} * p.tokens * p.q_heads : 0;
+  }
   return c;
 }
 
 uint64_t WorkspaceBytes(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
-  return CutOf(p, cus).rows * (p.cache.head_dim + 2) * 4;
+  const Cut c = CutOf(p, cus);
+  return (c.rows + c.tile_rows) * (p.cache.head_dim + 2) * 4;
 }
 
 RoostStatus Admit(const RoostAmdPagedAttentionF4Params& p, uint64_t& pages) {
@@ -579,10 +992,23 @@ RoostStatus Admit(const RoostAmdPagedAttentionF4Params& p, uint64_t& pages) {
   return gate.status();
 }
 
+template <int D, int kWaves>
+void LaunchTiles(const Args& a, const Cut& c, hipStream_t s) {
+  const uint32_t grid = c.tiles * a.cache.kv_heads * c.tile_splits;
+  if (a.capped) {
+    TileAttentionKernel<D, kWaves, true><<<grid, 64 * kWaves, 0, s>>>(a);
+  } else {
+    TileAttentionKernel<D, kWaves, false><<<grid, 64 * kWaves, 0, s>>>(a);
+  }
+  if (c.tile_splits > 1) TileMergeKernel<D, kWaves><<<dim3(c.tiles * a.cache.kv_heads, 8 * kWaves), 256, 0, s>>>(a);
+}
+
 template <int D>
 void Launch(const Args& a, const Cut& c, hipStream_t s) {
+  if (c.by_tile) LaunchTiles<D, TileWaves(D)>(a, c, s);
+  if (!c.by_row) return;
   const dim3 grid(a.cache.kv_heads, c.splits, a.batch);
-  if (c.tiles == 1) {
+  if (c.row_tiles == 1) {
     RowAttentionKernel<D, 1><<<grid, 64 * kRowWaves, 0, s>>>(a);
   } else {
     RowAttentionKernel<D, 2><<<grid, 64 * kRowWaves, 0, s>>>(a);
@@ -630,6 +1056,9 @@ extern "C" ROOST_API RoostStatus roost_amd_paged_attention_f4_run(RoostContext* 
     if (p.tokens == 0 || p.batch == 0) return ROOST_STATUS_OK;
     ROOST_GATE_RETURN(roost::OnDevice(gate, ctx));
     const Cut c = CutOf(p, ctx->compute_units);
+    gate.Expect(uint64_t{c.tiles} * p.cache.kv_heads * c.tile_splits < (1u << 23), ROOST_STATUS_UNSUPPORTED,
+                "%u tokens of %u heads: more tiles than one launch takes", p.tokens, p.q_heads);
+    ROOST_GATE_RETURN(gate);
     Args a{};
     a.q = static_cast<const uint16_t*>(p.q.address);
     a.out = static_cast<uint16_t*>(p.output.address);
@@ -650,7 +1079,10 @@ extern "C" ROOST_API RoostStatus roost_amd_paged_attention_f4_run(RoostContext* 
     a.causal = p.causal, a.window = p.window_left;
     a.part_o = ws != nullptr ? static_cast<float*>(ws->device) : nullptr;
     a.part_ml = a.part_o + c.rows * p.cache.head_dim;
-    a.splits = c.splits, a.part = c.part, a.short_tokens = c.short_tokens, a.row_limit = 0x7FFFFFFF;
+    a.tile_o = a.part_ml + 2 * c.rows;
+    a.tile_ml = a.tile_o + c.tile_rows * p.cache.head_dim;
+    a.splits = c.splits, a.part = c.part, a.short_tokens = c.short_tokens, a.row_limit = c.row_limit;
+    a.tile_splits = c.tile_splits;
     const hipStream_t s = roost::Stream(stream);
     if (p.cache.head_dim == 64) {
       Launch<64>(a, c, s);
