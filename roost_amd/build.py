@@ -39,8 +39,10 @@ def hipcc() -> str:
 
 
 # Per-source code-generation options. The GDN scan keeps its MFMA accumulators in architectural VGPRs (its
-# compute wavefronts read them with VALU every chunk; the AGPR form costs a copy per read).
-SOURCE_FLAGS = {"gated_delta_rule.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# compute wavefronts read them with VALU every chunk; the AGPR form costs a copy per read), and so does the attention over
+# 4-bit caches (their rescaling would copy every accumulator out and back).
+SOURCE_FLAGS = {"gated_delta_rule.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                "paged_attention_f4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src: str) -> Path:

@@ -53,22 +53,50 @@ struct Args {
   uint32_t capped, causal;
   int32_t window;
   // How the work is cut.
-  float *part_o, *part_ml;   // partial rows: sums before division, and (maximum, sum)
-  uint32_t splits, part;     // a sequence's keys in at most `splits` parts of `part`, the last one open-ended
+  float *part_o, *part_ml;   // the row kernel's partial rows: sums before division, and (maximum, sum)
+  uint32_t *cut;             // what it tells its merge: all units, then those before each sequence; NULL: nothing is split
+  uint32_t places;           // workgroups that share the units
+  uint32_t max_units;        // of a sequence: all sequences' together, in all KV heads, stay below 2^32
   uint32_t short_tokens;     // sequences of at most so many tokens may be split
   uint32_t row_limit;        // the row kernel takes sequences of at most so many rows, the tile kernel the others
   float *tile_o, *tile_ml;   // the tile kernel's partial rows, in at most tile_splits parts of its keys
   uint32_t tile_splits;
 };
 
+// The sum over the lanes up to this one, by lane shifts within rows of 16 and two broadcasts over them.
+__device__ __forceinline__ uint32_t WaveScan(uint32_t v) {
+  const auto add = [&](uint32_t o) { v += o; };
+  add(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x111, 0xf, 0xf, false)));
+  add(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x112, 0xf, 0xf, false)));
+  add(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x114, 0xf, 0xf, false)));
+  add(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x118, 0xf, 0xf, false)));
+  add(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x142, 0xa, 0xf, false)));
+  add(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x143, 0xc, 0xf, false)));
+  return v;
+}
+__device__ __forceinline__ uint32_t LaneOf(uint32_t v, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+__device__ __forceinline__ uint32_t WaveSum(uint32_t v) { return LaneOf(WaveScan(v), 63); }
+
 // ---- A sequence ---------------------------------------------------------------------------------------------------------
 
 struct Sequence {
   int32_t first, count;   // tokens
   int32_t keys;
-  int32_t blocks;         // entries at `pages`
-  const int32_t* pages;
+  int32_t blocks;         // its entries of the tables, from `entry` on
+  int64_t entry;
 };
+
+// Lane `from`'s sequence.
+__device__ __forceinline__ Sequence SequenceOfLane(const Sequence& s, int from) {
+  const auto of = [&](int32_t v) { return __builtin_amdgcn_readlane(v, from); };
+  Sequence t;
+  t.first = of(s.first), t.count = of(s.count), t.keys = of(s.keys), t.blocks = of(s.blocks);
+  t.entry = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(of(static_cast<int32_t>(s.entry)))) |
+                                 static_cast<uint64_t>(static_cast<uint32_t>(of(static_cast<int32_t>(s.entry >> 32)))) << 32);
+  return t;
+}
 
 __device__ __forceinline__ Sequence SequenceOf(const Args& a, uint32_t b) {
   Sequence s;
@@ -78,19 +106,19 @@ __device__ __forceinline__ Sequence SequenceOf(const Args& a, uint32_t b) {
   const uint32_t shift = a.cache.page_shift;
   int64_t keys = 0;
   s.blocks = 0;
-  s.pages = a.tables;
+  s.entry = 0;
   if (a.indptr != nullptr) {
     const int64_t begin = a.indptr[b], end = min(static_cast<int64_t>(a.indptr[b + 1]), static_cast<int64_t>(a.table_entries));
     if (begin >= 0 && end > begin) {
       s.blocks = static_cast<int32_t>(end - begin);
-      s.pages = a.tables + begin;
+      s.entry = begin;
       keys = ((end - begin - 1) << shift) + min(max(a.lens[b], 0), 1 << shift);
     }
   } else {
     const int32_t row = a.sequences != nullptr ? a.sequences[b] : static_cast<int32_t>(b);
     if (static_cast<uint32_t>(row) < a.table_rows) {
       s.blocks = static_cast<int32_t>(a.max_blocks);
-      s.pages = a.tables + static_cast<uint64_t>(row) * a.max_blocks;
+      s.entry = static_cast<int64_t>(row) * a.max_blocks;
       keys = min(static_cast<int64_t>(max(a.lens[row], 0)), static_cast<int64_t>(a.max_blocks) << shift);
     }
   }
@@ -103,11 +131,30 @@ __device__ __forceinline__ int32_t FirstKey(const Args& a, const Sequence& s, in
   return a.window < 0 ? 0 : max(0, s.keys - s.count + token - a.window) & ~15;
 }
 
-// Parts that the keys [begin, end) of a sequence go in.
-__device__ __forceinline__ uint32_t PartsOf(const Args& a, int32_t begin, int32_t end) {
-  if (end <= begin) return 1;
-  return min(static_cast<uint32_t>(end - begin + a.part - 1) / a.part, a.splits);
+constexpr int32_t kUnit = 128;            // keys: what the work of a batch is counted and cut in
+constexpr uint32_t kMaxScheduled = 704;   // sequences of a batch whose keys may be split (their units' room in LDS)
+
+// Whether the row kernel takes a sequence, and the units that its keys are (at most max_units: a last one takes what is left). 0:
+// not its own. One unit where the sequence is not to be split.
+__device__ __forceinline__ uint32_t UnitsOf(const Args& a, const Sequence& s) {
+  const int64_t rows = static_cast<int64_t>(s.count) * a.group;
+  if (rows == 0 || rows > static_cast<int64_t>(a.row_limit)) return 0;
+  if (s.count > static_cast<int32_t>(a.short_tokens)) return 1;
+  const int32_t units = (s.keys - FirstKey(a, s, 0) + kUnit - 1) / kUnit;
+  return min(static_cast<uint32_t>(max(units, 1)), a.max_units);
 }
+
+// All units, sequence by sequence, in each KV head after KV head, dealt to `places` workgroups in turn, the first of them one
+// more: the units of place c, and the place of unit x.
+struct Deal {
+  uint32_t each, more;  // more: places that have each + 1
+  __device__ __forceinline__ Deal(uint32_t units, uint32_t places) : each(units / places), more(units - each * places) {}
+  __device__ __forceinline__ uint32_t Begin(uint32_t c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ uint32_t PlaceOf(uint32_t x) const {
+    const uint32_t longer = more * (each + 1);
+    return x < longer ? x / (each + 1) : more + (x - longer) / each;
+  }
+};
 
 // ---- The row kernel -----------------------------------------------------------------------------------------------------------
 // Up to 16 kTiles rows (a few tokens' query heads of one KV head) against one part of a sequence's keys: decode. Bound by the
@@ -115,101 +162,168 @@ __device__ __forceinline__ uint32_t PartsOf(const Args& a, int32_t begin, int32_
 //
 // Operands of v_mfma_f32_16x16x32_bf16, lane l = 16 g + m: A[m][8 g + j], B[8 g + j][m], result [4 g + i][m].
 //   S^T = K Q^T: key m of 16 as A, query row m as B. The contraction runs over the dims in any order, so lane (m, g) takes its
-//   key's 16 bytes g, dims 32 g .. 32 g + 31 (head_dim 128): one scale a lane, word s the operand of step s, and 16 keys' codes
-//   are one load of 1 KB.
+//   key's 16 bytes g, dims 32 g .. 32 g + 31 (head_dim 128): one scale a lane, word s the operand of step s.
 //   O^T = V^T P^T: dim as A, keys contracted. Lane (m, g) of S^T holds rows' scores of keys 4 g + i of both 16-key groups; as B
 //   it needs eight keys: those. So keys are contracted in the order 16 (j / 4) + 4 g + j % 4, and p goes from result to operand
 //   without leaving the lane. A's lane (m, g) takes dims D / 16 m .. of those eight keys: one word a key (head_dim 128), eight
 //   dims a lane, dim d of the word the operand of product d.
-// Four wavefronts take the part's keys in turn by quarters; no barrier until their results meet in LDS.
-
+//
+// Four wavefronts take the part's steps of 32 keys in turn, each through a ring of its own in LDS that global_load_lds fills:
+// 34 D bytes a step, kStages steps under way without a register, no barrier until the results meet. A step's copies are awaited
+// by count.
+//
+// The units (128 keys of one KV head) of all sequences are dealt evenly to as many workgroups as the chip holds at once, each a
+// run of them, whatever sequences and KV heads that run through: a sequence's length then costs what it reads and no
+// workgroup waits for another. A KV head that a run holds whole is written out; of one that is cut, each workgroup leaves sums
+// for the merge: a run is cut at its two ends at most, so two places a workgroup hold them. Every workgroup finds its run by itself
+// from the lengths on the device, which a captured call cannot know before.
 constexpr int kRowWaves = 4;
 constexpr int kStep = 32;  // keys a wavefront takes at a time
 
-// Codes and scales of one step's keys in a lane.
 template <int D>
-struct RowStage {
-  uint32_t k[2][D / 32];  // words of the lane's key in each group of 16
-  uint32_t ks[2][D == 256 ? 2 : 1];
-  uint32_t v[8][D == 256 ? 2 : 1];  // D = 64: the low half
-  uint32_t vs[2];                   // four keys' scale bytes in each group
+struct RowRing {
+  static constexpr int kCodes = kStep * D / 2;            // bytes of K's, and of V's, codes of a step
+  static constexpr int kScales = 2 * D < 256 ? 256 : 2 * D;  // of both scales: [K, V][group][block][16 keys], at least one copy's
+  static constexpr int kStage = 2 * kCodes + kScales;
+  static constexpr int kCopies = 2 * kCodes / 1024 + kScales / 256;
+  static constexpr int kStages = D == 256 ? 2 : 3;
+  static constexpr int kResident = D == 256 ? 2 : D == 128 ? 3 : 4;  // workgroups a CU holds: LDS and registers
 };
 
-template <int D, int kTiles>
-__global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
+// The memory that p points at in each lane to LDS, 16 (or 4) bytes a lane, one behind the other from `lds` on. M0 is read
+// a wait state after its write.
+__device__ __forceinline__ void Copy16(const void* p, uint32_t lds) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(p), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void Copy4(const void* p, uint32_t lds) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(p), "s"(lds) : "memory");
+}
+
+typedef __attribute__((address_space(3))) unsigned char LdsByte;
+__device__ __forceinline__ uint32_t LdsAddress(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const LdsByte*)p));
+}
+
+template <int D, int kTiles, bool kCap>
+__global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : D == 128 ? 3 : 4) RowAttentionKernel(Args a) {
+  typedef RowRing<D> Ring;
   constexpr int kWords = D / 32;   // of a lane's key
   constexpr int kDt = D / 16;      // dims of a lane's V word(s): products of 16 dims each
   constexpr int kBlocks = D / 32;
-  __shared__ float red_o[kRowWaves][16][D];
-  __shared__ float red_ml[kRowWaves][2][16];
-
-  const uint32_t head = blockIdx.x, part = blockIdx.y;
-  const Sequence s = SequenceOf(a, blockIdx.z);
-  const int32_t rows = s.count * static_cast<int32_t>(a.group);
-  if (rows == 0 || rows > static_cast<int32_t>(a.row_limit)) return;
-  const int32_t begin = FirstKey(a, s, 0), end = s.keys;
-  const bool split = s.count <= static_cast<int32_t>(a.short_tokens);
-  const uint32_t parts = split ? PartsOf(a, begin, end) : 1;
-  if (part >= parts) return;
-  const int32_t k0 = begin + static_cast<int32_t>(part * a.part);
-  const int32_t k1 = part + 1 == parts ? end : k0 + static_cast<int32_t>(a.part);
+  constexpr int kStages = Ring::kStages;
+  struct Result {
+    float o[kRowWaves][16][D];
+    float ml[kRowWaves][2][16];
+  };
+  constexpr int kBytes = kRowWaves * kStages * Ring::kStage;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[kBytes > sizeof(Result) ? kBytes : sizeof(Result)];
+  Result& result = *reinterpret_cast<Result*>(lds);  // once all wavefronts are through with their rings
 
   const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // The wavefront's quarter, in whole steps.
-  const int32_t steps = max(0, (k1 - k0 + kStep - 1) / kStep), each = (steps + kRowWaves - 1) / kRowWaves;
-  const int32_t step0 = min(w * each, steps), my_steps = min(each, steps - step0);
-  const int32_t my0 = k0 + step0 * kStep;
-  const uint32_t shift = a.cache.page_shift, in_page = (1u << shift) - 1;
-
-  // Page ids of 64 groups of 16 keys, one a lane; -1 for a page that is none.
-  int32_t ids = -1;
-  const auto load_ids = [&](int32_t step) {
-    const int32_t key = my0 + step * kStep + 16 * lane, at = key >> shift;
-    ids = -1;
-    if (key < k1 && at < s.blocks) ids = s.pages[at];
-    if (static_cast<uint32_t>(ids) >= a.cache.pages) ids = -1;
+  const uint32_t heads = a.cache.kv_heads;
+  __shared__ uint16_t units[kMaxScheduled];
+  // Workgroup i runs on die i % 8: each die takes neighbouring runs, so that the scales of two heads, which share a line of
+  // memory, come to one L2.
+  const uint32_t share = (a.places + 7) / 8, place = blockIdx.x % 8 * share + blockIdx.x / 8;
+  if (blockIdx.x / 8 >= share || place >= a.places) return;
+  // The run [x, end) of units; the sequence of x, the units before it and its own.
+  uint32_t x = 0, end = 0, before = 0, b = place / heads, own = 1;
+  Sequence s;
+  const auto find = [&](uint32_t mine) {  // mine: the units of sequence `lane`, for a batch of up to 64
+    const uint32_t y = x / heads;
+    uint32_t base = 0, sum = 0;
+    for (;; base += 64) {
+      const uint32_t here = a.batch <= 64 ? mine : base + lane < a.batch ? units[base + lane] : 0;
+      const uint32_t to = sum + WaveScan(here);
+      const uint64_t past = __ballot(y < to);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        b = base + static_cast<uint32_t>(at);
+        own = LaneOf(here, at);
+        before = LaneOf(to, at) - own;
+        return;
+      }
+      sum = LaneOf(to, 63);
+    }
   };
-  // A group's rows: its codes start at row * D / 2, its scales of block b at srow + (b << shift). Pages that are none: page 0,
-  // whose keys are masked.
-  const auto load = [&](int32_t step, RowStage<D>& st) {
+  uint32_t mine = 0;
+  if (a.cut != nullptr) {
+    uint32_t sum = 0;
+    Sequence of{};
+    if (a.batch <= 64) {
+      if (lane < a.batch) of = SequenceOf(a, lane), mine = UnitsOf(a, of);
+      sum = WaveSum(mine);
+    } else {
+      for (uint32_t i = threadIdx.x; i < a.batch; i += 64 * kRowWaves) units[i] = static_cast<uint16_t>(UnitsOf(a, SequenceOf(a, i)));
+      __syncthreads();
+      for (uint32_t i = lane; i < a.batch; i += 64) sum += units[i];
+      sum = WaveSum(sum);
+    }
+    const Deal deal(sum * heads, a.places);
+    x = deal.Begin(place), end = deal.Begin(place + 1);
+    if (place == 0 && threadIdx.x == 0) a.cut[0] = sum;
+    if (x >= end) return;
+    find(mine);
+    s = a.batch <= 64 ? SequenceOfLane(of, static_cast<int>(b)) : SequenceOf(a, b);
+  } else {
+    s = SequenceOf(a, b);
+    if (UnitsOf(a, s) == 0) return;
+  }
+
+#pragma unroll 1
+  for (bool opening = true;; opening = false) {
+  // One KV head's part of the run.
+  const uint32_t head = a.cut != nullptr ? (x - before * heads) / own : place % heads;
+  const uint32_t from = a.cut != nullptr ? x - before * heads - head * own : 0;
+  const uint32_t to = a.cut != nullptr ? min(own, from + (end - x)) : 1;
+  const bool whole = from == 0 && to == own;
+  const int32_t rows = s.count * static_cast<int32_t>(a.group);
+  if (a.cut != nullptr && from == 0 && head == 0 && threadIdx.x == 0) a.cut[1 + b] = before;
+  const int32_t k0 = FirstKey(a, s, 0) + static_cast<int32_t>(from) * kUnit;
+  const int32_t k1 = to == own ? s.keys : k0 + static_cast<int32_t>(to - from) * kUnit;
+
+  const int32_t steps = max(0, (k1 - k0 + kStep - 1) / kStep), my_steps = (steps + kRowWaves - 1 - w) / kRowWaves;
+  const auto key_of = [&](int32_t step) { return k0 + (step * kRowWaves + w) * kStep; };
+  const uint32_t shift = a.cache.page_shift, in_page = (1u << shift) - 1;
+  unsigned char* const ring = lds + w * kStages * Ring::kStage;
+
+  // Page ids of a window of 32 steps, a group of 16 keys a lane; -1 for a page that is none.
+  const auto ids_of = [&](int32_t window) {
+    const int32_t key = key_of(window * 32 + lane / 2) + 16 * (lane & 1), at = key >> shift;
+    int32_t id = -1;
+    if (key < k1 && at < s.blocks) id = a.tables[s.entry + at];
+    return static_cast<uint32_t>(id) < a.cache.pages ? id : -1;
+  };
+
+  // One step's codes and scales to the ring. Pages that are none: page 0, whose keys are masked.
+  const auto issue = [&](int32_t step, int32_t ids) {
+    const uint32_t to = LdsAddress(ring) + static_cast<uint32_t>(step % kStages) * Ring::kStage;
+    uint64_t row[2], scale_row[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int32_t id = __builtin_amdgcn_readlane(ids, (2 * step + t) & 63);
-      const uint32_t key = static_cast<uint32_t>(my0 + step * kStep + 16 * t) & in_page;
+      const uint32_t key = static_cast<uint32_t>(key_of(step) + 16 * t) & in_page;
       const uint64_t head_page = static_cast<uint64_t>(max(id, 0)) * a.cache.kv_heads + head;
-      const uint64_t row = (head_page << shift) + key;
-      const uint64_t srow = ((head_page * kBlocks) << shift) + key;
-      const uint8_t* kc = a.cache.k + row * (D / 2);
-      const uint8_t* ksc = a.cache.k_scales + srow;
-      const uint8_t* vc = a.cache.v + row * (D / 2);
-      const uint8_t* vsc = a.cache.v_scales + srow;
-      if constexpr (D == 64) {
-        const U2 x = *reinterpret_cast<const U2*>(kc + m * 32 + 8 * g);
-        st.k[t][0] = x[0], st.k[t][1] = x[1];
-        st.ks[t][0] = ksc[((g >> 1) << shift) + m];
-      } else {
+      row[t] = ((head_page << shift) + key) * (D / 2);
+      scale_row[t] = ((head_page * kBlocks) << shift) + key;
+    }
 #pragma unroll
-        for (int h = 0; h < D / 128; ++h) {
-          const U4 x = *reinterpret_cast<const U4*>(kc + m * (D / 2) + 64 * h + 16 * g);
+    for (int i = 0; i < Ring::kCodes / 1024; ++i) {
+      const uint32_t byte = 1024 * i + 16 * lane;  // of [group][16 keys x D / 2]
+      const uint64_t from = (D == 64 ? (lane < 32 ? row[0] : row[1]) : row[i / (D / 128)]) + byte % (8 * D);
+      Copy16(a.cache.k + from, to + 1024 * i);
+      Copy16(a.cache.v + from, to + Ring::kCodes + 1024 * i);
+    }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) st.k[t][4 * h + i] = x[i];
-          st.ks[t][h] = ksc[((4 * h + g) << shift) + m];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* p = vc + (4 * g + i) * (D / 2) + m * (D / 32);
-        if constexpr (D == 64) {
-          st.v[4 * t + i][0] = *reinterpret_cast<const uint16_t*>(p);
-        } else if constexpr (D == 128) {
-          st.v[4 * t + i][0] = *reinterpret_cast<const uint32_t*>(p);
-        } else {
-          const U2 x = *reinterpret_cast<const U2*>(p);
-          st.v[4 * t + i][0] = x[0], st.v[4 * t + i][1] = x[1];
-        }
-      }
-      st.vs[t] = *reinterpret_cast<const uint32_t*>(vsc + ((m / (512 / D)) << shift) + 4 * g);
+    for (int i = 0; i < Ring::kScales / 256; ++i) {
+      const uint32_t x = 64 * i + lane, block = x / 4 % kBlocks, t = x / (4 * kBlocks) % 2, value = x / (8 * kBlocks) % 2;
+      const uint64_t from = (t == 0 ? scale_row[0] : scale_row[1]) + (block << shift) + 4 * (x % 4);
+      Copy4((value ? a.cache.v_scales : a.cache.k_scales) + from, to + 2 * Ring::kCodes + 256 * i);
     }
   };
 
@@ -217,7 +331,6 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
     // Query rows: lane m's of each 16.
     int32_t pos[kTiles];
     U4 q[kTiles][kWords];
-    int64_t row_at[kTiles];  // token * q_heads + head, or -1
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
       const int32_t r = (tile * kTiles + n) * 16 + m;
@@ -225,7 +338,6 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
       const int32_t token = ok ? r / static_cast<int32_t>(a.group) : 0;
       const uint32_t h = head * a.group + (ok ? r - token * static_cast<int32_t>(a.group) : 0);
       pos[n] = ok ? s.keys - s.count + token : -1;
-      row_at[n] = ok ? static_cast<int64_t>(s.first + token) * a.q_heads + h : -1;
       const uint16_t* qr = a.q + static_cast<uint64_t>(s.first + token) * a.q_stride + static_cast<uint64_t>(h) * D;
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
@@ -246,15 +358,73 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
 #pragma unroll
         for (int d = 0; d < kDt; ++d) o[n][d] = F4v{0, 0, 0, 0};
       }
-      const auto compute = [&](int32_t step, RowStage<D>& st) {
-        const int32_t key0 = my0 + step * kStep;
-        const int32_t id0 = __builtin_amdgcn_readlane(ids, (2 * step) & 63);
-        const int32_t id1 = __builtin_amdgcn_readlane(ids, (2 * step + 1) & 63);
-        const bool edge = key0 + kStep > k1 || (id0 | id1) < 0;
+      int32_t ids = ids_of(0), ids_next = my_steps > 32 ? ids_of(1) : -1;
+      uint64_t bad_issued = __ballot(ids < 0), bad = bad_issued;  // groups without a page, of the window issued from, and of this one
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) {
+        if (i < my_steps) issue(i, ids);
+      }
+#pragma unroll 1
+      for (int32_t step = 0; step < my_steps; ++step) {
+        if ((step & 31) == 0) bad = bad_issued;
+        if (step + kStages <= my_steps) {
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * Ring::kCopies) : "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        // The lane's share of the step: key m's codes and scales in each group, its dims of the eight keys and their scales.
+        uint32_t kc[2][kWords], ks[2][D == 256 ? 2 : 1], vc[8][D == 256 ? 2 : 1], vs[2];
+        {
+          const unsigned char* at = ring + static_cast<uint32_t>(step % kStages) * Ring::kStage;
+          const unsigned char* sc = at + 2 * Ring::kCodes;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if constexpr (D == 64) {
+              const U2 x = *reinterpret_cast<const U2*>(at + 512 * t + 32 * m + 8 * g);
+              kc[t][0] = x[0], kc[t][1] = x[1];
+              ks[t][0] = sc[16 * (t * kBlocks + g / 2) + m];
+            } else {
+#pragma unroll
+              for (int h = 0; h < D / 128; ++h) {
+                const U4 x = *reinterpret_cast<const U4*>(at + 8 * D * t + m * (D / 2) + 64 * h + 16 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kc[t][4 * h + i] = x[i];
+                ks[t][h] = sc[16 * (t * kBlocks + 4 * h + g) + m];
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const unsigned char* p = at + Ring::kCodes + 8 * D * t + (4 * g + i) * (D / 2) + m * (D / 32);
+              if constexpr (D == 64) {
+                vc[4 * t + i][0] = *reinterpret_cast<const uint16_t*>(p);
+              } else if constexpr (D == 128) {
+                vc[4 * t + i][0] = *reinterpret_cast<const uint32_t*>(p);
+              } else {
+                const U2 x = *reinterpret_cast<const U2*>(p);
+                vc[4 * t + i][0] = x[0], vc[4 * t + i][1] = x[1];
+              }
+            }
+            vs[t] = *reinterpret_cast<const uint32_t*>(sc + 32 * kBlocks + 16 * (t * kBlocks + m / (512 / D)) + 4 * g);
+          }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the next copies may take the stage
+        if (step + kStages < my_steps) {
+          const int32_t next = step + kStages;
+          if ((next & 31) == 0) {
+            ids = ids_next;
+            bad_issued = __ballot(ids < 0);
+            if (next + 32 < my_steps) ids_next = ids_of(next / 32 + 1);
+          }
+          issue(next, ids);
+        }
+
+        const int32_t key0 = key_of(step);
+        const uint32_t none = static_cast<uint32_t>(bad >> ((2 * step) & 63)) & 3;  // groups without a page
+        const bool edge = key0 + kStep > k1 || none != 0;
         const bool mask = edge || (a.causal && key0 + kStep > s.keys - s.count + 1) ||
                           (a.window >= 0 && key0 < s.keys - 1 - a.window);
         const auto absent = [&](int t, int i) {  // key 16 t + 4 g + i is none of the part's
-          return key0 + 16 * t + 4 * g + i >= k1 || (t == 0 ? id0 : id1) < 0;
+          return key0 + 16 * t + 4 * g + i >= k1 || (none >> t & 1) != 0;
         };
         F4v sc[kTiles][2];
 #pragma unroll
@@ -263,23 +433,25 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
           for (int n = 0; n < kTiles; ++n) sc[n][t] = F4v{0, 0, 0, 0};
 #pragma unroll
           for (int i = 0; i < kWords; ++i) {
-            const float scale = F4Scale(st.ks[t][D == 256 ? i / 4 : 0]);
-            const uint32_t c = st.k[t][i];
+            const float scale = F4Scale(ks[t][D == 256 ? i / 4 : 0]);
+            const uint32_t c = kc[t][i];
             const U4 kk{FromF4<0>(c, scale), FromF4<1>(c, scale), FromF4<2>(c, scale), FromF4<3>(c, scale)};
 #pragma unroll
             for (int n = 0; n < kTiles; ++n) sc[n][t] = Mfma16(kk, q[n][i], sc[n][t]);
           }
         }
-        float vscale[8];
         uint32_t nan_keys = 0;
+        if (edge || careful) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < 2; ++t) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t byte = st.vs[t] >> (8 * i) & 0xFF;
-            if (edge && absent(t, i)) byte = 127;  // whatever lies there: finite, times p = 0
-            if (careful && byte > kF4ByteHigh) byte = 127, nan_keys |= 1u << (4 * t + i);
-            vscale[4 * t + i] = F4Scale(byte);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t byte = vs[t] >> (8 * i) & 0xFF;
+              const bool nan = careful && byte > kF4ByteHigh;
+              const bool off = absent(t, i);
+              if (nan && !off) nan_keys |= 1u << (4 * t + i);
+              if (nan || off) vs[t] = (vs[t] & ~(0xFFu << (8 * i))) | 127u << (8 * i);  // finite, whatever lies there, times p = 0
+            }
           }
         }
         U4 p[kTiles];
@@ -288,8 +460,8 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
           float y[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            y[j] = sc[n][j / 4][j % 4] * a.scale_log2;
-            if (a.capped) y[j] = Capped(y[j], a.cap);
+            y[j] = sc[n][j / 4][j % 4];
+            if constexpr (kCap) y[j] = Capped(y[j] * a.scale_log2, a.cap);
           }
           if (mask) {
 #pragma unroll
@@ -300,9 +472,11 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
               y[j] = off ? -INFINITY : y[j];
             }
           }
+          const float scale = kCap ? 1.0f : a.scale_log2;  // positive: the largest score stays the largest
           float mx = y[0];
 #pragma unroll
           for (int j = 1; j < 8; ++j) mx = fmaxf(mx, y[j]);
+          mx *= scale;
           if (__any(mx > top[n] + kGrow)) {
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -316,7 +490,7 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
           const float base = top[n] == -INFINITY ? 0.0f : top[n];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            y[j] = __builtin_amdgcn_exp2f(y[j] - base);
+            y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], scale, -base));
             sum[n] += y[j];
           }
           p[n] = U4{PackBf16Rne(y[0], y[1]), PackBf16Rne(y[2], y[3]), PackBf16Rne(y[4], y[5]), PackBf16Rne(y[6], y[7])};
@@ -325,7 +499,7 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
         const auto two = [&](auto pair, int word, int out) {
           uint32_t c[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) c[j] = FromF4<decltype(pair)::value>(st.v[j][word], vscale[j]);
+          for (int j = 0; j < 8; ++j) c[j] = FromF4<decltype(pair)::value>(vc[j][word], F4Scale(vs[j / 4] >> (8 * (j % 4)) & 0xFF));
           U4 lo, hi;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -366,77 +540,74 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
             }
           }
         }
-      };
-      RowStage<D> even, odd;
-      for (int32_t first = 0; first < my_steps; first += 32) {  // 64 groups' page ids
-        load_ids(first);
-        const int32_t last = min(my_steps, first + 32);
-        load(first, even);
-        for (int32_t i = first; i < last; i += 2) {
-          if (i + 1 < last) load(i + 1, odd);
-          compute(i, even);
-          if (i + 1 >= last) break;
-          if (i + 2 < last) load(i + 2, even);
-          compute(i + 1, odd);
-        }
       }
     };
-    pass(false);
-    bool nan = false;
+    bool careful = false;
+#pragma unroll 1
+    for (;;) {
+      pass(careful);
+      if (careful) break;
+      bool nan = false;
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n)
+      for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-      for (int d = 0; d < kDt; ++d)
+        for (int d = 0; d < kDt; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) nan |= o[n][d][i] != o[n][d][i];
-    if (__any(nan)) pass(true);
+          for (int i = 0; i < 4; ++i) nan |= o[n][d][i] != o[n][d][i];
+      if (!__any(nan)) break;
+      careful = true;
+    }
 
     // The four wavefronts' results meet, 16 rows at a time.
 #pragma unroll
     for (int n = 0; n < kTiles; ++n) {
+      const int32_t row0 = (tile * kTiles + n) * 16;
       float l = sum[n];
       l += __shfl_xor(l, 16);
       l += __shfl_xor(l, 32);
-      if (n > 0 || tile > 0) __syncthreads();  // the rows before are read
-      if (g == 0) red_ml[w][0][m] = top[n], red_ml[w][1][m] = l;
+      __syncthreads();  // the rings, or the rows before, are read
+      if (g == 0) result.ml[w][0][m] = top[n], result.ml[w][1][m] = l;
+      if (row0 + m < rows) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int d = 0; d < kDt; d += 4) {
-          *reinterpret_cast<F4v*>(&red_o[w][m][(4 * g + i) * kDt + d]) =
-              F4v{o[n][d][i], o[n][d + 1][i], o[n][d + 2][i], o[n][d + 3][i]};
-        }
+          for (int d = 0; d < kDt; d += 4) {
+            *reinterpret_cast<F4v*>(&result.o[w][m][(4 * g + i) * kDt + d]) =
+                F4v{o[n][d][i], o[n][d + 1][i], o[n][d + 2][i], o[n][d + 3][i]};
+          }
+      }
       __syncthreads();
       constexpr int kThreadsPerRow = 16, kPer = D / kThreadsPerRow;  // 16 rows x 16 threads
       const int r = threadIdx.x / kThreadsPerRow, d0 = (threadIdx.x % kThreadsPerRow) * kPer;
-      const int32_t row = (tile * kTiles + n) * 16 + r;
+      const int32_t row = row0 + r;
       if (row >= rows) continue;
-      float big = red_ml[0][0][r];
+      float big = result.ml[0][0][r];
 #pragma unroll
-      for (int x = 1; x < kRowWaves; ++x) big = fmaxf(big, red_ml[x][0][r]);
+      for (int x = 1; x < kRowWaves; ++x) big = fmaxf(big, result.ml[x][0][r]);
       float total = 0.0f, f[kRowWaves], y[kPer];
 #pragma unroll
       for (int x = 0; x < kRowWaves; ++x) {
-        f[x] = red_ml[x][0][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(red_ml[x][0][r] - big);
-        total += red_ml[x][1][r] * f[x];
+        f[x] = result.ml[x][0][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(result.ml[x][0][r] - big);
+        total += result.ml[x][1][r] * f[x];
       }
 #pragma unroll
       for (int d = 0; d < kPer; ++d) {
         y[d] = 0.0f;
 #pragma unroll
-        for (int x = 0; x < kRowWaves; ++x) y[d] += red_o[x][r][d0 + d] * f[x];
+        for (int x = 0; x < kRowWaves; ++x) y[d] += result.o[x][r][d0 + d] * f[x];
       }
       const int32_t token = row / static_cast<int32_t>(a.group);
       const uint32_t h = head * a.group + static_cast<uint32_t>(row - token * static_cast<int32_t>(a.group));
-      if (parts > 1) {
-        const uint64_t at = ((static_cast<uint64_t>(blockIdx.z) * a.splits + part) * a.short_tokens + token) * a.q_heads + h;
+      if (!whole) {
+        // A part that began in an earlier run opens this one; else it goes on in the next.
+        const uint64_t at = (2 * static_cast<uint64_t>(place) + (opening && from != 0 ? 0 : 1)) * a.short_tokens * a.group +
+                            static_cast<uint32_t>(row);
 #pragma unroll
         for (int d = 0; d < kPer; d += 4) {
           *reinterpret_cast<F4v*>(a.part_o + at * D + d0 + d) = F4v{y[d], y[d + 1], y[d + 2], y[d + 3]};
         }
         if (d0 == 0) a.part_ml[2 * at] = big, a.part_ml[2 * at + 1] = total;
-        continue;
-      }
+      } else {
       const float inv = total > 0.0f ? 1.0f / total : total == total ? 0.0f : NAN;
       const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + h;
 #pragma unroll
@@ -447,7 +618,16 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
       if (a.lse != nullptr && d0 == 0) {
         a.lse[at] = total > 0.0f ? big + __builtin_amdgcn_logf(total) : total == total ? -INFINITY : NAN;
       }
+      }
     }
+    __syncthreads();  // the results are read: the rings may be filled again
+  }
+  x += to - from;
+  if (x >= end) return;
+  if (x >= (before + own) * heads) {
+    find(mine);
+    s = SequenceOf(a, b = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b))));
+  }
   }
 }
 
@@ -467,8 +647,6 @@ __global__ void __launch_bounds__(64 * kRowWaves) RowAttentionKernel(Args a) {
 // the key, and their 16-byte pieces by the next bits of it, which does the same for the transposing reads of 8 keys x 64 bytes.
 
 constexpr int kTileKeys = 64;
-
-typedef __attribute__((address_space(3))) unsigned char LdsByte;
 
 __device__ __forceinline__ U2 LdsTranspose(const unsigned char* base, uint32_t off) {
   auto* p = reinterpret_cast<__attribute__((address_space(3))) I4h*>(const_cast<LdsByte*>((const LdsByte*)base + off));
@@ -604,7 +782,7 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
       ids[i] = -1;
       if (!piece_of(i, value, key, block) || t >= tiles) continue;
       const int32_t k = k0 + t * kTileKeys + key, entry = k >> shift;
-      if ((k & ~15) < k1 && entry < s.blocks) ids[i] = s.pages[entry];
+      if ((k & ~15) < k1 && entry < s.blocks) ids[i] = a.tables[s.entry + entry];
     }
   };
   const auto load_codes = [&](int32_t t) {
@@ -804,34 +982,62 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
   if (a.lse != nullptr && g == 0) a.lse[at] = sum > 0.0f ? top + __builtin_amdgcn_logf(sum) : sum == sum ? -INFINITY : NAN;
 }
 
-// One row's parts, in order, by a wavefront. first: its first partial row, `step` rows between parts; at: its output row.
-template <int D>
-__device__ __forceinline__ void MergeRow(const Args& a, const float* part_o, const float* part_ml, uint64_t first, uint64_t step,
-                                         uint32_t parts, uint64_t at) {
-  constexpr int kPer = D / 64;
-  const int lane = threadIdx.x & 63;
-  float big = -INFINITY;
-  for (uint32_t p = lane; p < parts; p += 64) big = fmaxf(big, part_ml[2 * (first + p * step)]);
+// One row's parts by a workgroup: D / 4 lanes a part, their loads together, then the lanes' sums. The order of the additions is that
+// of the parts' numbers, whichever workgroup wrote them when. row_of(p): part p's partial row; at: the output row.
+template <int D, typename F>
+__device__ __forceinline__ void MergeRow(const Args& a, const float* part_o, const float* part_ml, F&& row_of, uint32_t parts,
+                                         uint64_t at) {
+  constexpr uint32_t kLanes = D / 4, kGroups = 256 / kLanes, kAtOnce = 4;
+  __shared__ float sums[kGroups][D + 4];
+  __shared__ float totals[kGroups], tops[kGroups];
+  const uint32_t group = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+  float top = -INFINITY, total = 0.0f;
+  F4v y{0, 0, 0, 0};
+  for (uint32_t p0 = group; p0 < parts; p0 += kGroups * kAtOnce) {
+    float m[kAtOnce], l[kAtOnce];
+    F4v v[kAtOnce];
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) big = fmaxf(big, __shfl_xor(big, x));
-  float total = 0.0f, y[kPer] = {};
-  for (uint32_t p = 0; p < parts; ++p) {
-    const uint64_t row = first + p * step;
-    const float m = part_ml[2 * row];
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - big);
-    total += part_ml[2 * row + 1] * f;
+    for (uint32_t i = 0; i < kAtOnce; ++i) {
+      const uint32_t p = p0 + i * kGroups;
+      m[i] = -INFINITY, l[i] = 0.0f, v[i] = F4v{0, 0, 0, 0};
+      if (p < parts) {
+        const uint64_t row = row_of(p);
+        m[i] = part_ml[2 * row], l[i] = part_ml[2 * row + 1];
+        v[i] = *reinterpret_cast<const F4v*>(part_o + row * D + d);
+      }
+    }
 #pragma unroll
-    for (int d = 0; d < kPer; ++d) y[d] += part_o[row * D + lane * kPer + d] * f;
+    for (uint32_t i = 0; i < kAtOnce; ++i) {
+      const float now = fmaxf(top, m[i]);
+      const float old = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - now);
+      const float by = m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[i] - now);
+      total = total * old + l[i] * by;
+      y = y * old + v[i] * by;
+      top = now;
+    }
+  }
+  *reinterpret_cast<F4v*>(&sums[group][d]) = y;
+  if (d == 0) totals[group] = total, tops[group] = top;
+  __syncthreads();
+  if (threadIdx.x >= kLanes) return;
+  top = tops[0];
+#pragma unroll
+  for (uint32_t i = 1; i < kGroups; ++i) top = fmaxf(top, tops[i]);
+  total = 0.0f, y = F4v{0, 0, 0, 0};
+#pragma unroll
+  for (uint32_t i = 0; i < kGroups; ++i) {
+    const float by = tops[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(tops[i] - top);
+    total += totals[i] * by;
+    y += *reinterpret_cast<const F4v*>(&sums[i][d]) * by;
   }
   const float inv = total > 0.0f ? 1.0f / total : total == total ? 0.0f : NAN;
-#pragma unroll
-  for (int d = 0; d < kPer; ++d) a.out[at * D + lane * kPer + d] = static_cast<uint16_t>(PackBf16Rne(y[d] * inv, 0.0f));
-  if (a.lse != nullptr && lane == 0) {
-    a.lse[at] = total > 0.0f ? big + __builtin_amdgcn_logf(total) : total == total ? -INFINITY : NAN;
+  *reinterpret_cast<U2*>(a.out + at * D + d) = U2{PackBf16Rne(y[0] * inv, y[1] * inv), PackBf16Rne(y[2] * inv, y[3] * inv)};
+  if (a.lse != nullptr && d == 0) {
+    a.lse[at] = total > 0.0f ? top + __builtin_amdgcn_logf(total) : total == total ? -INFINITY : NAN;
   }
 }
 
-// Block (tile and KV head, rows by fours).
+// Block (tile and KV head, row).
 template <int D, int kWaves>
 __global__ void __launch_bounds__(256) TileMergeKernel(Args a) {
   const uint32_t head = blockIdx.x % a.cache.kv_heads;
@@ -841,36 +1047,48 @@ __global__ void __launch_bounds__(256) TileMergeKernel(Args a) {
   const Sequence s = SequenceOf(a, b);
   const TileKeys range = KeysOfTile(a, s, tile, 32 * kWaves);
   const int32_t group = static_cast<int32_t>(a.group);
-  const int32_t row = tile * 32 * kWaves + static_cast<int32_t>(blockIdx.y * 4 + threadIdx.x / 64);
+  const int32_t row = tile * 32 * kWaves + static_cast<int32_t>(blockIdx.y);
   if (range.parts <= 1 || row >= s.count * group) return;
   const int32_t token = row / group;
   const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + head * a.group + static_cast<uint32_t>(row - token * group);
-  MergeRow<D>(a, a.tile_o, a.tile_ml, at, static_cast<uint64_t>(a.tokens) * a.q_heads, range.parts, at);
+  MergeRow<D>(a, a.tile_o, a.tile_ml, [&](uint32_t p) { return p * (static_cast<uint64_t>(a.tokens) * a.q_heads) + at; },
+              range.parts, at);
 }
 
-// A split sequence's parts. Block (rows of a KV head by fours, KV head, sequence).
+// A split sequence's parts. Block (row of a KV head, or the first of several, KV head, sequence).
 template <int D>
 __global__ void __launch_bounds__(256) RowMergeKernel(Args a) {
   const Sequence s = SequenceOf(a, blockIdx.z);
-  const int32_t group = static_cast<int32_t>(a.group), rows = s.count * group;
-  const int32_t row = static_cast<int32_t>(blockIdx.x * 4 + threadIdx.x / 64);
-  if (row >= rows || rows > static_cast<int32_t>(a.row_limit) || s.count > static_cast<int32_t>(a.short_tokens)) return;
-  const uint32_t parts = PartsOf(a, FirstKey(a, s, 0), s.keys);
-  if (parts <= 1) return;
-  const int32_t token = row / group;
-  const uint32_t h = blockIdx.y * a.group + static_cast<uint32_t>(row - token * group);
-  const uint64_t step = static_cast<uint64_t>(a.short_tokens) * a.q_heads;
-  const uint64_t first = static_cast<uint64_t>(blockIdx.z) * a.splits * step + static_cast<uint64_t>(token) * a.q_heads + h;
-  MergeRow<D>(a, a.part_o, a.part_ml, first, step, parts, static_cast<uint64_t>(s.first + token) * a.q_heads + h);
+  const uint32_t all = a.cut[0], before = a.cut[1 + blockIdx.z], units = UnitsOf(a, s), heads = a.cache.kv_heads;
+  if (units <= 1) return;
+  const Deal deal(all * heads, a.places);
+  const uint32_t begin = before * heads + blockIdx.y * units, first = deal.PlaceOf(begin), last = deal.PlaceOf(begin + units - 1);
+  if (first == last) return;  // whole
+  const int32_t group = static_cast<int32_t>(a.group);
+  const uint64_t rows = static_cast<uint64_t>(a.short_tokens) * a.group;
+  for (int32_t row = static_cast<int32_t>(blockIdx.x); row < s.count * group; row += static_cast<int32_t>(gridDim.x)) {
+    const int32_t token = row / group;
+    const uint32_t h = blockIdx.y * a.group + static_cast<uint32_t>(row - token * group);
+    MergeRow<D>(a, a.part_o, a.part_ml,
+                [&](uint32_t p) { return (2 * static_cast<uint64_t>(first + p) + (p == 0 ? 1 : 0)) * rows + static_cast<uint32_t>(row); },
+                last - first + 1, static_cast<uint64_t>(s.first + token) * a.q_heads + h);
+    __syncthreads();
+  }
 }
 
 // ---- Admission and launch --------------------------------------------------------------------------------------------------
 
 constexpr int TileWaves(uint32_t d) { return d == 256 ? 4 : 8; }
+constexpr uint32_t Resident(uint32_t d) {
+  return d == 256 ? RowRing<256>::kResident : d == 128 ? RowRing<128>::kResident : RowRing<64>::kResident;
+}
 
 struct Cut {
   uint32_t row_tiles;     // of 16 rows in the row kernel
-  uint32_t splits, part, short_tokens;
+  uint32_t short_tokens;
+  uint32_t places;        // its workgroups
+  uint32_t merge_rows;    // of a KV head that its merge is expected to have
+  bool merge;
   uint64_t rows;          // its partial rows
   bool by_row, by_tile;   // which kernels run
   uint32_t row_limit;
@@ -889,21 +1107,22 @@ Cut CutOf(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
   };
   // Which kernels: sequences of up to 16 rows (32 where a token alone has more than 16) go row by row, longer ones by tiles. One
   // kernel is enough where no sequence is expected for the other; it then takes all, so an expectation that fails costs time only.
+  // At head_dim 256 two tiles of 16 rows do not fit a wavefront's registers, and 32 rows take two turns.
   const uint64_t expected = uint64_t{p.max_q_len ? std::min(p.max_q_len, p.tokens) : p.tokens} * group;
-  c.row_tiles = group > 16 || (expected > 16 && expected <= 32) ? 2 : 1;
-  const uint32_t few = 16 * c.row_tiles;
+  c.row_tiles = p.cache.head_dim < 256 && (group > 16 || (expected > 16 && expected <= 32)) ? 2 : 1;
+  const uint32_t few = std::max(16 * c.row_tiles, group);
   c.short_tokens = few / group;
   c.by_tile = expected > few;
   c.by_row = !c.by_tile || p.batch > 1;
   c.row_limit = !c.by_tile ? 0x7FFFFFFF : c.by_row ? few : 0;
   if (c.by_row) {
-    const uint64_t wanted = roost::CeilDiv(4 * cus, std::max<uint64_t>(1, uint64_t{p.batch} * p.cache.kv_heads));
-    const uint64_t k = seen(c.short_tokens), splits = std::max<uint64_t>(1, std::min<uint64_t>(wanted, roost::CeilDiv(k, 128)));
-    c.part = static_cast<uint32_t>(roost::RoundUp(roost::CeilDiv(k, splits), 64));
-    c.splits = static_cast<uint32_t>(roost::CeilDiv(k, c.part));
-    c.rows = c.splits > 1 ? uint64_t{p.batch} * c.splits * c.short_tokens * p.q_heads : 0;
-  } else {
-    c.splits = 1, c.part = kMostKeys;
+    // As many workgroups as the chip holds at once, or one for each unit of keys where fewer are expected; one for each KV head of
+    // a batch that is too large to be dealt.
+    const uint64_t least = uint64_t{p.batch} * p.cache.kv_heads, units = roost::CeilDiv(seen(c.short_tokens), kUnit);
+    c.merge = p.batch <= kMaxScheduled;
+    c.places = static_cast<uint32_t>(c.merge ? std::min(uint64_t{cus} * Resident(p.cache.head_dim), least * units) : least);
+    c.merge_rows = std::min(c.short_tokens, p.max_q_len ? p.max_q_len : c.short_tokens) * group;
+    c.rows = c.merge ? 2 * uint64_t{c.places} * c.short_tokens * group : 0;
   }
   c.tile_splits = 1;
   if (c.by_tile) {
@@ -919,7 +1138,7 @@ Cut CutOf(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
 
 uint64_t WorkspaceBytes(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
   const Cut c = CutOf(p, cus);
-  return (c.rows + c.tile_rows) * (p.cache.head_dim + 2) * 4;
+  return (c.rows + c.tile_rows) * (p.cache.head_dim + 2) * 4 + (c.merge ? 4 * (uint64_t{p.batch} + 1) : 0);
 }
 
 RoostStatus Admit(const RoostAmdPagedAttentionF4Params& p, uint64_t& pages) {
@@ -1000,21 +1219,24 @@ void LaunchTiles(const Args& a, const Cut& c, hipStream_t s) {
   } else {
     TileAttentionKernel<D, kWaves, false><<<grid, 64 * kWaves, 0, s>>>(a);
   }
-  if (c.tile_splits > 1) TileMergeKernel<D, kWaves><<<dim3(c.tiles * a.cache.kv_heads, 8 * kWaves), 256, 0, s>>>(a);
+  if (c.tile_splits > 1) TileMergeKernel<D, kWaves><<<dim3(c.tiles * a.cache.kv_heads, 32 * kWaves), 256, 0, s>>>(a);
 }
 
 template <int D>
 void Launch(const Args& a, const Cut& c, hipStream_t s) {
   if (c.by_tile) LaunchTiles<D, TileWaves(D)>(a, c, s);
   if (!c.by_row) return;
-  const dim3 grid(a.cache.kv_heads, c.splits, a.batch);
-  if (c.row_tiles == 1) {
-    RowAttentionKernel<D, 1><<<grid, 64 * kRowWaves, 0, s>>>(a);
+  const uint32_t grid = (c.places + 7) / 8 * 8;  // whole rounds of the dies
+  if (D == 256 || c.row_tiles == 1) {
+    a.capped ? RowAttentionKernel<D, 1, true><<<grid, 64 * kRowWaves, 0, s>>>(a)
+             : RowAttentionKernel<D, 1, false><<<grid, 64 * kRowWaves, 0, s>>>(a);
   } else {
-    RowAttentionKernel<D, 2><<<grid, 64 * kRowWaves, 0, s>>>(a);
+    constexpr int kTiles = D == 256 ? 1 : 2;
+    a.capped ? RowAttentionKernel<D, kTiles, true><<<grid, 64 * kRowWaves, 0, s>>>(a)
+             : RowAttentionKernel<D, kTiles, false><<<grid, 64 * kRowWaves, 0, s>>>(a);
   }
-  if (c.splits > 1) {
-    RowMergeKernel<D><<<dim3((c.short_tokens * a.group + 3) / 4, a.cache.kv_heads, a.batch), 256, 0, s>>>(a);
+  if (c.merge) {
+    RowMergeKernel<D><<<dim3(c.merge_rows, a.cache.kv_heads, a.batch), 256, 0, s>>>(a);
   }
 }
 
@@ -1081,7 +1303,10 @@ extern "C" ROOST_API RoostStatus roost_amd_paged_attention_f4_run(RoostContext* 
     a.part_ml = a.part_o + c.rows * p.cache.head_dim;
     a.tile_o = a.part_ml + 2 * c.rows;
     a.tile_ml = a.tile_o + c.tile_rows * p.cache.head_dim;
-    a.splits = c.splits, a.part = c.part, a.short_tokens = c.short_tokens, a.row_limit = c.row_limit;
+    a.cut = c.merge ? reinterpret_cast<uint32_t*>(a.tile_ml + 2 * c.tile_rows) : nullptr;
+    a.places = c.places;
+    a.max_units = std::min(65535u, 0xFFFFFFFFu / (kMaxScheduled * p.cache.kv_heads));
+    a.short_tokens = c.short_tokens, a.row_limit = c.row_limit;
     a.tile_splits = c.tile_splits;
     const hipStream_t s = roost::Stream(stream);
     if (p.cache.head_dim == 64) {
