@@ -197,6 +197,12 @@ __device__ __forceinline__ void Copy16(const void* p, uint32_t lds) {
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(m0) : "v"(p), "s"(lds) : "memory");
 }
+// A byte a lane, each to a word of its own.
+__device__ __forceinline__ void Copy1(const void* p, uint32_t lds) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(p), "s"(lds) : "memory");
+}
 __device__ __forceinline__ void Copy4(const void* p, uint32_t lds) {
   uint32_t m0;
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
@@ -635,9 +641,10 @@ __global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : 
 // 32 kWaves rows of one sequence and KV head (rows are its tokens' query heads, token by token) against the keys that they see, 64
 // at a time: prompt chunks. Bound by the matrix instructions and, beside them, by LDS reads and the softmax.
 //
-// A tile's codes come through registers, a lane a block of 32 dims (16 bytes, one scale), and go to LDS as bf16 once for all
-// wavefronts: 64 conversions a lane and tile at head_dim 128 and 256 rows, where converting in each wavefront would take 192. Codes
-// of the next tile are under way during a tile's products; LDS holds two tiles, so there is one barrier a tile.
+// A tile's codes go to LDS as bf16 once for all wavefronts, a lane a block of 32 dims (16 bytes, one scale): 16 conversions a lane
+// and tile at head_dim 128 and 256 rows, where converting in each wavefront would take 128. Codes of the next tile are under way
+// during a tile's products, straight into LDS, where each lane finds its own again: held in registers they would not fit beside
+// 32 rows' queries and sums at head_dim 256. LDS holds two converted tiles, so there is one barrier a tile.
 //
 // v_mfma_f32_32x32x16_bf16, lane l = 32 g + m: A[m][8 g + j], B[8 g + j][m], result register v at [8 (v / 4) + 4 g + v % 4][m].
 //   S^T = K Q^T with 32 keys as A and the wavefront's 32 rows as B. A lane then holds, of its row, keys 4 g + i of each 8; the
@@ -653,11 +660,13 @@ __device__ __forceinline__ U2 LdsTranspose(const unsigned char* base, uint32_t o
   return __builtin_bit_cast(U2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
 }
 
-template <int D>
+template <int D, int kWaves, int kPieces>
 struct TileLds {
   static constexpr int kKeyRow = 2 * D + 16;
   unsigned char k[2][kTileKeys * kKeyRow];
   unsigned char v[2][kTileKeys * 2 * D];
+  U4 codes[kWaves][kPieces][64];        // of the next tile, a block a lane
+  uint32_t scales[kWaves][kPieces][64];
   uint32_t bad[3];                // groups of 16 keys without a page, of this tile, the next and the one after
   uint32_t nan[3][kTileKeys];     // blocks of V that are NaN; only kept in a careful pass
 };
@@ -720,8 +729,10 @@ template <int D, int kWaves, bool kCap>
 __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(Args a) {
   constexpr int kThreads = 64 * kWaves, kRows = 32 * kWaves;
   constexpr int kKs = D / 16, kDt = D / 32;
+  constexpr int kHalves = D == 64 ? 2 : 1;  // of a tile's keys that are scored together (at 128 the registers of two cost 1%)
   constexpr int kPieces = (4 * D + kThreads - 1) / kThreads;  // blocks of 32 codes that a lane stages
-  __shared__ __attribute__((aligned(16))) TileLds<D> lds;
+  typedef TileLds<D, kWaves, kPieces> Lds;
+  __shared__ __attribute__((aligned(16))) Lds lds;
 
   const uint32_t head = blockIdx.x % a.cache.kv_heads, split = blockIdx.x / a.cache.kv_heads % a.tile_splits;
   uint32_t b = 0;
@@ -736,83 +747,88 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
   const int32_t k1 = min(range.end, k0 + range.part);
   const int32_t tiles = k1 > k0 ? (k1 - k0 + kTileKeys - 1) / kTileKeys : 0;
 
-  const int tid = threadIdx.x, lane = tid & 63, m = lane & 31, g = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t group = static_cast<int32_t>(a.group), rows = s.count * group;
-  const int32_t r = tile * kRows + 32 * w + m;
-  const bool row_ok = r < rows;
-  const int32_t token = row_ok ? r / group : 0;
-  const uint32_t h = head * a.group + static_cast<uint32_t>(row_ok ? r - token * group : 0);
   const int32_t before = s.keys - s.count;  // the first token's position
-  const int32_t pos = before + token;
+  // Lane `id`'s row: its token, -1 where there is none, and its query head.
+  const auto row_of = [&](int id, int32_t& token, uint32_t& h) {
+    const int32_t r = tile * kRows + 32 * w + (id & 31);
+    token = r < rows ? r / group : -1;
+    h = head * a.group + static_cast<uint32_t>(r < rows ? r - token * group : 0);
+  };
   // Positions of the wavefront's first and last row.
   const int32_t low = before + (tile * kRows + 32 * w) / group;
   const int32_t high = before + min((tile * kRows + 32 * w + 31) / group, s.count - 1);
   const bool idle = tile * kRows + 32 * w >= rows;  // the wavefront has no row, and only stages
-  const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + h;
 
   U4 q[kKs];
   {
-    const uint16_t* qr = a.q + static_cast<uint64_t>(s.first + token) * a.q_stride + static_cast<uint64_t>(h) * D + 8 * g;
+    int32_t token;
+    uint32_t h;
+    row_of(tid, token, h);
+    const uint16_t* qr = a.q + static_cast<uint64_t>(s.first + max(token, 0)) * a.q_stride + static_cast<uint64_t>(h) * D + 8 * g;
 #pragma unroll
     for (int i = 0; i < kKs; ++i) {
       const U4 x = *reinterpret_cast<const U4*>(qr + 16 * i);
-      q[i] = row_ok ? x : U4{0, 0, 0, 0};
+      q[i] = token >= 0 ? x : U4{0, 0, 0, 0};
     }
   }
 
-  // Staging: piece tid + i kThreads of [K, V] x 64 keys x blocks.
+  // Staging: piece tid + i kThreads of [K, V] x 64 keys x blocks. From head_dim 128 on a wavefront's 64 pieces are of one page.
   const uint32_t shift = a.cache.page_shift, in_page = (1u << shift) - 1;
-  const auto piece_of = [&](int i, bool& value, int32_t& key, uint32_t& block) {
-    const int p = tid + i * kThreads;
+  const auto piece_of = [&](int i, int id, bool& value, int32_t& key, uint32_t& block) {
+    const int p = id + i * kThreads;
     value = p >= 2 * D;
     key = (p & (2 * D - 1)) / (D / 32);
     block = static_cast<uint32_t>(p) & (D / 32 - 1);
     return p < 4 * D;
   };
   int32_t ids[kPieces];
-  U4 codes[kPieces];
-  uint32_t scales[kPieces];
-  const auto load_ids = [&](int32_t t) {
+  uint32_t none = 0;  // pieces of the tile under way that have no page
+  const auto load_ids = [&](int32_t t, int id) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       bool value;
       int32_t key;
       uint32_t block;
       ids[i] = -1;
-      if (!piece_of(i, value, key, block) || t >= tiles) continue;
+      if (!piece_of(i, id, value, key, block) || t >= tiles) continue;
       const int32_t k = k0 + t * kTileKeys + key, entry = k >> shift;
       if ((k & ~15) < k1 && entry < s.blocks) ids[i] = a.tables[s.entry + entry];
     }
   };
-  const auto load_codes = [&](int32_t t) {
+  const auto load_codes = [&](int32_t t, int id) {
+    none = 0;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       bool value;
       int32_t key;
       uint32_t block;
-      if (!piece_of(i, value, key, block)) continue;
-      if (static_cast<uint32_t>(ids[i]) >= a.cache.pages) ids[i] = -1;
+      if (!piece_of(i, id, value, key, block)) continue;
+      int32_t page = D == 64 ? ids[i] : __builtin_amdgcn_readfirstlane(ids[i]);
+      if (static_cast<uint32_t>(page) >= a.cache.pages) none |= 1u << i, page = 0;  // masked: any codes will do
       const uint32_t within = static_cast<uint32_t>(k0 + t * kTileKeys + key) & in_page;
-      const uint64_t head_page = static_cast<uint64_t>(max(ids[i], 0)) * a.cache.kv_heads + head;
-      codes[i] = *reinterpret_cast<const U4*>((value ? a.cache.v : a.cache.k) + ((head_page << shift) + within) * (D / 2) + 16 * block);
-      scales[i] = (value ? a.cache.v_scales : a.cache.k_scales)[((head_page * (D / 32) + block) << shift) + within];
-      if (ids[i] < 0) scales[i] |= 0x100;  // no key
+      const uint64_t head_page = static_cast<uint64_t>(page) * a.cache.kv_heads + head;
+      Copy16((value ? a.cache.v : a.cache.k) + ((head_page << shift) + within) * (D / 2) + 16 * block, LdsAddress(lds.codes[w][i]));
+      Copy1((value ? a.cache.v_scales : a.cache.k_scales) + ((head_page * (D / 32) + block) << shift) + within,
+            LdsAddress(lds.scales[w][i]));
     }
   };
-  const auto store = [&](int32_t t, bool careful) {
+  const auto store = [&](int32_t t, int id, bool careful) {
     const int slot = t % 3;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       bool value;
       int32_t key;
       uint32_t block;
-      if (!piece_of(i, value, key, block)) continue;
-      const bool none = (scales[i] & 0x100) != 0;
-      if (none && block == 0) atomicOr(&lds.bad[slot], 1u << (key / 16));
-      uint32_t byte = scales[i] & 0xFF;
+      if (!piece_of(i, id, value, key, block)) continue;
+      if ((none >> i & 1) && block == 0) atomicOr(&lds.bad[slot], 1u << (key / 16));
+      const U4 codes = lds.codes[w][i][id & 63];
+      uint32_t byte = lds.scales[w][i][id & 63];
       if (value) {
-        if (none || k0 + t * kTileKeys + key >= k1) byte = 127;  // whatever lies there: finite, times p = 0
+        if ((none >> i & 1) || k0 + t * kTileKeys + key >= k1) byte = 127;  // whatever lies there: finite, times p = 0
         if (careful && byte > kF4ByteHigh) {
           byte = 127;
           atomicOr(&lds.nan[slot][key], 1u << block);
@@ -822,12 +838,13 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
       unsigned char* const to = value ? lds.v[t & 1] : lds.k[t & 1];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t c = codes[i][j];
+        const uint32_t c = codes[j];
         const U4 x{FromF4<0>(c, scale), FromF4<1>(c, scale), FromF4<2>(c, scale), FromF4<3>(c, scale)};
-        const uint32_t off = value ? ValueAt<D>(key, block, j) : key * TileLds<D>::kKeyRow + 64 * block + 16 * j;
+        const uint32_t off = value ? ValueAt<D>(key, block, j) : key * Lds::kKeyRow + 64 * block + 16 * j;
         *reinterpret_cast<U4*>(to + off) = x;
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the next codes may come
   };
 
   F16v o[kDt];
@@ -842,26 +859,33 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
     if (careful && tid < 64) lds.nan[0][tid] = lds.nan[1][tid] = lds.nan[2][tid] = 0;
     __syncthreads();
     if (tiles > 0) {
-      load_ids(0);
-      load_codes(0);
-      load_ids(1);
-      store(0, careful);
+      load_ids(0, tid);
+      load_codes(0, tid);
+      load_ids(1, tid);
+      store(0, tid, careful);
     }
+#pragma unroll 1
     for (int32_t t = 0; t < tiles; ++t) {
       __syncthreads();  // tile t is in LDS; nobody reads tile t - 1 any more
       const int slot = t % 3, after = (t + 2) % 3;
+      // What depends on the lane is made anew from its number each time: kept, it would not fit the registers at head_dim 256,
+      // and at 64 leave room for one workgroup a CU instead of two (four prompts of 1,000 to 2,000 tokens on prefixes, 32 heads
+      // over 8: 105 us, kept 125). At 128 there is room, and it is kept (655 us; anew 720).
+      int tid = threadIdx.x;
+      if constexpr (D != 128) asm volatile("" : "+v"(tid));
+      const int lane = tid & 63, m = lane & 31, g = lane >> 5;
       if (tid == 0) lds.bad[after] = 0;
       if (careful && tid < 64) lds.nan[after][tid] = 0;
       if (t + 1 < tiles) {
-        load_codes(t + 1);
-        load_ids(t + 2);
+        load_codes(t + 1, tid);
+        load_ids(t + 2, tid);
       }
       const int32_t kb = k0 + t * kTileKeys;
       if (!idle && !(a.causal && kb > high)) {
         const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(lds.bad[slot])));
         const bool mask = kb + kTileKeys > k1 || (a.causal && kb + kTileKeys - 1 > low) || bad != 0 ||
                           (a.window >= 0 && kb < high - a.window);
-        const unsigned char* kt = lds.k[t & 1] + m * TileLds<D>::kKeyRow + 16 * g;
+        const unsigned char* kt = lds.k[t & 1] + m * Lds::kKeyRow + 16 * g;
         const unsigned char* vt = lds.v[t & 1];
         // The transposing read of four keys x 16 dims by 16 lanes: lane 16 c + j addresses key j / 4, dims 4 (j % 4) of it.
         const uint32_t j = lane & 15, key4 = 4 * g + j / 4, piece = 2 * (lane >> 4 & 1) + (j % 4) / 2;
@@ -869,33 +893,66 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
 #pragma unroll
         for (int f = 0; f < 2; ++f) va[f] = ValueAt<D>(key4 + 8 * f, 0, piece) + 8 * (j & 1);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (a.causal && kb + 32 * half > high) break;
-          F16v sc;
+        for (int half = 0; half < 2; half += kHalves) {
+          if (kHalves == 1 && a.causal && kb + 32 * half > high) break;
+          F16v sc[kHalves];
 #pragma unroll
-          for (int v = 0; v < 16; ++v) sc[v] = 0.0f;
+          for (int x = 0; x < kHalves; ++x)
 #pragma unroll
-          for (int i = 0; i < kKs; ++i) {
-            sc = Mfma32(*reinterpret_cast<const U4*>(kt + 32 * half * TileLds<D>::kKeyRow + 32 * i), q[i], sc);
+            for (int v = 0; v < 16; ++v) sc[x][v] = 0.0f;
+          // Operands are read two steps ahead of the products that use them: left alone, the compiler waits out every read in front
+          // of its product at this number of registers. The same for V below.
+          const unsigned char* kr = kt + 32 * half * Lds::kKeyRow;
+          constexpr int kAhead = 2;
+          U4 ka[kAhead][kHalves];
+          const auto key = [&](int i, int x) { return *reinterpret_cast<const U4*>(kr + 32 * x * Lds::kKeyRow + 32 * i); };
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int x = 0; x < kHalves; ++x) ka[i][x] = key(i, x);
+#pragma unroll
+          for (int i = 0; i < kKs; ++i)
+#pragma unroll
+            for (int x = 0; x < kHalves; ++x) {
+              const U4 k = ka[i % kAhead][x];
+              if (i + kAhead < kKs) ka[i % kAhead][x] = key(i + kAhead, x);
+              sc[x] = Mfma32(k, q[i], sc[x]);
+            }
+          __builtin_amdgcn_sched_group_barrier(0x100, kAhead * kHalves, 0);
+#pragma unroll
+          for (int i = 0; i < (kKs - kAhead) * kHalves; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
           }
+          __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kHalves, 0);
           if constexpr (kCap) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) sc[v] = Capped(sc[v] * a.scale_log2, a.cap);
+            for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+              for (int v = 0; v < 16; ++v) sc[x][v] = Capped(sc[x][v] * a.scale_log2, a.cap);
           }
           if (mask) {
+            int32_t token;
+            uint32_t h;
+            row_of(tid, token, h);
+            const int32_t pos = before + token;
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-              const int kk = 32 * half + 8 * (v / 4) + 4 * g + v % 4;
-              const int32_t key = kb + kk;
-              const bool off = (key >= k1) | ((a.causal != 0) & (key > pos)) | ((a.window >= 0) & (key < pos - a.window)) |
-                               ((bad >> (kk / 16) & 1) != 0);
-              sc[v] = off ? -INFINITY : sc[v];
-            }
+            for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+              for (int v = 0; v < 16; ++v) {
+                const int kk = 32 * (half + x) + 8 * (v / 4) + 4 * g + v % 4;
+                const int32_t key = kb + kk;
+                const bool off = (key >= k1) | ((a.causal != 0) & (key > pos)) | ((a.window >= 0) & (key < pos - a.window)) |
+                                 ((bad >> (kk / 16) & 1) != 0);
+                sc[x][v] = off ? -INFINITY : sc[x][v];
+              }
           }
           const float scale = kCap ? 1.0f : a.scale_log2;
-          float mx = sc[0];
+          float mx = sc[0][0];
 #pragma unroll
-          for (int v = 1; v < 16; ++v) mx = fmaxf(mx, sc[v]);
+          for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[x][v]);
           mx *= scale;
           if (__any(mx > top + kGrow)) {
             mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -909,28 +966,41 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
             top = now;
           }
           const float base = top == -INFINITY ? 0.0f : top;
-          U4 p[2];
+          // Half after half: the exponentials of the second run beside the first's products.
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float y[8];
+          for (int x = 0; x < kHalves; ++x) {
+            U4 p[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              y[e] = __builtin_amdgcn_exp2f(fmaf(sc[8 * c + e], scale, -base));
-              sum += y[e];
+            for (int c = 0; c < 2; ++c) {
+              float y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                y[e] = __builtin_amdgcn_exp2f(fmaf(sc[x][8 * c + e], scale, -base));
+                sum += y[e];
+              }
+              p[c] = U4{PackBf16Rne(y[0], y[1]), PackBf16Rne(y[2], y[3]), PackBf16Rne(y[4], y[5]), PackBf16Rne(y[6], y[7])};
             }
-            p[c] = U4{PackBf16Rne(y[0], y[1]), PackBf16Rne(y[2], y[3]), PackBf16Rne(y[4], y[5]), PackBf16Rne(y[6], y[7])};
-          }
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int d = 0; d < kDt; ++d) {
-              const uint32_t row = 16 * (2 * half + c) * 2 * D;
+            const auto value = [&](int n) {  // the operand of product n: 16 keys n / kDt, dims 32 (n % kDt) ..
+              const uint32_t row = 16 * (2 * (half + x) + n / kDt) * 2 * D, d = n % kDt;
               const U2 lo = LdsTranspose(vt, (va[0] ^ (64 * d)) + row), hi = LdsTranspose(vt, (va[1] ^ (64 * d)) + row);
-              o[d] = Mfma32(U4{lo[0], lo[1], hi[0], hi[1]}, p[c], o[d]);
+              return U4{lo[0], lo[1], hi[0], hi[1]};
+            };
+            U4 vv[kAhead];
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n) vv[n] = value(n);
+#pragma unroll
+            for (int n = 0; n < 2 * kDt; ++n) {
+              const U4 v = vv[n % kAhead];
+              if (n + kAhead < 2 * kDt) vv[n % kAhead] = value(n + kAhead);
+              o[n % kDt] = Mfma32(v, p[n / kDt], o[n % kDt]);
             }
           }
           if (careful) {
-            for (int kk = 32 * half; kk < 32 * half + 32; ++kk) {
+            int32_t token;
+            uint32_t h;
+            row_of(tid, token, h);
+            const int32_t pos = before + token;
+            for (int kk = 32 * half; kk < 32 * (half + kHalves); ++kk) {
               const uint32_t blocks = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(lds.nan[slot][kk])));
               if (blocks == 0) continue;
               const int32_t key = kb + kk;
@@ -946,7 +1016,7 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
           }
         }
       }
-      if (t + 1 < tiles) store(t + 1, careful);
+      if (t + 1 < tiles) store(t + 1, tid, careful);
     }
   };
   pass(false);
@@ -958,7 +1028,11 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
   if (__syncthreads_or(nan)) pass(true);
 
   sum += __shfl_xor(sum, 32);
-  if (!row_ok) return;
+  int32_t token;
+  uint32_t h;
+  row_of(tid, token, h);
+  if (token < 0) return;
+  const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + h;
   if (range.parts > 1) {
     const uint64_t row = static_cast<uint64_t>(split) * a.tokens * a.q_heads + at;
 #pragma unroll
@@ -1037,9 +1111,10 @@ __device__ __forceinline__ void MergeRow(const Args& a, const float* part_o, con
   }
 }
 
-// Block (tile and KV head, row).
+// Block (tile and KV head, 1,024 / D rows of it): D / 4 lanes a row, up to four parts' loads together.
 template <int D, int kWaves>
 __global__ void __launch_bounds__(256) TileMergeKernel(Args a) {
+  constexpr int32_t kLanes = D / 4, kRows = 256 / kLanes;
   const uint32_t head = blockIdx.x % a.cache.kv_heads;
   uint32_t b = 0;
   int32_t tile = 0;
@@ -1047,12 +1122,40 @@ __global__ void __launch_bounds__(256) TileMergeKernel(Args a) {
   const Sequence s = SequenceOf(a, b);
   const TileKeys range = KeysOfTile(a, s, tile, 32 * kWaves);
   const int32_t group = static_cast<int32_t>(a.group);
-  const int32_t row = tile * 32 * kWaves + static_cast<int32_t>(blockIdx.y);
+  const int32_t row = tile * 32 * kWaves + static_cast<int32_t>(blockIdx.y) * kRows + static_cast<int32_t>(threadIdx.x) / kLanes;
   if (range.parts <= 1 || row >= s.count * group) return;
-  const int32_t token = row / group;
+  const int32_t token = row / group, d = static_cast<int32_t>(threadIdx.x) % kLanes * 4;
   const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + head * a.group + static_cast<uint32_t>(row - token * group);
-  MergeRow<D>(a, a.tile_o, a.tile_ml, [&](uint32_t p) { return p * (static_cast<uint64_t>(a.tokens) * a.q_heads) + at; },
-              range.parts, at);
+  const uint64_t step = static_cast<uint64_t>(a.tokens) * a.q_heads;
+  float top = -INFINITY, total = 0.0f;
+  F4v y{0, 0, 0, 0};
+  for (uint32_t p0 = 0; p0 < range.parts; p0 += 4) {
+    float m[4], l[4];
+    F4v v[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      m[i] = -INFINITY, l[i] = 0.0f, v[i] = F4v{0, 0, 0, 0};
+      if (p0 + i < range.parts) {
+        const uint64_t r = (p0 + i) * step + at;
+        m[i] = a.tile_ml[2 * r], l[i] = a.tile_ml[2 * r + 1];
+        v[i] = *reinterpret_cast<const F4v*>(a.tile_o + r * D + d);
+      }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const float now = fmaxf(top, m[i]);
+      const float old = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - now);
+      const float by = m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[i] - now);
+      total = total * old + l[i] * by;
+      y = y * old + v[i] * by;
+      top = now;
+    }
+  }
+  const float inv = total > 0.0f ? 1.0f / total : total == total ? 0.0f : NAN;
+  *reinterpret_cast<U2*>(a.out + at * D + d) = U2{PackBf16Rne(y[0] * inv, y[1] * inv), PackBf16Rne(y[2] * inv, y[3] * inv)};
+  if (a.lse != nullptr && d == 0) {
+    a.lse[at] = total > 0.0f ? top + __builtin_amdgcn_logf(total) : total == total ? -INFINITY : NAN;
+  }
 }
 
 // A split sequence's parts. Block (row of a KV head, or the first of several, KV head, sequence).
@@ -1078,9 +1181,34 @@ __global__ void __launch_bounds__(256) RowMergeKernel(Args a) {
 
 // ---- Admission and launch --------------------------------------------------------------------------------------------------
 
-constexpr int TileWaves(uint32_t d) { return d == 256 ? 4 : 8; }
+constexpr int TileWaves(uint32_t) { return 8; }
 constexpr uint32_t Resident(uint32_t d) {
   return d == 256 ? RowRing<256>::kResident : d == 128 ? RowRing<128>::kResident : RowRing<64>::kResident;
+}
+
+// Into how many parts the tile kernel's keys are best cut, by what its workgroups were measured to take: 12 us (16 at head_dim
+// 256) to begin and end, 1.42, 2.0 and 4.1 us for each 64 keys at head_dim 64, 128 and 256, and for more parts than one the
+// merge, 4 us, 1.5 for each part, and the partial rows once out and in at 8 TB/s (they stay in the last cache). With G tiles of all KV heads and room for R workgroups, G S / R
+// rounds follow each other: whole ones where all tiles see as many keys, any number where a causal prompt's first tiles see few.
+// Measured, us, without parts / with the S chosen here: 512 tokens behind 8,000, 32 heads over 8 of 128: 283 / 100 (4); 512
+// behind 500, 8 heads of 256 over 2: 80 / 39 (8); 3,000 alone at 256: 211 / 94 (4); four of 1,000 to 2,000 on prefixes: 176 / 141 (2) at
+// 256, and at 64, 32 heads over 8, 103 (2 parts: 124).
+uint32_t TileSplits(const RoostAmdPagedAttentionF4Params& p, uint64_t groups, uint64_t keys, uint32_t cus) {
+  const uint32_t d = p.cache.head_dim;
+  const double ends = d == 256 ? 16 : 12, step = d == 256 ? 4.1 : d == 128 ? 2.0 : 1.42;
+  const double room = d == 64 ? 2.0 * cus : cus, steps = std::max(1.0, keys / 64.0);
+  const double fresh = p.causal ? std::min<double>(p.max_q_len ? p.max_q_len : p.tokens, keys) : 0;
+  const double mean = 1 - fresh / (2.0 * keys);  // of the keys that the last tile sees, what a tile does
+  const double row_us = double(p.tokens) * p.q_heads * d * 8 / 8e6;
+  uint32_t best = 1;
+  double least = 0;
+  for (uint32_t s = 1; s <= 16 && (s == 1 || keys >= 128 * s); ++s) {
+    const double rounds = std::max(1.0, groups * s / room), one = ends + step * steps / s;
+    const double alike = std::ceil(rounds) * one, unlike = std::max(one, rounds * (ends + step * steps / s * mean));
+    const double us = (2 * mean - 1) * alike + (2 - 2 * mean) * unlike + (s > 1 ? 4 + s * (1.5 + row_us) : 0);
+    if (s == 1 || us < least) best = s, least = us;
+  }
+  return best;
 }
 
 struct Cut {
@@ -1129,8 +1257,7 @@ Cut CutOf(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
     const uint64_t rows = 32 * TileWaves(p.cache.head_dim), all = uint64_t{p.tokens} * group;
     const uint64_t longer = std::min<uint64_t>(p.batch, all / (c.row_limit + 1));  // sequences that it can have
     c.tiles = static_cast<uint32_t>(all / rows + longer);
-    const uint64_t groups = std::max<uint64_t>(1, roost::CeilDiv(all, rows) * p.cache.kv_heads);
-    if (4 * groups < 3 * cus) c.tile_splits = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(cus / groups, seen(p.tokens) / 512)));
+    c.tile_splits = TileSplits(p, roost::CeilDiv(all, rows) * p.cache.kv_heads, seen(rows / group), cus);
     c.tile_rows = c.tile_splits > 1 ? uint64_t{c.tile_splits} * p.tokens * p.q_heads : 0;
   }
   return c;
@@ -1219,7 +1346,7 @@ void LaunchTiles(const Args& a, const Cut& c, hipStream_t s) {
   } else {
     TileAttentionKernel<D, kWaves, false><<<grid, 64 * kWaves, 0, s>>>(a);
   }
-  if (c.tile_splits > 1) TileMergeKernel<D, kWaves><<<dim3(c.tiles * a.cache.kv_heads, 32 * kWaves), 256, 0, s>>>(a);
+  if (c.tile_splits > 1) TileMergeKernel<D, kWaves><<<dim3(c.tiles * a.cache.kv_heads, 32 * kWaves * D / 1024), 256, 0, s>>>(a);
 }
 
 template <int D>
