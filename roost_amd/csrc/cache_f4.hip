@@ -75,47 +75,55 @@ __device__ __forceinline__ void Load8(const T* p, float (&x)[8]) {
   }
 }
 
-// blockIdx.y: 0 for K, 1 for V.
+// K's row and V's: both rows' loads go out together.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) CacheWriteF4Kernel(Args a) {
   const Place p = PlaceOf(a);
   if (!p.live) return;  // whole rows, so a block's four lanes stay together
-  const bool v = blockIdx.y != 0;
-  float x[8];
-  Load8(static_cast<const T*>(v ? a.v : a.k) + p.token * (v ? a.v_stride : a.k_stride) +
-            (((uint64_t{p.head} << a.vec_shift) + p.vec) << 3), x);
-  uint32_t top = 0;
+  const uint64_t at = ((uint64_t{p.head} << a.vec_shift) + p.vec) << 3;
+  float x[2][8];
+  Load8(static_cast<const T*>(a.k) + p.token * a.k_stride + at, x[0]);
+  Load8(static_cast<const T*>(a.v) + p.token * a.v_stride + at, x[1]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
-  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
-  const uint32_t byte = F4ScaleByte(top);
-  const uint32_t codes = byte == kF4ByteNan ? 0 : ToF4(x, F4Scale(byte));
-  *reinterpret_cast<uint32_t*>((v ? a.cache.v : a.cache.k) + p.codes) = codes;
-  if ((p.vec & 3) == 0) (v ? a.cache.v_scales : a.cache.k_scales)[p.scale] = static_cast<uint8_t>(byte);
+  for (int v = 0; v < 2; ++v) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[v][i]) & 0x7FFFFFFFu);
+    // The block's four lanes: a swap of neighbours, then of pairs.
+    top = max(top, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0xB1, 0xf, 0xf, false)));
+    top = max(top, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0x4E, 0xf, 0xf, false)));
+    const uint32_t byte = F4ScaleByte(top);
+    const uint32_t codes = byte == kF4ByteNan ? 0 : ToF4(x[v], F4Scale(byte));
+    *reinterpret_cast<uint32_t*>((v ? a.cache.v : a.cache.k) + p.codes) = codes;
+    if ((p.vec & 3) == 0) (v ? a.cache.v_scales : a.cache.k_scales)[p.scale] = static_cast<uint8_t>(byte);
+  }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) CacheReadF4Kernel(Args a) {
   const Place p = PlaceOf(a);
   if (!p.live) return;
-  const bool v = blockIdx.y != 0;
-  const uint32_t codes = *reinterpret_cast<const uint32_t*>((v ? a.cache.v : a.cache.k) + p.codes);
-  const float scale = F4Scale((v ? a.cache.v_scales : a.cache.k_scales)[p.scale]);
-  const U4 w{FromF4<0>(codes, scale), FromF4<1>(codes, scale), FromF4<2>(codes, scale), FromF4<3>(codes, scale)};
-  T* to = static_cast<T*>(v ? a.v : a.k) + p.token * (v ? a.v_stride : a.k_stride) +
-          (((uint64_t{p.head} << a.vec_shift) + p.vec) << 3);
-  if constexpr (sizeof(T) == 4) {
-    U4 lo, hi;
+  const uint64_t at = ((uint64_t{p.head} << a.vec_shift) + p.vec) << 3;
+  const uint32_t codes[2] = {*reinterpret_cast<const uint32_t*>(a.cache.k + p.codes),
+                             *reinterpret_cast<const uint32_t*>(a.cache.v + p.codes)};
+  const float scale[2] = {F4Scale(a.cache.k_scales[p.scale]), F4Scale(a.cache.v_scales[p.scale])};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      lo[2 * i] = w[i] << 16, lo[2 * i + 1] = w[i] & 0xFFFF0000u;
-      hi[2 * i] = w[2 + i] << 16, hi[2 * i + 1] = w[2 + i] & 0xFFFF0000u;
+  for (int v = 0; v < 2; ++v) {
+    const U4 w{FromF4<0>(codes[v], scale[v]), FromF4<1>(codes[v], scale[v]), FromF4<2>(codes[v], scale[v]),
+               FromF4<3>(codes[v], scale[v])};
+    T* to = static_cast<T*>(v ? a.v : a.k) + p.token * (v ? a.v_stride : a.k_stride) + at;
+    if constexpr (sizeof(T) == 4) {
+      U4 lo, hi;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        lo[2 * i] = w[i] << 16, lo[2 * i + 1] = w[i] & 0xFFFF0000u;
+        hi[2 * i] = w[2 + i] << 16, hi[2 * i + 1] = w[2 + i] & 0xFFFF0000u;
+      }
+      reinterpret_cast<U4*>(to)[0] = lo;
+      reinterpret_cast<U4*>(to)[1] = hi;
+    } else {
+      *reinterpret_cast<U4*>(to) = w;
     }
-    reinterpret_cast<U4*>(to)[0] = lo;
-    reinterpret_cast<U4*>(to)[1] = hi;
-  } else {
-    *reinterpret_cast<U4*>(to) = w;
   }
 }
 
@@ -184,7 +192,7 @@ RoostStatus Run(RoostContext* ctx, const void* params, void* stream, const char*
     a.cache = roost::ViewOf(p.cache, pages);
     a.rows = p.tokens * p.cache.kv_heads;
     a.vec_shift = static_cast<uint32_t>(__builtin_ctz(p.cache.head_dim / 8));
-    const dim3 grid(static_cast<uint32_t>(roost::CeilDiv(a.rows, kThreads >> a.vec_shift)), 2);
+    const dim3 grid(static_cast<uint32_t>(roost::CeilDiv(a.rows, kThreads >> a.vec_shift)));
     const hipStream_t s = roost::Stream(stream);
     const bool f32 = p.k.dtype == ROOST_DTYPE_F32;
     if (!write) {

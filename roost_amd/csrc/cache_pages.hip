@@ -50,6 +50,11 @@ __device__ __forceinline__ unsigned char* ColumnAt(const Pools& p, uint32_t c, u
   return o.address + layer * o.layer_bytes + uint64_t{16} * (c - layer * o.per_page);
 }
 
+// Copied and moved pages are passed through once: their lines give way first in the L2 (1,200 pages of 408 KiB copied: 209 us,
+// 215 by ordinary accesses). A fork's parent page is not: its other children read it too (128 forks of 16: 44 us, 54 so).
+__device__ __forceinline__ U4 Load(const unsigned char* at) { return __builtin_nontemporal_load(reinterpret_cast<const U4*>(at)); }
+__device__ __forceinline__ void Store(unsigned char* at, U4 v) { __builtin_nontemporal_store(v, reinterpret_cast<U4*>(at)); }
+
 // ---- CacheCopy ------------------------------------------------------------------------------------------------------------
 
 // Whether pair (src, dst) has to keep its place among the others: it reads or writes a page that another writes, or writes
@@ -126,13 +131,13 @@ __global__ void __launch_bounds__(kThreads) CacheCopyKernel(Pools pools, const i
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       if (mine && i < static_cast<int>(n) && !(skip >> i & 1)) {
-        v[i] = *reinterpret_cast<const U4*>(at + pairs[first + i].x * page_bytes);
+        v[i] = Load(at + pairs[first + i].x * page_bytes);
       }
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       if (mine && i < static_cast<int>(n) && !(skip >> i & 1)) {
-        *reinterpret_cast<U4*>(at + pairs[first + i].y * page_bytes) = v[i];
+        Store(at + pairs[first + i].y * page_bytes, v[i]);
       }
     }
     return;
@@ -250,15 +255,20 @@ __global__ void __launch_bounds__(kThreads) ScanKernel(Tables t, Scratch s, Requ
     return;
   }
 
-  __shared__ int32_t named[kMaxRequests];  // the sequence that a request writes
+  __shared__ __attribute__((aligned(16))) int32_t named[kMaxRequests];  // the sequence that a request writes
   for (uint32_t i = threadIdx.x; i < r.count; i += kThreads) named[i] = kFork ? r.list[2 * i + 1] : r.list[i];
   __syncthreads();
   const auto needed = [&](uint32_t i) -> int32_t {  // pages, or -1 for a request that is refused
     const int32_t to = named[i];
     if (static_cast<uint32_t>(to) >= t.sequences) return -1;
-    for (uint32_t j = 0; j < i; ++j) {
-      if (named[j] == to) return -1;
+    // Four names a read and no way out of the loop: the reads overlap (128 requests: 13 us one by one).
+    bool again = false;
+#pragma unroll 4
+    for (uint32_t j = 0; j < i; j += 4) {
+      const int4 four = *reinterpret_cast<const int4*>(&named[j]);
+      again |= (four.x == to) | (j + 1 < i && four.y == to) | (j + 2 < i && four.z == to) | (j + 3 < i && four.w == to);
     }
+    if (again) return -1;
     const int64_t have = LengthOf(t, to);
     if constexpr (kFork) {
       const int32_t from = r.list[2 * i];
@@ -457,11 +467,14 @@ __global__ void __launch_bounds__(kThreads) PlacesKernel(Tables t, Scratch s, in
       if (in % 64 != 0) n += static_cast<uint32_t>(__popcll(w[in / 64] & ((uint64_t{1} << (in % 64)) - 1)));
     }
     below_live = n;
-    uint32_t before = blockIdx.x > 0 ? ends[blockIdx.x - 1] : 0;  // used pages before each of the chunk's words
-    for (uint32_t k = 0; k < kWords; ++k) {
-      words[k] = before;
-      before += static_cast<uint32_t>(__popcll(s.bits[uint64_t{blockIdx.x} * kWords + k]));
-    }
+  }
+  if (threadIdx.x >= 64 && threadIdx.x < 64 + kWords) {  // used pages before each of the chunk's words
+    const uint32_t k = threadIdx.x - 64;
+    const uint64_t* w = s.bits + uint64_t{blockIdx.x} * kWords;
+    uint32_t before = blockIdx.x > 0 ? ends[blockIdx.x - 1] : 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; ++i) before += i < k ? static_cast<uint32_t>(__popcll(w[i])) : 0;
+    words[k] = before;
   }
   __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) s.counts[s.chunks] = live - below_live;  // movers
@@ -481,43 +494,40 @@ __global__ void __launch_bounds__(kThreads) PlacesKernel(Tables t, Scratch s, in
   }
 }
 
-// Units of work, dealt over the grid: first each sequence's row, then kBatch moving pages' share of 256 columns.
+// Every sequence's row, dealt over the grid; and blockIdx.x: 256 columns of the moving pages, kBatch at a time, whose groups
+// blockIdx.y deals. A thread keeps its column, so an address is one product a page.
 __global__ void __launch_bounds__(kThreads) MoveKernel(Tables t, Scratch s, Pools pools) {
   const uint32_t movers = s.counts[s.chunks];
   if (movers == 0) return;
-  const uint64_t pieces = (pools.columns + kThreads - 1) / kThreads;
-  const uint64_t units = t.sequences + pieces * ((movers + kBatch - 1) / kBatch);
-  for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    if (u < t.sequences) {
-      int32_t* row = t.blocks + u * t.max_blocks;
-      const int32_t n = PagesOf(LengthOf(t, static_cast<uint32_t>(u)), t.page_shift);
-      for (int32_t b = static_cast<int32_t>(threadIdx.x); b < n; b += kThreads) {
-        const int32_t p = row[b];
-        if (static_cast<uint32_t>(p) >= t.pages) continue;
-        const int32_t place = s.place[p];
-        if (place >= 0) row[b] = s.holes[place];
-      }
-      continue;
+  for (uint64_t q = uint64_t{blockIdx.y} * gridDim.x + blockIdx.x; q < t.sequences; q += uint64_t{gridDim.y} * gridDim.x) {
+    int32_t* row = t.blocks + q * t.max_blocks;
+    const int32_t n = PagesOf(LengthOf(t, static_cast<uint32_t>(q)), t.page_shift);
+    for (int32_t b = static_cast<int32_t>(threadIdx.x); b < n; b += kThreads) {
+      const int32_t p = row[b];
+      if (static_cast<uint32_t>(p) >= t.pages) continue;
+      const int32_t place = s.place[p];
+      if (place >= 0) row[b] = s.holes[place];
     }
-    const uint32_t group = static_cast<uint32_t>((u - t.sequences) / pieces);
-    const uint32_t piece = static_cast<uint32_t>((u - t.sequences) % pieces);
-    const uint32_t c = piece * kThreads + threadIdx.x, first = group * kBatch, n = min(movers - first, uint32_t{kBatch});
-    if (piece == 0 && threadIdx.x < n) {
+  }
+  const uint32_t c = blockIdx.x * kThreads + threadIdx.x;
+  const bool mine = c < pools.columns;
+  uint64_t bytes;
+  unsigned char* const at = ColumnAt(pools, min(c, pools.columns - 1), bytes);
+  for (uint32_t first = blockIdx.y * kBatch; first < movers; first += gridDim.y * kBatch) {
+    const uint32_t n = min(movers - first, uint32_t{kBatch});
+    if (blockIdx.x == 0 && threadIdx.x < n) {
       const int32_t from = s.movers[first + threadIdx.x], to = s.holes[first + threadIdx.x];
       t.refs[to] = t.refs[from];
       t.refs[from] = 0;
     }
-    if (c >= pools.columns) continue;
-    uint64_t bytes;
-    unsigned char* const at = ColumnAt(pools, c, bytes);
     U4 v[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (i < static_cast<int>(n)) v[i] = *reinterpret_cast<const U4*>(at + s.movers[first + i] * bytes);
+      if (mine && i < static_cast<int>(n)) v[i] = Load(at + s.movers[first + i] * bytes);
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (i < static_cast<int>(n)) *reinterpret_cast<U4*>(at + s.holes[first + i] * bytes) = v[i];
+      if (mine && i < static_cast<int>(n)) Store(at + s.holes[first + i] * bytes, v[i]);
     }
   }
 }
@@ -700,9 +710,11 @@ RoostStatus Run(RoostContext* ctx, const void* params, const RoostWorkspace* ws,
     } else {
       ScanKernel<false><<<s.chunks, kThreads, 0, st>>>(a.tables, s, a.requests, 1);
       PlacesKernel<<<s.chunks, kThreads, 0, st>>>(a.tables, s, a.requests.status);
-      // The number of moving pages is the device's: at most half the pool's, whose units the grid does not exceed.
-      const uint64_t units = p.sequences + roost::CeilDiv(a.pools.columns, kThreads) * roost::CeilDiv(p.pages, 2 * kBatch);
-      MoveKernel<<<static_cast<uint32_t>(std::min<uint64_t>(units, 8 * ctx->compute_units)), kThreads, 0, st>>>(a.tables, s, a.pools);
+      // The number of moving pages is the device's, at most half the pool's. 64 workgroups a CU end evenly over the chip (910 MB
+      // moved: 369 us, 460 with 8), and 16,384 that find nothing to move cost 5 us.
+      const auto pieces = static_cast<uint32_t>(roost::CeilDiv(a.pools.columns, kThreads));
+      const uint64_t groups = std::min<uint64_t>(roost::CeilDiv(p.pages, 2 * kBatch), roost::CeilDiv(uint64_t{64} * ctx->compute_units, pieces));
+      MoveKernel<<<dim3(pieces, static_cast<uint32_t>(groups)), kThreads, 0, st>>>(a.tables, s, a.pools);
     }
     return roost::HipStatus(hipGetLastError(), op, "kernel launch");
   });

@@ -690,20 +690,15 @@ __device__ __forceinline__ bool FindTile(const Args& a, uint32_t rank, uint32_t 
       const uint32_t rows = static_cast<uint32_t>(min(max(a.cu[base + lane + 1], first), most) - first) * a.group;
       tiles = rows > a.row_limit ? (rows + rows_a_tile - 1) / rows_a_tile : 0;
     }
-    uint32_t end = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t o = static_cast<uint32_t>(__shfl_up(static_cast<int>(end), d));
-      if (lane >= d) end += o;
-    }
+    const uint32_t end = WaveScan(tiles);
     const uint64_t here = __ballot(rank < end);
     if (here != 0) {
       const int at = __builtin_ctzll(here);
       b = base + static_cast<uint32_t>(at);
-      tile = static_cast<int32_t>(__builtin_amdgcn_readlane(static_cast<int>(end), at)) - 1 - static_cast<int32_t>(rank);
+      tile = static_cast<int32_t>(LaneOf(end, at)) - 1 - static_cast<int32_t>(rank);
       return true;
     }
-    rank -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(end), 63));
+    rank -= LaneOf(end, 63);
   }
   return false;
 }
