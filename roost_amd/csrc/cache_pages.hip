@@ -121,7 +121,9 @@ __global__ void __launch_bounds__(kThreads) CacheCopyKernel(Pools pools, const i
       if constexpr (kMarked) {
         met = threadIdx.x == 0 && Meets(marks, p);
       } else {
-        for (uint32_t j = threadIdx.x; j < count; j += kThreads) met |= j != first + i && InPools(all[j], pages) && Meets(p, all[j]);
+        for (uint32_t j = threadIdx.x; j < count; j += kThreads) {
+          met |= j != first + i && InPools(all[j], pages) && Meets(p, all[j]);
+        }
       }
       if (met) atomicOr(&meets[0], 1u << i);
     }
@@ -557,7 +559,8 @@ void AdmitPools(roost::Gate& gate, const RoostAmdPagePool* pools, uint32_t count
                 static_cast<unsigned long long>(p.page_bytes))
         .Expect(p.layers == 1 || (p.layer_bytes % 16 == 0 && p.layer_bytes >= p.page_bytes * pages &&
                                   p.layer_bytes <= (uint64_t{1} << 40)),
-                ROOST_STATUS_INVALID_ARGUMENT, "pool %u: layers %llu bytes apart: no multiple of 16, below %u pages of %llu, or above 2^40", i,
+                ROOST_STATUS_INVALID_ARGUMENT,
+                "pool %u: layers %llu bytes apart: no multiple of 16, below %u pages of %llu, or above 2^40", i,
                 static_cast<unsigned long long>(p.layer_bytes), pages, static_cast<unsigned long long>(p.page_bytes));
     if (!gate.ok()) return;
     const uint64_t mine = p.page_bytes / 16 * p.layers;
@@ -631,19 +634,24 @@ RoostStatus Admit(const RoostAmdCachePagesParams& p, const char* op, Call call, 
         .Aligned("slot_mapping", p.slot_mapping.address, 8);
   }
   const uint64_t statuses = call == Call::kCompact ? 1 : p.count;
-  if (call != Call::kFree) gate.OptionalTensor("status", p.status, ROOST_DTYPE_I32, statuses).Aligned("status", p.status.address, 4);
+  if (call != Call::kFree) {
+    gate.OptionalTensor("status", p.status, ROOST_DTYPE_I32, statuses).Aligned("status", p.status.address, 4);
+  }
   ROOST_GATE_RETURN(gate);
   const bool pools = call == Call::kFork || call == Call::kCompact;
   if (pools) AdmitPools(gate, p.pools, p.pool_count, p.pages, a.pools);
   ROOST_GATE_RETURN(gate);
-  const auto of = [](const RoostDeviceSpan& s, uint64_t elements, uint64_t bytes) { return roost::ExtentOf(s.address, elements * bytes); };
+  const auto of = [](const RoostDeviceSpan& s, uint64_t elements, uint64_t bytes) {
+    return roost::ExtentOf(s.address, elements * bytes);
+  };
   // Everything that the call writes, then what it only reads.
+  const uint64_t requests = call == Call::kCompact ? 0 : uint64_t{p.count} * (call == Call::kFork ? 2 : 1);
   const roost::Extent spans[] = {of(p.block_tables, entries, 4),
                                  of(p.lengths, p.sequences, 4),
                                  of(p.refs, p.pages, 4),
                                  call == Call::kFree ? roost::Extent{} : of(p.status, statuses, 4),
                                  call == Call::kGrow ? of(p.slot_mapping, p.slot_mapping.length, 8) : roost::Extent{},
-                                 call == Call::kCompact ? roost::Extent{} : of(p.requests, uint64_t{p.count} * (call == Call::kFork ? 2 : 1), 4),
+                                 of(p.requests, requests, 4),
                                  call == Call::kGrow ? of(p.cu_seqlens, p.count + 1, 4) : roost::Extent{}};
   for (int i = 0; i < 7; ++i) {
     for (int j = 0; j < i && j < 5; ++j) {
@@ -713,7 +721,8 @@ RoostStatus Run(RoostContext* ctx, const void* params, const RoostWorkspace* ws,
       // The number of moving pages is the device's, at most half the pool's. 64 workgroups a CU end evenly over the chip (910 MB
       // moved: 369 us, 460 with 8), and 16,384 that find nothing to move cost 5 us.
       const auto pieces = static_cast<uint32_t>(roost::CeilDiv(a.pools.columns, kThreads));
-      const uint64_t groups = std::min<uint64_t>(roost::CeilDiv(p.pages, 2 * kBatch), roost::CeilDiv(uint64_t{64} * ctx->compute_units, pieces));
+      const uint64_t groups =
+          std::min<uint64_t>(roost::CeilDiv(p.pages, 2 * kBatch), roost::CeilDiv(uint64_t{64} * ctx->compute_units, pieces));
       MoveKernel<<<dim3(pieces, static_cast<uint32_t>(groups)), kThreads, 0, st>>>(a.tables, s, a.pools);
     }
     return roost::HipStatus(hipGetLastError(), op, "kernel launch");
@@ -744,7 +753,8 @@ extern "C" ROOST_API RoostStatus roost_amd_cache_copy_workspace(RoostContext* ct
 extern "C" ROOST_API RoostStatus roost_amd_cache_copy_run(RoostContext* ctx, const void* params, const RoostWorkspace* ws,
                                                           void* stream) {
   roost::Gate gate(kCopy);
-  gate.Expect(ctx != nullptr, ROOST_STATUS_INVALID_ARGUMENT, "no context was passed").Header(params, sizeof(RoostAmdCacheCopyParams));
+  gate.Expect(ctx != nullptr, ROOST_STATUS_INVALID_ARGUMENT, "no context was passed")
+      .Header(params, sizeof(RoostAmdCacheCopyParams));
   ROOST_GATE_RETURN(gate);
   const auto& p = *static_cast<const RoostAmdCacheCopyParams*>(params);
   return roost::CatchAll(kCopy, [&]() -> RoostStatus {

@@ -158,7 +158,8 @@ struct Deal {
 
 // ---- The row kernel -----------------------------------------------------------------------------------------------------------
 // Up to 16 kTiles rows (a few tokens' query heads of one KV head) against one part of a sequence's keys: decode. Bound by the
-// cache's bytes, 1.06 D a key and KV head.
+// cache's bytes, 1.06 D a key and KV head: 64 sequences of 500 to 16,000 keys, 32 heads over 8 of 128, 632 MB, take 128 us (4.9
+// TB/s of the 5.1 that a copy reaches) and the merge of their parts 6.
 //
 // Operands of v_mfma_f32_16x16x32_bf16, lane l = 16 g + m: A[m][8 g + j], B[8 g + j][m], result [4 g + i][m].
 //   S^T = K Q^T: key m of 16 as A, query row m as B. The contraction runs over the dims in any order, so lane (m, g) takes its
@@ -265,7 +266,9 @@ __global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : 
       if (lane < a.batch) of = SequenceOf(a, lane), mine = UnitsOf(a, of);
       sum = WaveSum(mine);
     } else {
-      for (uint32_t i = threadIdx.x; i < a.batch; i += 64 * kRowWaves) units[i] = static_cast<uint16_t>(UnitsOf(a, SequenceOf(a, i)));
+      for (uint32_t i = threadIdx.x; i < a.batch; i += 64 * kRowWaves) {
+        units[i] = static_cast<uint16_t>(UnitsOf(a, SequenceOf(a, i)));
+      }
       __syncthreads();
       for (uint32_t i = lane; i < a.batch; i += 64) sum += units[i];
       sum = WaveSum(sum);
@@ -283,363 +286,365 @@ __global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : 
 
 #pragma unroll 1
   for (bool opening = true;; opening = false) {
-  // One KV head's part of the run.
-  const uint32_t head = a.cut != nullptr ? (x - before * heads) / own : place % heads;
-  const uint32_t from = a.cut != nullptr ? x - before * heads - head * own : 0;
-  const uint32_t to = a.cut != nullptr ? min(own, from + (end - x)) : 1;
-  const bool whole = from == 0 && to == own;
-  const int32_t rows = s.count * static_cast<int32_t>(a.group);
-  if (a.cut != nullptr && from == 0 && head == 0 && threadIdx.x == 0) a.cut[1 + b] = before;
-  const int32_t k0 = FirstKey(a, s, 0) + static_cast<int32_t>(from) * kUnit;
-  const int32_t k1 = to == own ? s.keys : k0 + static_cast<int32_t>(to - from) * kUnit;
+    // One KV head's part of the run.
+    const uint32_t head = a.cut != nullptr ? (x - before * heads) / own : place % heads;
+    const uint32_t from = a.cut != nullptr ? x - before * heads - head * own : 0;
+    const uint32_t to = a.cut != nullptr ? min(own, from + (end - x)) : 1;
+    const bool whole = from == 0 && to == own;
+    const int32_t rows = s.count * static_cast<int32_t>(a.group);
+    if (a.cut != nullptr && from == 0 && head == 0 && threadIdx.x == 0) a.cut[1 + b] = before;
+    const int32_t k0 = FirstKey(a, s, 0) + static_cast<int32_t>(from) * kUnit;
+    const int32_t k1 = to == own ? s.keys : k0 + static_cast<int32_t>(to - from) * kUnit;
 
-  const int32_t steps = max(0, (k1 - k0 + kStep - 1) / kStep), my_steps = (steps + kRowWaves - 1 - w) / kRowWaves;
-  const auto key_of = [&](int32_t step) { return k0 + (step * kRowWaves + w) * kStep; };
-  const uint32_t shift = a.cache.page_shift, in_page = (1u << shift) - 1;
-  unsigned char* const ring = lds + w * kStages * Ring::kStage;
+    const int32_t steps = max(0, (k1 - k0 + kStep - 1) / kStep), my_steps = (steps + kRowWaves - 1 - w) / kRowWaves;
+    const auto key_of = [&](int32_t step) { return k0 + (step * kRowWaves + w) * kStep; };
+    const uint32_t shift = a.cache.page_shift, in_page = (1u << shift) - 1;
+    unsigned char* const ring = lds + w * kStages * Ring::kStage;
 
-  // Page ids of a window of 32 steps, a group of 16 keys a lane; -1 for a page that is none.
-  const auto ids_of = [&](int32_t window) {
-    const int32_t key = key_of(window * 32 + lane / 2) + 16 * (lane & 1), at = key >> shift;
-    int32_t id = -1;
-    if (key < k1 && at < s.blocks) id = a.tables[s.entry + at];
-    return static_cast<uint32_t>(id) < a.cache.pages ? id : -1;
-  };
+    // Page ids of a window of 32 steps, a group of 16 keys a lane; -1 for a page that is none.
+    const auto ids_of = [&](int32_t window) {
+      const int32_t key = key_of(window * 32 + lane / 2) + 16 * (lane & 1), at = key >> shift;
+      int32_t id = -1;
+      if (key < k1 && at < s.blocks) id = a.tables[s.entry + at];
+      return static_cast<uint32_t>(id) < a.cache.pages ? id : -1;
+    };
 
-  // One step's codes and scales to the ring. Pages that are none: page 0, whose keys are masked.
-  const auto issue = [&](int32_t step, int32_t ids) {
-    const uint32_t to = LdsAddress(ring) + static_cast<uint32_t>(step % kStages) * Ring::kStage;
-    uint64_t row[2], scale_row[2];
+    // One step's codes and scales to the ring. Pages that are none: page 0, whose keys are masked.
+    const auto issue = [&](int32_t step, int32_t ids) {
+      const uint32_t to = LdsAddress(ring) + static_cast<uint32_t>(step % kStages) * Ring::kStage;
+      uint64_t row[2], scale_row[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int32_t id = __builtin_amdgcn_readlane(ids, (2 * step + t) & 63);
-      const uint32_t key = static_cast<uint32_t>(key_of(step) + 16 * t) & in_page;
-      const uint64_t head_page = static_cast<uint64_t>(max(id, 0)) * a.cache.kv_heads + head;
-      row[t] = ((head_page << shift) + key) * (D / 2);
-      scale_row[t] = ((head_page * kBlocks) << shift) + key;
-    }
-#pragma unroll
-    for (int i = 0; i < Ring::kCodes / 1024; ++i) {
-      const uint32_t byte = 1024 * i + 16 * lane;  // of [group][16 keys x D / 2]
-      const uint64_t from = (D == 64 ? (lane < 32 ? row[0] : row[1]) : row[i / (D / 128)]) + byte % (8 * D);
-      Copy16(a.cache.k + from, to + 1024 * i);
-      Copy16(a.cache.v + from, to + Ring::kCodes + 1024 * i);
-    }
-#pragma unroll
-    for (int i = 0; i < Ring::kScales / 256; ++i) {
-      const uint32_t x = 64 * i + lane, block = x / 4 % kBlocks, t = x / (4 * kBlocks) % 2, value = x / (8 * kBlocks) % 2;
-      const uint64_t from = (t == 0 ? scale_row[0] : scale_row[1]) + (block << shift) + 4 * (x % 4);
-      Copy4((value ? a.cache.v_scales : a.cache.k_scales) + from, to + 2 * Ring::kCodes + 256 * i);
-    }
-  };
-
-  for (int32_t tile = 0; tile * 16 * kTiles < rows; ++tile) {
-    // Query rows: lane m's of each 16.
-    int32_t pos[kTiles];
-    U4 q[kTiles][kWords];
-#pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      const int32_t r = (tile * kTiles + n) * 16 + m;
-      const bool ok = r < rows;
-      const int32_t token = ok ? r / static_cast<int32_t>(a.group) : 0;
-      const uint32_t h = head * a.group + (ok ? r - token * static_cast<int32_t>(a.group) : 0);
-      pos[n] = ok ? s.keys - s.count + token : -1;
-      const uint16_t* qr = a.q + static_cast<uint64_t>(s.first + token) * a.q_stride + static_cast<uint64_t>(h) * D;
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        const int d = D == 64 ? 16 * g + 8 * i : 128 * (i / 4) + 32 * g + 8 * (i % 4);
-        const U4 x = *reinterpret_cast<const U4*>(qr + d);
-        q[n][i] = ok ? x : U4{0, 0, 0, 0};
+      for (int t = 0; t < 2; ++t) {
+        const int32_t id = __builtin_amdgcn_readlane(ids, (2 * step + t) & 63);
+        const uint32_t key = static_cast<uint32_t>(key_of(step) + 16 * t) & in_page;
+        const uint64_t head_page = static_cast<uint64_t>(max(id, 0)) * a.cache.kv_heads + head;
+        row[t] = ((head_page << shift) + key) * (D / 2);
+        scale_row[t] = ((head_page * kBlocks) << shift) + key;
       }
-    }
-
-    F4v o[kTiles][kDt];
-    float top[kTiles], sum[kTiles];
-    // careful: a block of V that is NaN multiplies as zeros, and makes the outputs of the rows that see it NaN by hand; without,
-    // its NaN would reach the rows that do not see it as well. Only taken where a first pass left a NaN.
-    const auto pass = [&](bool careful) {
 #pragma unroll
-      for (int n = 0; n < kTiles; ++n) {
-        top[n] = -INFINITY, sum[n] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < kDt; ++d) o[n][d] = F4v{0, 0, 0, 0};
+      for (int i = 0; i < Ring::kCodes / 1024; ++i) {
+        const uint32_t byte = 1024 * i + 16 * lane;  // of [group][16 keys x D / 2]
+        const uint64_t from = (D == 64 ? (lane < 32 ? row[0] : row[1]) : row[i / (D / 128)]) + byte % (8 * D);
+        Copy16(a.cache.k + from, to + 1024 * i);
+        Copy16(a.cache.v + from, to + Ring::kCodes + 1024 * i);
       }
-      int32_t ids = ids_of(0), ids_next = my_steps > 32 ? ids_of(1) : -1;
-      uint64_t bad_issued = __ballot(ids < 0), bad = bad_issued;  // groups without a page, of the window issued from, and of this one
 #pragma unroll
-      for (int i = 0; i < kStages; ++i) {
-        if (i < my_steps) issue(i, ids);
-      }
-#pragma unroll 1
-      for (int32_t step = 0; step < my_steps; ++step) {
-        if ((step & 31) == 0) bad = bad_issued;
-        if (step + kStages <= my_steps) {
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * Ring::kCopies) : "memory");
-        } else {
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
-        // The lane's share of the step: key m's codes and scales in each group, its dims of the eight keys and their scales.
-        uint32_t kc[2][kWords], ks[2][D == 256 ? 2 : 1], vc[8][D == 256 ? 2 : 1], vs[2];
-        {
-          const unsigned char* at = ring + static_cast<uint32_t>(step % kStages) * Ring::kStage;
-          const unsigned char* sc = at + 2 * Ring::kCodes;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if constexpr (D == 64) {
-              const U2 x = *reinterpret_cast<const U2*>(at + 512 * t + 32 * m + 8 * g);
-              kc[t][0] = x[0], kc[t][1] = x[1];
-              ks[t][0] = sc[16 * (t * kBlocks + g / 2) + m];
-            } else {
-#pragma unroll
-              for (int h = 0; h < D / 128; ++h) {
-                const U4 x = *reinterpret_cast<const U4*>(at + 8 * D * t + m * (D / 2) + 64 * h + 16 * g);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) kc[t][4 * h + i] = x[i];
-                ks[t][h] = sc[16 * (t * kBlocks + 4 * h + g) + m];
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const unsigned char* p = at + Ring::kCodes + 8 * D * t + (4 * g + i) * (D / 2) + m * (D / 32);
-              if constexpr (D == 64) {
-                vc[4 * t + i][0] = *reinterpret_cast<const uint16_t*>(p);
-              } else if constexpr (D == 128) {
-                vc[4 * t + i][0] = *reinterpret_cast<const uint32_t*>(p);
-              } else {
-                const U2 x = *reinterpret_cast<const U2*>(p);
-                vc[4 * t + i][0] = x[0], vc[4 * t + i][1] = x[1];
-              }
-            }
-            vs[t] = *reinterpret_cast<const uint32_t*>(sc + 32 * kBlocks + 16 * (t * kBlocks + m / (512 / D)) + 4 * g);
-          }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the next copies may take the stage
-        if (step + kStages < my_steps) {
-          const int32_t next = step + kStages;
-          if ((next & 31) == 0) {
-            ids = ids_next;
-            bad_issued = __ballot(ids < 0);
-            if (next + 32 < my_steps) ids_next = ids_of(next / 32 + 1);
-          }
-          issue(next, ids);
-        }
-
-        const int32_t key0 = key_of(step);
-        const uint32_t none = static_cast<uint32_t>(bad >> ((2 * step) & 63)) & 3;  // groups without a page
-        const bool edge = key0 + kStep > k1 || none != 0;
-        const bool mask = edge || (a.causal && key0 + kStep > s.keys - s.count + 1) ||
-                          (a.window >= 0 && key0 < s.keys - 1 - a.window);
-        const auto absent = [&](int t, int i) {  // key 16 t + 4 g + i is none of the part's
-          return key0 + 16 * t + 4 * g + i >= k1 || (none >> t & 1) != 0;
-        };
-        F4v sc[kTiles][2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) sc[n][t] = F4v{0, 0, 0, 0};
-#pragma unroll
-          for (int i = 0; i < kWords; ++i) {
-            const float scale = F4Scale(ks[t][D == 256 ? i / 4 : 0]);
-            const uint32_t c = kc[t][i];
-            const U4 kk{FromF4<0>(c, scale), FromF4<1>(c, scale), FromF4<2>(c, scale), FromF4<3>(c, scale)};
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n) sc[n][t] = Mfma16(kk, q[n][i], sc[n][t]);
-          }
-        }
-        uint32_t nan_keys = 0;
-        if (edge || careful) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t byte = vs[t] >> (8 * i) & 0xFF;
-              const bool nan = careful && byte > kF4ByteHigh;
-              const bool off = absent(t, i);
-              if (nan && !off) nan_keys |= 1u << (4 * t + i);
-              if (nan || off) vs[t] = (vs[t] & ~(0xFFu << (8 * i))) | 127u << (8 * i);  // finite, whatever lies there, times p = 0
-            }
-          }
-        }
-        U4 p[kTiles];
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-          float y[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            y[j] = sc[n][j / 4][j % 4];
-            if constexpr (kCap) y[j] = Capped(y[j] * a.scale_log2, a.cap);
-          }
-          if (mask) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int32_t key = key0 + 16 * (j / 4) + 4 * g + j % 4;
-              const bool off = absent(j / 4, j % 4) | ((a.causal != 0) & (key > pos[n])) |
-                               ((a.window >= 0) & (key < pos[n] - a.window));
-              y[j] = off ? -INFINITY : y[j];
-            }
-          }
-          const float scale = kCap ? 1.0f : a.scale_log2;  // positive: the largest score stays the largest
-          float mx = y[0];
-#pragma unroll
-          for (int j = 1; j < 8; ++j) mx = fmaxf(mx, y[j]);
-          mx *= scale;
-          if (__any(mx > top[n] + kGrow)) {
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float now = mx > top[n] ? mx : top[n];
-            const float by = top[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[n] - now);
-            sum[n] *= by;
-#pragma unroll
-            for (int d = 0; d < kDt; ++d) o[n][d] *= by;
-            top[n] = now;
-          }
-          const float base = top[n] == -INFINITY ? 0.0f : top[n];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], scale, -base));
-            sum[n] += y[j];
-          }
-          p[n] = U4{PackBf16Rne(y[0], y[1]), PackBf16Rne(y[2], y[3]), PackBf16Rne(y[4], y[5]), PackBf16Rne(y[6], y[7])};
-        }
-        // Two dims of eight keys, then each dim's eight keys.
-        const auto two = [&](auto pair, int word, int out) {
-          uint32_t c[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) c[j] = FromF4<decltype(pair)::value>(vc[j][word], F4Scale(vs[j / 4] >> (8 * (j % 4)) & 0xFF));
-          U4 lo, hi;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            lo[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x05040100u);
-            hi[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x07060302u);
-          }
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) {
-            o[n][out] = Mfma16(lo, p[n], o[n][out]);
-            o[n][out + 1] = Mfma16(hi, p[n], o[n][out + 1]);
-          }
-        };
-#pragma unroll
-        for (int word = 0; word < (D == 256 ? 2 : 1); ++word) {
-          two(std::integral_constant<int, 0>{}, word, 8 * word);
-          two(std::integral_constant<int, 1>{}, word, 8 * word + 2);
-          if constexpr (D > 64) {
-            two(std::integral_constant<int, 2>{}, word, 8 * word + 4);
-            two(std::integral_constant<int, 3>{}, word, 8 * word + 6);
-          }
-        }
-        if (careful) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            for (uint64_t lanes = __ballot(nan_keys >> j & 1); lanes != 0; lanes &= lanes - 1) {
-              const int from = __builtin_ctzll(lanes);  // dims D / 16 (from % 16) .. of a key of its group
-              const int32_t key = key0 + 16 * (j / 4) + 4 * (from >> 4) + j % 4;
-#pragma unroll
-              for (int n = 0; n < kTiles; ++n) {
-                if ((a.causal && key > pos[n]) || (a.window >= 0 && key < pos[n] - a.window)) continue;
-#pragma unroll
-                for (int d = 0; d < kDt; ++d)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    if (4 * g + i == (from & 15)) o[n][d][i] = NAN;
-                  }
-              }
-            }
-          }
-        }
+      for (int i = 0; i < Ring::kScales / 256; ++i) {
+        const uint32_t x = 64 * i + lane, block = x / 4 % kBlocks, t = x / (4 * kBlocks) % 2, value = x / (8 * kBlocks) % 2;
+        const uint64_t from = (t == 0 ? scale_row[0] : scale_row[1]) + (block << shift) + 4 * (x % 4);
+        Copy4((value ? a.cache.v_scales : a.cache.k_scales) + from, to + 2 * Ring::kCodes + 256 * i);
       }
     };
-    bool careful = false;
-#pragma unroll 1
-    for (;;) {
-      pass(careful);
-      if (careful) break;
-      bool nan = false;
-#pragma unroll
-      for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-        for (int d = 0; d < kDt; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) nan |= o[n][d][i] != o[n][d][i];
-      if (!__any(nan)) break;
-      careful = true;
-    }
 
-    // The four wavefronts' results meet, 16 rows at a time.
+    for (int32_t tile = 0; tile * 16 * kTiles < rows; ++tile) {
+      // Query rows: lane m's of each 16.
+      int32_t pos[kTiles];
+      U4 q[kTiles][kWords];
 #pragma unroll
-    for (int n = 0; n < kTiles; ++n) {
-      const int32_t row0 = (tile * kTiles + n) * 16;
-      float l = sum[n];
-      l += __shfl_xor(l, 16);
-      l += __shfl_xor(l, 32);
-      __syncthreads();  // the rings, or the rows before, are read
-      if (g == 0) result.ml[w][0][m] = top[n], result.ml[w][1][m] = l;
-      if (row0 + m < rows) {
+      for (int n = 0; n < kTiles; ++n) {
+        const int32_t r = (tile * kTiles + n) * 16 + m;
+        const bool ok = r < rows;
+        const int32_t token = ok ? r / static_cast<int32_t>(a.group) : 0;
+        const uint32_t h = head * a.group + (ok ? r - token * static_cast<int32_t>(a.group) : 0);
+        pos[n] = ok ? s.keys - s.count + token : -1;
+        const uint16_t* qr = a.q + static_cast<uint64_t>(s.first + token) * a.q_stride + static_cast<uint64_t>(h) * D;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int d = 0; d < kDt; d += 4) {
-            *reinterpret_cast<F4v*>(&result.o[w][m][(4 * g + i) * kDt + d]) =
-                F4v{o[n][d][i], o[n][d + 1][i], o[n][d + 2][i], o[n][d + 3][i]};
-          }
-      }
-      __syncthreads();
-      constexpr int kThreadsPerRow = 16, kPer = D / kThreadsPerRow;  // 16 rows x 16 threads
-      const int r = threadIdx.x / kThreadsPerRow, d0 = (threadIdx.x % kThreadsPerRow) * kPer;
-      const int32_t row = row0 + r;
-      if (row >= rows) continue;
-      float big = result.ml[0][0][r];
-#pragma unroll
-      for (int x = 1; x < kRowWaves; ++x) big = fmaxf(big, result.ml[x][0][r]);
-      float total = 0.0f, f[kRowWaves], y[kPer];
-#pragma unroll
-      for (int x = 0; x < kRowWaves; ++x) {
-        f[x] = result.ml[x][0][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(result.ml[x][0][r] - big);
-        total += result.ml[x][1][r] * f[x];
-      }
-#pragma unroll
-      for (int d = 0; d < kPer; ++d) {
-        y[d] = 0.0f;
-#pragma unroll
-        for (int x = 0; x < kRowWaves; ++x) y[d] += result.o[x][r][d0 + d] * f[x];
-      }
-      const int32_t token = row / static_cast<int32_t>(a.group);
-      const uint32_t h = head * a.group + static_cast<uint32_t>(row - token * static_cast<int32_t>(a.group));
-      if (!whole) {
-        // A part that began in an earlier run opens this one; else it goes on in the next.
-        const uint64_t at = (2 * static_cast<uint64_t>(place) + (opening && from != 0 ? 0 : 1)) * a.short_tokens * a.group +
-                            static_cast<uint32_t>(row);
-#pragma unroll
-        for (int d = 0; d < kPer; d += 4) {
-          *reinterpret_cast<F4v*>(a.part_o + at * D + d0 + d) = F4v{y[d], y[d + 1], y[d + 2], y[d + 3]};
+        for (int i = 0; i < kWords; ++i) {
+          const int d = D == 64 ? 16 * g + 8 * i : 128 * (i / 4) + 32 * g + 8 * (i % 4);
+          const U4 x = *reinterpret_cast<const U4*>(qr + d);
+          q[n][i] = ok ? x : U4{0, 0, 0, 0};
         }
-        if (d0 == 0) a.part_ml[2 * at] = big, a.part_ml[2 * at + 1] = total;
-      } else {
-      const float inv = total > 0.0f ? 1.0f / total : total == total ? 0.0f : NAN;
-      const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + h;
+      }
+
+      F4v o[kTiles][kDt];
+      float top[kTiles], sum[kTiles];
+      // careful: a block of V that is NaN multiplies as zeros, and makes the outputs of the rows that see it NaN by hand; without,
+      // its NaN would reach the rows that do not see it as well. Only taken where a first pass left a NaN.
+      const auto pass = [&](bool careful) {
 #pragma unroll
-      for (int d = 0; d < kPer; d += 4) {
-        *reinterpret_cast<U2*>(a.out + at * D + d0 + d) = U2{PackBf16Rne(y[d] * inv, y[d + 1] * inv),
-                                                             PackBf16Rne(y[d + 2] * inv, y[d + 3] * inv)};
+        for (int n = 0; n < kTiles; ++n) {
+          top[n] = -INFINITY, sum[n] = 0.0f;
+#pragma unroll
+          for (int d = 0; d < kDt; ++d) o[n][d] = F4v{0, 0, 0, 0};
+        }
+        int32_t ids = ids_of(0), ids_next = my_steps > 32 ? ids_of(1) : -1;
+        uint64_t bad_issued = __ballot(ids < 0), bad = bad_issued;  // groups without a page: of the window issued from, of this one
+#pragma unroll
+        for (int i = 0; i < kStages; ++i) {
+          if (i < my_steps) issue(i, ids);
+        }
+#pragma unroll 1
+        for (int32_t step = 0; step < my_steps; ++step) {
+          if ((step & 31) == 0) bad = bad_issued;
+          if (step + kStages <= my_steps) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * Ring::kCopies) : "memory");
+          } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          }
+          // The lane's share of the step: key m's codes and scales in each group, its dims of the eight keys and their scales.
+          uint32_t kc[2][kWords], ks[2][D == 256 ? 2 : 1], vc[8][D == 256 ? 2 : 1], vs[2];
+          {
+            const unsigned char* at = ring + static_cast<uint32_t>(step % kStages) * Ring::kStage;
+            const unsigned char* sc = at + 2 * Ring::kCodes;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if constexpr (D == 64) {
+                const U2 x = *reinterpret_cast<const U2*>(at + 512 * t + 32 * m + 8 * g);
+                kc[t][0] = x[0], kc[t][1] = x[1];
+                ks[t][0] = sc[16 * (t * kBlocks + g / 2) + m];
+              } else {
+#pragma unroll
+                for (int h = 0; h < D / 128; ++h) {
+                  const U4 x = *reinterpret_cast<const U4*>(at + 8 * D * t + m * (D / 2) + 64 * h + 16 * g);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) kc[t][4 * h + i] = x[i];
+                  ks[t][h] = sc[16 * (t * kBlocks + 4 * h + g) + m];
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const unsigned char* p = at + Ring::kCodes + 8 * D * t + (4 * g + i) * (D / 2) + m * (D / 32);
+                if constexpr (D == 64) {
+                  vc[4 * t + i][0] = *reinterpret_cast<const uint16_t*>(p);
+                } else if constexpr (D == 128) {
+                  vc[4 * t + i][0] = *reinterpret_cast<const uint32_t*>(p);
+                } else {
+                  const U2 x = *reinterpret_cast<const U2*>(p);
+                  vc[4 * t + i][0] = x[0], vc[4 * t + i][1] = x[1];
+                }
+              }
+              vs[t] = *reinterpret_cast<const uint32_t*>(sc + 32 * kBlocks + 16 * (t * kBlocks + m / (512 / D)) + 4 * g);
+            }
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the next copies may take the stage
+          if (step + kStages < my_steps) {
+            const int32_t next = step + kStages;
+            if ((next & 31) == 0) {
+              ids = ids_next;
+              bad_issued = __ballot(ids < 0);
+              if (next + 32 < my_steps) ids_next = ids_of(next / 32 + 1);
+            }
+            issue(next, ids);
+          }
+
+          const int32_t key0 = key_of(step);
+          const uint32_t none = static_cast<uint32_t>(bad >> ((2 * step) & 63)) & 3;  // groups without a page
+          const bool edge = key0 + kStep > k1 || none != 0;
+          const bool mask = edge || (a.causal && key0 + kStep > s.keys - s.count + 1) ||
+                            (a.window >= 0 && key0 < s.keys - 1 - a.window);
+          const auto absent = [&](int t, int i) {  // key 16 t + 4 g + i is none of the part's
+            return key0 + 16 * t + 4 * g + i >= k1 || (none >> t & 1) != 0;
+          };
+          F4v sc[kTiles][2];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) sc[n][t] = F4v{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+              const float scale = F4Scale(ks[t][D == 256 ? i / 4 : 0]);
+              const uint32_t c = kc[t][i];
+              const U4 kk{FromF4<0>(c, scale), FromF4<1>(c, scale), FromF4<2>(c, scale), FromF4<3>(c, scale)};
+#pragma unroll
+              for (int n = 0; n < kTiles; ++n) sc[n][t] = Mfma16(kk, q[n][i], sc[n][t]);
+            }
+          }
+          uint32_t nan_keys = 0;
+          if (edge || careful) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t byte = vs[t] >> (8 * i) & 0xFF;
+                const bool nan = careful && byte > kF4ByteHigh;
+                const bool off = absent(t, i);
+                if (nan && !off) nan_keys |= 1u << (4 * t + i);
+                if (nan || off) vs[t] = (vs[t] & ~(0xFFu << (8 * i))) | 127u << (8 * i);  // finite, times p = 0
+              }
+            }
+          }
+          U4 p[kTiles];
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              y[j] = sc[n][j / 4][j % 4];
+              if constexpr (kCap) y[j] = Capped(y[j] * a.scale_log2, a.cap);
+            }
+            if (mask) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int32_t key = key0 + 16 * (j / 4) + 4 * g + j % 4;
+                const bool off = absent(j / 4, j % 4) | ((a.causal != 0) & (key > pos[n])) |
+                                 ((a.window >= 0) & (key < pos[n] - a.window));
+                y[j] = off ? -INFINITY : y[j];
+              }
+            }
+            const float scale = kCap ? 1.0f : a.scale_log2;  // positive: the largest score stays the largest
+            float mx = y[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, y[j]);
+            mx *= scale;
+            if (__any(mx > top[n] + kGrow)) {
+              mx = fmaxf(mx, __shfl_xor(mx, 16));
+              mx = fmaxf(mx, __shfl_xor(mx, 32));
+              const float now = mx > top[n] ? mx : top[n];
+              const float by = top[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[n] - now);
+              sum[n] *= by;
+#pragma unroll
+              for (int d = 0; d < kDt; ++d) o[n][d] *= by;
+              top[n] = now;
+            }
+            const float base = top[n] == -INFINITY ? 0.0f : top[n];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], scale, -base));
+              sum[n] += y[j];
+            }
+            p[n] = U4{PackBf16Rne(y[0], y[1]), PackBf16Rne(y[2], y[3]), PackBf16Rne(y[4], y[5]), PackBf16Rne(y[6], y[7])};
+          }
+          // Two dims of eight keys, then each dim's eight keys.
+          const auto two = [&](auto pair, int word, int out) {
+            uint32_t c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              c[j] = FromF4<decltype(pair)::value>(vc[j][word], F4Scale(vs[j / 4] >> (8 * (j % 4)) & 0xFF));
+            }
+            U4 lo, hi;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              lo[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x05040100u);
+              hi[j] = __builtin_amdgcn_perm(c[2 * j + 1], c[2 * j], 0x07060302u);
+            }
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) {
+              o[n][out] = Mfma16(lo, p[n], o[n][out]);
+              o[n][out + 1] = Mfma16(hi, p[n], o[n][out + 1]);
+            }
+          };
+#pragma unroll
+          for (int word = 0; word < (D == 256 ? 2 : 1); ++word) {
+            two(std::integral_constant<int, 0>{}, word, 8 * word);
+            two(std::integral_constant<int, 1>{}, word, 8 * word + 2);
+            if constexpr (D > 64) {
+              two(std::integral_constant<int, 2>{}, word, 8 * word + 4);
+              two(std::integral_constant<int, 3>{}, word, 8 * word + 6);
+            }
+          }
+          if (careful) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              for (uint64_t lanes = __ballot(nan_keys >> j & 1); lanes != 0; lanes &= lanes - 1) {
+                const int from = __builtin_ctzll(lanes);  // dims D / 16 (from % 16) .. of a key of its group
+                const int32_t key = key0 + 16 * (j / 4) + 4 * (from >> 4) + j % 4;
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                  if ((a.causal && key > pos[n]) || (a.window >= 0 && key < pos[n] - a.window)) continue;
+#pragma unroll
+                  for (int d = 0; d < kDt; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                      if (4 * g + i == (from & 15)) o[n][d][i] = NAN;
+                    }
+                }
+              }
+            }
+          }
+        }
+      };
+      bool careful = false;
+#pragma unroll 1
+      for (;;) {
+        pass(careful);
+        if (careful) break;
+        bool nan = false;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int d = 0; d < kDt; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nan |= o[n][d][i] != o[n][d][i];
+        if (!__any(nan)) break;
+        careful = true;
       }
-      if (a.lse != nullptr && d0 == 0) {
-        a.lse[at] = total > 0.0f ? big + __builtin_amdgcn_logf(total) : total == total ? -INFINITY : NAN;
+
+      // The four wavefronts' results meet, 16 rows at a time.
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) {
+        const int32_t row0 = (tile * kTiles + n) * 16;
+        float l = sum[n];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        __syncthreads();  // the rings, or the rows before, are read
+        if (g == 0) result.ml[w][0][m] = top[n], result.ml[w][1][m] = l;
+        if (row0 + m < rows) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < kDt; d += 4) {
+              *reinterpret_cast<F4v*>(&result.o[w][m][(4 * g + i) * kDt + d]) =
+                  F4v{o[n][d][i], o[n][d + 1][i], o[n][d + 2][i], o[n][d + 3][i]};
+            }
+        }
+        __syncthreads();
+        constexpr int kThreadsPerRow = 16, kPer = D / kThreadsPerRow;  // 16 rows x 16 threads
+        const int r = threadIdx.x / kThreadsPerRow, d0 = (threadIdx.x % kThreadsPerRow) * kPer;
+        const int32_t row = row0 + r;
+        if (row >= rows) continue;
+        float big = result.ml[0][0][r];
+#pragma unroll
+        for (int x = 1; x < kRowWaves; ++x) big = fmaxf(big, result.ml[x][0][r]);
+        float total = 0.0f, f[kRowWaves], y[kPer];
+#pragma unroll
+        for (int x = 0; x < kRowWaves; ++x) {
+          f[x] = result.ml[x][0][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(result.ml[x][0][r] - big);
+          total += result.ml[x][1][r] * f[x];
+        }
+#pragma unroll
+        for (int d = 0; d < kPer; ++d) {
+          y[d] = 0.0f;
+#pragma unroll
+          for (int x = 0; x < kRowWaves; ++x) y[d] += result.o[x][r][d0 + d] * f[x];
+        }
+        const int32_t token = row / static_cast<int32_t>(a.group);
+        const uint32_t h = head * a.group + static_cast<uint32_t>(row - token * static_cast<int32_t>(a.group));
+        if (!whole) {
+          // A part that began in an earlier run opens this one; else it goes on in the next.
+          const uint64_t at = (2 * static_cast<uint64_t>(place) + (opening && from != 0 ? 0 : 1)) * a.short_tokens * a.group +
+                              static_cast<uint32_t>(row);
+#pragma unroll
+          for (int d = 0; d < kPer; d += 4) {
+            *reinterpret_cast<F4v*>(a.part_o + at * D + d0 + d) = F4v{y[d], y[d + 1], y[d + 2], y[d + 3]};
+          }
+          if (d0 == 0) a.part_ml[2 * at] = big, a.part_ml[2 * at + 1] = total;
+        } else {
+          const float inv = total > 0.0f ? 1.0f / total : total == total ? 0.0f : NAN;
+          const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + h;
+#pragma unroll
+          for (int d = 0; d < kPer; d += 4) {
+            *reinterpret_cast<U2*>(a.out + at * D + d0 + d) = U2{PackBf16Rne(y[d] * inv, y[d + 1] * inv),
+                                                                 PackBf16Rne(y[d + 2] * inv, y[d + 3] * inv)};
+        }
+        if (a.lse != nullptr && d0 == 0) {
+          a.lse[at] = total > 0.0f ? big + __builtin_amdgcn_logf(total) : total == total ? -INFINITY : NAN;
+        }
+        }
       }
-      }
+      __syncthreads();  // the results are read: the rings may be filled again
     }
-    __syncthreads();  // the results are read: the rings may be filled again
-  }
-  x += to - from;
-  if (x >= end) return;
-  if (x >= (before + own) * heads) {
-    find(mine);
-    s = SequenceOf(a, b = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b))));
-  }
+    x += to - from;
+    if (x >= end) return;
+    if (x >= (before + own) * heads) {
+      find(mine);
+      s = SequenceOf(a, b = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(b))));
+    }
   }
 }
 
 // ---- The tile kernel ----------------------------------------------------------------------------------------------------------
-// 32 kWaves rows of one sequence and KV head (rows are its tokens' query heads, token by token) against the keys that they see, 64
-// at a time: prompt chunks. Bound by the matrix instructions and, beside them, by LDS reads and the softmax.
+// 256 rows of one sequence and KV head (rows are its tokens' query heads, token by token) against the keys that they see, 64 at a
+// time: prompt chunks. Bound by the matrix instructions and, beside them, by LDS reads and the softmax.
 //
 // A tile's codes go to LDS as bf16 once for all wavefronts, a lane a block of 32 dims (16 bytes, one scale): 16 conversions a lane
 // and tile at head_dim 128 and 256 rows, where converting in each wavefront would take 128. Codes of the next tile are under way
@@ -653,6 +658,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : 
 // LDS: K rows are padded by 16 bytes, so that 16 keys' reads of 16 bytes meet no bank twice; V's 64-byte chunks are swizzled by
 // the key, and their 16-byte pieces by the next bits of it, which does the same for the transposing reads of 8 keys x 64 bytes.
 
+constexpr int kTileWaves = 8;
 constexpr int kTileKeys = 64;
 
 __device__ __forceinline__ U2 LdsTranspose(const unsigned char* base, uint32_t off) {
@@ -660,13 +666,13 @@ __device__ __forceinline__ U2 LdsTranspose(const unsigned char* base, uint32_t o
   return __builtin_bit_cast(U2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
 }
 
-template <int D, int kWaves, int kPieces>
+template <int D, int kPieces>
 struct TileLds {
   static constexpr int kKeyRow = 2 * D + 16;
   unsigned char k[2][kTileKeys * kKeyRow];
   unsigned char v[2][kTileKeys * 2 * D];
-  U4 codes[kWaves][kPieces][64];        // of the next tile, a block a lane
-  uint32_t scales[kWaves][kPieces][64];
+  U4 codes[kTileWaves][kPieces][64];        // of the next tile, a block a lane
+  uint32_t scales[kTileWaves][kPieces][64];
   uint32_t bad[3];                // groups of 16 keys without a page, of this tile, the next and the one after
   uint32_t nan[3][kTileKeys];     // blocks of V that are NaN; only kept in a careful pass
 };
@@ -720,13 +726,13 @@ __device__ __forceinline__ TileKeys KeysOfTile(const Args& a, const Sequence& s,
   return k;
 }
 
-template <int D, int kWaves, bool kCap>
-__global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(Args a) {
-  constexpr int kThreads = 64 * kWaves, kRows = 32 * kWaves;
+template <int D, bool kCap>
+__global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttentionKernel(Args a) {
+  constexpr int kThreads = 64 * kTileWaves, kRows = 32 * kTileWaves;
   constexpr int kKs = D / 16, kDt = D / 32;
   constexpr int kHalves = D == 64 ? 2 : 1;  // of a tile's keys that are scored together (at 128 the registers of two cost 1%)
   constexpr int kPieces = (4 * D + kThreads - 1) / kThreads;  // blocks of 32 codes that a lane stages
-  typedef TileLds<D, kWaves, kPieces> Lds;
+  typedef TileLds<D, kPieces> Lds;
   __shared__ __attribute__((aligned(16))) Lds lds;
 
   const uint32_t head = blockIdx.x % a.cache.kv_heads, split = blockIdx.x / a.cache.kv_heads % a.tile_splits;
@@ -1051,8 +1057,8 @@ __global__ void __launch_bounds__(64 * kWaves, kWaves / 4) TileAttentionKernel(A
   if (a.lse != nullptr && g == 0) a.lse[at] = sum > 0.0f ? top + __builtin_amdgcn_logf(sum) : sum == sum ? -INFINITY : NAN;
 }
 
-// One row's parts by a workgroup: D / 4 lanes a part, their loads together, then the lanes' sums. The order of the additions is that
-// of the parts' numbers, whichever workgroup wrote them when. row_of(p): part p's partial row; at: the output row.
+// One row's parts by a workgroup: D / 4 lanes a part, their loads together, then the lanes' sums. The order of the additions is
+// that of the parts' numbers, whichever workgroup wrote them when. row_of(p): part p's partial row; at: the output row.
 template <int D, typename F>
 __device__ __forceinline__ void MergeRow(const Args& a, const float* part_o, const float* part_ml, F&& row_of, uint32_t parts,
                                          uint64_t at) {
@@ -1107,20 +1113,21 @@ __device__ __forceinline__ void MergeRow(const Args& a, const float* part_o, con
 }
 
 // Block (tile and KV head, 1,024 / D rows of it): D / 4 lanes a row, up to four parts' loads together.
-template <int D, int kWaves>
+template <int D>
 __global__ void __launch_bounds__(256) TileMergeKernel(Args a) {
   constexpr int32_t kLanes = D / 4, kRows = 256 / kLanes;
   const uint32_t head = blockIdx.x % a.cache.kv_heads;
   uint32_t b = 0;
   int32_t tile = 0;
-  if (!FindTile(a, blockIdx.x / a.cache.kv_heads, 32 * kWaves, b, tile)) return;
+  if (!FindTile(a, blockIdx.x / a.cache.kv_heads, 32 * kTileWaves, b, tile)) return;
   const Sequence s = SequenceOf(a, b);
-  const TileKeys range = KeysOfTile(a, s, tile, 32 * kWaves);
+  const TileKeys range = KeysOfTile(a, s, tile, 32 * kTileWaves);
   const int32_t group = static_cast<int32_t>(a.group);
-  const int32_t row = tile * 32 * kWaves + static_cast<int32_t>(blockIdx.y) * kRows + static_cast<int32_t>(threadIdx.x) / kLanes;
+  const int32_t row = tile * 32 * kTileWaves + static_cast<int32_t>(blockIdx.y * kRows + threadIdx.x / kLanes);
   if (range.parts <= 1 || row >= s.count * group) return;
   const int32_t token = row / group, d = static_cast<int32_t>(threadIdx.x) % kLanes * 4;
-  const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + head * a.group + static_cast<uint32_t>(row - token * group);
+  const uint32_t h = head * a.group + static_cast<uint32_t>(row - token * group);
+  const uint64_t at = static_cast<uint64_t>(s.first + token) * a.q_heads + h;
   const uint64_t step = static_cast<uint64_t>(a.tokens) * a.q_heads;
   float top = -INFINITY, total = 0.0f;
   F4v y{0, 0, 0, 0};
@@ -1168,7 +1175,9 @@ __global__ void __launch_bounds__(256) RowMergeKernel(Args a) {
     const int32_t token = row / group;
     const uint32_t h = blockIdx.y * a.group + static_cast<uint32_t>(row - token * group);
     MergeRow<D>(a, a.part_o, a.part_ml,
-                [&](uint32_t p) { return (2 * static_cast<uint64_t>(first + p) + (p == 0 ? 1 : 0)) * rows + static_cast<uint32_t>(row); },
+                [&](uint32_t p) {
+                  return (2 * static_cast<uint64_t>(first + p) + (p == 0 ? 1 : 0)) * rows + static_cast<uint32_t>(row);
+                },
                 last - first + 1, static_cast<uint64_t>(s.first + token) * a.q_heads + h);
     __syncthreads();
   }
@@ -1176,18 +1185,17 @@ __global__ void __launch_bounds__(256) RowMergeKernel(Args a) {
 
 // ---- Admission and launch --------------------------------------------------------------------------------------------------
 
-constexpr int TileWaves(uint32_t) { return 8; }
 constexpr uint32_t Resident(uint32_t d) {
   return d == 256 ? RowRing<256>::kResident : d == 128 ? RowRing<128>::kResident : RowRing<64>::kResident;
 }
 
 // Into how many parts the tile kernel's keys are best cut, by what its workgroups were measured to take: 12 us (16 at head_dim
 // 256) to begin and end, 1.42, 2.0 and 4.1 us for each 64 keys at head_dim 64, 128 and 256, and for more parts than one the
-// merge, 4 us, 1.5 for each part, and the partial rows once out and in at 8 TB/s (they stay in the last cache). With G tiles of all KV heads and room for R workgroups, G S / R
-// rounds follow each other: whole ones where all tiles see as many keys, any number where a causal prompt's first tiles see few.
-// Measured, us, without parts / with the S chosen here: 512 tokens behind 8,000, 32 heads over 8 of 128: 283 / 100 (4); 512
-// behind 500, 8 heads of 256 over 2: 80 / 39 (8); 3,000 alone at 256: 211 / 94 (4); four of 1,000 to 2,000 on prefixes: 176 / 141 (2) at
-// 256, and at 64, 32 heads over 8, 103 (2 parts: 124).
+// merge, 4 us, 1.5 for each part, and the partial rows once out and in at 8 TB/s (they stay in the last cache). With G tiles of
+// all KV heads and room for R workgroups, G S / R rounds follow each other: whole ones where all tiles see as many keys, any
+// number where a causal prompt's first tiles see few. Measured, us, without parts / with the S chosen here: 512 tokens behind
+// 8,000, 32 heads over 8 of 128: 283 / 100 (4); 512 behind 500, 8 heads of 256 over 2: 80 / 39 (8); 3,000 alone at 256: 211 / 94
+// (4); four of 1,000 to 2,000 on prefixes: 176 / 141 (2) at 256, and at 64, 32 heads over 8, 103 (2 parts: 124).
 uint32_t TileSplits(const RoostAmdPagedAttentionF4Params& p, uint64_t groups, uint64_t keys, uint32_t cus) {
   const uint32_t d = p.cache.head_dim;
   const double ends = d == 256 ? 16 : 12, step = d == 256 ? 4.1 : d == 128 ? 2.0 : 1.42;
@@ -1249,7 +1257,7 @@ Cut CutOf(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
   }
   c.tile_splits = 1;
   if (c.by_tile) {
-    const uint64_t rows = 32 * TileWaves(p.cache.head_dim), all = uint64_t{p.tokens} * group;
+    const uint64_t rows = 32 * kTileWaves, all = uint64_t{p.tokens} * group;
     const uint64_t longer = std::min<uint64_t>(p.batch, all / (c.row_limit + 1));  // sequences that it can have
     c.tiles = static_cast<uint32_t>(all / rows + longer);
     c.tile_splits = TileSplits(p, roost::CeilDiv(all, rows) * p.cache.kv_heads, seen(rows / group), cus);
@@ -1323,8 +1331,8 @@ RoostStatus Admit(const RoostAmdPagedAttentionF4Params& p, uint64_t& pages) {
        {roost::ExtentOf(p.q.address, p.tokens, 2 * stride, 2 * width), roost::ExtentOf(p.cache.k.address, pages * page * 16),
         roost::ExtentOf(p.cache.v.address, pages * page * 16), roost::ExtentOf(p.cache.k_scales.address, pages * page),
         roost::ExtentOf(p.cache.v_scales.address, pages * page), roost::ExtentOf(p.cu_seqlens.address, 4 * (uint64_t{p.batch} + 1)),
-        roost::ExtentOf(p.block_tables.address, 4 * p.block_tables.length), roost::ExtentOf(p.kv_lens.address, 4 * p.kv_lens.length),
-        roost::ExtentOf(p.kv_indptr.address, 4 * (uint64_t{p.batch} + 1)),
+        roost::ExtentOf(p.block_tables.address, 4 * p.block_tables.length),
+        roost::ExtentOf(p.kv_lens.address, 4 * p.kv_lens.length), roost::ExtentOf(p.kv_indptr.address, 4 * (uint64_t{p.batch} + 1)),
         roost::ExtentOf(p.sequences.address, 4 * uint64_t{p.batch})}) {
     gate.Expect(!roost::Overlap(out, other) && !roost::Overlap(lse, other), ROOST_STATUS_INVALID_ARGUMENT,
                 "output or lse overlaps an input of the call");
@@ -1333,20 +1341,20 @@ RoostStatus Admit(const RoostAmdPagedAttentionF4Params& p, uint64_t& pages) {
   return gate.status();
 }
 
-template <int D, int kWaves>
+template <int D>
 void LaunchTiles(const Args& a, const Cut& c, hipStream_t s) {
   const uint32_t grid = c.tiles * a.cache.kv_heads * c.tile_splits;
   if (a.capped) {
-    TileAttentionKernel<D, kWaves, true><<<grid, 64 * kWaves, 0, s>>>(a);
+    TileAttentionKernel<D, true><<<grid, 64 * kTileWaves, 0, s>>>(a);
   } else {
-    TileAttentionKernel<D, kWaves, false><<<grid, 64 * kWaves, 0, s>>>(a);
+    TileAttentionKernel<D, false><<<grid, 64 * kTileWaves, 0, s>>>(a);
   }
-  if (c.tile_splits > 1) TileMergeKernel<D, kWaves><<<dim3(c.tiles * a.cache.kv_heads, 32 * kWaves * D / 1024), 256, 0, s>>>(a);
+  if (c.tile_splits > 1) TileMergeKernel<D><<<dim3(c.tiles * a.cache.kv_heads, 32 * kTileWaves * D / 1024), 256, 0, s>>>(a);
 }
 
 template <int D>
 void Launch(const Args& a, const Cut& c, hipStream_t s) {
-  if (c.by_tile) LaunchTiles<D, TileWaves(D)>(a, c, s);
+  if (c.by_tile) LaunchTiles<D>(a, c, s);
   if (!c.by_row) return;
   const uint32_t grid = (c.places + 7) / 8 * 8;  // whole rounds of the dies
   if (D == 256 || c.row_tiles == 1) {
@@ -1401,7 +1409,9 @@ extern "C" ROOST_API RoostStatus roost_amd_paged_attention_f4_run(RoostContext* 
     ROOST_GATE_RETURN(roost::OnDevice(gate, ctx));
     const Cut c = CutOf(p, ctx->compute_units);
     gate.Expect(uint64_t{c.tiles} * p.cache.kv_heads * c.tile_splits < (1u << 23), ROOST_STATUS_UNSUPPORTED,
-                "%u tokens of %u heads: more tiles than one launch takes", p.tokens, p.q_heads);
+                "%u tokens of %u heads: more tiles than one launch takes", p.tokens, p.q_heads)
+        .Expect(c.places < (1u << 24) - 8, ROOST_STATUS_UNSUPPORTED, "%u sequences of %u KV heads: more than one launch takes",
+                p.batch, p.cache.kv_heads);
     ROOST_GATE_RETURN(gate);
     Args a{};
     a.q = static_cast<const uint16_t*>(p.q.address);
