@@ -1258,12 +1258,13 @@ Cut CutOf(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
   // Which kernels: sequences of up to 16 rows (32 where a token alone has more than 16) go row by row, longer ones by tiles. One
   // kernel is enough where no sequence is expected for the other; it then takes all, so an expectation that fails costs time only.
   // At head_dim 256 two tiles of 16 rows do not fit a wavefront's registers, and 32 rows take two turns.
-  const uint64_t expected = uint64_t{p.max_q_len ? std::min(p.max_q_len, p.tokens) : p.tokens} * group;
+  const uint64_t longest = p.max_q_len ? std::min(p.max_q_len, p.tokens) : p.tokens, expected = longest * group;
   c.row_tiles = p.cache.head_dim < 256 && (group > 16 || (expected > 16 && expected <= 32)) ? 2 : 1;
   const uint32_t few = std::max(16 * c.row_tiles, group);
   c.short_tokens = few / group;
   c.by_tile = expected > few;
-  c.by_row = !c.by_tile || p.batch > 1;
+  // A sequence has what the others leave of the tokens, at least. The row kernel's launches cost 8 us where it finds nothing.
+  c.by_row = !c.by_tile || p.tokens <= (p.batch - 1) * longest + c.short_tokens;
   c.row_limit = !c.by_tile ? 0x7FFFFFFF : c.by_row ? few : 0;
   if (c.by_row) {
     // As many workgroups as the chip holds at once, or one for each unit of keys where fewer are expected; one for each KV head of

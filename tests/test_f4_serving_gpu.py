@@ -257,3 +257,13 @@ def test_on_another_stream(session):
     stream.synchronize()
     a.check()
     own.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_short_sequence_that_the_hints_rule_out(session, dim):
+    """Two sequences of which max_q_len leaves neither short; one is, and one has no tokens at all."""
+    for lens in ([(1, 500), (100, 300)], [(0, 40), (90, 90)], [(3, 3), (61, 70), (64, 900)]):
+        a = fc.Attention(70, lens, dim=dim, pad=2)
+        a.hints = dict(max_q_len=40, max_kv_len=100)
+        a.run(session)
+        a.check(str(lens))
