@@ -655,8 +655,10 @@ __global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : 
 //   S^T = K Q^T with 32 keys as A and the wavefront's 32 rows as B. A lane then holds, of its row, keys 4 g + i of each 8; the
 //   products O^T = V^T P^T contract the keys in that order, so p stays in its lane, and V^T's operand (dim m, four keys twice) is
 //   read from LDS by transposing reads.
-// LDS: K rows are padded by 16 bytes, so that 16 keys' reads of 16 bytes meet no bank twice; V's 64-byte chunks are swizzled by
-// the key, and their 16-byte pieces by the next bits of it, which does the same for the transposing reads of 8 keys x 64 bytes.
+// LDS: reads of 16 bytes a lane want 16 rows' pieces apart in 256 bytes, the converted codes' stores eight lanes' apart in 128
+// (counted: eight lanes a cycle). K rows are padded by 16 bytes for the first; V's 64-byte chunks change places by the key for the
+// transposing reads of four keys x 64 bytes. The stores' eight lanes have 8 / (D / 32) keys, so pieces change places by what those
+// bits do not tell apart: no conflict is left (28% of the LDS cycles at head_dim 128 before: 639 us, now 607).
 
 constexpr int kTileWaves = 8;
 constexpr int kTileKeys = 64;
@@ -677,11 +679,19 @@ struct TileLds {
   uint32_t nan[3][kTileKeys];     // blocks of V that are NaN; only kept in a careful pass
 };
 
-// Where block `block`, piece `piece` (8 dims) of a key lies in LDS.
+// Where block `block`, piece `piece` (8 dims) of a key lies in LDS, V's and K's, and how V's pieces change places.
+template <int D>
+constexpr uint32_t SwapOf(uint32_t key, uint32_t block) {
+  return D == 64 ? key & 3 : D == 128 ? ((key ^ key >> 2) & 3) ^ (block & 2) : block >> 1;
+}
 template <int D>
 __device__ __forceinline__ uint32_t ValueAt(uint32_t key, uint32_t block, uint32_t piece) {
   const uint32_t swap = D == 64 ? key >> 1 & 1 : key & 3;
-  return key * 2 * D + ((block ^ swap) * 64) + ((piece ^ (key >> 2 & 3)) * 16);
+  return key * 2 * D + ((block ^ swap) * 64) + ((piece ^ SwapOf<D>(key, block)) * 16);
+}
+template <int D>
+__device__ __forceinline__ uint32_t KeyAt(uint32_t key, uint32_t block, uint32_t piece) {
+  return key * (2 * D + 16) + 64 * block + 16 * (D == 64 ? piece : piece ^ (block & 2)) + (D == 256 ? 16 * (block >> 2) : 0);
 }
 
 // Tile `rank` of all sequences' that have more rows than row_limit; a sequence's last tiles first, whose rows see most keys.
@@ -841,7 +851,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
       for (int j = 0; j < 4; ++j) {
         const uint32_t c = codes[j];
         const U4 x{FromF4<0>(c, scale), FromF4<1>(c, scale), FromF4<2>(c, scale), FromF4<3>(c, scale)};
-        const uint32_t off = value ? ValueAt<D>(key, block, j) : key * Lds::kKeyRow + 64 * block + 16 * j;
+        const uint32_t off = value ? ValueAt<D>(key, block, j) : KeyAt<D>(key, block, j);
         *reinterpret_cast<U4*>(to + off) = x;
       }
     }
@@ -906,7 +916,9 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
           const unsigned char* kr = kt + 32 * half * Lds::kKeyRow;
           constexpr int kAhead = 2;
           U4 ka[kAhead][kHalves];
-          const auto key = [&](int i, int x) { return *reinterpret_cast<const U4*>(kr + 32 * x * Lds::kKeyRow + 32 * i); };
+          const auto key = [&](int i, int x) {  // dims 16 i + 8 g .. of the lane's key
+            return *reinterpret_cast<const U4*>(kr + 32 * x * Lds::kKeyRow + KeyAt<D>(0, i / 2, 2 * (i % 2)));
+          };
 #pragma unroll
           for (int i = 0; i < kAhead; ++i)
 #pragma unroll
@@ -971,8 +983,8 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
 #pragma unroll
           for (int x = 0; x < kHalves; ++x) {
             const auto value = [&](int n) {  // the operand of product n: 16 keys n / kDt, dims 32 (n % kDt) ..
-              const uint32_t row = 16 * (2 * (half + x) + n / kDt) * 2 * D, d = n % kDt;
-              const U2 lo = LdsTranspose(vt, (va[0] ^ (64 * d)) + row), hi = LdsTranspose(vt, (va[1] ^ (64 * d)) + row);
+              const uint32_t row = 16 * (2 * (half + x) + n / kDt) * 2 * D, d = n % kDt, swap = 64 * d | 16 * SwapOf<D>(0, d);
+              const U2 lo = LdsTranspose(vt, (va[0] ^ swap) + row), hi = LdsTranspose(vt, (va[1] ^ swap) + row);
               return U4{lo[0], lo[1], hi[0], hi[1]};
             };
             U4 vv[kAhead];
@@ -1004,8 +1016,8 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
               o[n % kDt] = Mfma32(v, p[n / kDt], o[n % kDt]);
             }
             // At 128 the first reads come in front of the exponentials and each product in front of the reads that it leaves room
-            // for: two prompts of 3,500 to 4,096 tokens on prefixes, 32 heads over 8, take 639 us, 653 in the compiler's order. At
-            // 64 and 256 that order is as fast or faster.
+            // for: 2% (two prompts of 3,500 to 4,096 tokens on prefixes, 32 heads over 8). At 64 and 256 that order is as fast or
+            // faster.
             if constexpr (D == 128) {
 #pragma unroll
               for (int n = 0; n < 2 * kDt; ++n) {
