@@ -1221,25 +1221,29 @@ constexpr uint32_t Resident(uint32_t d) {
 }
 
 // Into how many parts the tile kernel's keys are best cut, by what its workgroups were measured to take: 12 us (16 at head_dim
-// 256) to begin and end, 1.42, 2.0 and 4.1 us for each 64 keys at head_dim 64, 128 and 256, and for more parts than one the
-// merge, 4 us, 1.5 for each part, and the partial rows once out and in at 8 TB/s (they stay in the last cache). With G tiles of
-// all KV heads and room for R workgroups, G S / R rounds follow each other: whole ones where all tiles see as many keys, any
-// number where a causal prompt's first tiles see few. Measured, us, without parts / with the S chosen here: 512 tokens behind
-// 8,000, 32 heads over 8 of 128: 283 / 100 (4); 512 behind 500, 8 heads of 256 over 2: 80 / 39 (8); 3,000 alone at 256: 211 / 94
-// (4); four of 1,000 to 2,000 on prefixes: 176 / 141 (2) at 256, and at 64, 32 heads over 8, 103 (2 parts: 124).
+// 256) to begin and end, 1.25, 2.0 and 4.1 us for each 64 keys at head_dim 64, 128 and 256 on a CU of their own (at 64 a CU holds
+// two, which then take twice as long), and for more parts than one the merge, 4 us, 0.9 for each part, and the partial rows once
+// out and in at 8 TB/s (they stay in the last cache). With G tiles of all KV heads, G S / CUs rounds follow each other: whole ones
+// where all tiles see as many keys, any number where a causal prompt's first tiles see few. Parts are whole 64 keys, so only an S
+// that they come out at counts. Measured, us, without parts / with the S chosen here: 512 tokens behind 8,000, 32 heads over 8 of
+// 128: 283 / 94 (4); 512 behind 500, 8 heads of 256 over 2: 80 / 38 (8); two of 100 behind 8,000, 32 heads over 8 of 64: 38 (8;
+// 4 parts 56, 12 parts 44); 3,000 alone at 256: 211 / 93 (4); four of 1,000 to 2,000 on prefixes: 176 / 132 (2) at 256, and at 64,
+// 32 heads over 8, 97 (2 parts: 124).
 uint32_t TileSplits(const RoostAmdPagedAttentionF4Params& p, uint64_t groups, uint64_t keys, uint32_t cus) {
   const uint32_t d = p.cache.head_dim;
-  const double ends = d == 256 ? 16 : 12, step = d == 256 ? 4.1 : d == 128 ? 2.0 : 1.42;
-  const double room = d == 64 ? 2.0 * cus : cus, steps = std::max(1.0, keys / 64.0);
+  const double ends = d == 256 ? 16 : 12, step = d == 256 ? 4.1 : d == 128 ? 2.0 : 1.25;
+  const uint64_t steps = roost::CeilDiv(keys, kTileKeys);
   const double fresh = p.causal ? std::min<double>(p.max_q_len ? p.max_q_len : p.tokens, keys) : 0;
   const double mean = 1 - fresh / (2.0 * keys);  // of the keys that the last tile sees, what a tile does
   const double row_us = double(p.tokens) * p.q_heads * d * 8 / 8e6;
   uint32_t best = 1;
   double least = 0;
-  for (uint32_t s = 1; s <= 16 && (s == 1 || keys >= 128 * s); ++s) {
-    const double rounds = std::max(1.0, groups * s / room), one = ends + step * steps / s;
-    const double alike = std::ceil(rounds) * one, unlike = std::max(one, rounds * (ends + step * steps / s * mean));
-    const double us = (2 * mean - 1) * alike + (2 - 2 * mean) * unlike + (s > 1 ? 4 + s * (1.5 + row_us) : 0);
+  for (uint32_t s = 1; s <= 16; ++s) {
+    const uint64_t part = roost::CeilDiv(steps, s);
+    if (roost::CeilDiv(steps, part) != s) continue;
+    const double rounds = std::max(1.0, double(groups) * s / cus), one = ends + step * part;
+    const double alike = std::ceil(rounds) * one, unlike = std::max(one, rounds * (ends + step * part * mean));
+    const double us = (2 * mean - 1) * alike + (2 - 2 * mean) * unlike + (s > 1 ? 4 + s * (0.9 + row_us) : 0);
     if (s == 1 || us < least) best = s, least = us;
   }
   return best;
