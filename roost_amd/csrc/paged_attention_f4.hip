@@ -1303,6 +1303,7 @@ Cut CutOf(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
 }
 
 uint64_t WorkspaceBytes(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
+  if (p.tokens == 0 || p.batch == 0) return 0;
   const Cut c = CutOf(p, cus);
   return (c.rows + c.tile_rows) * (p.cache.head_dim + 2) * 4 + (c.merge ? 4 * (uint64_t{p.batch} + 1) : 0);
 }
