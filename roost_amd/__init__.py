@@ -864,7 +864,7 @@ def _pools(pools):
     if not pools:
         raise ValueError("pools: none given")
     found = (abi.PagePool * len(pools))()
-    pages = pools[0].shape[1]
+    pages = pools[0].shape[1] if pools[0].dim() > 1 else "pages"
     for i, t in enumerate(pools):
         if t.dim() < 2 or t.shape[1] != pages:
             raise ValueError(f"pool {i}: shape {tuple(t.shape)}, not [layers, {pages}, ...]")

@@ -1302,10 +1302,15 @@ Cut CutOf(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
   return c;
 }
 
-uint64_t WorkspaceBytes(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
-  if (p.tokens == 0 || p.batch == 0) return 0;
-  const Cut c = CutOf(p, cus);
+uint64_t WorkspaceBytes(const RoostAmdPagedAttentionF4Params& p, const Cut& c) {
   return (c.rows + c.tile_rows) * (p.cache.head_dim + 2) * 4 + (c.merge ? 4 * (uint64_t{p.batch} + 1) : 0);
+}
+
+void AdmitLaunch(roost::Gate& gate, const RoostAmdPagedAttentionF4Params& p, const Cut& c) {
+  gate.Expect(uint64_t{c.tiles} * p.cache.kv_heads * c.tile_splits < (1u << 23), ROOST_STATUS_UNSUPPORTED,
+              "%u tokens of %u heads: more tiles than one launch takes", p.tokens, p.q_heads)
+      .Expect(c.places < (1u << 24) - 8, ROOST_STATUS_UNSUPPORTED, "%u sequences of %u KV heads: more than one launch takes",
+              p.batch, p.cache.kv_heads);
 }
 
 RoostStatus Admit(const RoostAmdPagedAttentionF4Params& p, uint64_t& pages) {
@@ -1421,7 +1426,13 @@ extern "C" ROOST_API RoostStatus roost_amd_paged_attention_f4_workspace(RoostCon
   return roost::CatchAll(kOp, [&]() -> RoostStatus {
     uint64_t pages = 0;
     ROOST_RETURN_IF_FAILED(Admit(p, pages));
-    sizes->device_bytes = WorkspaceBytes(p, ctx->compute_units);
+    sizes->device_bytes = 0;
+    if (p.tokens > 0 && p.batch > 0) {
+      const Cut c = CutOf(p, ctx->compute_units);
+      AdmitLaunch(gate, p, c);
+      ROOST_GATE_RETURN(gate);
+      sizes->device_bytes = WorkspaceBytes(p, c);
+    }
     sizes->pinned_host_bytes = sizes->plan_bytes = 0;
     sizes->device_alignment = 256;
     return ROOST_STATUS_OK;
@@ -1438,18 +1449,15 @@ extern "C" ROOST_API RoostStatus roost_amd_paged_attention_f4_run(RoostContext* 
   return roost::CatchAll(kOp, [&]() -> RoostStatus {
     uint64_t pages = 0;
     ROOST_RETURN_IF_FAILED(Admit(p, pages));
-    const uint64_t bytes = WorkspaceBytes(p, ctx->compute_units);
+    if (p.tokens == 0 || p.batch == 0) return ROOST_STATUS_OK;
+    const Cut c = CutOf(p, ctx->compute_units);
+    AdmitLaunch(gate, p, c);
+    ROOST_GATE_RETURN(gate);
+    const uint64_t bytes = WorkspaceBytes(p, c);
     gate.Expect(roost::HasDeviceRegion(ws, bytes), ROOST_STATUS_WORKSPACE_TOO_SMALL,
                 "the call needs %llu bytes of 256-byte aligned device workspace", static_cast<unsigned long long>(bytes));
     ROOST_GATE_RETURN(gate);
-    if (p.tokens == 0 || p.batch == 0) return ROOST_STATUS_OK;
     ROOST_GATE_RETURN(roost::OnDevice(gate, ctx));
-    const Cut c = CutOf(p, ctx->compute_units);
-    gate.Expect(uint64_t{c.tiles} * p.cache.kv_heads * c.tile_splits < (1u << 23), ROOST_STATUS_UNSUPPORTED,
-                "%u tokens of %u heads: more tiles than one launch takes", p.tokens, p.q_heads)
-        .Expect(c.places < (1u << 24) - 8, ROOST_STATUS_UNSUPPORTED, "%u sequences of %u KV heads: more than one launch takes",
-                p.batch, p.cache.kv_heads);
-    ROOST_GATE_RETURN(gate);
     Args a{};
     a.q = static_cast<const uint16_t*>(p.q.address);
     a.out = static_cast<uint16_t*>(p.output.address);

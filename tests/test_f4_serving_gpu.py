@@ -267,3 +267,41 @@ def test_a_short_sequence_that_the_hints_rule_out(session, dim):
         a.hints = dict(max_q_len=40, max_kv_len=100)
         a.run(session)
         a.check(str(lens))
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(96, 48, 64), (72, 24, 128), (130, 130, 64), (40, 40, 256)])
+def test_many_heads(session, q_heads, kv_heads, dim):
+    a = fc.Attention(80, [(1, 300), (2, 17), (90, 140), (1, 1)], q_heads=q_heads, kv_heads=kv_heads, dim=dim)
+    a.run(session)
+    a.check()
+
+
+def test_a_sequence_named_twice(session):
+    """Two entries of a batch may ask the same sequence."""
+    a = fc.Attention(81, [(1, 700), (4, 700), (60, 700)], dim=128)
+    a.sequences = a.i32([1, 1, 1])
+    a.page_ids = [a.page_ids[1]] * 3
+    a.run(session)
+    a.check()
+
+
+def test_two_calls_at_once(session):
+    """Two sessions, a stream and a workspace each, on the same cache; neither waits for the other."""
+    made = []
+    for i in range(2):
+        stream = torch.cuda.Stream()
+        a = fc.Attention(82, [(1, 9000), (64, 2000), (1, 40)], dim=128)
+        if i:
+            a.q.copy_(torch.randn(a.q.shape, generator=a.g, device="cuda"))
+            a.cache = made[0][1].cache
+        made.append((roost_amd.OpSession(session.lib, device=0, stream=stream), a, a.params()))
+    for own, _, p in made:
+        roost_amd.paged_attention_f4_workspace(own, p)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for own, _, p in made:
+            roost_amd.paged_attention_f4(own, p)
+    torch.cuda.synchronize()
+    for own, a, _ in made:
+        a.check()
+        own.close()
