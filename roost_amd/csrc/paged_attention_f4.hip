@@ -643,11 +643,12 @@ __global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : 
 }
 
 // ---- The tile kernel ----------------------------------------------------------------------------------------------------------
-// 256 rows of one sequence and KV head (rows are its tokens' query heads, token by token) against the keys that they see, 64 at a
-// time: prompt chunks. Bound by the matrix instructions and, beside them, by LDS reads and the softmax.
+// 256 rows of one sequence and KV head (rows are its tokens' query heads, token by token) against the keys that they see, 64 or
+// 128 at a time: prompt chunks. Bound by the matrix instructions and, beside them, by the softmax and LDS reads: 1.0 PFLOP/s over
+// two prompts of 3,500 to 4,096 tokens on prefixes, 32 heads over 8 of 128.
 //
 // A tile's codes go to LDS as bf16 once for all wavefronts, a lane a block of 32 dims (16 bytes, one scale): 16 conversions a lane
-// and tile at head_dim 128 and 256 rows, where converting in each wavefront would take 128. Codes of the next tile are under way
+// for 64 keys at head_dim 128, where converting in each wavefront would take 128. Codes of the next tile are under way
 // during a tile's products, straight into LDS, where each lane finds its own again: held in registers they would not fit beside
 // 32 rows' queries and sums at head_dim 256. LDS holds two converted tiles, so there is one barrier a tile.
 //
@@ -661,22 +662,22 @@ __global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : 
 // bits do not tell apart: no conflict is left (28% of the LDS cycles at head_dim 128 before: 639 us, now 607).
 
 constexpr int kTileWaves = 8;
-constexpr int kTileKeys = 64;
+constexpr int kTileKeys = 64;  // what a tile's keys are cut into parts by
 
 __device__ __forceinline__ U2 LdsTranspose(const unsigned char* base, uint32_t off) {
   auto* p = reinterpret_cast<__attribute__((address_space(3))) I4h*>(const_cast<LdsByte*>((const LdsByte*)base + off));
   return __builtin_bit_cast(U2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
 }
 
-template <int D, int kPieces>
+template <int D, int kKeys, int kPieces>
 struct TileLds {
   static constexpr int kKeyRow = 2 * D + 16;
-  unsigned char k[2][kTileKeys * kKeyRow];
-  unsigned char v[2][kTileKeys * 2 * D];
+  unsigned char k[2][kKeys * kKeyRow];
+  unsigned char v[2][kKeys * 2 * D];
   U4 codes[kTileWaves][kPieces][64];        // of the next tile, a block a lane
   uint32_t scales[kTileWaves][kPieces][64];
   uint32_t bad[3];                // groups of 16 keys without a page, of this tile, the next and the one after
-  uint32_t nan[3][kTileKeys];     // blocks of V that are NaN; only kept in a careful pass
+  uint32_t nan[3][kKeys];     // blocks of V that are NaN; only kept in a careful pass
 };
 
 // Where block `block`, piece `piece` (8 dims) of a key lies in LDS, V's and K's, and how V's pieces change places.
@@ -741,8 +742,12 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
   constexpr int kThreads = 64 * kTileWaves, kRows = 32 * kTileWaves;
   constexpr int kKs = D / 16, kDt = D / 32;
   constexpr int kHalves = D == 64 ? 2 : 1;  // of a tile's keys that are scored together (at 128 the registers of two cost 1%)
-  constexpr int kPieces = (4 * D + kThreads - 1) / kThreads;  // blocks of 32 codes that a lane stages
-  typedef TileLds<D, kPieces> Lds;
+  // Keys at a time: as many as LDS holds twice (at 64 beside a second workgroup). 128 instead of 64 at head_dim 128, half the
+  // barriers: 606 -> 566 us for two prompts of 3,500 to 4,096 tokens on prefixes, 166 -> 147 for four of 2,000 to 4,000.
+  constexpr int kKeys = D == 128 ? 128 : 64;
+  constexpr int kBlocks = kKeys * D / 32;     // of K's, and of V's, of a tile
+  constexpr int kPieces = (2 * kBlocks + kThreads - 1) / kThreads;  // blocks of 32 codes that a lane stages
+  typedef TileLds<D, kKeys, kPieces> Lds;
   __shared__ __attribute__((aligned(16))) Lds lds;
 
   const uint32_t head = blockIdx.x % a.cache.kv_heads, split = blockIdx.x / a.cache.kv_heads % a.tile_splits;
@@ -756,7 +761,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
   if (split >= range.parts) return;
   const int32_t k0 = range.begin + static_cast<int32_t>(split) * range.part;
   const int32_t k1 = min(range.end, k0 + range.part);
-  const int32_t tiles = k1 > k0 ? (k1 - k0 + kTileKeys - 1) / kTileKeys : 0;
+  const int32_t tiles = k1 > k0 ? (k1 - k0 + kKeys - 1) / kKeys : 0;
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -790,10 +795,10 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
   const uint32_t shift = a.cache.page_shift, in_page = (1u << shift) - 1;
   const auto piece_of = [&](int i, int id, bool& value, int32_t& key, uint32_t& block) {
     const int p = id + i * kThreads;
-    value = p >= 2 * D;
-    key = (p & (2 * D - 1)) / (D / 32);
+    value = p >= kBlocks;
+    key = (p & (kBlocks - 1)) / (D / 32);
     block = static_cast<uint32_t>(p) & (D / 32 - 1);
-    return p < 4 * D;
+    return p < 2 * kBlocks;
   };
   int32_t ids[kPieces];
   uint32_t none = 0;  // pieces of the tile under way that have no page
@@ -805,7 +810,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
       uint32_t block;
       ids[i] = -1;
       if (!piece_of(i, id, value, key, block) || t >= tiles) continue;
-      const int32_t k = k0 + t * kTileKeys + key, entry = k >> shift;
+      const int32_t k = k0 + t * kKeys + key, entry = k >> shift;
       if ((k & ~15) < k1 && entry < s.blocks) ids[i] = a.tables[s.entry + entry];
     }
   };
@@ -819,7 +824,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
       if (!piece_of(i, id, value, key, block)) continue;
       int32_t page = D == 64 ? ids[i] : __builtin_amdgcn_readfirstlane(ids[i]);
       if (static_cast<uint32_t>(page) >= a.cache.pages) none |= 1u << i, page = 0;  // masked: any codes will do
-      const uint32_t within = static_cast<uint32_t>(k0 + t * kTileKeys + key) & in_page;
+      const uint32_t within = static_cast<uint32_t>(k0 + t * kKeys + key) & in_page;
       const uint64_t head_page = static_cast<uint64_t>(page) * a.cache.kv_heads + head;
       Copy16((value ? a.cache.v : a.cache.k) + ((head_page << shift) + within) * (D / 2) + 16 * block, LdsAddress(lds.codes[w][i]));
       Copy1((value ? a.cache.v_scales : a.cache.k_scales) + ((head_page * (D / 32) + block) << shift) + within,
@@ -839,7 +844,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
       const U4 codes = lds.codes[w][i][id & 63];
       uint32_t byte = lds.scales[w][i][id & 63];
       if (value) {
-        if ((none >> i & 1) || k0 + t * kTileKeys + key >= k1) byte = 127;  // whatever lies there: finite, times p = 0
+        if ((none >> i & 1) || k0 + t * kKeys + key >= k1) byte = 127;  // whatever lies there: finite, times p = 0
         if (careful && byte > kF4ByteHigh) {
           byte = 127;
           atomicOr(&lds.nan[slot][key], 1u << block);
@@ -867,7 +872,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
 #pragma unroll
       for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
     if (tid < 3) lds.bad[tid] = 0;
-    if (careful && tid < 64) lds.nan[0][tid] = lds.nan[1][tid] = lds.nan[2][tid] = 0;
+    if (careful && tid < kKeys) lds.nan[0][tid] = lds.nan[1][tid] = lds.nan[2][tid] = 0;
     __syncthreads();
     if (tiles > 0) {
       load_ids(0, tid);
@@ -886,15 +891,15 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
       if constexpr (D != 128) asm volatile("" : "+v"(tid));
       const int lane = tid & 63, m = lane & 31, g = lane >> 5;
       if (tid == 0) lds.bad[after] = 0;
-      if (careful && tid < 64) lds.nan[after][tid] = 0;
+      if (careful && tid < kKeys) lds.nan[after][tid] = 0;
       if (t + 1 < tiles) {
         load_codes(t + 1, tid);
         load_ids(t + 2, tid);
       }
-      const int32_t kb = k0 + t * kTileKeys;
+      const int32_t kb = k0 + t * kKeys;
       if (!idle && !(a.causal && kb > high)) {
         const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(lds.bad[slot])));
-        const bool mask = kb + kTileKeys > k1 || (a.causal && kb + kTileKeys - 1 > low) || bad != 0 ||
+        const bool mask = kb + kKeys > k1 || (a.causal && kb + kKeys - 1 > low) || bad != 0 ||
                           (a.window >= 0 && kb < high - a.window);
         const unsigned char* kt = lds.k[t & 1] + m * Lds::kKeyRow + 16 * g;
         const unsigned char* vt = lds.v[t & 1];
@@ -903,9 +908,9 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
         uint32_t va[2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) va[f] = ValueAt<D>(key4 + 8 * f, 0, piece) + 8 * (j & 1);
-#pragma unroll
-        for (int half = 0; half < 2; half += kHalves) {
-          if (kHalves == 1 && a.causal && kb + 32 * half > high) break;
+#pragma unroll (D == 256 ? 1 : kKeys / 32)  // at 256, by 3% faster so: fewer registers are kept over both halves
+        for (int half = 0; half < kKeys / 32; half += kHalves) {
+          if (half > 0 && (kb + 32 * half >= k1 || (a.causal && kb + 32 * half > high))) break;
           F16v sc[kHalves];
 #pragma unroll
           for (int x = 0; x < kHalves; ++x)
@@ -1221,7 +1226,7 @@ constexpr uint32_t Resident(uint32_t d) {
 }
 
 // Into how many parts the tile kernel's keys are best cut, by what its workgroups were measured to take: 12 us (16 at head_dim
-// 256) to begin and end, 1.25, 2.0 and 4.1 us for each 64 keys at head_dim 64, 128 and 256 on a CU of their own (at 64 a CU holds
+// 256) to begin and end, 1.25, 1.8 and 4.1 us for each 64 keys at head_dim 64, 128 and 256 on a CU of their own (at 64 a CU holds
 // two, which then take twice as long), and for more parts than one the merge, 4 us, 0.9 for each part, and the partial rows once
 // out and in at 8 TB/s (they stay in the last cache). With G tiles of all KV heads, G S / CUs rounds follow each other: whole ones
 // where all tiles see as many keys, any number where a causal prompt's first tiles see few. Parts are whole 64 keys, so only an S
@@ -1231,7 +1236,7 @@ constexpr uint32_t Resident(uint32_t d) {
 // 32 heads over 8, 97 (2 parts: 124).
 uint32_t TileSplits(const RoostAmdPagedAttentionF4Params& p, uint64_t groups, uint64_t keys, uint32_t cus) {
   const uint32_t d = p.cache.head_dim;
-  const double ends = d == 256 ? 16 : 12, step = d == 256 ? 4.1 : d == 128 ? 2.0 : 1.25;
+  const double ends = d == 256 ? 16 : 12, step = d == 256 ? 4.1 : d == 128 ? 1.8 : 1.25;
   const uint64_t steps = roost::CeilDiv(keys, kTileKeys);
   const double fresh = p.causal ? std::min<double>(p.max_q_len ? p.max_q_len : p.tokens, keys) : 0;
   const double mean = 1 - fresh / (2.0 * keys);  // of the keys that the last tile sees, what a tile does
