@@ -742,9 +742,10 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
   constexpr int kThreads = 64 * kTileWaves, kRows = 32 * kTileWaves;
   constexpr int kKs = D / 16, kDt = D / 32;
   constexpr int kHalves = D == 64 ? 2 : 1;  // of a tile's keys that are scored together (at 128 the registers of two cost 1%)
-  // Keys at a time: as many as LDS holds twice (at 64 beside a second workgroup). 128 instead of 64 at head_dim 128, half the
-  // barriers: 606 -> 566 us for two prompts of 3,500 to 4,096 tokens on prefixes, 166 -> 147 for four of 2,000 to 4,000.
-  constexpr int kKeys = D == 128 ? 128 : 64;
+  // Keys at a time: as many as LDS holds twice, two workgroups' at head_dim 64. 128 instead of 64, half the barriers: 606 -> 566 us
+  // for two prompts of 3,500 to 4,096 tokens on prefixes at 128, 166 -> 147 for four of 2,000 to 4,000; 96 -> 92 for four of 1,000
+  // to 2,000 at 64.
+  constexpr int kKeys = D == 256 ? 64 : 128;
   constexpr int kBlocks = kKeys * D / 32;     // of K's, and of V's, of a tile
   constexpr int kPieces = (2 * kBlocks + kThreads - 1) / kThreads;  // blocks of 32 codes that a lane stages
   typedef TileLds<D, kKeys, kPieces> Lds;
@@ -776,6 +777,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
   // Positions of the wavefront's first and last row.
   const int32_t low = before + (tile * kRows + 32 * w) / group;
   const int32_t high = before + min((tile * kRows + 32 * w + 31) / group, s.count - 1);
+  const int32_t last = a.causal ? min(high, k1 - 1) : k1 - 1;  // the last key of the part that its rows see
   const bool idle = tile * kRows + 32 * w >= rows;  // the wavefront has no row, and only stages
 
   U4 q[kKs];
@@ -897,7 +899,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
         load_ids(t + 2, tid);
       }
       const int32_t kb = k0 + t * kKeys;
-      if (!idle && !(a.causal && kb > high)) {
+      if (!idle && kb <= last) {
         const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(lds.bad[slot])));
         const bool mask = kb + kKeys > k1 || (a.causal && kb + kKeys - 1 > low) || bad != 0 ||
                           (a.window >= 0 && kb < high - a.window);
@@ -910,7 +912,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
         for (int f = 0; f < 2; ++f) va[f] = ValueAt<D>(key4 + 8 * f, 0, piece) + 8 * (j & 1);
 #pragma unroll (D == 256 ? 1 : kKeys / 32)  // at 256, by 3% faster so: fewer registers are kept over both halves
         for (int half = 0; half < kKeys / 32; half += kHalves) {
-          if (half > 0 && (kb + 32 * half >= k1 || (a.causal && kb + 32 * half > high))) break;
+          if (half > 0 && kb + 32 * half > last) break;
           F16v sc[kHalves];
 #pragma unroll
           for (int x = 0; x < kHalves; ++x)
