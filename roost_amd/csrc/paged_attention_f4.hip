@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : 
 // LDS: reads of 16 bytes a lane want 16 rows' pieces apart in 256 bytes, the converted codes' stores eight lanes' apart in 128
 // (counted: eight lanes a cycle). K rows are padded by 16 bytes for the first; V's 64-byte chunks change places by the key for the
 // transposing reads of four keys x 64 bytes. The stores' eight lanes have 8 / (D / 32) keys, so pieces change places by what those
-// bits do not tell apart: no conflict is left (28% of the LDS cycles at head_dim 128 before: 639 us, now 607).
+// bits do not tell apart: no conflict is left (28% of the LDS cycles at head_dim 128 before; 5% of the time).
 
 constexpr int kTileWaves = 8;
 constexpr int kTileKeys = 64;  // what a tile's keys are cut into parts by
@@ -888,7 +888,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
       const int slot = t % 3, after = (t + 2) % 3;
       // What depends on the lane is made anew from its number each time: kept, it would not fit the registers at head_dim 256,
       // and at 64 leave room for one workgroup a CU instead of two (four prompts of 1,000 to 2,000 tokens on prefixes, 32 heads
-      // over 8: 105 us, kept 125). At 128 there is room, and it is kept (655 us; anew 720).
+      // over 8: 105 us, kept 125). At 128 there is room, and it is kept (544 us; anew 620).
       int tid = threadIdx.x;
       if constexpr (D != 128) asm volatile("" : "+v"(tid));
       const int lane = tid & 63, m = lane & 31, g = lane >> 5;
@@ -1229,7 +1229,7 @@ constexpr uint32_t Resident(uint32_t d) {
 
 // Into how many parts the tile kernel's keys are best cut, by what its workgroups were measured to take: 12 us (16 at head_dim
 // 256) to begin and end, 1.25, 1.8 and 4.1 us for each 64 keys at head_dim 64, 128 and 256 on a CU of their own (at 64 a CU holds
-// two, which then take twice as long), and for more parts than one the merge, 4 us, 0.9 for each part, and the partial rows once
+// two, which then take twice as long), and for more parts than one the merge, 4 us, 0.97 for each part, and the partial rows once
 // out and in at 8 TB/s (they stay in the last cache). With G tiles of all KV heads, G S / CUs rounds follow each other: whole ones
 // where all tiles see as many keys, any number where a causal prompt's first tiles see few. Parts are whole 64 keys, so only an S
 // that they come out at counts. Measured, us, without parts / with the S chosen here: 512 tokens behind 8,000, 32 heads over 8 of
@@ -1250,7 +1250,7 @@ uint32_t TileSplits(const RoostAmdPagedAttentionF4Params& p, uint64_t groups, ui
     if (roost::CeilDiv(steps, part) != s) continue;
     const double rounds = std::max(1.0, double(groups) * s / cus), one = ends + step * part;
     const double alike = std::ceil(rounds) * one, unlike = std::max(one, rounds * (ends + step * part * mean));
-    const double us = (2 * mean - 1) * alike + (2 - 2 * mean) * unlike + (s > 1 ? 4 + s * (0.9 + row_us) : 0);
+    const double us = (2 * mean - 1) * alike + (2 - 2 * mean) * unlike + (s > 1 ? 4 + s * (0.97 + row_us) : 0);
     if (s == 1 || us < least) best = s, least = us;
   }
   return best;
