@@ -188,8 +188,13 @@ struct RowRing {
   static constexpr int kStage = 2 * kCodes + kScales;
   static constexpr int kCopies = 2 * kCodes / 1024 + kScales / 256;
   static constexpr int kStages = D == 256 ? 2 : 3;
-  static constexpr int kResident = D == 256 ? 2 : D == 128 ? 3 : 4;  // workgroups a CU holds: LDS and registers
 };
+
+// Workgroups of the row kernel that a CU holds, which its launch bounds ask for and the host deals the keys to. One tile of rows: 4,
+// 3 and 2 at head_dim 64, 128 and 256, by LDS (29, 54 and 71 KB) and registers (128, 167 and 215); two tiles: 2, by registers (174
+// and 230). Dealt to more than it holds, a second round follows: 64 sequences of 5 tokens and 500 to 16,000 keys, 32 heads over 8 of
+// 128, take 192 us, dealt to 3 a CU 206; a token of 32 heads a KV head 65 against 80.
+constexpr uint32_t RowsResident(uint32_t d, uint32_t tiles) { return tiles == 2 || d == 256 ? 2 : d == 128 ? 3 : 4; }
 
 // The memory that p points at in each lane to LDS, 16 (or 4) bytes a lane, one behind the other from `lds` on. M0 is read
 // a wait state after its write.
@@ -216,7 +221,7 @@ __device__ __forceinline__ uint32_t LdsAddress(const void* p) {
 }
 
 template <int D, int kTiles, bool kCap>
-__global__ void __launch_bounds__(64 * kRowWaves, kTiles == 2 || D == 256 ? 2 : D == 128 ? 3 : 4) RowAttentionKernel(Args a) {
+__global__ void __launch_bounds__(64 * kRowWaves, RowsResident(D, kTiles)) RowAttentionKernel(Args a) {
   typedef RowRing<D> Ring;
   constexpr int kWords = D / 32;   // of a lane's key
   constexpr int kDt = D / 16;      // dims of a lane's V word(s): products of 16 dims each
@@ -1223,10 +1228,6 @@ __global__ void __launch_bounds__(256) RowMergeKernel(Args a) {
 
 // ---- Admission and launch --------------------------------------------------------------------------------------------------
 
-constexpr uint32_t Resident(uint32_t d) {
-  return d == 256 ? RowRing<256>::kResident : d == 128 ? RowRing<128>::kResident : RowRing<64>::kResident;
-}
-
 // Into how many parts the tile kernel's keys are best cut, by what its workgroups were measured to take: 12 us (16 at head_dim
 // 256) to begin and end, 1.25, 1.8 and 4.1 us for each 64 keys at head_dim 64, 128 and 256 on a CU of their own (at 64 a CU holds
 // two, which then take twice as long), and for more parts than one the merge, 4 us, 0.97 for each part, and the partial rows once
@@ -1294,7 +1295,8 @@ Cut CutOf(const RoostAmdPagedAttentionF4Params& p, uint32_t cus) {
     // a batch that is too large to be dealt.
     const uint64_t least = uint64_t{p.batch} * p.cache.kv_heads, units = roost::CeilDiv(seen(c.short_tokens), kUnit);
     c.merge = p.batch <= kMaxScheduled;
-    c.places = static_cast<uint32_t>(c.merge ? std::min(uint64_t{cus} * Resident(p.cache.head_dim), least * units) : least);
+    const uint64_t held = uint64_t{cus} * RowsResident(p.cache.head_dim, c.row_tiles);
+    c.places = static_cast<uint32_t>(c.merge ? std::min(held, least * units) : least);
     c.merge_rows = std::min(c.short_tokens, p.max_q_len ? p.max_q_len : c.short_tokens) * group;
     c.rows = c.merge ? 2 * uint64_t{c.places} * c.short_tokens * group : 0;
   }
