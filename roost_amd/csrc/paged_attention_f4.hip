@@ -5,6 +5,8 @@
 // for each 32 dims, and become bf16 exactly (v_cvt_scalef32_pk_bf16_fp4, two codes an instruction, the scale included), so the
 // products are those of the bf16 matrix instructions with f32 sums. Each p is rounded to bf16 once in front of its product.
 
+#include <cfloat>
+#include <cmath>
 #include <initializer_list>
 #include <type_traits>
 
@@ -33,11 +35,28 @@ __device__ __forceinline__ F16v Mfma32(U4 a, U4 b, F16v c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(B8, a), __builtin_bit_cast(B8, b), c, 0, 0, 0);
 }
 
-struct SoftCap {  // cap tanh(s / cap) in log2 units: capl - 2 capl / (1 + 2^(k y)), y the scaled score
-  float capl, k;
+// cap tanh(s / cap) in log2 units, y the scaled score. What a kernel is built with:
+//   kNearCap, caps up to 128: capl - 2 capl / (1 + 2^(k y)), off by at most 8 2^-23 cap whatever the score: 1.3e-4, below what rounding
+//     p to bf16 makes of a score.
+//   kFarCap, above: that would lose the score itself (0.02 at a cap of 1e5). With z = |y| / capl up to 1/4 y times a polynomial in
+//     z^2, tanh(z) / z to 4e-9 (fitted for the least largest error), from there on as near: off by at most 16 2^-23 of the score.
+//     A kernel of its own, for three times the instructions and more registers: a prompt chunk of 3,500 tokens on 500, 32 heads over 8
+//     of 128, takes 265 us, with a near cap 195, with none 142; a decode batch 133, 127 and 122.
+enum Cap : int { kNoCap, kNearCap, kFarCap };
+constexpr float kNearMost = 128.0f;  // the largest cap of kNearCap
+struct SoftCap {
+  float capl, k;  // k: 2 / cap, for kFarCap 1 / capl
 };
+template <int kCap>
 __device__ __forceinline__ float Capped(float y, SoftCap c) {
-  return c.capl - 2.0f * c.capl * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * c.k));
+  if constexpr (kCap == kNearCap) {
+    return c.capl - 2.0f * c.capl * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y * c.k));
+  } else {
+    const float z = fabsf(y) * c.k, z2 = z * z;
+    const float little = y * fmaf(z2, fmaf(z2, fmaf(z2, -0.05143305f, 0.13324264f), -0.33333242f), 1.0f);
+    const float much = c.capl * fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * 2.88539008f)), 1.0f);
+    return z <= 0.25f ? little : copysignf(much, y);
+  }
 }
 
 struct Args {
@@ -50,7 +69,7 @@ struct Args {
   uint32_t batch, tokens, q_heads, group, table_rows, max_blocks;
   float scale_log2;  // of the scores, times log2(e)
   SoftCap cap;
-  uint32_t capped, causal;
+  uint32_t causal;
   int32_t window;
   // How the work is cut.
   float *part_o, *part_ml;   // the row kernel's partial rows: sums before division, and (maximum, sum)
@@ -220,7 +239,7 @@ __device__ __forceinline__ uint32_t LdsAddress(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const LdsByte*)p));
 }
 
-template <int D, int kTiles, bool kCap>
+template <int D, int kTiles, int kCap>
 __global__ void __launch_bounds__(64 * kRowWaves, RowsResident(D, kTiles)) RowAttentionKernel(Args a) {
   typedef RowRing<D> Ring;
   constexpr int kWords = D / 32;   // of a lane's key
@@ -475,7 +494,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, RowsResident(D, kTiles)) RowAt
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               y[j] = sc[n][j / 4][j % 4];
-              if constexpr (kCap) y[j] = Capped(y[j] * a.scale_log2, a.cap);
+              if constexpr (kCap != kNoCap) y[j] = Capped<kCap>(y[j] * a.scale_log2, a.cap);
             }
             if (mask) {
 #pragma unroll
@@ -486,7 +505,7 @@ __global__ void __launch_bounds__(64 * kRowWaves, RowsResident(D, kTiles)) RowAt
                 y[j] = off ? -INFINITY : y[j];
               }
             }
-            const float scale = kCap ? 1.0f : a.scale_log2;  // positive: the largest score stays the largest
+            const float scale = kCap != kNoCap ? 1.0f : a.scale_log2;  // positive: the largest score stays the largest
             float mx = y[0];
 #pragma unroll
             for (int j = 1; j < 8; ++j) mx = fmaxf(mx, y[j]);
@@ -742,7 +761,7 @@ __device__ __forceinline__ TileKeys KeysOfTile(const Args& a, const Sequence& s,
   return k;
 }
 
-template <int D, bool kCap>
+template <int D, int kCap>
 __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttentionKernel(Args a) {
   constexpr int kThreads = 64 * kTileWaves, kRows = 32 * kTileWaves;
   constexpr int kKs = D / 16, kDt = D / 32;
@@ -950,11 +969,11 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
           }
           __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kHalves, 0);
-          if constexpr (kCap) {
+          if constexpr (kCap != kNoCap) {
 #pragma unroll
             for (int x = 0; x < kHalves; ++x)
 #pragma unroll
-              for (int v = 0; v < 16; ++v) sc[x][v] = Capped(sc[x][v] * a.scale_log2, a.cap);
+              for (int v = 0; v < 16; ++v) sc[x][v] = Capped<kCap>(sc[x][v] * a.scale_log2, a.cap);
           }
           if (mask) {
             int32_t token;
@@ -972,7 +991,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
                 sc[x][v] = off ? -INFINITY : sc[x][v];
               }
           }
-          const float scale = kCap ? 1.0f : a.scale_log2;
+          const float scale = kCap != kNoCap ? 1.0f : a.scale_log2;
           float mx = sc[0][0];
 #pragma unroll
           for (int x = 0; x < kHalves; ++x)
@@ -1392,29 +1411,19 @@ RoostStatus Admit(const RoostAmdPagedAttentionF4Params& p, uint64_t& pages) {
   return gate.status();
 }
 
-template <int D>
-void LaunchTiles(const Args& a, const Cut& c, hipStream_t s) {
-  const uint32_t grid = c.tiles * a.cache.kv_heads * c.tile_splits;
-  if (a.capped) {
-    TileAttentionKernel<D, true><<<grid, 64 * kTileWaves, 0, s>>>(a);
-  } else {
-    TileAttentionKernel<D, false><<<grid, 64 * kTileWaves, 0, s>>>(a);
-  }
-  if (c.tile_splits > 1) TileMergeKernel<D><<<dim3(c.tiles * a.cache.kv_heads, 32 * kTileWaves * D / 1024), 256, 0, s>>>(a);
-}
-
-template <int D>
+template <int D, int kCap>
 void Launch(const Args& a, const Cut& c, hipStream_t s) {
-  if (c.by_tile) LaunchTiles<D>(a, c, s);
+  if (c.by_tile) TileAttentionKernel<D, kCap><<<c.tiles * a.cache.kv_heads * c.tile_splits, 64 * kTileWaves, 0, s>>>(a);
+  if (c.by_tile && c.tile_splits > 1) {
+    TileMergeKernel<D><<<dim3(c.tiles * a.cache.kv_heads, 32 * kTileWaves * D / 1024), 256, 0, s>>>(a);
+  }
   if (!c.by_row) return;
   const uint32_t grid = (c.places + 7) / 8 * 8;  // whole rounds of the dies
-  if (D == 256 || c.row_tiles == 1) {
-    a.capped ? RowAttentionKernel<D, 1, true><<<grid, 64 * kRowWaves, 0, s>>>(a)
-             : RowAttentionKernel<D, 1, false><<<grid, 64 * kRowWaves, 0, s>>>(a);
+  constexpr int kTiles = D == 256 ? 1 : 2;
+  if (c.row_tiles < kTiles) {
+    RowAttentionKernel<D, 1, kCap><<<grid, 64 * kRowWaves, 0, s>>>(a);
   } else {
-    constexpr int kTiles = D == 256 ? 1 : 2;
-    a.capped ? RowAttentionKernel<D, kTiles, true><<<grid, 64 * kRowWaves, 0, s>>>(a)
-             : RowAttentionKernel<D, kTiles, false><<<grid, 64 * kRowWaves, 0, s>>>(a);
+    RowAttentionKernel<D, kTiles, kCap><<<grid, 64 * kRowWaves, 0, s>>>(a);
   }
   if (c.merge) {
     RowMergeKernel<D><<<dim3(c.merge_rows, a.cache.kv_heads, a.batch), 256, 0, s>>>(a);
@@ -1482,8 +1491,12 @@ extern "C" ROOST_API RoostStatus roost_amd_paged_attention_f4_run(RoostContext* 
     const float scale = p.sm_scale != 0.0f ? p.sm_scale : 1.0f / std::sqrt(static_cast<float>(p.cache.head_dim));
     constexpr float kLog2e = 1.44269504f;
     a.scale_log2 = scale * kLog2e;
-    a.capped = p.logits_soft_cap > 0.0f;
-    if (a.capped) a.cap = {p.logits_soft_cap * kLog2e, 2.0f / p.logits_soft_cap};
+    const int kind = p.logits_soft_cap <= 0.0f ? kNoCap : p.logits_soft_cap <= kNearMost ? kNearCap : kFarCap;
+    if (kind != kNoCap) {
+      // Held to finite numbers at both ends: a cap times log2(e) may pass f32, and so may its reciprocal.
+      const float cap = p.logits_soft_cap, capl = std::min(cap * kLog2e, FLT_MAX);
+      a.cap = {capl, kind == kFarCap ? static_cast<float>(1 / (double{cap} * kLog2e)) : std::min(2.0f / cap, FLT_MAX)};
+    }
     a.causal = p.causal, a.window = p.window_left;
     a.part_o = ws != nullptr ? static_cast<float*>(ws->device) : nullptr;
     a.part_ml = a.part_o + c.rows * p.cache.head_dim;
@@ -1495,12 +1508,22 @@ extern "C" ROOST_API RoostStatus roost_amd_paged_attention_f4_run(RoostContext* 
     a.short_tokens = c.short_tokens, a.row_limit = c.row_limit;
     a.tile_splits = c.tile_splits;
     const hipStream_t s = roost::Stream(stream);
-    if (p.cache.head_dim == 64) {
-      Launch<64>(a, c, s);
-    } else if (p.cache.head_dim == 128) {
-      Launch<128>(a, c, s);
+    const auto launch = [&](auto cap) {
+      constexpr int kCap = decltype(cap)::value;
+      if (p.cache.head_dim == 64) {
+        Launch<64, kCap>(a, c, s);
+      } else if (p.cache.head_dim == 128) {
+        Launch<128, kCap>(a, c, s);
+      } else {
+        Launch<256, kCap>(a, c, s);
+      }
+    };
+    if (kind == kNoCap) {
+      launch(std::integral_constant<int, kNoCap>{});
+    } else if (kind == kNearCap) {
+      launch(std::integral_constant<int, kNearCap>{});
     } else {
-      Launch<256>(a, c, s);
+      launch(std::integral_constant<int, kFarCap>{});
     }
     return roost::HipStatus(hipGetLastError(), kOp, "kernel launch");
   });
