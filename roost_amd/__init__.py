@@ -567,6 +567,15 @@ def gdn_chunk_layer(session: OpSession, conv_params, gates_params, gdn_params, n
 
 # ---- the fused ops between the residual stream and the projections (AddRmsNorm, AddRmsNormQuant, SiluMulQuant, GemmLora) ----
 
+def _stride(name, what, stride, least):
+    """A row stride as a record's 32 bits carry it."""
+    if stride < least:
+        raise ValueError(f"{name}: {what} are {stride} elements apart, below their {least}")
+    if stride >= 2 ** 32:
+        raise ValueError(f"{name}: {what} are {stride} elements apart, 2^32 or more")
+    return stride
+
+
 def _rows(t, name, rows, dim, dtypes=None):
     """(span, row stride) of a [rows, dim] tensor whose columns are contiguous; an empty span for None."""
     if t is None:
@@ -577,9 +586,7 @@ def _rows(t, name, rows, dim, dtypes=None):
         raise ValueError(f"{name}: {t.dtype} is not one of {dtypes}")
     if dim > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: columns are {t.stride(1)} elements apart, not 1")
-    stride = t.stride(0) if rows > 1 else dim
-    if stride < dim:
-        raise ValueError(f"{name}: rows are {stride} elements apart, below their {dim} columns")
+    stride = _stride(name, "rows", t.stride(0) if rows > 1 else dim, dim)
     return span(t, length=0 if rows == 0 else (rows - 1) * stride + dim), stride
 
 
@@ -768,9 +775,7 @@ def _token_heads(t, name, tokens, heads, dim):
         raise ValueError(f"{name}: shape {tuple(t.shape)}, not {(tokens, heads, dim)}")
     if dim > 1 and t.stride(2) != 1 or heads > 1 and t.stride(1) != dim:
         raise ValueError(f"{name}: strides {t.stride()}: a token's heads have to be contiguous")
-    stride = t.stride(0) if tokens > 1 else heads * dim
-    if stride < heads * dim:
-        raise ValueError(f"{name}: tokens are {stride} elements apart, below their {heads * dim} elements")
+    stride = _stride(name, "tokens", t.stride(0) if tokens > 1 else heads * dim, heads * dim)
     return span(t, length=0 if tokens == 0 else (tokens - 1) * stride + heads * dim), stride
 
 
