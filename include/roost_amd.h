@@ -412,7 +412,7 @@ typedef struct RoostAmdPagedAttentionF4Params {
   uint32_t max_blocks;
   uint32_t max_q_len;
   uint32_t max_kv_len;
-  float sm_scale;        /* 0 = 1/sqrt(head_dim) */
+  float sm_scale;        /* at most 2^126; 0 = 1/sqrt(head_dim) */
   float logits_soft_cap; /* 0 = off */
   int32_t window_left;   /* -1 = no sliding window */
   uint32_t causal;

@@ -1360,6 +1360,8 @@ RoostStatus Admit(const RoostAmdPagedAttentionF4Params& p, uint64_t& pages) {
       .Expect(p.window_left < 0 || p.causal == 1, ROOST_STATUS_UNSUPPORTED, "a window without causal has no kernel here")
       .Expect(p.sm_scale >= 0.0f && p.sm_scale < INFINITY, ROOST_STATUS_INVALID_ARGUMENT,
               "sm_scale = %g is not 0 (1/sqrt(head_dim)) or positive and finite", p.sm_scale)
+      .Expect(p.sm_scale <= 0x1p126f, ROOST_STATUS_UNSUPPORTED, "sm_scale = %g, above 2^126: its product with log2(e) passes f32",
+              p.sm_scale)
       .Expect(p.logits_soft_cap >= 0.0f && p.logits_soft_cap < INFINITY, ROOST_STATUS_INVALID_ARGUMENT,
               "logits_soft_cap = %g is not 0 or positive and finite", p.logits_soft_cap);
   ROOST_GATE_RETURN(gate);
