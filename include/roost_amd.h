@@ -374,8 +374,8 @@ ROOST_API RoostStatus roost_amd_cache_read_f4_run(RoostContext* ctx, const void*
 
 /* PagedAttentionF4: attention of a step's queries over such a cache, decode rows, prompt chunks and both in one call. Sequence
  * b's queries are rows cu_seqlens[b] .. cu_seqlens[b + 1] of q and stand at its last positions: with n of them and `len` keys,
- * query i is at position len - n + i and sees the keys up to it (all of them unless causal), from position - window_left on
- * where window_left >= 0. Per query head h with KV head h / (q_heads / kv_heads):
+ * query i is at position len - n + i and sees the keys up to it, from position - window_left on where window_left >= 0; all keys,
+ * wherever it stands, unless causal (a window needs causal). Per query head h with KV head h / (q_heads / kv_heads):
  *   s_j = sm_scale q . k_j, with logits_soft_cap > 0 then cap tanh(s_j / cap); p = softmax(s); out = sum_j p_j v_j;
  *   lse = log2 sum_j exp(s_j).
  * A query that sees no key has zero output and an lse of minus infinity. Rows of no sequence (behind cu_seqlens[batch], in a
@@ -385,12 +385,16 @@ ROOST_API RoostStatus roost_amd_cache_read_f4_run(RoostContext* ctx, const void*
  *     sequences[b], or b where sequences is NULL;
  *   - kv_indptr [batch + 1], block_tables [.] and kv_lens [batch] as the plan region's kv_indptr, kv_indices and
  *     kv_last_page_len; max_blocks, table_rows and sequences are 0.
- * A page id outside the pool holds no keys; a row outside the tables has none; lengths are cut to the row's pages. Queries past
- * the keys (n > len) see none; cu_seqlens[0] = 0 and cu_seqlens does not go backwards (else the rows in question are undefined
+ * A page id outside the pool holds no keys; a row outside the tables has none; lengths are cut to the row's pages. Causal
+ * queries in front of the first key (n > len) see none; cu_seqlens[0] = 0 and cu_seqlens does not go backwards (else the rows in question are undefined
  * or unwritten, and nothing outside the spans is read or written).
  * max_q_len and max_kv_len are the largest n and len that the caller expects (0: unknown). They choose how the work is cut and
- * bound nothing: longer sequences are computed too, only less evenly spread.
- * Scores and sums are f32; each probability is rounded to bf16 once, in front of its product with v. q is 16-byte aligned, its
+ * bound nothing: longer sequences are computed too, only less evenly spread. Without max_q_len a step of decode rows also launches
+ * what prompt chunks need. In a batch of more than 704 sequences each one's keys stay with one workgroup a KV head.
+ * Unlike RoostPagedAttentionParams, a window_left of 0 (each query sees itself) is taken, and of the negative ones -1 alone; a
+ * negative cap and a window without causal are refused.
+ * Scores and sums are f32; each probability is rounded to bf16 once, in front of its product with v. The sums before their division
+ * stay in f32 where |v| < 2^120 / len. q is 16-byte aligned, its
  * token stride a multiple of 8; q_heads is a multiple of kv_heads, at most 32 to each; tokens are below 2^24. */
 typedef struct RoostAmdPagedAttentionF4Params {
   uint32_t struct_size;
