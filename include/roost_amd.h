@@ -386,16 +386,16 @@ ROOST_API RoostStatus roost_amd_cache_read_f4_run(RoostContext* ctx, const void*
  *   - kv_indptr [batch + 1], block_tables [.] and kv_lens [batch] as the plan region's kv_indptr, kv_indices and
  *     kv_last_page_len; max_blocks, table_rows and sequences are 0.
  * A page id outside the pool holds no keys; a row outside the tables has none; lengths are cut to the row's pages. Causal
- * queries in front of the first key (n > len) see none; cu_seqlens[0] = 0 and cu_seqlens does not go backwards (else the rows in question are undefined
- * or unwritten, and nothing outside the spans is read or written).
+ * queries in front of the first key (n > len) see none; cu_seqlens[0] = 0 and cu_seqlens does not go backwards (else the rows in
+ * question are undefined or unwritten, and nothing outside the spans is read or written).
  * max_q_len and max_kv_len are the largest n and len that the caller expects (0: unknown). They choose how the work is cut and
  * bound nothing: longer sequences are computed too, only less evenly spread. Without max_q_len a step of decode rows also launches
  * what prompt chunks need. In a batch of more than 704 sequences each one's keys stay with one workgroup a KV head.
  * Unlike RoostPagedAttentionParams, a window_left of 0 (each query sees itself) is taken, and of the negative ones -1 alone; a
  * negative cap and a window without causal are refused.
- * Scores and sums are f32; each probability is rounded to bf16 once, in front of its product with v. The sums before their division
- * stay in f32 where |v| < 2^120 / len. q is 16-byte aligned, its
- * token stride a multiple of 8; q_heads is a multiple of kv_heads, at most 32 to each; tokens are below 2^24. */
+ * Scores and sums are f32; each probability is rounded to bf16 once, in front of its product with v. The sums before their
+ * division stay in f32 where |v| < 2^120 / len. q is 16-byte aligned, its token stride a multiple of 8; q_heads is a multiple of
+ * kv_heads, at most 32 to each; tokens are below 2^24. */
 typedef struct RoostAmdPagedAttentionF4Params {
   uint32_t struct_size;
   uint32_t abi_minor;

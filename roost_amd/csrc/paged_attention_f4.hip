@@ -36,12 +36,12 @@ __device__ __forceinline__ F16v Mfma32(U4 a, U4 b, F16v c) {
 }
 
 // cap tanh(s / cap) in log2 units, y the scaled score. What a kernel is built with:
-//   kNearCap, caps up to 128: capl - 2 capl / (1 + 2^(k y)), off by at most 8 2^-23 cap whatever the score: 1.3e-4, below what rounding
-//     p to bf16 makes of a score.
+//   kNearCap, caps up to 128: capl - 2 capl / (1 + 2^(k y)), off by at most 8 2^-23 cap whatever the score: 1.3e-4, below what
+//     rounding p to bf16 makes of a score.
 //   kFarCap, above: that would lose the score itself (0.02 at a cap of 1e5). With z = |y| / capl up to 1/4 y times a polynomial in
 //     z^2, tanh(z) / z to 4e-9 (fitted for the least largest error), from there on as near: off by at most 16 2^-23 of the score.
-//     A kernel of its own, for three times the instructions and more registers: a prompt chunk of 3,500 tokens on 500, 32 heads over 8
-//     of 128, takes 265 us, with a near cap 195, with none 142; a decode batch 133, 127 and 122.
+//     A kernel of its own, for three times the instructions and more registers: a prompt chunk of 3,500 tokens on 500, 32 heads
+//     over 8 of 128, takes 265 us, with a near cap 195, with none 142; a decode batch 133, 127 and 122.
 enum Cap : int { kNoCap, kNearCap, kFarCap };
 constexpr float kNearMost = 128.0f;  // the largest cap of kNearCap
 struct SoftCap {
@@ -178,7 +178,7 @@ struct Deal {
 // ---- The row kernel -----------------------------------------------------------------------------------------------------------
 // Up to 16 kTiles rows (a few tokens' query heads of one KV head) against one part of a sequence's keys: decode. Bound by the
 // cache's bytes, 1.06 D a key and KV head: 64 sequences of 500 to 16,000 keys, 32 heads over 8 of 128, 632 MB, take 128 us (4.9
-// TB/s of the 5.1 that a copy reaches) and the merge of their parts 6.
+// TB/s; a copy reaches 5.1, a stream that only reads 7.0) and the merge of their parts 6.
 //
 // Operands of v_mfma_f32_16x16x32_bf16, lane l = 16 g + m: A[m][8 g + j], B[8 g + j][m], result [4 g + i][m].
 //   S^T = K Q^T: key m of 16 as A, query row m as B. The contraction runs over the dims in any order, so lane (m, g) takes its
@@ -209,10 +209,10 @@ struct RowRing {
   static constexpr int kStages = D == 256 ? 2 : 3;
 };
 
-// Workgroups of the row kernel that a CU holds, which its launch bounds ask for and the host deals the keys to. One tile of rows: 4,
-// 3 and 2 at head_dim 64, 128 and 256, by LDS (29, 54 and 71 KB) and registers (128, 167 and 215); two tiles: 2, by registers (174
-// and 230). Dealt to more than it holds, a second round follows: 64 sequences of 5 tokens and 500 to 16,000 keys, 32 heads over 8 of
-// 128, take 192 us, dealt to 3 a CU 206; a token of 32 heads a KV head 65 against 80.
+// Workgroups of the row kernel that a CU holds, which its launch bounds ask for and the host deals the keys to. One tile of rows:
+// 4, 3 and 2 at head_dim 64, 128 and 256, by LDS (29, 54 and 71 KB) and registers (128, 168 and 216); two tiles: 2, by registers
+// (174 and 230). Dealt to more than it holds, a second round follows: 64 sequences of 5 tokens and 500 to 16,000 keys, 32 heads
+// over 8 of 128, take 192 us, dealt to 3 a CU 206; a token of 32 heads a KV head 65 against 80.
 constexpr uint32_t RowsResident(uint32_t d, uint32_t tiles) { return tiles == 2 || d == 256 ? 2 : d == 128 ? 3 : 4; }
 
 // The memory that p points at in each lane to LDS, 16 (or 4) bytes a lane, one behind the other from `lds` on. M0 is read
@@ -910,9 +910,10 @@ __global__ void __launch_bounds__(64 * kTileWaves, kTileWaves / 4) TileAttention
     for (int32_t t = 0; t < tiles; ++t) {
       __syncthreads();  // tile t is in LDS; nobody reads tile t - 1 any more
       const int slot = t % 3, after = (t + 2) % 3;
-      // What depends on the lane is made anew from its number each time: kept, it would not fit the registers at head_dim 256,
-      // and at 64 leave room for one workgroup a CU instead of two (four prompts of 1,000 to 2,000 tokens on prefixes, 32 heads
-      // over 8: 105 us, kept 125). At 128 there is room, and it is kept (544 us; anew 620).
+      // What depends on the lane is made anew from its number each time: kept, it would at 64 leave room for one workgroup a CU
+      // instead of two (four prompts of 1,000 to 2,000 tokens on prefixes, 32 heads over 8: 105 us, kept 125). At 128 there is
+      // room, and it is kept (544 us; anew 620). At 256 all 256 registers are taken and 10 more values go to scratch (kept: 51):
+      // in front of and behind this loop and in a careful pass; with a cap a query operand's four are read in it too.
       int tid = threadIdx.x;
       if constexpr (D != 128) asm volatile("" : "+v"(tid));
       const int lane = tid & 63, m = lane & 31, g = lane >> 5;
